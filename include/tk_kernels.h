@@ -397,6 +397,85 @@ TK_API int tk_silu_mul(tk_dtype_t dtype, const void* gate, const void* up, void*
 TK_API int tk_silu_mul_amax(tk_dtype_t dtype, const void* gate, const void* up, void* y, int64_t n,
                             float* amax_out, void* stream);
 
+/* ---- training: dropout ---------------------------------------------------------
+ * y[i] = keep_i ? T(x[i] / (1 - p)) : 0 over n contiguous elements, without a
+ * stored mask: element i takes word i % 4 of the Philox4x32-10 block with
+ * counter (i / 4, offset) and key seed, and is kept when the word is at least
+ * round(p * 2^32).  0 <= p <= 1 (1 drops everything; a dropped element is 0
+ * whatever its value).  The backward pass is the same call on the gradient.  y
+ * may be x; other overlaps are not allowed.  seed and offset are host values,
+ * so a captured call replays its mask.  The reference's attention refuses
+ * dropout_p (torch_kunlun/kunlun/attention.py:36-107) for want of a generator. */
+TK_API int tk_dropout(tk_dtype_t dtype, const void* x, void* y, int64_t n, double p, uint64_t seed,
+                      uint64_t offset, void* stream);
+
+/* ---- training: norms around a block ----------------------------------------------
+ * The norm behind a transformer block with its dropout, gate and residual
+ * scale, and the norm before the next block, on contiguous [rows, cols]
+ * tensors of one dtype:
+ *
+ *   u     = post_norm ? Norm(f) * post_weight + post_bias : f
+ *   d     = dropout(u; p, seed, offset)      (element row * cols + col)
+ *   x_new = residual_scale * x + gate * d
+ *   h     = Norm(x_new) * weight + bias
+ *
+ * Norm subtracts the row's mean (TK_NORM_LAYER) and divides by
+ * sqrt(mean square + eps).  NULL weights stand for 1, NULL biases for 0, a
+ * NULL gate for 1.  gate is [gate_rows, cols]: row r uses gate row
+ * r / (rows / gate_rows) (1: one for each channel; the batch size: one for
+ * each sample; rows: one for each token).  Sums and statistics are fp32; each
+ * output is rounded once.  stats (NULL or 16-byte aligned, [rows][4]) receives
+ * mean and rstd of f (post norm only) and of x_new for the backward pass.
+ * cols <= 32768.  Outputs must not overlap inputs.  Extends layer_norm
+ * (csrc/ops_nn.cpp:85-130) and the adds around it (csrc/ops.cpp:117-149). */
+typedef enum { TK_NORM_LAYER = 0, TK_NORM_RMS = 1 } tk_norm_t;
+
+typedef struct {
+    tk_dtype_t dtype;
+    tk_norm_t norm;
+    int64_t rows, cols;
+    const void* x;
+    const void* f;
+    const void* weight;
+    const void* bias;
+    int post_norm;
+    const void* post_weight;
+    const void* post_bias;
+    const void* gate;
+    int64_t gate_rows; /* ignored without a gate */
+    float residual_scale, eps;
+    double p;
+    uint64_t seed, offset;
+    void* x_new;
+    void* h;
+    float* stats;
+} tk_residual_norm_desc_t;
+
+TK_API int tk_residual_norm(const tk_residual_norm_desc_t* desc, void* stream);
+
+/* Its gradients.  fwd holds the forward call's sizes, parameters, x_new and
+ * stats, and f where there is a post norm or a gate; its x, h and bias are not
+ * read.  grad_x_new and grad_h are the gradients of the outputs (NULL: zero,
+ * not both).  Each result may be NULL: dx, df [rows, cols], dweight, dbias,
+ * dpost_weight, dpost_bias [cols], dgate [gate_rows, cols].  Column sums are
+ * fp32 in a fixed order (deterministic). */
+typedef struct {
+    tk_residual_norm_desc_t fwd;
+    const void* grad_x_new;
+    const void* grad_h;
+    void* dx;
+    void* df;
+    void* dweight;
+    void* dbias;
+    void* dpost_weight;
+    void* dpost_bias;
+    void* dgate;
+} tk_residual_norm_grad_desc_t;
+
+TK_API size_t tk_residual_norm_backward_workspace_size(const tk_residual_norm_grad_desc_t* desc);
+TK_API int tk_residual_norm_backward(const tk_residual_norm_grad_desc_t* desc, void* workspace,
+                                     size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

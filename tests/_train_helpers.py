@@ -1,0 +1,124 @@
+"""64-bit references of the training operators and the bounds their tests use.
+
+`philox_words` is Philox4x32-10 (Salmon, Moraes, Dror and Shaw, SC 2011) in
+numpy integers.  `residual_norm64` evaluates the residual norm and its
+gradients from the formulas, with the sum of the absolute values of the terms
+each result is built from: a result's error is at most one ulp of T (its
+rounding, which a binary32 error can move across a boundary) plus a relative
+error of those terms.
+"""
+import numpy as np
+import torch
+
+U32 = 2.0 ** -24          # half a binary32 step, relative
+HALF_STEP = {torch.float16: 2.0 ** -11, torch.float32: 2.0 ** -24}
+# Roundings on a term's way through one row sum: at most 24 additions in a
+# thread and 5 + 9 levels across threads, then a handful of products.
+K = 48
+
+
+def philox_words(n, seed, offset):
+    i = np.arange((n + 3) // 4, dtype=np.uint64)
+    lo = np.uint64(0xFFFFFFFF)
+    s = np.uint64(32)
+    c = [i & lo, i >> s, np.full_like(i, offset & 0xFFFFFFFF), np.full_like(i, offset >> 32)]
+    k = [seed & 0xFFFFFFFF, seed >> 32]
+    for _ in range(10):
+        a, b = c[0] * np.uint64(0xD2511F53), c[2] * np.uint64(0xCD9E8D57)
+        c = [(b >> s) ^ c[1] ^ np.uint64(k[0]), b & lo, (a >> s) ^ c[3] ^ np.uint64(k[1]), a & lo]
+        k = [(k[0] + 0x9E3779B9) & 0xFFFFFFFF, (k[1] + 0xBB67AE85) & 0xFFFFFFFF]
+    return np.stack(c, axis=1).reshape(-1)[:n]
+
+
+def keep_mask(shape, p, seed, offset):
+    n = int(np.prod(shape))
+    return torch.from_numpy(philox_words(n, seed, offset) >= np.uint64(round(p * 2.0 ** 32))).reshape(shape)
+
+
+def ulp(v, dtype):
+    bits, low = (10, -14) if dtype == torch.float16 else (23, -126)
+    return 2.0 ** (torch.floor(torch.log2(v.abs().clamp_min(2.0 ** low))) - bits)
+
+
+def assert_within(got, want, bound, what):
+    assert got.shape == want.shape, (what, got.shape, want.shape)
+    err = (got.double() - want).abs()
+    bad = ~(err <= bound)
+    assert not bad.any(), (f"{what}: {int(bad.sum())} of {err.numel()} beyond the bound, first at "
+                           f"{bad.nonzero()[:3].tolist()}: got {got.double()[bad][:3].tolist()}, "
+                           f"want {want[bad][:3].tolist()}, bound {bound.expand_as(err)[bad][:3].tolist()}")
+
+
+def _norm64(v, rms, eps):
+    mean = torch.zeros_like(v[..., :1]) if rms else v.mean(-1, keepdim=True)
+    rstd = ((v - mean).square().mean(-1, keepdim=True) + eps).rsqrt()
+    return (v - mean) * rstd, rstd, v.abs().amax(-1, keepdim=True) * rstd
+
+
+def residual_norm64(x, f, weight=None, bias=None, post=False, post_weight=None, post_bias=None, gate=None,
+                    rms=False, scale=1.0, eps=1e-5, keep=None, p=0.0, gx=None, gh=None):
+    """{name: (value, bound)} in float64 on the rounded inputs; gradients when
+    gx / gh are given (the missing one counts as zero)."""
+    dtype = x.dtype
+    d = {n: t.double() for n, t in dict(x=x, f=f, w=weight, b=bias, pw=post_weight, pb=post_bias, gate=gate,
+                                        gx=gx, gh=gh).items() if t is not None}
+    one = torch.ones((), dtype=torch.float64)
+    w, b, pw, pb, gt = d.get("w", one), d.get("b", 0 * one), d.get("pw", one), d.get("pb", 0 * one), d.get("gate", one)
+    drop = one if keep is None else keep.double() / (1.0 - p) if p < 1 else torch.zeros_like(d["x"])
+    u, m_u, c_u = d["f"], d["f"].abs(), 0.0
+    if post:
+        q, rq, aq = _norm64(d["f"], rms, eps)
+        c_q = K * U32 * (1 + aq)
+        u, m_u, c_u = q * pw + pb, (1 + q.abs()) * pw.abs() + pb.abs(), c_q
+    x_new = scale * d["x"] + gt * drop * u
+    m_x = abs(scale) * d["x"].abs() + (gt * drop).abs() * m_u
+    e_x = (c_u + 8 * U32) * m_x                       # binary32 error of x_new
+    n, rn, an = _norm64(x_new, rms, eps)
+    # n moves with x_new's error, its own row sums and (in the backward pass) x_new's rounding
+    c_n = K * U32 * (1 + an) + 2 * e_x.amax(-1, keepdim=True) * rn
+    h = n * w + b
+    out = {"x_new": (x_new, ulp(x_new, dtype) + e_x),
+           "h": (h, ulp(h, dtype) + (c_n + 4 * U32) * ((1 + n.abs()) * w.abs() + b.abs()))}
+    if gx is None and gh is None:
+        return out
+    zero = torch.zeros_like(x_new)
+    vx, vh = d.get("gx", zero), d.get("gh", zero)
+    c_b = c_n + HALF_STEP[dtype] * an                 # n from the rounded x_new
+    t = vh * w
+    mean = (lambda v: torch.zeros_like(v[..., :1])) if rms else (lambda v: v.mean(-1, keepdim=True))
+    both = lambda v: v.mean(-1, keepdim=True)  # noqa: E731
+    g = vx + rn * (t - mean(t) - n * both(t * n))
+    m_g = vx.abs() + rn * (t.abs() + (1 + n.abs()) * (both(t.abs()) + both((t * n).abs())))
+    e_g = (c_b + K * U32) * 2 * m_g
+    rows = x.numel() // x.shape[-1]
+    dims = tuple(range(x.dim() - 1))
+
+    def total(name, v, err, mag, over=dims, shape=None):
+        s = v.sum(over, keepdim=shape is not None)
+        e = (err + (rows + 64) * U32 * mag).sum(over, keepdim=shape is not None)
+        out[name] = (s, ulp(s, dtype) + e)
+
+    out["x"] = (scale * g, ulp(scale * g, dtype) + abs(scale) * e_g)
+    total("weight", vh * n, vh.abs() * c_b * (1 + n.abs()), (vh * n).abs())
+    total("bias", vh, 0 * zero, vh.abs())
+    e_u = (c_u + 8 * U32) * m_u * drop.abs()
+    if gate is not None:
+        v, e, m = g * drop * u, e_g * (drop * u).abs() + m_g * e_u, m_g * drop.abs() * m_u
+        if gate.dim() == 1:
+            total("gate", v, e, m)
+        else:
+            over = tuple(i for i in range(x.dim() - 1) if gate.shape[i] != x.shape[i])
+            if over:
+                total("gate", v, e, m, over, True)
+            else:
+                out["gate"] = (v, ulp(v, dtype) + e + 4 * U32 * m)
+    gu, e_gu, m_gu = gt * drop * g, (gt * drop).abs() * (e_g + 4 * U32 * m_g), (gt * drop).abs() * m_g
+    if post:
+        total("post_weight", gu * q, e_gu * (1 + q.abs()) + m_gu * c_q * (1 + q.abs()), m_gu * (1 + q.abs()))
+        total("post_bias", gu, e_gu, m_gu)
+        t, e_t, m_t = gu * pw, e_gu * pw.abs(), m_gu * pw.abs()
+        gu = rq * (t - mean(t) - q * both(t * q))
+        spread = lambda v: v + (1 + q.abs()) * (both(v) + both(v * q.abs()))  # noqa: E731
+        e_gu = rq * (spread(e_t) + 2 * (c_q + K * U32) * spread(m_t))
+    out["f"] = (gu, ulp(gu, dtype) + e_gu)
+    return out

@@ -1,0 +1,151 @@
+"""What needs no GPU of the training operators: the generator's published
+vectors, the 64-bit references against torch's autograd, and the argument
+checks that come before any device work."""
+import ctypes
+
+import numpy as np
+import pytest
+import torch
+
+from tests import _train_helpers as R
+from torch_kunlun_b200 import _capi as C
+
+
+def test_philox_known_answers():
+    # the published test vectors of Philox4x32-10: counter, key -> words
+    def block(counter, key):
+        lo = counter[0] | counter[1] << 32
+        c = [counter[0], counter[1], counter[2], counter[3]]
+        k = [key[0], key[1]]
+        for _ in range(10):
+            a, b = c[0] * 0xD2511F53, c[2] * 0xCD9E8D57
+            c = [(b >> 32) ^ c[1] ^ k[0], b & 0xFFFFFFFF, (a >> 32) ^ c[3] ^ k[1], a & 0xFFFFFFFF]
+            k = [(k[0] + 0x9E3779B9) & 0xFFFFFFFF, (k[1] + 0xBB67AE85) & 0xFFFFFFFF]
+        return c, lo
+    assert block([0] * 4, [0] * 2)[0] == [0x6627E8D5, 0xE169C58D, 0xBC57AC4C, 0x9B00DBD8]
+    assert block([0xFFFFFFFF] * 4, [0xFFFFFFFF] * 2)[0] == [0x408F276D, 0x41C83B0E, 0xA20BC7C6, 0x6D5451FD]
+    assert block([0x243F6A88, 0x85A308D3, 0x13198A2E, 0x03707344], [0xA4093822, 0x299F31D0])[0] == \
+        [0xD16CFE09, 0x94FDCCEB, 0x5001E420, 0x24126EA1]
+    words = R.philox_words(8, 0x299F31D0A4093822, 0x0370734413198A2E)
+    for i in range(2):
+        assert list(words[4 * i:4 * i + 4]) == block([i, 0, 0x13198A2E, 0x03707344], [0xA4093822, 0x299F31D0])[0]
+    assert words.dtype == np.uint64
+
+
+@pytest.mark.parametrize("rms", [False, True])
+@pytest.mark.parametrize("post", [False, True])
+def test_residual_norm_reference_matches_autograd(rms, post):
+    g = torch.Generator().manual_seed(3)
+    n = lambda *s: torch.randn(*s, generator=g, dtype=torch.float32)  # noqa: E731
+    x, f, w, b, gate = n(2, 5, 12), n(2, 5, 12), n(12), n(12), n(2, 1, 12)
+    pw, pb = (n(12), n(12)) if post else (None, None)
+    gx, gh, keep = n(2, 5, 12), n(2, 5, 12), torch.rand(2, 5, 12, generator=g) > 0.3
+    got = R.residual_norm64(x, f, w, b, post, pw, pb, gate, rms, 0.7, 1e-5, keep, 0.3, gx, gh)
+    leaves = {k: v.double().requires_grad_() for k, v in dict(x=x, f=f, weight=w, bias=b, post_weight=pw, post_bias=pb, gate=gate).items() if v is not None}
+
+    def norm(v, w, b):
+        m = 0 if rms else v.mean(-1, keepdim=True)
+        return (v - m) / ((v - m).square().mean(-1, keepdim=True) + 1e-5).sqrt() * w + b
+
+    u = norm(leaves["f"], leaves["post_weight"], leaves["post_bias"]) if post else leaves["f"]
+    x_new = 0.7 * leaves["x"] + leaves["gate"] * u * keep.double() / 0.7
+    h = norm(x_new, leaves["weight"], leaves["bias"])
+    grads = torch.autograd.grad([x_new, h], list(leaves.values()), [gx.double(), gh.double()])
+    for k, v in {"x_new": x_new, "h": h, **dict(zip(leaves, grads))}.items():
+        assert torch.allclose(got[k][0], v, rtol=1e-10, atol=1e-10), k
+
+
+def test_dropout_refuses_bad_arguments_before_the_device():
+    L = C.lib()
+    assert L.tk_dropout(5, 16, 16, 4, 0.1, 1, 0, None) == 1
+    assert L.tk_dropout(0, 16, 16, -1, 0.1, 1, 0, None) == 1
+    assert L.tk_dropout(0, None, 16, 4, 0.1, 1, 0, None) == 1
+    for p in (-0.5, 1.5, float("nan")):
+        assert L.tk_dropout(0, 16, 16, 4, p, 1, 0, None) == 1
+        assert b"[0, 1]" in L.tk_last_error_string()
+    assert L.tk_dropout(0, None, None, 0, 0.1, 1, 0, None) == 0  # nothing to do
+
+
+def _norm_desc(**kw):
+    d = C.ResidualNormDesc()
+    d.dtype, d.norm, d.rows, d.cols, d.residual_scale, d.eps = 0, 0, 4, 16, 1.0, 1e-5
+    for k, v in kw.items():
+        setattr(d, k, v)
+    return d
+
+
+@pytest.mark.parametrize("fields,status", [
+    (dict(dtype=7), 1), (dict(norm=2), 1), (dict(rows=-1), 1), (dict(cols=0), 1), (dict(cols=32769), 2),
+    (dict(p=1.5), 1), (dict(p=float("nan")), 1), (dict(post_weight=16), 1), (dict(gate=16, gate_rows=3), 1),
+    (dict(gate=16, gate_rows=0), 1), (dict(rows=1 << 62), 1), (dict(), 1)])  # the last: NULL tensors
+def test_residual_norm_refuses_bad_arguments_before_the_device(fields, status):
+    L = C.lib()
+    d = _norm_desc(**fields)
+    assert L.tk_residual_norm(ctypes.byref(d), None) == status
+    g = C.ResidualNormGradDesc()
+    g.fwd = d
+    assert L.tk_residual_norm_backward(ctypes.byref(g), None, 0, None) == status
+    if fields:
+        assert L.tk_residual_norm_backward_workspace_size(ctypes.byref(g)) == 0
+    assert L.tk_residual_norm(None, None) == 1 and L.tk_residual_norm_backward(None, None, 0, None) == 1
+
+
+def test_residual_norm_backward_needs_its_inputs():
+    L = C.lib()
+    g = C.ResidualNormGradDesc()
+    g.fwd = _norm_desc(x_new=16, stats=16)
+    assert L.tk_residual_norm_backward(ctypes.byref(g), None, 0, None) == 1
+    assert b"no incoming gradient" in L.tk_last_error_string()
+    g.grad_h = 16
+    g.fwd.post_norm = 1
+    assert L.tk_residual_norm_backward(ctypes.byref(g), None, 0, None) == 1
+    assert b"f is needed" in L.tk_last_error_string()
+    g.fwd.stats = 8
+    assert L.tk_residual_norm_backward(ctypes.byref(g), None, 0, None) == 1
+    assert L.tk_residual_norm(ctypes.byref(_norm_desc(rows=0)), None) == 0
+
+
+@pytest.mark.parametrize("rows,units", [(1, 1), (5, 3), (148, 148), (1000, 296), (16384, 296), (97, 96)])
+def test_row_ranges_partition_and_unit_of_inverts(rows, units):
+    # unit_begin / unit_of of residual_norm.cu
+    begin = [u * rows // units for u in range(units + 1)]
+    assert begin[0] == 0 and begin[-1] == rows and all(a < b for a, b in zip(begin, begin[1:]))
+    for r in range(rows):
+        u = ((r + 1) * units - 1) // rows
+        assert begin[u] <= r < begin[u + 1]
+
+
+@pytest.mark.parametrize("rows,units,gate_rows", [(12, 5, 3), (4001 * 3, 296, 3), (811 * 13, 148, 811), (96, 7, 96 // 2), (300, 13, 1)])
+def test_gate_segments_reach_the_column_kernel_once(rows, units, gate_rows):
+    """Every gate row is finished exactly once: by the unit that holds it whole,
+    or by the item of the first unit boundary inside it, over the slots its
+    units wrote."""
+    period = rows // gate_rows
+    begin = [u * rows // units for u in range(units + 1)]
+    unit_of = lambda r: ((r + 1) * units - 1) // rows  # noqa: E731
+    written, finished = {}, {}
+    for u in range(units):
+        lo = begin[u]
+        while lo < begin[u + 1]:
+            row = lo // period
+            hi = min(begin[u + 1], (row + 1) * period)
+            if lo == row * period and hi == (row + 1) * period:
+                finished[row] = finished.get(row, 0) + 1
+            else:
+                slot = 2 * u + (0 if lo == begin[u] else 1)
+                assert slot not in written
+                written[slot] = (row, hi - lo)
+            lo = hi
+    for u in range(1, units):
+        row = begin[u] // period
+        if begin[u] % period == 0 or unit_of(row * period) != u - 1:
+            continue
+        last = unit_of((row + 1) * period - 1)
+        covered = 0
+        for v in range(u - 1, last + 1):
+            got_row, n = written.pop(2 * v + (0 if begin[v] // period == row else 1))
+            assert got_row == row
+            covered += n
+        assert covered == period
+        finished[row] = finished.get(row, 0) + 1
+    assert not written and finished == {r: 1 for r in range(gate_rows)}

@@ -28,6 +28,7 @@ EXPORTED = [
     "tk_softmax", "tk_layer_norm", "tk_qgemm_noalloc", "tk_sdpa_workspace_size", "tk_sdpa_q16",
     "tk_reduce_sum", "tk_conv3d_workspace_size", "tk_conv3d_q16", "tk_qgemm_scatter_rows",
     "tk_conv3d_wgrad_workspace_size", "tk_conv3d_wgrad_q16", "tk_silu_mul_amax",
+    "tk_dropout", "tk_residual_norm", "tk_residual_norm_backward_workspace_size", "tk_residual_norm_backward",
 ]
 
 
@@ -84,6 +85,24 @@ class ConvWgradDesc(ctypes.Structure):
         ("amax_x", ctypes.c_void_p), ("amax_g", ctypes.c_void_p)]
 
 
+class ResidualNormDesc(ctypes.Structure):
+    """Mirror of tk_residual_norm_desc_t."""
+    _fields_ = ([("dtype", ctypes.c_int), ("norm", ctypes.c_int), ("rows", ctypes.c_int64), ("cols", ctypes.c_int64)] +
+                [(n, ctypes.c_void_p) for n in ("x", "f", "weight", "bias")] +
+                [("post_norm", ctypes.c_int)] +
+                [(n, ctypes.c_void_p) for n in ("post_weight", "post_bias", "gate")] +
+                [("gate_rows", ctypes.c_int64), ("residual_scale", ctypes.c_float), ("eps", ctypes.c_float),
+                 ("p", ctypes.c_double), ("seed", ctypes.c_uint64), ("offset", ctypes.c_uint64)] +
+                [(n, ctypes.c_void_p) for n in ("x_new", "h", "stats")])
+
+
+class ResidualNormGradDesc(ctypes.Structure):
+    """Mirror of tk_residual_norm_grad_desc_t."""
+    _fields_ = ([("fwd", ResidualNormDesc)] +
+                [(n, ctypes.c_void_p) for n in ("grad_x_new", "grad_h", "dx", "df", "dweight", "dbias",
+                                                "dpost_weight", "dpost_bias", "dgate")])
+
+
 def lib() -> ctypes.CDLL:
     global _lib
     if _lib is None:
@@ -111,6 +130,11 @@ def lib() -> ctypes.CDLL:
         L.tk_conv3d_wgrad_workspace_size.argtypes = [ctypes.POINTER(ConvWgradDesc)]
         L.tk_conv3d_wgrad_workspace_size.restype = ctypes.c_size_t
         L.tk_conv3d_wgrad_q16.argtypes = [ctypes.POINTER(ConvWgradDesc), vp, ctypes.c_size_t, vp]
+        L.tk_dropout.argtypes = [i32, vp, vp, i64, ctypes.c_double, ctypes.c_uint64, ctypes.c_uint64, vp]
+        L.tk_residual_norm.argtypes = [ctypes.POINTER(ResidualNormDesc), vp]
+        L.tk_residual_norm_backward_workspace_size.argtypes = [ctypes.POINTER(ResidualNormGradDesc)]
+        L.tk_residual_norm_backward_workspace_size.restype = ctypes.c_size_t
+        L.tk_residual_norm_backward.argtypes = [ctypes.POINTER(ResidualNormGradDesc), vp, ctypes.c_size_t, vp]
         _lib = L
     return _lib
 

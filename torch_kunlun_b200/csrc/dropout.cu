@@ -1,0 +1,139 @@
+// dropout.cu -- y = keep ? T(x * 1 / (1 - p)) : 0 with the mask of
+// tk_philox.cuh, recomputed wherever it is needed and never stored; the
+// backward pass is the same call on the gradient.
+//
+// Two bytes per fp16 element each way bound it (4 bytes in all); the ten
+// Philox rounds of four elements cost 20 wide multiplies, which run while the
+// thread's loads are in flight.
+#include <cuda_fp16.h>
+
+#include "tk_internal.h"
+#include "tk_philox.cuh"
+
+namespace tk {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kUnroll = 2;  // octets of elements in flight per thread
+
+template <typename T>
+struct Octet {  // 8 elements as one (fp16) or two (fp32) 16-byte vectors
+    static constexpr int N = sizeof(T) / 2;
+    uint4 v[N];
+    __device__ __forceinline__ void load(const T* p) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = __ldcs(reinterpret_cast<const uint4*>(p) + i);
+    }
+    __device__ __forceinline__ void store(T* p) const {
+#pragma unroll
+        for (int i = 0; i < N; ++i) __stcs(reinterpret_cast<uint4*>(p) + i, v[i]);
+    }
+};
+
+__device__ __forceinline__ uint32_t scale2(uint32_t pair, float s, uint32_t keep) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&pair));
+    const __half2 h = __floats2half2_rn(f.x * s, f.y * s);
+    const uint32_t bits = *reinterpret_cast<const uint32_t*>(&h);
+    return bits & ((keep & 1u ? 0x0000FFFFu : 0u) | (keep & 2u ? 0xFFFF0000u : 0u));
+}
+
+__device__ __forceinline__ void apply(Octet<__half>& o, float s, uint32_t keep) {
+    o.v[0].x = scale2(o.v[0].x, s, keep);
+    o.v[0].y = scale2(o.v[0].y, s, keep >> 2);
+    o.v[0].z = scale2(o.v[0].z, s, keep >> 4);
+    o.v[0].w = scale2(o.v[0].w, s, keep >> 6);
+}
+
+__device__ __forceinline__ uint32_t scale1(uint32_t bits, float s, uint32_t keep) {
+    return keep & 1u ? __float_as_uint(__uint_as_float(bits) * s) : 0u;
+}
+
+__device__ __forceinline__ void apply(Octet<float>& o, float s, uint32_t keep) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        o.v[i].x = scale1(o.v[i].x, s, keep >> (4 * i));
+        o.v[i].y = scale1(o.v[i].y, s, keep >> (4 * i + 1));
+        o.v[i].z = scale1(o.v[i].z, s, keep >> (4 * i + 2));
+        o.v[i].w = scale1(o.v[i].w, s, keep >> (4 * i + 3));
+    }
+}
+
+__device__ __forceinline__ float to_f(__half v) { return __half2float(v); }
+__device__ __forceinline__ float to_f(float v) { return v; }
+__device__ __forceinline__ void from_f(float v, __half& o) { o = __float2half_rn(v); }
+__device__ __forceinline__ void from_f(float v, float& o) { o = v; }
+
+// n elements, 16-byte aligned pointers: octets by vectors, the last n % 8
+// elements one thread each.
+template <typename T>
+__global__ void __launch_bounds__(kThreads) dropout_kernel(const T* x, T* y, int64_t n,
+                                                           const DropoutParams d) {
+    const int64_t octets = n / 8;
+    const int64_t base = static_cast<int64_t>(blockIdx.x) * kThreads * kUnroll + threadIdx.x;
+    Octet<T> o[kUnroll];
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+        const int64_t i = base + u * kThreads;
+        if (i < octets) o[u].load(x + 8 * i);
+    }
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+        const int64_t i = base + u * kThreads;
+        if (i < octets) {
+            apply(o[u], d.scale, dropout_keep8(d, i));
+            o[u].store(y + 8 * i);
+        }
+    }
+    const int64_t tail = octets * 8 + threadIdx.x;
+    if (blockIdx.x == gridDim.x - 1 && tail < n) {
+        from_f(dropout_keep1(d, tail) ? to_f(x[tail]) * d.scale : 0.0f, y[tail]);
+    }
+}
+
+// Pointers off a 16-byte boundary: one block of four elements per thread.
+template <typename T>
+__global__ void __launch_bounds__(kThreads) dropout_any_kernel(const T* x, T* y, int64_t n,
+                                                               const DropoutParams d) {
+    const int64_t b = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
+    if (4 * b >= n) return;
+    uint32_t w[4];
+    philox4x32_10(b, d.offset, d.seed, w);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const int64_t i = 4 * b + j;
+        if (i < n) from_f(w[j] >= d.threshold && !d.none_kept ? to_f(x[i]) * d.scale : 0.0f, y[i]);
+    }
+}
+
+template <typename T>
+int dropout_launch(const void* x, void* y, int64_t n, const DropoutParams& d, cudaStream_t s) {
+    const T* xp = static_cast<const T*>(x);
+    T* yp = static_cast<T*>(y);
+    if (((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(y)) & 15) == 0) {
+        const int64_t blocks = std::max<int64_t>(1, ceil_div(n / 8, kThreads * kUnroll));
+        TK_CHECK_ARG(blocks <= 0x7FFFFFFF, "tk_dropout: too many elements");
+        dropout_kernel<T><<<static_cast<unsigned>(blocks), kThreads, 0, s>>>(xp, yp, n, d);
+    } else {
+        const int64_t blocks = ceil_div(ceil_div(n, 4), kThreads);
+        TK_CHECK_ARG(blocks <= 0x7FFFFFFF, "tk_dropout: too many elements");
+        dropout_any_kernel<T><<<static_cast<unsigned>(blocks), kThreads, 0, s>>>(xp, yp, n, d);
+    }
+    return launch_status("dropout");
+}
+
+}  // namespace
+}  // namespace tk
+
+extern "C" int tk_dropout(tk_dtype_t dtype, const void* x, void* y, int64_t n, double p, uint64_t seed,
+                          uint64_t offset, void* stream) {
+    TK_CHECK_ARG(dtype == TK_DTYPE_F16 || dtype == TK_DTYPE_F32, "tk_dropout: bad dtype %d",
+                 static_cast<int>(dtype));
+    TK_CHECK_ARG(n >= 0, "tk_dropout: n must not be negative");
+    TK_CHECK_ARG(p >= 0.0 && p <= 1.0, "tk_dropout: p must be in [0, 1], got %g", p);
+    if (n == 0) return TK_OK;
+    TK_CHECK_ARG(x != nullptr && y != nullptr, "tk_dropout: NULL pointer");
+    const tk::DropoutParams d = tk::dropout_params(p, seed, offset);
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    return dtype == TK_DTYPE_F16 ? tk::dropout_launch<__half>(x, y, n, d, s)
+                                 : tk::dropout_launch<float>(x, y, n, d, s);
+}

@@ -118,4 +118,13 @@ at::Tensor sdpa(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
                 const std::optional<at::Tensor>& mask, bool is_causal, std::optional<double> scale,
                 bool fused);
 
+// ---- training ops exposed to Python (differentiable) ----
+at::Tensor dropout(const at::Tensor& x, double p, uint64_t seed, uint64_t offset);
+std::tuple<at::Tensor, at::Tensor> residual_norm(
+    const at::Tensor& x, const at::Tensor& f, const std::optional<at::Tensor>& weight,
+    const std::optional<at::Tensor>& bias, bool rms, bool post_norm,
+    const std::optional<at::Tensor>& post_weight, const std::optional<at::Tensor>& post_bias,
+    const std::optional<at::Tensor>& gate, double residual_scale, double eps, double p, uint64_t seed,
+    uint64_t offset);
+
 }  // namespace torch_kunlun

@@ -109,6 +109,12 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("sdpa", &sdpa, py::arg("query"), py::arg("key"), py::arg("value"),
           py::arg("attn_mask") = py::none(), py::arg("is_causal") = false,
           py::arg("scale") = py::none(), py::arg("fused") = true);
+    m.def("dropout", &dropout, py::arg("x"), py::arg("p"), py::arg("seed"), py::arg("offset") = 0);
+    m.def("residual_norm", &residual_norm, py::arg("x"), py::arg("f"), py::arg("weight") = py::none(),
+          py::arg("bias") = py::none(), py::arg("rms") = false, py::arg("post_norm") = false,
+          py::arg("post_weight") = py::none(), py::arg("post_bias") = py::none(),
+          py::arg("gate") = py::none(), py::arg("residual_scale") = 1.0, py::arg("eps") = 1e-5,
+          py::arg("p") = 0.0, py::arg("seed") = 0, py::arg("offset") = 0);
     m.def("abi_version", [] { return tk_abi_version(); });
     torch_kunlun::register_peer(m);
 }

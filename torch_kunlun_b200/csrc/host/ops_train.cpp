@@ -1,0 +1,268 @@
+// ops_train.cpp -- the training operators of the kunlun backend that have no
+// aten name: dropout with a recomputed mask and the residual norm, each an
+// autograd function over one or two calls of the C ABI.
+//
+// The reference stops at linear, convolution, relu and MSE gradients
+// (csrc/autograd.cpp) and at a forward layer_norm (csrc/ops_nn.cpp:85-130);
+// these ops follow its float16/float32 rules.  Their backward passes are not
+// differentiable themselves and say so.
+#include <torch/csrc/autograd/custom_function.h>
+
+#include "kunlun.h"
+
+namespace torch_kunlun {
+
+namespace {
+
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+struct DeviceScope {
+    int prev;
+    explicit DeviceScope(int dev) : prev(current_device()) {
+        if (dev >= 0 && dev != prev) cudaSetDevice(dev);
+    }
+    ~DeviceScope() { cudaSetDevice(prev); }
+};
+
+// An autograd function takes an absent tensor as an empty optional.
+using Optional = std::optional<at::Tensor>;
+Optional optional(const at::Tensor& t) { return t.defined() ? Optional(t) : Optional(); }
+at::Tensor or_undefined(const Optional& t) { return t.has_value() ? *t : at::Tensor(); }
+
+void check_input(const at::Tensor& t, const char* op) {
+    TORCH_CHECK(t.defined() && t.device().type() == c10::DeviceType::PrivateUse1, "kunlun ", op,
+                " requires kunlun tensors, got ", t.device());
+    TORCH_CHECK(t.scalar_type() == at::kHalf || t.scalar_type() == at::kFloat, "kunlun ", op,
+                " supports float16/float32, got ", t.scalar_type());
+}
+
+// A parameter of x's dtype on x's device, contiguous; undefined when absent.
+at::Tensor param(const std::optional<at::Tensor>& t, const at::Tensor& x, const char* op, const char* name) {
+    if (!t.has_value() || !t->defined()) return at::Tensor();
+    TORCH_CHECK(t->device() == x.device(), "kunlun ", op, ": ", name, " is on ", t->device(), ", expected ", x.device());
+    TORCH_CHECK(t->scalar_type() == x.scalar_type(), "kunlun ", op, ": ", name, " must be ", x.scalar_type(), ", got ",
+                t->scalar_type());
+    return t->contiguous();
+}
+
+bool needs_grad(std::initializer_list<at::Tensor> ts) {
+    if (!at::GradMode::is_enabled()) return false;
+    for (const at::Tensor& t : ts)
+        if (t.defined() && t.requires_grad()) return true;
+    return false;
+}
+
+void check_single_backward(const char* op) {
+    TORCH_CHECK(!at::GradMode::is_enabled(), "kunlun ", op, ": gradients of its backward pass (create_graph=True) are not implemented");
+}
+
+void* ptr(const at::Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
+
+// ---- dropout --------------------------------------------------------------------
+
+at::Tensor dropout_run(const at::Tensor& x, double p, uint64_t seed, uint64_t offset) {
+    at::Tensor xc = x.contiguous();
+    at::Tensor y = at::empty(xc.sizes(), xc.options());
+    const int dev = xc.device().index();
+    DeviceScope g(dev);
+    check_tk(tk_dropout(tk_dtype(xc.scalar_type()), ptr(xc), ptr(y), xc.numel(), p, seed, offset, current_stream(dev)),
+             "tk_dropout");
+    return y;
+}
+
+struct Dropout : torch::autograd::Function<Dropout> {
+    static at::Tensor forward(AutogradContext* ctx, const at::Tensor& x, double p, int64_t seed, int64_t offset) {
+        ctx->saved_data["p"] = p;
+        ctx->saved_data["seed"] = seed;
+        ctx->saved_data["offset"] = offset;
+        return dropout_run(x, p, static_cast<uint64_t>(seed), static_cast<uint64_t>(offset));
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        check_single_backward("dropout");
+        at::Tensor gx = dropout_run(grads[0], ctx->saved_data["p"].toDouble(),
+                                    static_cast<uint64_t>(ctx->saved_data["seed"].toInt()),
+                                    static_cast<uint64_t>(ctx->saved_data["offset"].toInt()));
+        return {gx, at::Tensor(), at::Tensor(), at::Tensor()};
+    }
+};
+
+// ---- residual norm ----------------------------------------------------------------
+
+struct NormOptions {
+    bool rms, post;
+    double scale, eps, p;
+    int64_t seed, offset;
+};
+
+tk_residual_norm_desc_t norm_desc(const at::Tensor& like, const NormOptions& o, const at::Tensor& weight,
+                                  const at::Tensor& post_weight, const at::Tensor& post_bias, const at::Tensor& gate) {
+    tk_residual_norm_desc_t d = {};
+    d.dtype = tk_dtype(like.scalar_type());
+    d.norm = o.rms ? TK_NORM_RMS : TK_NORM_LAYER;
+    d.cols = like.size(-1);
+    d.rows = like.numel() / d.cols;
+    d.weight = ptr(weight);
+    d.post_norm = o.post ? 1 : 0;
+    d.post_weight = ptr(post_weight);
+    d.post_bias = ptr(post_bias);
+    d.gate = ptr(gate);
+    d.gate_rows = gate.defined() ? gate.numel() / d.cols : 0;
+    d.residual_scale = static_cast<float>(o.scale);
+    d.eps = static_cast<float>(o.eps);
+    d.p = o.p;
+    d.seed = static_cast<uint64_t>(o.seed);
+    d.offset = static_cast<uint64_t>(o.offset);
+    return d;
+}
+
+std::tuple<at::Tensor, at::Tensor> norm_run(const at::Tensor& x, const at::Tensor& f, const at::Tensor& weight,
+                                            const at::Tensor& bias, const at::Tensor& post_weight,
+                                            const at::Tensor& post_bias, const at::Tensor& gate, const NormOptions& o,
+                                            const at::Tensor& stats) {
+    const int dev = x.device().index();
+    DeviceScope g(dev);
+    at::Tensor x_new = at::empty(x.sizes(), x.options()), h = at::empty(x.sizes(), x.options());
+    tk_residual_norm_desc_t d = norm_desc(x, o, weight, post_weight, post_bias, gate);
+    d.x = ptr(x);
+    d.f = ptr(f);
+    d.bias = ptr(bias);
+    d.x_new = ptr(x_new);
+    d.h = ptr(h);
+    d.stats = stats.defined() ? stats.data_ptr<float>() : nullptr;
+    check_tk(tk_residual_norm(&d, current_stream(dev)), "tk_residual_norm");
+    return {x_new, h};
+}
+
+struct ResidualNorm : torch::autograd::Function<ResidualNorm> {
+    static variable_list forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& f, const Optional& weight_in,
+                                 const Optional& bias_in, const Optional& post_weight_in, const Optional& post_bias_in,
+                                 const Optional& gate_in, const NormOptions& o) {
+        const at::Tensor weight = or_undefined(weight_in), bias = or_undefined(bias_in),
+                         post_weight = or_undefined(post_weight_in), post_bias = or_undefined(post_bias_in),
+                         gate = or_undefined(gate_in);
+        const int64_t rows = x.numel() / x.size(-1);
+        at::Tensor stats;
+        {
+            DeviceScope g(x.device().index());
+            stats = at::empty({rows, 4}, x.options().dtype(at::kFloat));
+        }
+        auto [x_new, h] = norm_run(x, f, weight, bias, post_weight, post_bias, gate, o, stats);
+        const bool need_f = o.post || gate.defined();
+        ctx->save_for_backward({x_new, need_f ? f : at::Tensor(), weight, post_weight, post_bias, gate, stats});
+        ctx->saved_data["flags"] = std::vector<bool>{o.rms,
+                                                     o.post,
+                                                     x.requires_grad(),
+                                                     f.requires_grad(),
+                                                     weight.defined() && weight.requires_grad(),
+                                                     bias.defined() && bias.requires_grad(),
+                                                     post_weight.defined() && post_weight.requires_grad(),
+                                                     post_bias.defined() && post_bias.requires_grad(),
+                                                     gate.defined() && gate.requires_grad()};
+        ctx->saved_data["reals"] = std::vector<double>{o.scale, o.eps, o.p};
+        ctx->saved_data["random"] = std::vector<int64_t>{o.seed, o.offset};
+        ctx->set_materialize_grads(false);
+        return {x_new, h};
+    }
+
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        check_single_backward("residual_norm");
+        variable_list out(8);
+        at::Tensor gx = grads[0], gh = grads[1];
+        if (!gx.defined() && !gh.defined()) return out;
+        const variable_list saved = ctx->get_saved_variables();
+        const at::Tensor &x_new = saved[0], &f = saved[1], &weight = saved[2], &post_weight = saved[3],
+                         &post_bias = saved[4], &gate = saved[5], &stats = saved[6];
+        const auto flag = ctx->saved_data["flags"].toBoolList();
+        const auto real = ctx->saved_data["reals"].toDoubleVector();
+        const auto random = ctx->saved_data["random"].toIntVector();
+        const NormOptions o = {flag[0], flag[1], real[0], real[1], real[2], random[0], random[1]};
+        if (gx.defined()) gx = gx.contiguous();
+        if (gh.defined()) gh = gh.contiguous();
+        const int dev = x_new.device().index();
+        DeviceScope g(dev);
+        auto fresh = [&](bool wanted, at::IntArrayRef shape) {
+            return wanted ? at::empty(shape, x_new.options()) : at::Tensor();
+        };
+        const int64_t cols = x_new.size(-1);
+        out[0] = fresh(flag[2], x_new.sizes());
+        out[1] = fresh(flag[3], x_new.sizes());
+        out[2] = fresh(flag[4], {cols});
+        out[3] = fresh(flag[5], {cols});
+        out[4] = fresh(flag[6], {cols});
+        out[5] = fresh(flag[7], {cols});
+        if (flag[8]) out[6] = at::empty(gate.sizes(), gate.options());
+        tk_residual_norm_grad_desc_t d = {};
+        d.fwd = norm_desc(x_new, o, weight, post_weight, post_bias, gate);
+        d.fwd.f = ptr(f);
+        d.fwd.x_new = ptr(x_new);
+        d.fwd.stats = stats.data_ptr<float>();
+        d.grad_x_new = ptr(gx);
+        d.grad_h = ptr(gh);
+        d.dx = ptr(out[0]);
+        d.df = ptr(out[1]);
+        d.dweight = ptr(out[2]);
+        d.dbias = ptr(out[3]);
+        d.dpost_weight = ptr(out[4]);
+        d.dpost_bias = ptr(out[5]);
+        d.dgate = ptr(out[6]);
+        const size_t bytes = tk_residual_norm_backward_workspace_size(&d);
+        TORCH_CHECK(bytes > 0, "kunlun residual_norm: ", tk_last_error_string());
+        at::Tensor ws = workspace(bytes, x_new.device());
+        check_tk(tk_residual_norm_backward(&d, aligned_base(ws), bytes, current_stream(dev)), "tk_residual_norm_backward");
+        return out;
+    }
+};
+
+}  // namespace
+
+at::Tensor dropout(const at::Tensor& x, double p, uint64_t seed, uint64_t offset) {
+    check_input(x, "dropout");
+    TORCH_CHECK(p >= 0.0 && p <= 1.0, "kunlun dropout: p must be in [0, 1], got ", p);
+    if (needs_grad({x})) return Dropout::apply(x, p, static_cast<int64_t>(seed), static_cast<int64_t>(offset));
+    at::AutoDispatchBelowADInplaceOrView guard;
+    return dropout_run(x, p, seed, offset);
+}
+
+std::tuple<at::Tensor, at::Tensor> residual_norm(
+    const at::Tensor& x_in, const at::Tensor& f_in, const std::optional<at::Tensor>& weight_in,
+    const std::optional<at::Tensor>& bias_in, bool rms, bool post_norm, const std::optional<at::Tensor>& post_weight_in,
+    const std::optional<at::Tensor>& post_bias_in, const std::optional<at::Tensor>& gate_in, double residual_scale,
+    double eps, double p, uint64_t seed, uint64_t offset) {
+    const char* op = "residual_norm";
+    check_input(x_in, op);
+    check_input(f_in, op);
+    TORCH_CHECK(x_in.dim() >= 1 && x_in.size(-1) >= 1, "kunlun residual_norm: x needs a last dimension of at least 1");
+    TORCH_CHECK(f_in.sizes().equals(x_in.sizes()), "kunlun residual_norm: f has shape ", f_in.sizes(), ", expected ", x_in.sizes());
+    TORCH_CHECK(p >= 0.0 && p <= 1.0, "kunlun residual_norm: p must be in [0, 1], got ", p);
+    TORCH_CHECK(post_norm || !((post_weight_in.has_value() && post_weight_in->defined()) ||
+                               (post_bias_in.has_value() && post_bias_in->defined())),
+                "kunlun residual_norm: post_weight and post_bias need post_norm=True");
+    const at::Tensor f = param(f_in, x_in, op, "f"), weight = param(weight_in, x_in, op, "weight"),
+                     bias = param(bias_in, x_in, op, "bias"), post_weight = param(post_weight_in, x_in, op, "post_weight"),
+                     post_bias = param(post_bias_in, x_in, op, "post_bias"), gate = param(gate_in, x_in, op, "gate"),
+                     x = x_in.contiguous();
+    const int64_t cols = x.size(-1);
+    for (const at::Tensor& t : {weight, bias, post_weight, post_bias})
+        TORCH_CHECK(!t.defined() || (t.dim() == 1 && t.size(0) == cols), "kunlun residual_norm: weights and biases must be [",
+                    cols, "], got ", t.sizes());
+    if (gate.defined() && !(gate.dim() == 1 && gate.size(0) == cols)) {
+        bool ok = gate.dim() == x.dim() && gate.size(-1) == cols, shared = false;
+        for (int64_t i = 0; ok && i + 1 < x.dim(); ++i) {
+            if (gate.size(i) != x.size(i)) shared = true;
+            ok = shared ? gate.size(i) == 1 : true;
+        }
+        TORCH_CHECK(ok, "kunlun residual_norm: gate must be [", cols, "] or x's shape ", x.sizes(),
+                    " with 1 in place of some last dimensions before the columns, got ", gate.sizes());
+    }
+    const NormOptions o = {rms, post_norm, residual_scale, eps, p, static_cast<int64_t>(seed), static_cast<int64_t>(offset)};
+    if (needs_grad({x, f, weight, bias, post_weight, post_bias, gate})) {
+        const variable_list r = ResidualNorm::apply(x, f, optional(weight), optional(bias), optional(post_weight),
+                                                    optional(post_bias), optional(gate), o);
+        return {r[0], r[1]};
+    }
+    at::AutoDispatchBelowADInplaceOrView guard;
+    return norm_run(x, f, weight, bias, post_weight, post_bias, gate, o, at::Tensor());
+}
+
+}  // namespace torch_kunlun

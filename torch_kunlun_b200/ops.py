@@ -7,6 +7,10 @@
   csrc/ops_nn.cpp:132-147, csrc/ops_extra.cpp:71).
 * ``silu_mul(gate, up)`` -- T(silu(gate)) * up, the gated-MLP product, in one
   elementwise pass.
+* ``dropout``, ``residual_norm`` -- differentiable training operators: dropout
+  whose mask is a function of (seed, offset, element index) and is never
+  stored, and the norms behind and before a transformer block with the block's
+  dropout, gate and residual scale in one pass.
 """
 
 from __future__ import annotations
@@ -83,5 +87,47 @@ def linear_from_limbs(a_limbs: torch.Tensor, b_limbs: torch.Tensor, k: int, amax
     return _C.linear_from_limbs(a_limbs, b_limbs, k, amax_a, amax_b, bias, ACT[act], out, dtype, gate, amax_out)
 
 
-__all__ = ["linear", "silu_mul", "silu_mul_amax", "amax", "linear_scaled", "quantize_limbs",
+def _u64(value: int, name: str) -> int:
+    value = int(value)
+    if not 0 <= value < 1 << 64:
+        raise ValueError(f"{name} must be in [0, 2**64), got {value}")
+    return value
+
+
+def dropout(x: torch.Tensor, p: float, seed: int, offset: int = 0) -> torch.Tensor:
+    """x / (1 - p) where the element is kept, 0 elsewhere (also for inf and
+    NaN).  Element i, in row-major order, is kept when word i % 4 of the
+    Philox4x32-10 block with counter (i // 4, offset) and key seed is at least
+    round(p * 2**32).  The same (seed, offset) gives the same mask on every call
+    and in the backward pass, so give each call of a step an offset of its
+    own.  0 <= p <= 1; float16 and float32."""
+    return _C.dropout(x, float(p), _u64(seed, "seed"), _u64(offset, "offset"))
+
+
+def residual_norm(x: torch.Tensor, f: torch.Tensor, weight: Optional[torch.Tensor] = None,
+                  bias: Optional[torch.Tensor] = None, *, norm: str = "layer", post_norm: bool = False,
+                  post_weight: Optional[torch.Tensor] = None, post_bias: Optional[torch.Tensor] = None,
+                  gate: Optional[torch.Tensor] = None, residual_scale: float = 1.0, eps: float = 1e-5,
+                  p: float = 0.0, seed: int = 0, offset: int = 0):
+    """(x_new, h) for a residual stream x and a block's output f [..., D]:
+
+        u     = Norm(f) * post_weight + post_bias if post_norm else f
+        x_new = residual_scale * x + gate * dropout(u, p, seed, offset)
+        h     = Norm(x_new) * weight + bias
+
+    Norm is "layer" (mean and variance) or "rms" (mean square), with eps under
+    the root.  h is the next block's input; a post-LayerNorm block takes h alone.
+    gate is [D], or x's shape with 1 in place of some last dimensions before D
+    ([B, 1, D] gates each sample).  All tensors share one dtype, float16 or
+    float32; sums are fp32 (of the unrounded x_new for h) and each output is
+    rounded once.  D is at most 32768.  Differentiable in every tensor; the
+    backward pass recomputes the mask and takes x_new as it was rounded."""
+    if norm not in ("layer", "rms"):
+        raise ValueError(f"norm must be 'layer' or 'rms', got {norm!r}")
+    return _C.residual_norm(x, f, weight, bias, norm == "rms", bool(post_norm), post_weight, post_bias, gate,
+                            float(residual_scale), float(eps), float(p), _u64(seed, "seed"),
+                            _u64(offset, "offset"))
+
+
+__all__ = ["linear", "dropout", "residual_norm", "silu_mul", "silu_mul_amax", "amax", "linear_scaled", "quantize_limbs",
            "linear_from_limbs", "ACT"]
