@@ -476,6 +476,57 @@ TK_API size_t tk_residual_norm_backward_workspace_size(const tk_residual_norm_gr
 TK_API int tk_residual_norm_backward(const tk_residual_norm_grad_desc_t* desc, void* workspace,
                                      size_t workspace_bytes, void* stream);
 
+/* ---- training: linear cross entropy ------------------------------------------------
+ * Softmax cross entropy of the logits z = x weight^T + bias without storing
+ * them: loss_i = logsumexp(z_i) - z_i[target_i], for x [rows, cols], weight
+ * [vocab, cols], optional bias [vocab] (one dtype, contiguous) and target
+ * [rows].  A row whose target is ignore_index counts nowhere (loss 0, gradient
+ * 0, whatever its x holds); any other target outside [0, vocab) makes its loss
+ * and the gradients NaN.  reduction: one loss per row, or their mean over the
+ * rows with a target (NaN without any) or sum.  Losses are fp32.  fp16
+ * products are exact and summed in fp32; fp32 operands enter as two binary16
+ * planes each (22 bits, or 2^-40 of the tensor's largest value).  The
+ * counterpart in training of mse_loss (csrc/autograd.cpp). */
+typedef enum { TK_REDUCE_NONE = 0, TK_REDUCE_MEAN = 1, TK_REDUCE_SUM = 2 } tk_reduction_t;
+
+typedef struct {
+    tk_dtype_t dtype;
+    int64_t rows, cols, vocab;
+    const void* x;
+    const void* weight;
+    const void* bias;
+    const int64_t* target;
+    int64_t ignore_index;
+    int reduction;
+    float* loss; /* [rows], or one value */
+    void* state; /* 16-byte aligned, tk_linear_ce_state_size bytes: what the
+                  * backward pass needs; NULL where there is none */
+} tk_linear_ce_desc_t;
+
+TK_API size_t tk_linear_ce_state_size(const tk_linear_ce_desc_t* desc);
+TK_API size_t tk_linear_ce_workspace_size(const tk_linear_ce_desc_t* desc);
+TK_API int tk_linear_ce(const tk_linear_ce_desc_t* desc, void* workspace, size_t workspace_bytes,
+                        void* stream);
+
+/* Its gradients: fwd is the forward call's descriptor with its state (loss is
+ * not read), grad_loss the gradient of the loss ([rows] or one value).  dx
+ * [rows, cols], dweight [vocab, cols] and dbias [vocab] may be NULL.  The
+ * logits are computed again in pieces of the vocabulary; softmax - onehot is
+ * held as binary16 (two planes for fp32) scaled by the largest |grad_loss|.
+ * Deterministic.  The state's scalars are written, so two backward passes of
+ * one state must not run at the same time. */
+typedef struct {
+    tk_linear_ce_desc_t fwd;
+    const float* grad_loss;
+    void* dx;
+    void* dweight;
+    void* dbias;
+} tk_linear_ce_grad_desc_t;
+
+TK_API size_t tk_linear_ce_backward_workspace_size(const tk_linear_ce_grad_desc_t* desc);
+TK_API int tk_linear_ce_backward(const tk_linear_ce_grad_desc_t* desc, void* workspace,
+                                 size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

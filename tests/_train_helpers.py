@@ -122,3 +122,66 @@ def residual_norm64(x, f, weight=None, bias=None, post=False, post_weight=None, 
         e_gu = rq * (spread(e_t) + 2 * (c_q + K * U32) * spread(m_t))
     out["f"] = (gu, ulp(gu, dtype) + e_gu)
     return out
+
+
+def linear_ce64(x, w, target, bias=None, ignore=-100, reduction="mean", grad=None):
+    """{name: (value, bound)} of the linear cross entropy and its gradients in
+    float64 (on the tensors' device), from their rounded values.
+
+    Bounds, from how the kernels compute:
+    * a product sum over k terms in steps of 16 on the tensor cores, each step
+      rounded (or cut) to binary32: (k / 16 + 16) 2^-23 of the terms' absolute
+      sum; binary16 factors are exact, fp32 ones enter as two binary16 planes
+      without the product of the low ones: three times the steps, and 4 * 2^-22
+      of the terms' absolute sum, and 2^-39 of the largest values per term;
+    * base-2 exponentials and logarithms: 2^-21 relative; the sums of
+      exponentials: 32 in a row, then at most V / 2048 + 32 joins;
+    * dz (softmax - onehot, at most 1) rounded to binary16 at 2^14 times its
+      value: half a step or half the smallest subnormal, 2^-39; two planes
+      keep 2^-22.
+    """
+    f16 = x.dtype == torch.float16
+    X, W = x.double(), w.double()
+    V, D = W.shape
+    used = target != ignore
+    X = torch.where(used[:, None], X, torch.zeros((), dtype=X.dtype, device=X.device))
+
+    def product_error(k, mag, amax=0.0):
+        e = (k * (1 if f16 else 3) / 16 + 16) * 2.0 ** -23 * mag
+        return e if f16 else e + 4 * 2.0 ** -22 * mag + k * 2.0 ** -39 * amax
+
+    z, mag = X @ W.T, X.abs() @ W.abs().T
+    if bias is not None:
+        z, mag = z + bias.double(), mag + bias.double().abs()
+    xm, wm = float(X.abs().max()) if X.numel() else 0.0, float(W.abs().max())
+    e_z = product_error(D, mag, xm * wm) + 2.0 ** -22 * z.abs()
+    lse = torch.logsumexp(z, 1)
+    at = torch.where(used, target, 0)[:, None]
+    hit = z.gather(1, at)[:, 0]
+    e_lse = e_z.amax(1) + 2.0 ** -20 + (64 + V / 2048) * 2.0 ** -24 + 2.0 ** -22 * lse.abs()
+    rows = torch.where(used, lse - hit, 0.0)
+    e_rows = torch.where(used, e_lse + (D / 64 + 12) * 2.0 ** -24 * mag.gather(1, at)[:, 0] + 2.0 ** -22 * (lse.abs() + hit.abs()), 0.0)
+    count = int(used.sum())
+    share = {"none": 1.0, "sum": 1.0, "mean": 1.0 / max(count, 1)}[reduction]
+    if reduction == "none":
+        out = {"loss": (rows, e_rows + ulp(rows, torch.float32))}
+    else:
+        total = rows.sum() * share
+        out = {"loss": (total, e_rows.sum() * share + ulp(total, torch.float32))}
+    if grad is None:
+        return out
+    g = torch.where(used, grad.double() * share, 0.0)
+    gmax = float(g.abs().max()) if g.numel() else 0.0
+    p = (z - lse[:, None]).exp()
+    dz = p.clone()
+    dz[torch.arange(len(dz), device=dz.device), at[:, 0]] -= 1.0
+    e_dz = p * (e_z + e_lse[:, None] + 2.0 ** -20) + (2.0 ** -11 if f16 else 2.0 ** -22) * dz.abs() + 2.0 ** -22 * dz.abs()
+    dz, e_dz = dz * g[:, None], e_dz * g.abs()[:, None] + torch.where(used, 2.0 ** -39 * gmax, 0.0)[:, None]
+    for name, a, e, b, k in (("x", dz, e_dz, W, V), ("weight", dz.T, e_dz.T, X, len(X))):
+        v, m = a @ b, a.abs() @ b.abs()
+        out[name] = (v, ulp(v, x.dtype) + e @ b.abs() + product_error(k, m, gmax * float(b.abs().max()) if b.numel() else 0.0)
+                     + 64 * 2.0 ** -24 * m)
+    if bias is not None:
+        s = dz.sum(0)
+        out["bias"] = (s, ulp(s, x.dtype) + e_dz.sum(0) + (len(X) / 8 + 64) * 2.0 ** -24 * dz.abs().sum(0))
+    return out

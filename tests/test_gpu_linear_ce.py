@@ -1,0 +1,313 @@
+"""The linear cross entropy against its 64-bit definition on the same rounded
+inputs (tests/_train_helpers.py derives the bounds), its gradients, masks and
+refusals, and the training operators in one step."""
+import pytest
+import torch
+import torch.nn.functional as F
+
+pytestmark = pytest.mark.gpu
+
+torch_kunlun = pytest.importorskip("torch_kunlun")
+kunlun = torch_kunlun.kunlun
+from tests import _train_helpers as R  # noqa: E402
+from torch_kunlun_b200 import _capi, ops  # noqa: E402
+
+DEV = "kunlun"
+F16, F32 = torch.float16, torch.float32
+
+
+def rnd(shape, seed, dtype=F16, scale=1.0):
+    g = torch.Generator().manual_seed(seed)
+    return (torch.randn(shape, generator=g) * scale).to(dtype)
+
+
+def ce_inputs(n, d, v, dtype, bias, ignored=0, seed=0):
+    g = torch.Generator().manual_seed(seed + 50)
+    t = {"x": rnd((n, d), seed, dtype), "weight": rnd((v, d), seed + 1, dtype, 2.0 / d ** 0.5)}
+    if bias:
+        t["bias"] = rnd((v,), seed + 2, dtype, 0.3)
+    target = torch.randint(0, v, (n,), generator=g)
+    target[torch.randperm(n, generator=g)[:ignored]] = -100
+    return t, target
+
+
+def run_ce(t, target, reduction, grad=None, ignore=-100, wanted=("x", "weight", "bias")):
+    dev = {k: v.to(DEV).requires_grad_(grad is not None and k in wanted) for k, v in t.items()}
+    loss = ops.linear_cross_entropy(dev["x"], dev["weight"], target.to(DEV), dev.get("bias"), ignore, reduction)
+    out = {"loss": loss}
+    if grad is not None:
+        names = [k for k in t if k in wanted]
+        out.update(zip(names, torch.autograd.grad(loss, [dev[k] for k in names], grad.to(DEV))))
+    assert _capi.device_error(0) == 0
+    return {k: v.detach().cpu() for k, v in out.items()}
+
+
+def check_ce(t, target, reduction, grad=None, ignore=-100, wanted=("x", "weight", "bias")):
+    got = run_ce(t, target, reduction, grad, ignore, wanted)
+    cu = {k: v.cuda() for k, v in t.items()}
+    want = R.linear_ce64(cu["x"], cu["weight"], target.cuda(), cu.get("bias"), ignore, reduction,
+                         None if grad is None else grad.cuda())
+    for k, v in got.items():
+        value, bound = want[k]
+        R.assert_within(v, value.cpu(), bound.cpu(), f"{k} {tuple(t['x'].shape)} {tuple(t['weight'].shape)} {t['x'].dtype} {reduction}")
+    return got
+
+
+def loss_grad(n, reduction, seed=0):
+    if reduction == "none":
+        return torch.randn(n, generator=torch.Generator().manual_seed(seed + 7))
+    return torch.tensor(256.0 if reduction == "mean" else 0.75)
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("n,d,v", [(1, 1, 1), (1, 8, 2), (3, 7, 5), (5, 64, 257), (16, 16, 128), (128, 256, 256), (130, 128, 300), (129, 768, 1000),
+                                   (257, 100, 1031), (300, 72, 5000), (64, 1024, 10007), (500, 31, 77), (5000, 96, 40), (1000, 264, 2560)])
+@pytest.mark.parametrize("reduction,bias", [("mean", False), ("none", True)])
+def test_linear_ce(n, d, v, dtype, reduction, bias):
+    t, target = ce_inputs(n, d, v, dtype, bias, seed=n + d + v)
+    check_ce(t, target, reduction, loss_grad(n, reduction))
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("n,ignored", [(1, 1), (40, 39), (300, 0), (300, 172), (300, 300), (2000, 1700)])
+def test_linear_ce_ignored_rows(n, ignored, dtype):
+    for reduction in ("none", "sum"):
+        t, target = ce_inputs(n, 80, 700, dtype, True, ignored, seed=n + ignored)
+        got = check_ce(t, target, reduction, loss_grad(n, reduction))
+        if reduction == "none":
+            assert not got["loss"][target == -100].any()
+        assert not got["x"][target == -100].any()
+
+
+def test_linear_ce_without_any_target():
+    t, _ = ce_inputs(9, 16, 30, F16, True)
+    target = torch.full((9,), -100)
+    got = run_ce(t, target, "mean", torch.tensor(1.0))
+    assert torch.isnan(got["loss"])
+    assert not got["x"].any() and not got["weight"].any() and not got["bias"].any()
+    assert run_ce(t, target, "sum")["loss"] == 0
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+def test_linear_ce_non_finite_ignored_rows_do_not_matter(dtype):
+    t, target = ce_inputs(150, 96, 500, dtype, False, 40, seed=3)
+    clean = run_ce(t, target, "mean", torch.tensor(64.0))
+    off = (target == -100).nonzero()[:, 0]
+    t["x"][off[0]] = float("nan")
+    t["x"][off[1]] = float("inf")
+    t["x"][off[2]] = torch.finfo(dtype).min
+    again = run_ce(t, target, "mean", torch.tensor(64.0))
+    for k in clean:
+        assert torch.equal(clean[k], again[k]), k
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+def test_linear_ce_non_finite_row_stays_in_its_row(dtype):
+    t, target = ce_inputs(140, 64, 300, dtype, False, seed=4)
+    t["x"][17, 3] = float("nan")
+    got = run_ce(t, target, "none", loss_grad(140, "none"))
+    assert torch.isnan(got["loss"][17]) and torch.isnan(got["x"][17]).all()
+    rest = torch.arange(140) != 17
+    assert torch.isfinite(got["loss"][rest]).all() and torch.isfinite(got["x"][rest]).all()
+
+
+def test_linear_ce_target_out_of_range_is_nan():
+    t, target = ce_inputs(20, 32, 100, F16, False, seed=5)
+    target[4], target[11] = 100, -1
+    got = run_ce(t, target, "none", torch.ones(20))
+    bad = torch.zeros(20, dtype=torch.bool)
+    bad[[4, 11]] = True
+    assert torch.isnan(got["loss"][bad]).all() and torch.isfinite(got["loss"][~bad]).all()
+    assert torch.isnan(got["x"][bad]).all() and torch.isfinite(got["x"][~bad]).all()
+
+
+def test_linear_ce_bias_of_minus_infinity_removes_a_word():
+    t, target = ce_inputs(30, 48, 300, F16, True, seed=6)
+    target[target == 299] = 0
+    target[target == 5] = 1
+    t["bias"][5] = t["bias"][299] = float("-inf")
+    got = run_ce(t, target, "none")
+    keep = [i for i in range(300) if i not in (5, 299)]
+    z = t["x"].double() @ t["weight"].double().T + t["bias"].double()
+    want = torch.logsumexp(z[:, keep], 1) - z.gather(1, target[:, None])[:, 0]
+    assert torch.allclose(got["loss"].double(), want, atol=2e-5, rtol=0)  # 2^-20 + (48/16 + 16) 2^-23 of |z| terms below 8
+
+
+def test_linear_ce_large_logits_do_not_overflow():
+    # a bare exponential of these logits overflows binary32
+    t, target = ce_inputs(60, 64, 400, F32, False, seed=8)
+    t["weight"] *= 100
+    check_ce(t, target, "mean", torch.tensor(1.0))
+
+
+@pytest.mark.parametrize("scale_x,scale_w", [(1e-8, 1e4), (1e6, 1e-5), (1e-20, 1e20)])
+def test_linear_ce_fp32_magnitudes(scale_x, scale_w):
+    t, target = ce_inputs(70, 120, 500, F32, False, seed=9)
+    t["x"] *= scale_x
+    t["weight"] *= scale_w
+    check_ce(t, target, "mean", torch.tensor(1.0))
+
+
+def test_linear_ce_other_ignore_index_and_leading_dimensions():
+    t, target = ce_inputs(24, 40, 90, F16, False, seed=10)
+    target[::3] = 0
+    check_ce(t, target, "mean", torch.tensor(32.0), ignore=0)
+    x3 = t["x"].view(2, 3, 4, 40).to(DEV)
+    loss = ops.linear_cross_entropy(x3, t["weight"].to(DEV), target.view(2, 3, 4).to(DEV), reduction="none")
+    assert loss.shape == (2, 3, 4) and loss.dtype == F32
+    flat = run_ce(t, target, "none")["loss"]
+    assert torch.equal(loss.cpu().view(-1), flat)
+
+
+def test_linear_ce_strided_and_misaligned_inputs():
+    t, target = ce_inputs(50, 64, 200, F16, True, seed=11)
+    plain = run_ce(t, target, "none")["loss"]
+    xt = t["x"].t().contiguous().to(DEV).t()
+    w = torch.empty(200 * 64 + 1, dtype=F16, device=DEV)
+    w[1:].copy_(t["weight"].view(-1).to(DEV))
+    b = torch.empty(201, dtype=F16, device=DEV)
+    b[1:].copy_(t["bias"].to(DEV))
+    got = ops.linear_cross_entropy(xt, w[1:].view(200, 64), target.to(DEV), b[1:], reduction="none").cpu()
+    assert torch.equal(got, plain)
+
+
+@pytest.mark.parametrize("dtype,n,d,v", [(F16, 16384, 64, 20003), (F32, 9000, 40, 20003)])
+def test_linear_ce_several_pieces_of_the_vocabulary(dtype, n, d, v):
+    # dz of all columns is larger than one piece
+    t, target = ce_inputs(n, d, v, dtype, True, n // 3, seed=12)
+    check_ce(t, target, "mean", torch.tensor(4096.0))
+
+
+@pytest.mark.parametrize("wanted", [("x",), ("weight",), ("bias",), ("x", "bias")])
+def test_linear_ce_some_gradients(wanted):
+    t, target = ce_inputs(90, 56, 310, F16, True, 8, seed=13)
+    check_ce(t, target, "mean", torch.tensor(128.0), wanted=wanted)
+
+
+def test_linear_ce_extreme_row_gradients():
+    # one row's gradient far above the others', a zero one, and none at all
+    t, target = ce_inputs(64, 72, 200, F16, False, seed=14)
+    g = torch.ones(64)
+    g[3], g[4] = 1000.0, 0.0
+    got = check_ce(t, target, "none", g)
+    assert not got["x"][4].any()
+    zero = run_ce(t, target, "none", torch.zeros(64))
+    assert not zero["x"].any() and not zero["weight"].any()
+
+
+def test_linear_ce_empty_batch():
+    t = {"x": torch.zeros(0, 16, dtype=F16), "weight": rnd((9, 16), 1), "bias": rnd((9,), 2)}
+    target = torch.zeros(0, dtype=torch.int64)
+    assert run_ce(t, target, "none")["loss"].shape == (0,)
+    assert run_ce(t, target, "sum")["loss"] == 0 and torch.isnan(run_ce(t, target, "mean")["loss"])
+    got = run_ce(t, target, "sum", torch.tensor(1.0))
+    assert got["x"].shape == (0, 16) and not got["weight"].any() and not got["bias"].any()
+
+
+def test_linear_ce_gradient_against_differences():
+    t, target = ce_inputs(20, 24, 60, F32, True, 3, seed=15)
+    got = run_ce(t, target, "mean", torch.tensor(1.0))
+    wide = {k: v.double() for k, v in t.items()}
+
+    def value(u):
+        z = u["x"] @ u["weight"].T + u["bias"]
+        return float(F.cross_entropy(z, target))
+
+    for k in t:
+        v = torch.randn(t[k].shape, generator=torch.Generator().manual_seed(5), dtype=torch.float64)
+        step = 1e-5
+        slope = (value({**wide, k: wide[k] + step * v}) - value({**wide, k: wide[k] - step * v})) / (2 * step)
+        # truncation step^2 and cancellation 2^-52 / step are far below 2^-18 of
+        # the gradient's terms, its binary32 error
+        assert abs(float((got[k].double() * v).sum()) - slope) <= 2.0 ** -18 * float((got[k].double() * v).abs().sum()) + 1e-8, k
+
+
+def test_linear_ce_is_deterministic_on_streams_and_with_reused_memory():
+    t, target = ce_inputs(700, 200, 3000, F16, True, 90, seed=16)
+    g = torch.tensor(512.0)
+    first = run_ce(t, target, "mean", g)
+    s = kunlun.Stream()
+    for _ in range(3):
+        with kunlun.stream(s):
+            junk = torch.empty(64 << 20, dtype=F16, device=DEV).fill_(float("nan"))  # what the workspace may hold
+            del junk
+            again = run_ce(t, target, "mean", g)
+        s.synchronize()
+        for k in first:
+            assert torch.equal(first[k], again[k]), k
+
+
+def test_linear_ce_backward_twice():
+    t, target = ce_inputs(100, 64, 300, F16, False, seed=17)
+    x = t["x"].to(DEV).requires_grad_()
+    loss = ops.linear_cross_entropy(x, t["weight"].to(DEV), target.to(DEV))
+    one, = torch.autograd.grad(loss, x, torch.tensor(2.0).to(DEV), retain_graph=True)
+    two, = torch.autograd.grad(loss, x, torch.tensor(4.0).to(DEV))
+    want = R.linear_ce64(t["x"], t["weight"], target, grad=torch.tensor(2.0))["x"]
+    R.assert_within(one.cpu(), *want, "first")
+    R.assert_within(two.cpu(), *R.linear_ce64(t["x"], t["weight"], target, grad=torch.tensor(4.0))["x"], "second")
+
+
+def test_linear_ce_refusals():
+    t, target = ce_inputs(6, 16, 40, F16, True)
+    x, w, b, y = t["x"].to(DEV), t["weight"].to(DEV), t["bias"].to(DEV), target.to(DEV)
+    with pytest.raises(ValueError, match="reduction"):
+        ops.linear_cross_entropy(x, w, y, reduction="max")
+    for bad in (lambda: ops.linear_cross_entropy(x, w[:, :8], y), lambda: ops.linear_cross_entropy(x, w.float(), y),
+                lambda: ops.linear_cross_entropy(x, w, y[:4]), lambda: ops.linear_cross_entropy(x, w, target),
+                lambda: ops.linear_cross_entropy(x, w, y.to(torch.int32)), lambda: ops.linear_cross_entropy(x, w, y, b[:3]),
+                lambda: ops.linear_cross_entropy(t["x"], t["weight"], target),
+                lambda: ops.linear_cross_entropy(x, w, y, b.cpu())):
+        with pytest.raises(RuntimeError, match="linear_cross_entropy"):
+            bad()
+    leaf = x.clone().requires_grad_()
+    with pytest.raises(RuntimeError, match="create_graph"):
+        torch.autograd.grad(ops.linear_cross_entropy(leaf, w, y), leaf, create_graph=True)
+
+
+def test_training_operators_in_one_step():
+    """Two blocks of linear - relu - linear under residual norms with dropout,
+    then the loss: every operator's results and gradients checked against its
+    64-bit form on the values and gradients it met in the step."""
+    n, d, v, hid = 96, 128, 500, 256
+    names = [("w1", (hid, d)), ("w2", (d, hid)), ("g", (d,)), ("b", (d,)), ("pg", (d,)), ("pb", (d,)), ("gate", (d,))]
+    params = [{k: (rnd(s, 10 * i + j, F16, 1 / s[-1] ** 0.5 if len(s) == 2 else 0.1) + (0 if len(s) == 2 or k in ("b", "pb") else 1)).to(F16)
+               for j, (k, s) in enumerate(names)} for i in range(2)]
+    dev = [{k: t.to(DEV).requires_grad_() for k, t in p.items()} for p in params]
+    x0 = rnd((n, d), 77)
+    head, target = rnd((v, d), 78, F16, 0.1), torch.randint(0, v, (n,), generator=torch.Generator().manual_seed(3))
+    target[::7] = -100
+    hd = head.to(DEV).requires_grad_()
+    x = x0.to(DEV).requires_grad_()
+    h, steps = x, []
+    for i, p in enumerate(dev):
+        f = F.linear(torch.relu(F.linear(h, p["w1"])), p["w2"])
+        x_new, h = ops.residual_norm(x, f, p["g"], p["b"], post_norm=True, post_weight=p["pg"], post_bias=p["pb"], gate=p["gate"], p=0.1, seed=42, offset=i)
+        for t in (x, f, x_new, h):
+            t.retain_grad()
+        steps.append((x, f, x_new, h))
+        x = x_new
+    y = ops.dropout(h, 0.2, 42, 9)
+    y.retain_grad()
+    loss = ops.linear_cross_entropy(y, hd, target.to(DEV))
+    loss.backward(torch.tensor(1024.0).to(DEV))
+    cpu = lambda t: None if t is None else t.detach().cpu()  # noqa: E731
+    want = R.linear_ce64(cpu(y), head, target, grad=torch.tensor(1024.0))
+    R.assert_within(cpu(loss), *want["loss"], "loss")
+    R.assert_within(cpu(y.grad), *want["x"], "dy")
+    R.assert_within(cpu(hd.grad), *want["weight"], "dhead")
+    keep = R.keep_mask(h.shape, 0.2, 42, 9)
+    last = torch.where(keep, cpu(y.grad).float() * torch.tensor(1.25), 0.0).to(F16)
+    assert torch.equal(cpu(h.grad), last)
+    for i in (1, 0):
+        xi, fi, xn, hi = steps[i]
+        p = params[i]
+        gx = cpu(xn.grad) if i == 0 else None
+        got = R.residual_norm64(cpu(xi), cpu(fi), p["g"], p["b"], True, p["pg"], p["pb"], p["gate"], False, 1.0, 1e-5,
+                                R.keep_mask(xi.shape, 0.1, 42, i), 0.1, gx, cpu(hi.grad))
+        R.assert_within(cpu(xn), *got["x_new"], f"x_new {i}")
+        R.assert_within(cpu(hi), *got["h"], f"h {i}")
+        R.assert_within(cpu(fi.grad), *got["f"], f"df {i}")
+        for k, name in (("g", "weight"), ("b", "bias"), ("pg", "post_weight"), ("pb", "post_bias"), ("gate", "gate")):
+            R.assert_within(cpu(dev[i][k].grad), *got[name], f"{name} {i}")
+        assert torch.isfinite(cpu(dev[i]["w1"].grad)).all() and cpu(dev[i]["w1"].grad).any()

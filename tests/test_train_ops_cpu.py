@@ -149,3 +149,74 @@ def test_gate_segments_reach_the_column_kernel_once(rows, units, gate_rows):
         assert covered == period
         finished[row] = finished.get(row, 0) + 1
     assert not written and finished == {r: 1 for r in range(gate_rows)}
+
+
+@pytest.mark.parametrize("reduction", ["none", "mean", "sum"])
+def test_linear_ce_reference_matches_torch(reduction):
+    g = torch.Generator().manual_seed(5)
+    x, w, b = (torch.randn(s, generator=g) for s in ((11, 6), (17, 6), (17,)))
+    target = torch.randint(0, 17, (11,), generator=g)
+    target[[2, 7]] = -100
+    up = torch.randn(11, generator=g) if reduction == "none" else torch.tensor(3.0)
+    got = R.linear_ce64(x, w, target, b, reduction=reduction, grad=up)
+    leaves = [t.double().requires_grad_() for t in (x, w, b)]
+    loss = torch.nn.functional.cross_entropy(leaves[0] @ leaves[1].T + leaves[2], target, reduction=reduction)
+    grads = torch.autograd.grad(loss, leaves, up.double())
+    for k, v in zip(("loss", "x", "weight", "bias"), (loss, *grads)):
+        assert torch.allclose(got[k][0], v, rtol=1e-10, atol=1e-10), k
+
+
+def _ce_desc(**kw):
+    d = C.LinearCeDesc()
+    d.dtype, d.rows, d.cols, d.vocab, d.reduction, d.ignore_index, d.loss = 0, 4, 16, 32, 1, -100, 16
+    for k, v in kw.items():
+        setattr(d, k, v)
+    return d
+
+
+@pytest.mark.parametrize("fields,status", [
+    (dict(dtype=3), 1), (dict(reduction=5), 1), (dict(rows=-1), 1), (dict(cols=0), 1), (dict(vocab=0), 1),
+    (dict(vocab=1 << 31), 2), (dict(rows=1 << 40), 2)])
+def test_linear_ce_refuses_bad_arguments_before_the_device(fields, status):
+    L = C.lib()
+    d = _ce_desc(**fields)
+    g = C.LinearCeGradDesc()
+    g.fwd = d
+    assert L.tk_linear_ce_workspace_size(ctypes.byref(d)) == 0 and L.tk_linear_ce_state_size(ctypes.byref(d)) == 0
+    assert L.tk_linear_ce_backward_workspace_size(ctypes.byref(g)) == 0
+    assert L.tk_linear_ce(ctypes.byref(d), None, 0, None) == status
+    assert L.tk_linear_ce_backward(ctypes.byref(g), None, 0, None) == status
+
+
+def test_linear_ce_needs_pointers_and_workspace():
+    L = C.lib()
+    assert L.tk_linear_ce(None, None, 0, None) == 1 and L.tk_linear_ce_backward(None, None, 0, None) == 1
+    d = _ce_desc()
+    assert L.tk_linear_ce(ctypes.byref(d), None, 0, None) == 1  # NULL tensors
+    d.x = d.weight = d.target = 1024  # never dereferenced: the workspace check fails first
+    assert L.tk_linear_ce(ctypes.byref(d), None, 0, None) == 4
+    need = L.tk_linear_ce_workspace_size(ctypes.byref(d))
+    assert L.tk_linear_ce(ctypes.byref(d), 512, need, None) == 4  # not 1024-byte aligned
+    assert L.tk_linear_ce(ctypes.byref(d), 1024, need - 1, None) == 4
+    g = C.LinearCeGradDesc()
+    g.fwd = d
+    assert L.tk_linear_ce_backward(ctypes.byref(g), None, 0, None) == 1  # no state
+    g.fwd.state, g.grad_loss = 1024, 1024
+    assert L.tk_linear_ce_backward(ctypes.byref(g), None, 0, None) == 4
+    g.dbias = 1024
+    assert L.tk_linear_ce_backward(ctypes.byref(g), None, 0, None) == 1 and b"bias" in L.tk_last_error_string()
+
+
+@pytest.mark.parametrize("dtype,rows,vocab", [(0, 1, 1), (0, 8192, 65536), (0, 16384, 30011), (1, 9000, 20003), (0, 200000, 140000), (1, 1 << 20, 300)])
+def test_linear_ce_workspace_is_bounded_by_its_pieces(dtype, rows, vocab):
+    """dz is held one piece at a time: at most 512 MiB, or one 256-column tile."""
+    L = C.lib()
+    g = C.LinearCeGradDesc()
+    g.fwd = _ce_desc(dtype=dtype, rows=rows, vocab=vocab, cols=64, weight=1024)
+    pad = (rows + 255) // 256 * 256
+    planes = 1 + dtype
+    packed = planes * pad * 64 * 2 + (planes * vocab * 64 * 2 if dtype else 0)
+    dz = max(512 << 20, pad * 2 * planes * 256)
+    acc = pad * 64 * 4
+    split = 2 * 148 * 128 * 256 * 4
+    assert L.tk_linear_ce_backward_workspace_size(ctypes.byref(g)) <= packed + dz + acc + split + 4 * pad + 8192

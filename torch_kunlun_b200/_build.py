@@ -26,7 +26,7 @@ CUDA_HOME = os.environ.get("CUDA_HOME", "/usr/local/cuda")
 NVCC = os.path.join(CUDA_HOME, "bin", "nvcc")
 
 KERNEL_SOURCES = ["capi.cu", "quant.cu", "qgemm.cu", "eltwise.cu", "rowops.cu", "conv.cu", "noalloc.cu", "attention.cu", "conv_tc.cu",
-                  "dropout.cu", "residual_norm.cu"]
+                  "dropout.cu", "residual_norm.cu", "cross_entropy.cu"]
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 KERNEL_LIB = os.path.join(PKG, "libtk_kernels.so")
 

@@ -29,6 +29,8 @@ EXPORTED = [
     "tk_reduce_sum", "tk_conv3d_workspace_size", "tk_conv3d_q16", "tk_qgemm_scatter_rows",
     "tk_conv3d_wgrad_workspace_size", "tk_conv3d_wgrad_q16", "tk_silu_mul_amax",
     "tk_dropout", "tk_residual_norm", "tk_residual_norm_backward_workspace_size", "tk_residual_norm_backward",
+    "tk_linear_ce_state_size", "tk_linear_ce_workspace_size", "tk_linear_ce", "tk_linear_ce_backward_workspace_size",
+    "tk_linear_ce_backward",
 ]
 
 
@@ -103,6 +105,19 @@ class ResidualNormGradDesc(ctypes.Structure):
                                                 "dpost_weight", "dpost_bias", "dgate")])
 
 
+class LinearCeDesc(ctypes.Structure):
+    """Mirror of tk_linear_ce_desc_t."""
+    _fields_ = ([("dtype", ctypes.c_int), ("rows", ctypes.c_int64), ("cols", ctypes.c_int64), ("vocab", ctypes.c_int64)] +
+                [(n, ctypes.c_void_p) for n in ("x", "weight", "bias", "target")] +
+                [("ignore_index", ctypes.c_int64), ("reduction", ctypes.c_int), ("loss", ctypes.c_void_p),
+                 ("state", ctypes.c_void_p)])
+
+
+class LinearCeGradDesc(ctypes.Structure):
+    """Mirror of tk_linear_ce_grad_desc_t."""
+    _fields_ = [("fwd", LinearCeDesc)] + [(n, ctypes.c_void_p) for n in ("grad_loss", "dx", "dweight", "dbias")]
+
+
 def lib() -> ctypes.CDLL:
     global _lib
     if _lib is None:
@@ -135,6 +150,12 @@ def lib() -> ctypes.CDLL:
         L.tk_residual_norm_backward_workspace_size.argtypes = [ctypes.POINTER(ResidualNormGradDesc)]
         L.tk_residual_norm_backward_workspace_size.restype = ctypes.c_size_t
         L.tk_residual_norm_backward.argtypes = [ctypes.POINTER(ResidualNormGradDesc), vp, ctypes.c_size_t, vp]
+        for name, desc in (("tk_linear_ce", LinearCeDesc), ("tk_linear_ce_backward", LinearCeGradDesc)):
+            getattr(L, name).argtypes = [ctypes.POINTER(desc), vp, ctypes.c_size_t, vp]
+            getattr(L, name + "_workspace_size").argtypes = [ctypes.POINTER(desc)]
+            getattr(L, name + "_workspace_size").restype = ctypes.c_size_t
+        L.tk_linear_ce_state_size.argtypes = [ctypes.POINTER(LinearCeDesc)]
+        L.tk_linear_ce_state_size.restype = ctypes.c_size_t
         _lib = L
     return _lib
 

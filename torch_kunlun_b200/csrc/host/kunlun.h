@@ -126,5 +126,7 @@ std::tuple<at::Tensor, at::Tensor> residual_norm(
     const std::optional<at::Tensor>& post_weight, const std::optional<at::Tensor>& post_bias,
     const std::optional<at::Tensor>& gate, double residual_scale, double eps, double p, uint64_t seed,
     uint64_t offset);
+at::Tensor linear_cross_entropy(const at::Tensor& x, const at::Tensor& weight, const at::Tensor& target,
+                                const std::optional<at::Tensor>& bias, int64_t ignore_index, int64_t reduction);
 
 }  // namespace torch_kunlun

@@ -115,6 +115,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
           py::arg("post_weight") = py::none(), py::arg("post_bias") = py::none(),
           py::arg("gate") = py::none(), py::arg("residual_scale") = 1.0, py::arg("eps") = 1e-5,
           py::arg("p") = 0.0, py::arg("seed") = 0, py::arg("offset") = 0);
+    m.def("linear_cross_entropy", &linear_cross_entropy, py::arg("x"), py::arg("weight"), py::arg("target"),
+          py::arg("bias") = py::none(), py::arg("ignore_index") = -100, py::arg("reduction") = 1);
     m.def("abi_version", [] { return tk_abi_version(); });
     torch_kunlun::register_peer(m);
 }

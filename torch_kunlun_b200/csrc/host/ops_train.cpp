@@ -1,6 +1,6 @@
 // ops_train.cpp -- the training operators of the kunlun backend that have no
-// aten name: dropout with a recomputed mask and the residual norm, each an
-// autograd function over one or two calls of the C ABI.
+// aten name: dropout with a recomputed mask, the residual norm and the linear
+// cross entropy, each an autograd function over one or two calls of the C ABI.
 //
 // The reference stops at linear, convolution, relu and MSE gradients
 // (csrc/autograd.cpp) and at a forward layer_norm (csrc/ops_nn.cpp:85-130);
@@ -214,7 +214,114 @@ struct ResidualNorm : torch::autograd::Function<ResidualNorm> {
     }
 };
 
+// ---- linear cross entropy ------------------------------------------------------------
+
+tk_linear_ce_desc_t ce_desc(const at::Tensor& x, const at::Tensor& weight, const at::Tensor& target, const at::Tensor& bias,
+                            int64_t ignore_index, int64_t reduction) {
+    tk_linear_ce_desc_t d = {};
+    d.dtype = tk_dtype(x.scalar_type());
+    d.rows = x.size(0);
+    d.cols = x.size(1);
+    d.vocab = weight.size(0);
+    d.x = ptr(x);
+    d.weight = ptr(weight);
+    d.bias = ptr(bias);
+    d.target = target.numel() > 0 ? target.data_ptr<int64_t>() : nullptr;
+    d.ignore_index = ignore_index;
+    d.reduction = static_cast<int>(reduction);
+    return d;
+}
+
+// x [N, D], weight [V, D], target [N]; `state` (when defined) is filled for
+// the backward pass.
+at::Tensor ce_run(tk_linear_ce_desc_t d, const at::Tensor& x, at::Tensor* state) {
+    const int dev = x.device().index();
+    DeviceScope g(dev);
+    const auto f32 = x.options().dtype(at::kFloat);
+    at::Tensor loss = d.reduction == TK_REDUCE_NONE ? at::empty({d.rows}, f32) : at::empty({}, f32);
+    d.loss = d.reduction == TK_REDUCE_NONE && d.rows == 0 ? nullptr : loss.data_ptr<float>();
+    const size_t bytes = tk_linear_ce_workspace_size(&d);
+    TORCH_CHECK(bytes > 0, "kunlun linear_cross_entropy: ", tk_last_error_string());
+    if (state != nullptr) {
+        *state = at::empty({static_cast<int64_t>(tk_linear_ce_state_size(&d))}, x.options().dtype(at::kByte));
+        d.state = state->data_ptr();
+    }
+    at::Tensor ws = workspace(bytes, x.device());
+    check_tk(tk_linear_ce(&d, aligned_base(ws), bytes, current_stream(dev)), "tk_linear_ce");
+    return loss;
+}
+
+struct LinearCrossEntropy : torch::autograd::Function<LinearCrossEntropy> {
+    static at::Tensor forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& weight, const at::Tensor& target,
+                              const Optional& bias_in, int64_t ignore_index, int64_t reduction) {
+        const at::Tensor bias = or_undefined(bias_in);
+        at::Tensor state;
+        at::Tensor loss = ce_run(ce_desc(x, weight, target, bias, ignore_index, reduction), x, &state);
+        ctx->save_for_backward({x, weight, target, bias, state});
+        ctx->saved_data["ints"] = std::vector<int64_t>{ignore_index, reduction, x.requires_grad(), weight.requires_grad(),
+                                                       bias.defined() && bias.requires_grad()};
+        ctx->set_materialize_grads(false);
+        return loss;
+    }
+
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        check_single_backward("linear_cross_entropy");
+        variable_list out(6);
+        if (!grads[0].defined()) return out;
+        const variable_list saved = ctx->get_saved_variables();
+        const at::Tensor &x = saved[0], &weight = saved[1], &target = saved[2], &bias = saved[3], &state = saved[4];
+        const auto ints = ctx->saved_data["ints"].toIntVector();
+        const int dev = x.device().index();
+        DeviceScope g(dev);
+        const at::Tensor grad = grads[0].contiguous();
+        if (ints[2]) out[0] = at::empty(x.sizes(), x.options());
+        if (ints[3]) out[1] = at::empty(weight.sizes(), weight.options());
+        if (ints[4]) out[3] = at::empty(bias.sizes(), bias.options());
+        tk_linear_ce_grad_desc_t d = {};
+        d.fwd = ce_desc(x, weight, target, bias, ints[0], ints[1]);
+        d.fwd.state = state.data_ptr();
+        d.grad_loss = grad.numel() > 0 ? grad.data_ptr<float>() : nullptr;
+        d.dx = ptr(out[0]);
+        d.dweight = ptr(out[1]);
+        d.dbias = ptr(out[3]);
+        const size_t bytes = tk_linear_ce_backward_workspace_size(&d);
+        TORCH_CHECK(bytes > 0, "kunlun linear_cross_entropy: ", tk_last_error_string());
+        at::Tensor ws = workspace(bytes, x.device());
+        check_tk(tk_linear_ce_backward(&d, aligned_base(ws), bytes, current_stream(dev)), "tk_linear_ce_backward");
+        return out;
+    }
+};
+
 }  // namespace
+
+at::Tensor linear_cross_entropy(const at::Tensor& x_in, const at::Tensor& weight_in, const at::Tensor& target_in,
+                                const std::optional<at::Tensor>& bias_in, int64_t ignore_index, int64_t reduction) {
+    const char* op = "linear_cross_entropy";
+    check_input(x_in, op);
+    TORCH_CHECK(x_in.dim() >= 1 && x_in.size(-1) >= 1, "kunlun linear_cross_entropy: x needs a last dimension of at least 1");
+    TORCH_CHECK(weight_in.defined() && weight_in.dim() == 2 && weight_in.size(0) >= 1 && weight_in.size(1) == x_in.size(-1),
+                "kunlun linear_cross_entropy: weight must be [vocab, ", x_in.size(-1), "], got ", weight_in.sizes());
+    TORCH_CHECK(target_in.device() == x_in.device() && target_in.scalar_type() == at::kLong,
+                "kunlun linear_cross_entropy: target must be int64 on ", x_in.device(), ", got ", target_in.scalar_type(),
+                " on ", target_in.device());
+    TORCH_CHECK(target_in.sizes().equals(x_in.sizes().slice(0, x_in.dim() - 1)),
+                "kunlun linear_cross_entropy: target has shape ", target_in.sizes(), ", expected x's leading dimensions of ",
+                x_in.sizes());
+    TORCH_CHECK(reduction >= 0 && reduction <= 2, "kunlun linear_cross_entropy: bad reduction ", reduction);
+    const at::Tensor weight = param(weight_in, x_in, op, "weight"), bias = param(bias_in, x_in, op, "bias");
+    TORCH_CHECK(!bias.defined() || (bias.dim() == 1 && bias.size(0) == weight.size(0)),
+                "kunlun linear_cross_entropy: bias must be [", weight.size(0), "], got ", bias.sizes());
+    const int64_t cols = x_in.size(-1), rows = x_in.numel() / cols;
+    const at::Tensor x = x_in.contiguous().view({rows, cols}), target = target_in.contiguous().view({rows});
+    at::Tensor loss;
+    if (needs_grad({x, weight, bias})) {
+        loss = LinearCrossEntropy::apply(x, weight, target, optional(bias), ignore_index, reduction);
+    } else {
+        at::AutoDispatchBelowADInplaceOrView guard;
+        loss = ce_run(ce_desc(x, weight, target, bias, ignore_index, reduction), x, nullptr);
+    }
+    return reduction == TK_REDUCE_NONE ? loss.view(target_in.sizes()) : loss;
+}
 
 at::Tensor dropout(const at::Tensor& x, double p, uint64_t seed, uint64_t offset) {
     check_input(x, "dropout");

@@ -11,6 +11,8 @@
   whose mask is a function of (seed, offset, element index) and is never
   stored, and the norms behind and before a transformer block with the block's
   dropout, gate and residual scale in one pass.
+* ``linear_cross_entropy`` -- the loss of a vocabulary projection and its
+  gradients without the logits.
 """
 
 from __future__ import annotations
@@ -129,5 +131,25 @@ def residual_norm(x: torch.Tensor, f: torch.Tensor, weight: Optional[torch.Tenso
                             _u64(offset, "offset"))
 
 
-__all__ = ["linear", "dropout", "residual_norm", "silu_mul", "silu_mul_amax", "amax", "linear_scaled", "quantize_limbs",
+REDUCTION = {"none": 0, "mean": 1, "sum": 2}
+
+
+def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Tensor,
+                         bias: Optional[torch.Tensor] = None, ignore_index: int = -100,
+                         reduction: str = "mean") -> torch.Tensor:
+    """cross_entropy(x @ weight^T + bias, target) without the logits, in fp32.
+
+    x [..., D], weight [V, D] and bias [V] share one dtype, float16 or float32;
+    target [...] is int64.  Rows whose target is ignore_index take no part (loss
+    and gradient 0, whatever x holds there) and cost nothing; any other target
+    outside [0, V) makes its loss NaN.  reduction is "mean" (over the rows with a
+    target), "sum" or "none" (target's shape).  Products are those of the tensors' own
+    values summed in fp32, not the int16-quantised ones of ``linear``.
+    Differentiable in x, weight and bias."""
+    if reduction not in REDUCTION:
+        raise ValueError(f"reduction must be one of {sorted(REDUCTION)}, got {reduction!r}")
+    return _C.linear_cross_entropy(x, weight, target, bias, int(ignore_index), REDUCTION[reduction])
+
+
+__all__ = ["linear", "dropout", "residual_norm", "linear_cross_entropy", "silu_mul", "silu_mul_amax", "amax", "linear_scaled", "quantize_limbs",
            "linear_from_limbs", "ACT"]
