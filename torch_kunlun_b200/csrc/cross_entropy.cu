@@ -26,13 +26,22 @@
 // 2^15)), 22 bits or 2^-40 of the largest value, and a product is the sum
 // hi*hi + hi*lo + lo*hi: the K loop runs over three pairs of planes.
 //
-// GEMM kernel (one persistent CTA per SM, 320 threads): warp 0 loads 64-deep
-// stages by TMA (128-byte swizzle), warp 1 issues tcgen05.mma kind::f16 into
-// two 256-column accumulators in TMEM, warps 2..9 run the epilogue of one
-// while the other fills.  Tiles are 128 x 256.
+// GEMM kernel (persistent pairs of CTAs, one CTA per SM, 320 threads each):
+// a pair computes 256 x 256 tiles, CTA r holding rows [128 r, + 128) of A and
+// of B in shared memory and of the result in TMEM, so each SM loads 32 KB per
+// 64 K values of a 256 x 256 tile.  Warp 0 of both CTAs loads its halves by
+// TMA (128-byte swizzle) onto the leader's barriers, warp 1 of the leader
+// issues tcgen05.mma cta_group::2 kind::f16 into two 256-column accumulators,
+// warps 2..9 of both CTAs run the epilogue of one while the other fills.
+//
+// The tensor core adds each 16-deep step into a binary32 accumulator that it
+// cuts rather than rounds, a bias that grows with K.  Where outputs are
+// binary32 (fp32 gradients, the loss) the K loop is cut into chunks that the
+// epilogue adds in registers.
 #include <cuda_fp16.h>
 
 #include <algorithm>
+#include <atomic>
 
 #include "tk_internal.h"
 #include "tk_ptx.cuh"
@@ -40,13 +49,19 @@
 namespace tk {
 namespace {
 
-constexpr int BM = 128, BN = 256, BK = 64;
-constexpr int STAGES = 4;
-constexpr int A_BYTES = BM * BK * 2, B_BYTES = BN * BK * 2;
+constexpr int BM = 256, BN = 256, BK = 64;     // a pair's tile
+constexpr int HM = BM / 2, HN = BN / 2;          // one CTA's operand rows
+constexpr int STAGES = 5;
+constexpr int A_BYTES = HM * BK * 2, B_BYTES = HN * BK * 2;
 constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
 constexpr int EPI_WARPS = 8;
 constexpr int THREADS = 64 + 32 * EPI_WARPS;
-constexpr int GEMM_SMEM = STAGES * STAGE_BYTES + 1024 + 256;
+// An epilogue warp turns 32 rows x 32 columns through its own 4.5 KB, so that
+// eight lanes store 128 consecutive bytes of a row (144-byte pitch: no bank
+// conflicts for 16-byte accesses).
+constexpr int PITCH = 36;
+constexpr int TURN_BYTES = EPI_WARPS * 32 * PITCH * 4;
+constexpr int GEMM_SMEM = STAGES * STAGE_BYTES + TURN_BYTES + 1024 + 256;
 constexpr int TMEM_COLS = 512;
 static_assert(GEMM_SMEM <= 232448, "shared memory budget");
 
@@ -59,7 +74,7 @@ struct Scalars {
     int count;           // rows with a target
     unsigned amax_x;     // binary32 bits of the largest finite |x|, |W| (fp32 operands)
     unsigned amax_w;
-    float z_log2;        // accumulator -> base-2 logit
+    unsigned rows_done;  // blocks of ce_rows_kernel that finished
     float gmax;          // max |g_i|
     float dx_scale, dw_scale, db_scale;  // accumulators -> gradients
 };
@@ -72,12 +87,13 @@ struct GemmParams {
     int m_tiles;   // < 0: from sc->count
     int k_blocks;  // per pair of planes; < 0: from sc->count
     int pairs;     // 1 (fp16 operands) or 3 (two planes each)
+    int chunk;     // K blocks per accumulator chunk
     int max_units; // tiles x K splits the workspace of a split reduction holds
+    int64_t vocab0, vocab;  // the piece's first column, all columns
     int group;     // M tiles that neighbouring CTAs share
     unsigned* err;
     // kStats / kDlogits
     const float* bias2;  // bias * log2(e), or NULL
-    int64_t vocab0, vocab;  // the piece's first column, all columns
     float2* part;           // [2 * n_tiles][rows_pad] maximum and sum
     int64_t rows_pad;
     const float* lse2;
@@ -90,7 +106,8 @@ struct GemmParams {
     const int* index;    // kGradX: output row of a packed row
     int64_t out_rows, out_cols;
     int out_f32, out_vec;
-    float* acc;          // [rows_pad][out_cols] sums over earlier pieces
+    float* acc;          // [rows_pad][acc_ld] sums over earlier pieces
+    int64_t acc_ld;
     int first, last;     // piece (kGradX)
     float* split;        // [max_units][BM][BN] partial tiles
 };
@@ -116,7 +133,12 @@ __device__ __forceinline__ Shape shape_of(const GemmParams& p) {
     return s;
 }
 
-// Work unit -> (K chunk, M tile, N tile); the chunk varies slowest, tiles run
+// First K block of a split.
+__device__ __forceinline__ int split_begin(const Shape& s, int ks) {
+    return static_cast<int>(static_cast<int64_t>(ks) * s.blocks / s.splits);
+}
+
+// Work unit -> (K split, M tile, N tile); the split varies slowest, tiles run
 // in groups of p.group M tiles so neighbours share operands in L2.
 __device__ __forceinline__ void decode_unit(const GemmParams& p, const Shape& s, int u, int& mt, int& nt, int& ks) {
     const int tiles = s.m_tiles * p.n_tiles;
@@ -131,12 +153,46 @@ __device__ __forceinline__ void decode_unit(const GemmParams& p, const Shape& s,
     nt = r / size;
 }
 
-__device__ __forceinline__ void tc_mma_f16(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+// D[tmem of both CTAs] (+)= A B^T over the pair's shared memory.
+__device__ __forceinline__ void tc_mma_f16_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
     asm volatile(
         "{\n\t.reg .pred p;\n\t"
         "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
         "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+
+// Arrive on the mbarrier at this offset in both CTAs of the pair once all
+// prior tcgen05 operations of this thread have completed.
+__device__ __forceinline__ void tc_commit_pair(uint32_t bar) {
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
+        "h"(static_cast<uint16_t>(3))
+        : "memory");
+}
+
+// The same on this CTA's mbarrier alone (one kernel uses one .cta_group).
+__device__ __forceinline__ void tc_commit_pair_local(uint32_t bar) {
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+
+__device__ __forceinline__ void tmem_alloc_pair(uint32_t dst_smem, uint32_t ncols) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(dst_smem), "r"(ncols) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+}
+
+__device__ __forceinline__ void tmem_dealloc_pair(uint32_t taddr, uint32_t ncols) {
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(ncols) : "memory");
+}
+
+// One box into this CTA's shared memory, completing on a barrier of the pair
+// (a shared::cluster address); c0, innermost, is a multiple of 8 elements.
+__device__ __forceinline__ void tma_load_3d_pair(uint32_t dst, const void* tmap, uint32_t cluster_bar, int c0, int c1, int c2) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(tmap)), "r"(cluster_bar), "r"(c0), "r"(c1), "r"(c2)
         : "memory");
 }
 
@@ -172,25 +228,32 @@ __device__ __forceinline__ uint32_t half2_bits(float a, float b) {
     return *reinterpret_cast<const uint32_t*>(&h);
 }
 
+// The power of two that takes the largest value into [2^14, 2^15).
+__device__ __forceinline__ float plane_scale(unsigned amax_bits) {
+    if (amax_bits == 0) return 1.0f;
+    const int e = max(static_cast<int>(amax_bits >> 23), 1) - 127;
+    return exp2f(static_cast<float>(max(-126, min(126, 14 - e))));
+}
+
 // 32 consecutive columns of one row: base-2 logits from the accumulators.
-__device__ __forceinline__ void logits2(const uint32_t (&acc)[32], float k, const float* bias2, int64_t col, int64_t vocab, float (&y)[32]) {
+__device__ __forceinline__ void logits2(const float* acc, float k, const float* bias2, int64_t col, int64_t vocab, float (&y)[32]) {
     if (bias2 != nullptr) {
         if (col + 32 <= vocab) {
 #pragma unroll
             for (int i = 0; i < 32; i += 4) {
                 const float4 b = __ldg(reinterpret_cast<const float4*>(bias2 + col + i));
-                y[i] = fmaf(__uint_as_float(acc[i]), k, b.x);
-                y[i + 1] = fmaf(__uint_as_float(acc[i + 1]), k, b.y);
-                y[i + 2] = fmaf(__uint_as_float(acc[i + 2]), k, b.z);
-                y[i + 3] = fmaf(__uint_as_float(acc[i + 3]), k, b.w);
+                y[i] = fmaf(acc[i], k, b.x);
+                y[i + 1] = fmaf(acc[i + 1], k, b.y);
+                y[i + 2] = fmaf(acc[i + 2], k, b.z);
+                y[i + 3] = fmaf(acc[i + 3], k, b.w);
             }
         } else {
 #pragma unroll
-            for (int i = 0; i < 32; ++i) y[i] = col + i < vocab ? fmaf(__uint_as_float(acc[i]), k, __ldg(bias2 + col + i)) : -INFINITY;
+            for (int i = 0; i < 32; ++i) y[i] = col + i < vocab ? fmaf(acc[i], k, __ldg(bias2 + col + i)) : -INFINITY;
         }
     } else {
 #pragma unroll
-        for (int i = 0; i < 32; ++i) y[i] = __uint_as_float(acc[i]) * k;
+        for (int i = 0; i < 32; ++i) y[i] = acc[i] * k;
         if (col + 32 > vocab) {
 #pragma unroll
             for (int i = 0; i < 32; ++i)
@@ -207,74 +270,90 @@ __device__ __forceinline__ void join(float& m, float& s, float m2, float s2) {
     m = top;
 }
 
-__device__ __forceinline__ void store_out(const GemmParams& p, int64_t row, int64_t col, const float (&v)[32]) {
-    if (p.out_f32) {
-        float* o = static_cast<float*>(p.out) + row * p.out_cols + col;
-        if (p.out_vec) {
+// The 32 x 32 block that the warp's lanes hold by rows (v: this lane's row),
+// handed out by columns: f(row, column, four values), eight lanes per row.
+template <typename F>
+__device__ __forceinline__ void turn(float* buf, int lane, const float* v, F f) {
+    __syncwarp();
 #pragma unroll
-            for (int i = 0; i < 32; i += 4)
-                if (col + i < p.out_cols) *reinterpret_cast<float4*>(o + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+    for (int i = 0; i < 32; i += 4) *reinterpret_cast<float4*>(buf + lane * PITCH + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+    __syncwarp();
+#pragma unroll
+    for (int r = 0; r < 32; r += 4) {
+        const int row = r + lane / 8, col = lane % 8 * 4;
+        f(row, col, *reinterpret_cast<const float4*>(buf + row * PITCH + col));
+    }
+}
+
+// Four finished values of a gradient: joined with the earlier pieces' sum,
+// kept for the next piece, or scaled, rounded and stored.
+template <int EPI>
+__device__ __forceinline__ void finish4(const GemmParams& p, int64_t m, int64_t rows, int64_t col, float scale, float4 f) {
+    if (m >= rows || col >= p.out_cols) return;
+    float v[4] = {f.x, f.y, f.z, f.w};
+    const bool four = col + 4 <= p.out_cols;
+    if (EPI == kGradX && !(p.first && p.last)) {
+        // rows of the sum are a multiple of four columns apart
+        float4* a = reinterpret_cast<float4*>(p.acc + m * p.acc_ld + col);
+        if (!p.first) {
+            const float4 e = *a;
+            v[0] += e.x, v[1] += e.y, v[2] += e.z, v[3] += e.w;
+        }
+        if (!p.last) {
+            *a = make_float4(v[0], v[1], v[2], v[3]);
+            return;
+        }
+    }
+    const int64_t at = (EPI == kGradX ? p.index[m] : m) * p.out_cols + col;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] *= scale;
+    if (p.out_f32) {
+        float* o = static_cast<float*>(p.out) + at;
+        if (p.out_vec && four) {
+            *reinterpret_cast<float4*>(o) = make_float4(v[0], v[1], v[2], v[3]);
         } else {
 #pragma unroll
-            for (int i = 0; i < 32; ++i)
+            for (int i = 0; i < 4; ++i)
                 if (col + i < p.out_cols) o[i] = v[i];
         }
     } else {
-        __half* o = static_cast<__half*>(p.out) + row * p.out_cols + col;
-        if (p.out_vec) {
-#pragma unroll
-            for (int i = 0; i < 32; i += 8)
-                if (col + i < p.out_cols)
-                    *reinterpret_cast<uint4*>(o + i) = make_uint4(half2_bits(v[i], v[i + 1]), half2_bits(v[i + 2], v[i + 3]),
-                                                                  half2_bits(v[i + 4], v[i + 5]), half2_bits(v[i + 6], v[i + 7]));
+        __half* o = static_cast<__half*>(p.out) + at;
+        if (p.out_vec && four) {
+            *reinterpret_cast<uint2*>(o) = make_uint2(half2_bits(v[0], v[1]), half2_bits(v[2], v[3]));
         } else {
 #pragma unroll
-            for (int i = 0; i < 32; ++i)
+            for (int i = 0; i < 4; ++i)
                 if (col + i < p.out_cols) o[i] = __float2half_rn(v[i]);
         }
     }
 }
 
-// A finished chunk of 32 columns of a gradient tile: joined with the earlier
-// pieces' sum, kept for the next piece or rounded and stored.
-template <int EPI>
-__device__ __forceinline__ void finish_grad(const GemmParams& p, int64_t m, int64_t rows, int64_t col, float scale, float (&v)[32]) {
-    if (m >= rows || col >= p.out_cols) return;
-    if (EPI == kGradX && !(p.first && p.last)) {
-        float* a = p.acc + m * p.out_cols + col;
-        if (!p.first) {
-#pragma unroll
-            for (int i = 0; i < 32; ++i)
-                if (col + i < p.out_cols) v[i] += a[i];
-        }
-        if (!p.last) {
-#pragma unroll
-            for (int i = 0; i < 32; ++i)
-                if (col + i < p.out_cols) a[i] = v[i];
-            return;
-        }
-    }
-#pragma unroll
-    for (int i = 0; i < 32; ++i) v[i] *= scale;
-    store_out(p, EPI == kGradX ? p.index[m] : m, col, v);
+// The scale that takes an accumulator to a base-2 logit.
+__device__ __forceinline__ float z_scale(const GemmParams& p) {
+    return p.pairs == 1 ? kLog2e : kLog2e / plane_scale(p.sc->amax_x) / plane_scale(p.sc->amax_w);
 }
 
-template <int EPI>
+// CHUNKED: the epilogue adds chunks of the K loop in registers (128 columns
+// of a row per thread).
+template <int EPI, bool CHUNKED>
 __global__ void __launch_bounds__(THREADS, 1)
 ce_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const GemmParams p) {
     constexpr bool A_MN = EPI == kGradW, B_MN = EPI == kGradX || EPI == kGradW;
     constexpr uint32_t IDESC = idesc_f16(BM, BN, A_MN, B_MN);
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
-    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + STAGES * STAGE_BYTES);
-    uint64_t* full_bar = bars;               // [STAGES] TMA -> MMA
-    uint64_t* empty_bar = bars + STAGES;     // [STAGES] MMA -> TMA
-    uint64_t* acc_full = bars + 2 * STAGES;  // [2] MMA -> epilogue
-    uint64_t* acc_empty = acc_full + 2;      // [2] epilogue -> MMA
-    uint64_t* drain_bar = acc_empty + 2;     // MMA teardown
+    float* turn_buf = reinterpret_cast<float*>(smem + STAGES * STAGE_BYTES);
+    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + STAGES * STAGE_BYTES + TURN_BYTES);
+    uint64_t* full_bar = bars;               // [STAGES] both CTAs' TMA -> MMA (leader's)
+    uint64_t* empty_bar = bars + STAGES;     // [STAGES] MMA -> TMA (each CTA's)
+    uint64_t* acc_full = bars + 2 * STAGES;  // [2] MMA -> epilogue (each CTA's)
+    uint64_t* acc_empty = acc_full + 2;      // [2] both CTAs' epilogue -> MMA (leader's)
+    uint64_t* drain_bar = acc_empty + 2;     // MMA teardown (leader's)
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain_bar + 1);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = cluster_ctarank();
+    const bool leader = rank == 0;
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < STAGES; ++s) {
@@ -283,7 +362,7 @@ ce_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(smem_u32(acc_full + i), 1);
-            mbar_init(smem_u32(acc_empty + i), EPI_WARPS);
+            mbar_init(smem_u32(acc_empty + i), 2 * EPI_WARPS);
         }
         mbar_init(smem_u32(drain_bar), 1);
         *abort_flag = 0;
@@ -291,19 +370,18 @@ ce_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
         tma_prefetch_desc(&tmA);
         tma_prefetch_desc(&tmB);
     }
-    if (warp == 1) {
-        tmem_alloc(smem_u32(tmem_slot), TMEM_COLS);
-        tmem_relinquish();
-    }
+    if (warp == 1) tmem_alloc_pair(smem_u32(tmem_slot), TMEM_COLS);
     tc_fence_before();
     __syncthreads();
+    cluster_sync_all();  // the pair's barriers are set before either CTA signals them
     tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
     pdl_wait();
     const Shape sh = shape_of<EPI>(p);
+    const int first_unit = blockIdx.x >> 1, unit_step = gridDim.x >> 1;
 
     if (warp == 0) {
-        // ---------------- TMA producer ----------------
+        // ---------------- TMA producer (both CTAs) ----------------
         int stage = 0;
         uint32_t phase = 0;
         uint32_t last_phase[STAGES];
@@ -314,11 +392,12 @@ ce_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
         }
         const int per_pair = sh.blocks / p.pairs;
         bool ok = true;
-        for (int u = blockIdx.x; u < sh.units && ok; u += gridDim.x) {
+        for (int u = first_unit; u < sh.units && ok; u += unit_step) {
             int mt, nt, ks;
             decode_unit(p, sh, u, mt, nt, ks);
-            const int kb1 = static_cast<int>(static_cast<int64_t>(ks + 1) * sh.blocks / sh.splits);
-            for (int kb = static_cast<int>(static_cast<int64_t>(ks) * sh.blocks / sh.splits); kb < kb1; ++kb) {
+            const int kb1 = split_begin(sh, ks + 1);
+            const int a0 = mt * BM + static_cast<int>(rank) * HM, b0 = nt * BN + static_cast<int>(rank) * HN;
+            for (int kb = split_begin(sh, ks); kb < kb1; ++kb) {
                 if (!mbar_wait_bounded(smem_u32(empty_bar + stage), phase ^ 1u, abort_flag, p.err, kDevErrWaitEmpty)) {
                     ok = false;
                     break;
@@ -327,20 +406,20 @@ ce_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
                     const int pair = kb / per_pair;
                     const int kx = (kb - pair * per_pair) * BK;
                     const int pa = pair == 2 ? 1 : 0, pb = pair == 1 ? 1 : 0;
-                    const uint32_t fb = smem_u32(full_bar + stage);
+                    if (leader) mbar_arrive_expect_tx(smem_u32(full_bar + stage), 2 * STAGE_BYTES);
+                    const uint32_t fb = mapa_shared(smem_u32(full_bar + stage), 0);
                     const uint32_t sa = smem_u32(smem + stage * STAGE_BYTES);
-                    mbar_arrive_expect_tx(fb, STAGE_BYTES);
                     if constexpr (A_MN) {
 #pragma unroll
-                        for (int i = 0; i < BM / 64; ++i) tma_load_3d(sa + i * BK * 128, &tmA, fb, mt * BM + i * 64, kx, pa);
+                        for (int i = 0; i < HM / 64; ++i) tma_load_3d_pair(sa + i * BK * 128, &tmA, fb, a0 + i * 64, kx, pa);
                     } else {
-                        tma_load_3d(sa, &tmA, fb, kx, mt * BM, pa);
+                        tma_load_3d_pair(sa, &tmA, fb, kx, a0, pa);
                     }
                     if constexpr (B_MN) {
 #pragma unroll
-                        for (int i = 0; i < BN / 64; ++i) tma_load_3d(sa + A_BYTES + i * BK * 128, &tmB, fb, nt * BN + i * 64, kx, pb);
+                        for (int i = 0; i < HN / 64; ++i) tma_load_3d_pair(sa + A_BYTES + i * BK * 128, &tmB, fb, b0 + i * 64, kx, pb);
                     } else {
-                        tma_load_3d(sa + A_BYTES, &tmB, fb, kx, nt * BN, pb);
+                        tma_load_3d_pair(sa + A_BYTES, &tmB, fb, kx, b0, pb);
                     }
                 }
                 __syncwarp();
@@ -352,90 +431,104 @@ ce_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
                 }
             }
         }
-        // Drain: every box this warp issued has landed before the CTA exits.
-        for (int s = 0; s < STAGES; ++s) {
-            if (used[s]) {
-                volatile int no_abort = 0;
-                mbar_wait_bounded(smem_u32(full_bar + s), last_phase[s], &no_abort, p.err, kDevErrWaitDrain);
+        // Drain: every box of the pair has landed before either CTA exits (the
+        // leader's barriers count both; the peer waits at the cluster barrier).
+        if (leader) {
+            for (int s = 0; s < STAGES; ++s) {
+                if (used[s]) {
+                    volatile int no_abort = 0;
+                    mbar_wait_bounded(smem_u32(full_bar + s), last_phase[s], &no_abort, p.err, kDevErrWaitDrain);
+                }
             }
         }
     } else if (warp == 1) {
-        // ---------------- MMA issuer ----------------
-        int stage = 0;
-        uint32_t phase = 0;
-        bool ok = true;
-        int local = 0;
-        for (int u = blockIdx.x; u < sh.units && ok; u += gridDim.x, ++local) {
-            const int buf = local & 1;
-            if (!mbar_wait_bounded(smem_u32(acc_empty + buf), ((local >> 1) & 1) ^ 1u, abort_flag, p.err, kDevErrWaitAccEmpty)) break;
-            tc_fence_after();
-            const uint32_t acc = tmem_base + buf * BN;
-            int mt, nt, ks;
-            decode_unit(p, sh, u, mt, nt, ks);
-            const int kb0 = static_cast<int>(static_cast<int64_t>(ks) * sh.blocks / sh.splits);
-            const int kb1 = static_cast<int>(static_cast<int64_t>(ks + 1) * sh.blocks / sh.splits);
-            for (int kb = kb0; kb < kb1; ++kb) {
-                if (!mbar_wait_bounded(smem_u32(full_bar + stage), phase, abort_flag, p.err, kDevErrWaitFull)) {
-                    ok = false;
-                    break;
-                }
-                tc_fence_after();
-                if (lane == 0) {
-                    const uint32_t sa = smem_u32(smem + stage * STAGE_BYTES);
-                    const uint64_t da = A_MN ? smem_desc_mnmajor_sw128(sa) : smem_desc_kmajor_sw128(sa);
-                    const uint64_t db = B_MN ? smem_desc_mnmajor_sw128(sa + A_BYTES) : smem_desc_kmajor_sw128(sa + A_BYTES);
-                    // 16 K values on: 32 bytes inside the swizzled row of a
-                    // K-major tile, two 1 KB atoms of an MN-major one
-                    constexpr uint64_t step_a = (A_MN ? 2048 : 32) >> 4, step_b = (B_MN ? 2048 : 32) >> 4;
+        // ---------------- MMA issuer (leader) ----------------
+        if (leader) {
+            int stage = 0;
+            uint32_t phase = 0;
+            bool ok = true;
+            int local = 0;  // accumulator chunks so far
+            for (int u = first_unit; u < sh.units && ok; u += unit_step) {
+                int mt, nt, ks;
+                decode_unit(p, sh, u, mt, nt, ks);
+                int kb = split_begin(sh, ks);
+                const int kb1 = split_begin(sh, ks + 1);
+                do {
+                    const int c0 = kb, c1 = CHUNKED ? min(kb1, kb + p.chunk) : kb1;
+                    const int buf = local & 1;
+                    if (!mbar_wait_bounded_cluster(smem_u32(acc_empty + buf), ((local >> 1) & 1) ^ 1u, abort_flag, p.err, kDevErrWaitAccEmpty)) {
+                        ok = false;
+                        break;
+                    }
+                    tc_fence_after();
+                    const uint32_t acc = tmem_base + buf * BN;
+                    for (; kb < c1; ++kb) {
+                        if (!mbar_wait_bounded(smem_u32(full_bar + stage), phase, abort_flag, p.err, kDevErrWaitFull)) {
+                            ok = false;
+                            break;
+                        }
+                        tc_fence_after();
+                        if (lane == 0) {
+                            const uint32_t sa = smem_u32(smem + stage * STAGE_BYTES);
+                            const uint64_t da = A_MN ? smem_desc_mnmajor_sw128(sa) : smem_desc_kmajor_sw128(sa);
+                            const uint64_t db = B_MN ? smem_desc_mnmajor_sw128(sa + A_BYTES) : smem_desc_kmajor_sw128(sa + A_BYTES);
+                            // 16 K values on: 32 bytes inside the swizzled row of a
+                            // K-major tile, two 1 KB atoms of an MN-major one
+                            constexpr uint64_t step_a = (A_MN ? 2048 : 32) >> 4, step_b = (B_MN ? 2048 : 32) >> 4;
 #pragma unroll
-                    for (int kk = 0; kk < BK / 16; ++kk)
-                        tc_mma_f16(acc, da + kk * step_a, db + kk * step_b, IDESC, kb > kb0 || kk > 0 ? 1u : 0u);
-                    tc_commit(smem_u32(empty_bar + stage));
-                }
-                __syncwarp();
-                if (++stage == STAGES) {
-                    stage = 0;
-                    phase ^= 1u;
-                }
+                            for (int kk = 0; kk < BK / 16; ++kk)
+                                tc_mma_f16_pair(acc, da + kk * step_a, db + kk * step_b, IDESC, kb > c0 || kk > 0 ? 1u : 0u);
+                            tc_commit_pair(smem_u32(empty_bar + stage));
+                        }
+                        __syncwarp();
+                        if (++stage == STAGES) {
+                            stage = 0;
+                            phase ^= 1u;
+                        }
+                    }
+                    if (!ok) break;
+                    if (lane == 0) tc_commit_pair(smem_u32(acc_full + buf));
+                    __syncwarp();
+                    ++local;
+                } while (kb < kb1);
             }
-            if (!ok) break;
-            if (lane == 0) tc_commit(smem_u32(acc_full + buf));
+            // Drain: all MMAs of this thread complete before TMEM is freed.
+            if (lane == 0) tc_commit_pair_local(smem_u32(drain_bar));
             __syncwarp();
+            volatile int no_abort = 0;
+            mbar_wait_bounded(smem_u32(drain_bar), 0, &no_abort, p.err, kDevErrWaitDrain);
         }
-        // Drain: all MMAs of this thread complete before TMEM is freed.
-        if (lane == 0) tc_commit(smem_u32(drain_bar));
-        __syncwarp();
-        volatile int no_abort = 0;
-        mbar_wait_bounded(smem_u32(drain_bar), 0, &no_abort, p.err, kDevErrWaitDrain);
     } else {
-        // ---------------- epilogue (warps 2..9) ----------------
+        // ---------------- epilogue (warps 2..9 of both CTAs) ----------------
         // A warp reads TMEM lanes [32 * (warp % 4), + 32), one row per lane,
         // and half of the tile's columns.
         const int quarter = warp & 3, half = (warp - 2) >> 2;
+        float* const buf_turn = turn_buf + (warp - 2) * 32 * PITCH;
         const int rows = p.sc->count;
         float scale = 1.0f;
-        if constexpr (EPI == kStats || EPI == kDlogits) scale = p.sc->z_log2;
+        if constexpr (EPI == kStats || EPI == kDlogits) scale = z_scale(p);
         if constexpr (EPI == kGradX) scale = p.sc->dx_scale;
         if constexpr (EPI == kGradW) scale = p.sc->dw_scale;
         int local = 0;
-        for (int u = blockIdx.x; u < sh.units; u += gridDim.x, ++local) {
+        bool ok = true;
+        for (int u = first_unit; u < sh.units && ok; u += unit_step) {
             int mt, nt, ks;
             decode_unit(p, sh, u, mt, nt, ks);
-            const int buf = local & 1;
-            if (!mbar_wait_bounded(smem_u32(acc_full + buf), (local >> 1) & 1, abort_flag, p.err, kDevErrWaitAccFull)) break;
-            tc_fence_after();
-            const uint32_t t0 = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + buf * BN + half * (BN / 2);
-            const int64_t m = static_cast<int64_t>(mt) * BM + quarter * 32 + lane;
+            const int blocks = split_begin(sh, ks + 1) - split_begin(sh, ks);
+            const int64_t m0 = static_cast<int64_t>(mt) * BM + rank * HM + quarter * 32;  // the warp's first row
+            const int64_t m = m0 + lane;
             const int64_t col0 = static_cast<int64_t>(nt) * BN + half * (BN / 2);
-            if constexpr (EPI == kStats) {
-                float top = -INFINITY, sum = 0.0f;
-#pragma unroll 1
-                for (int c = 0; c < BN / 2; c += 32) {
-                    uint32_t acc[32];
+            float top = -INFINITY, sum = 0.0f;  // kStats
+            const bool live = m < rows;         // kDlogits
+            const float lse = EPI == kDlogits && live ? p.lse2[m] : 0.0f;
+            const float g = EPI == kDlogits && live ? p.grow[m] * kDzScale : 0.0f;
+            const int64_t hit = EPI == kDlogits && live ? p.target[m] - p.vocab0 : -1;
+            // 32 columns of this lane's row, from column col0 + c of the tile
+            auto take = [&](int c, const float* acc) {
+                const int64_t col = col0 + c;
+                if constexpr (EPI == kStats) {
                     float y[32];
-                    tmem_ld_32x32b_x32(t0 + c, acc);
-                    tc_wait_ld();
-                    logits2(acc, scale, p.bias2, col0 + c, p.vocab, y);
+                    logits2(acc, scale, p.bias2, col, p.vocab, y);
                     float cm = y[0];
 #pragma unroll
                     for (int i = 1; i < 32; ++i) cm = fmaxf(cm, y[i]);
@@ -444,23 +537,8 @@ ce_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
 #pragma unroll
                     for (int i = 0; i < 32; ++i) cs += exp2_sfu(y[i] - ref);
                     join(top, sum, cm, cs);
-                }
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(smem_u32(acc_empty + buf));
-                p.part[(static_cast<int64_t>(nt) * 2 + half) * p.rows_pad + m] = make_float2(top, sum);
-            } else if constexpr (EPI == kDlogits) {
-                const bool live = m < rows;
-                const float lse = live ? p.lse2[m] : 0.0f;
-                const float g = live ? p.grow[m] * kDzScale : 0.0f;
-                const int64_t hit = live ? p.target[m] - p.vocab0 : -1;
-#pragma unroll 1
-                for (int c = 0; c < BN / 2; c += 32) {
-                    uint32_t acc[32];
+                } else if constexpr (EPI == kDlogits) {
                     float y[32];
-                    tmem_ld_32x32b_x32(t0 + c, acc);
-                    tc_wait_ld();
-                    const int64_t col = col0 + c;
                     logits2(acc, scale, p.bias2, p.vocab0 + col, p.vocab, y);
 #pragma unroll
                     for (int i = 0; i < 32; ++i) y[i] = live ? exp2_sfu(y[i] - lse) * g : 0.0f;
@@ -469,89 +547,104 @@ ce_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
 #pragma unroll
                         for (int i = 0; i < 32; ++i) y[i] -= i == j ? g : 0.0f;
                     }
-                    __half* o = p.dz + m * p.dz_ld + col;
-#pragma unroll
-                    for (int i = 0; i < 32; i += 8) {
-                        const uint4 hi = make_uint4(half2_bits(y[i], y[i + 1]), half2_bits(y[i + 2], y[i + 3]),
-                                                    half2_bits(y[i + 4], y[i + 5]), half2_bits(y[i + 6], y[i + 7]));
-                        *reinterpret_cast<uint4*>(o + i) = hi;
+                    turn(buf_turn, lane, y, [&](int r, int cc, float4 f) {
+                        __half* o = p.dz + (m0 + r) * p.dz_ld + col + cc;
+                        const uint2 hi = make_uint2(half2_bits(f.x, f.y), half2_bits(f.z, f.w));
+                        *reinterpret_cast<uint2*>(o) = hi;
                         if (p.dz_plane != 0) {
-                            const __half2* h = reinterpret_cast<const __half2*>(&hi);
-                            uint32_t lo[4];
-#pragma unroll
-                            for (int t = 0; t < 4; ++t) {
-                                const float2 f = __half22float2(h[t]);
-                                lo[t] = half2_bits(y[i + 2 * t] - f.x, y[i + 2 * t + 1] - f.y);
-                            }
-                            *reinterpret_cast<uint4*>(o + p.dz_plane + i) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                            const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&hi.x));
+                            const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&hi.y));
+                            *reinterpret_cast<uint2*>(o + p.dz_plane) = make_uint2(half2_bits(f.x - a.x, f.y - a.y), half2_bits(f.z - b.x, f.w - b.y));
                         }
-                    }
+                    });
+                } else {
+                    const int64_t limit = EPI == kGradX ? rows : p.out_rows;
+                    turn(buf_turn, lane, acc, [&](int r, int cc, float4 f) {
+                        if (sh.splits > 1) {
+                            *reinterpret_cast<float4*>(p.split + (static_cast<int64_t>(u) * BM + rank * HM + quarter * 32 + r) * BN + half * (BN / 2) + c + cc) = f;
+                        } else {
+                            finish4<EPI>(p, m0 + r, limit, col + cc, scale, f);
+                        }
+                    });
                 }
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(smem_u32(acc_empty + buf));
-            } else {
-                const bool some = static_cast<int64_t>(ks + 1) * sh.blocks / sh.splits > static_cast<int64_t>(ks) * sh.blocks / sh.splits;
-                const int64_t limit = EPI == kGradX ? rows : p.out_rows;
-#pragma unroll 1
-                for (int c = 0; c < BN / 2; c += 32) {
-                    uint32_t acc[32];
-                    float v[32];
-                    tmem_ld_32x32b_x32(t0 + c, acc);
-                    tc_wait_ld();
+            };
+            const int chunks = CHUNKED ? max(1, (blocks + p.chunk - 1) / p.chunk) : 1;
+            float v[CHUNKED ? BN / 2 : 32];
+            if constexpr (CHUNKED) {
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) v[i] = some ? __uint_as_float(acc[i]) : 0.0f;
-                    if (sh.splits > 1) {
-                        float* t = p.split + (static_cast<int64_t>(u) * BM + quarter * 32 + lane) * BN + half * (BN / 2) + c;
-#pragma unroll
-                        for (int i = 0; i < 32; i += 4) *reinterpret_cast<float4*>(t + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
-                    } else {
-                        finish_grad<EPI>(p, m, limit, col0 + c, scale, v);
-                    }
-                }
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(smem_u32(acc_empty + buf));
+                for (int i = 0; i < BN / 2; ++i) v[i] = 0.0f;
             }
+            for (int k = 0; k < chunks; ++k, ++local) {
+                const int buf = local & 1;
+                if (!mbar_wait_bounded(smem_u32(acc_full + buf), (local >> 1) & 1, abort_flag, p.err, kDevErrWaitAccFull)) {
+                    ok = false;
+                    break;
+                }
+                tc_fence_after();
+                const uint32_t t0 = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + buf * BN + half * (BN / 2);
+                if constexpr (CHUNKED) {
+#pragma unroll
+                    for (int c = 0; c < BN / 2; c += 32) {
+                        uint32_t acc[32];
+                        tmem_ld_32x32b_x32(t0 + c, acc);
+                        tc_wait_ld();
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) v[c + i] += blocks > 0 ? __uint_as_float(acc[i]) : 0.0f;
+                    }
+                } else {
+#pragma unroll 1
+                    for (int c = 0; c < BN / 2; c += 32) {
+                        uint32_t acc[32];
+                        tmem_ld_32x32b_x32(t0 + c, acc);
+                        tc_wait_ld();
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) v[i] = blocks > 0 ? __uint_as_float(acc[i]) : 0.0f;
+                        take(c, v);
+                    }
+                }
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive_remote(mapa_shared(smem_u32(acc_empty + buf), 0));
+            }
+            if (!ok) break;
+            if constexpr (CHUNKED) {
+#pragma unroll
+                for (int c = 0; c < BN / 2; c += 32) take(c, v + c);
+            }
+            if constexpr (EPI == kStats) p.part[(static_cast<int64_t>(nt) * 2 + half) * p.rows_pad + m] = make_float2(top, sum);
         }
     }
     tc_fence_before();
     __syncthreads();
+    cluster_sync_all();  // neither CTA leaves while the other signals it or reads its operands
     tc_fence_after();
-    if (warp == 1) tmem_dealloc(tmem_base, TMEM_COLS);
+    if (warp == 1) tmem_dealloc_pair(tmem_base, TMEM_COLS);
 }
 
-// Adds the K chunks of split tiles in their order.  One block per 8 rows of a
-// tile, 8 threads of 32 columns per row.
+// Adds the K splits of the tiles in their order, four rows of a tile per block
+// of 256 threads, four columns per thread.
 template <int EPI>
-__global__ void __launch_bounds__(64) ce_split_kernel(const GemmParams p) {
+__global__ void __launch_bounds__(256) ce_split_kernel(const GemmParams p) {
     pdl_wait();
     const Shape sh = shape_of<EPI>(p);
     if (sh.splits <= 1) return;
     const int tiles = sh.m_tiles * p.n_tiles;
     const int64_t limit = EPI == kGradX ? p.sc->count : p.out_rows;
     const float scale = EPI == kGradX ? p.sc->dx_scale : p.sc->dw_scale;
-    for (int b = blockIdx.x; b < tiles * (BM / 8); b += gridDim.x) {
-        const int tile = b / (BM / 8);
-        const int row = (b % (BM / 8)) * 8 + static_cast<int>(threadIdx.x) / 8;
-        const int c = static_cast<int>(threadIdx.x % 8) * 32;
+    for (int b = blockIdx.x; b < tiles * (BM / 4); b += gridDim.x) {
+        const int tile = b / (BM / 4);
+        const int row = b % (BM / 4) * 4 + static_cast<int>(threadIdx.x) / 64;
+        const int c = static_cast<int>(threadIdx.x % 64) * 4;
         int mt, nt, ks;
         decode_unit(p, sh, tile, mt, nt, ks);
-        float v[32];
-#pragma unroll
-        for (int i = 0; i < 32; ++i) v[i] = 0.0f;
+        const int64_t m = static_cast<int64_t>(mt) * BM + row, col = static_cast<int64_t>(nt) * BN + c;
+        if (m >= limit || col >= p.out_cols) continue;
+        float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         for (int k = 0; k < sh.splits; ++k) {
-            const float4* t = reinterpret_cast<const float4*>(p.split + ((static_cast<int64_t>(k) * tiles + tile) * BM + row) * BN + c);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float4 f = t[i];
-                v[4 * i] += f.x;
-                v[4 * i + 1] += f.y;
-                v[4 * i + 2] += f.z;
-                v[4 * i + 3] += f.w;
-            }
+            const float4 f = *reinterpret_cast<const float4*>(p.split + ((static_cast<int64_t>(k) * tiles + tile) * BM + row) * BN + c);
+            v.x += f.x, v.y += f.y, v.z += f.z, v.w += f.w;
         }
-        finish_grad<EPI>(p, static_cast<int64_t>(mt) * BM + row, limit, static_cast<int64_t>(nt) * BN + c, scale, v);
+        finish4<EPI>(p, m, limit, col, scale, v);
     }
 }
 
@@ -603,7 +696,7 @@ ce_index_kernel(const int64_t* target, int64_t rows, int64_t vocab, int64_t igno
         sc->count = base;
         sc->amax_x = 0;
         sc->amax_w = 0;
-        sc->z_log2 = kLog2e;
+        sc->rows_done = 0;
     }
 }
 
@@ -624,35 +717,75 @@ __global__ void __launch_bounds__(256) ce_amax_kernel(const float* x, const floa
     if ((threadIdx.x & 31) == 0 && top != 0) atomicMax(is_w ? &sc->amax_w : &sc->amax_x, top);
 }
 
-// The power of two that takes the largest value into [2^14, 2^15).
-__device__ __forceinline__ float plane_scale(unsigned amax_bits) {
-    if (amax_bits == 0) return 1.0f;
-    const int e = max(static_cast<int>(amax_bits >> 23), 1) - 127;
-    return exp2f(static_cast<float>(max(-126, min(126, 14 - e))));
+// Eight consecutive elements of a row whose address is off a 16-byte boundary:
+// whole 16-byte vectors around them, shifted into place (`begin` and `end` bound
+// the tensor; vectors that would leave it, and the end of a row, go one element
+// at a time).
+template <typename T>
+__device__ __forceinline__ void load8_any(const T* p, int64_t left, const void* begin, const void* end, float (&v)[8]) {
+    constexpr int W = sizeof(T) == 2 ? 8 : 12;  // 32-bit words of the vectors read
+    const uintptr_t at = reinterpret_cast<uintptr_t>(p);
+    const uintptr_t a = at & ~static_cast<uintptr_t>(15);
+    if (left < 8 || a < reinterpret_cast<uintptr_t>(begin) || a + 4 * W > reinterpret_cast<uintptr_t>(end)) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = i < left ? load_f(p, i) : 0.0f;
+        return;
+    }
+    uint32_t w[W + 2];
+#pragma unroll
+    for (int i = 0; i < W / 4; ++i) {
+        const uint4 u = *reinterpret_cast<const uint4*>(a + 16 * i);
+        w[4 * i] = u.x, w[4 * i + 1] = u.y, w[4 * i + 2] = u.z, w[4 * i + 3] = u.w;
+    }
+    w[W] = w[W + 1] = 0;
+    const int shift = static_cast<int>(at - a) >> 2;
+    if (shift & 2) {
+#pragma unroll
+        for (int i = 0; i < W; ++i) w[i] = w[i + 2];
+    }
+    if (shift & 1) {
+#pragma unroll
+        for (int i = 0; i < W; ++i) w[i] = w[i + 1];
+    }
+    if constexpr (sizeof(T) == 2) {
+        const int half = at & 2 ? 16 : 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t u = __funnelshift_r(w[i], w[i + 1], half);
+            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&u));
+            v[2 * i] = f.x;
+            v[2 * i + 1] = f.y;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(w[i]);
+    }
 }
 
-// Rows as binary16 planes with a padded row length: x's listed rows (and zero
-// rows up to a multiple of kRowPad) or W's rows.
+// Rows as binary16 planes, `ld` elements apart (a multiple of 8, zero past cols).
+template <typename T>
+struct PackJob {
+    const T* src;
+    const int* index;  // row r of the planes is row index[r] of src; NULL: r
+    __half* dst;       // NULL: nothing to pack
+    int64_t rows, cols, ld, plane;
+    bool vec;          // 16-byte aligned rows, cols a multiple of 8
+};
+
 template <typename T, int PLANES>
-__global__ void __launch_bounds__(128)
-ce_pack_kernel(const T* src, const int* index, const Scalars* sc, int64_t src_rows, int64_t cols, __half* dst, int64_t ld, int64_t plane, bool vec) {
-    pdl_wait();
-    const int64_t live = index != nullptr ? sc->count : src_rows;
-    const int64_t rows = index != nullptr ? (live + kRowPad - 1) / kRowPad * kRowPad : src_rows;
-    float s = 1.0f;
-    if constexpr (PLANES == 2) s = plane_scale(index != nullptr ? sc->amax_x : sc->amax_w);
-    for (int64_t r = blockIdx.x; r < rows; r += gridDim.x) {
-        const T* from = r < live ? src + (index != nullptr ? static_cast<int64_t>(index[r]) : r) * cols : nullptr;
-        __half* to = dst + r * ld;
-        for (int64_t c = static_cast<int64_t>(threadIdx.x) * 8; c < ld; c += 128 * 8) {
+__device__ __forceinline__ void pack_rows(const PackJob<T>& j, int64_t live, int64_t rows, float s, int64_t block, int64_t blocks) {
+    const void* end = j.src + j.rows * j.cols;
+    for (int64_t r = block; r < rows; r += blocks) {
+        const T* from = r < live ? j.src + (j.index != nullptr ? static_cast<int64_t>(j.index[r]) : r) * j.cols : nullptr;
+        __half* to = j.dst + r * j.ld;
+        for (int64_t c = static_cast<int64_t>(threadIdx.x) * 8; c < j.ld; c += blockDim.x * 8) {
             float v[8];
             if (from == nullptr) {
 #pragma unroll
                 for (int i = 0; i < 8; ++i) v[i] = 0.0f;
-            } else if (vec) {  // 16-byte aligned rows, cols a multiple of 8
+            } else if (j.vec) {
                 if constexpr (sizeof(T) == 2) {
-                    const uint4 u = *reinterpret_cast<const uint4*>(from + c);
-                    *reinterpret_cast<uint4*>(to + c) = u;
+                    *reinterpret_cast<uint4*>(to + c) = *reinterpret_cast<const uint4*>(from + c);
                     continue;
                 } else {
                     const float4 a = *reinterpret_cast<const float4*>(from + c), b = *reinterpret_cast<const float4*>(from + c + 4);
@@ -660,8 +793,7 @@ ce_pack_kernel(const T* src, const int* index, const Scalars* sc, int64_t src_ro
                     v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
                 }
             } else {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) v[i] = c + i < cols ? load_f(from, c + i) : 0.0f;
+                load8_any(from + c, j.cols - c, j.src, end, v);
             }
             uint32_t hi[4], lo[4];
 #pragma unroll
@@ -673,20 +805,30 @@ ce_pack_kernel(const T* src, const int* index, const Scalars* sc, int64_t src_ro
                 lo[t] = half2_bits(isfinite(f.x) ? a - f.x : 0.0f, isfinite(f.y) ? b - f.y : 0.0f);
             }
             *reinterpret_cast<uint4*>(to + c) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-            if constexpr (PLANES == 2) *reinterpret_cast<uint4*>(to + plane + c) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+            if constexpr (PLANES == 2) *reinterpret_cast<uint4*>(to + j.plane + c) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
         }
     }
 }
 
-template <typename T>
-__global__ void __launch_bounds__(256) ce_bias_kernel(const T* bias, int64_t vocab, float* bias2) {
-    const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-    if (i < vocab) bias2[i] = load_f(bias, i) * kLog2e;
-}
+constexpr int kPackThreads = 128;
 
-__global__ void ce_scale_kernel(Scalars* sc) {
+// Packs x's listed rows (zero rows after them up to a multiple of kRowPad), W
+// where it is not read in place, and the bias in base 2: blocks [0, x_blocks),
+// the next w_blocks, the rest.
+template <typename T, int PLANES>
+__global__ void __launch_bounds__(kPackThreads)
+ce_pack_kernel(const PackJob<T> x, const PackJob<T> w, const Scalars* sc, int x_blocks, int w_blocks, const T* bias, float* bias2) {
     pdl_wait();
-    sc->z_log2 = kLog2e / plane_scale(sc->amax_x) / plane_scale(sc->amax_w);
+    const int b = static_cast<int>(blockIdx.x);
+    if (b < x_blocks) {
+        const int64_t live = sc->count;
+        pack_rows<T, PLANES>(x, live, (live + kRowPad - 1) / kRowPad * kRowPad, PLANES == 2 ? plane_scale(sc->amax_x) : 1.0f, b, x_blocks);
+    } else if (b < x_blocks + w_blocks) {
+        pack_rows<T, PLANES>(w, w.rows, w.rows, PLANES == 2 ? plane_scale(sc->amax_w) : 1.0f, b - x_blocks, w_blocks);
+    } else {
+        const int64_t i = static_cast<int64_t>(b - x_blocks - w_blocks) * kPackThreads + threadIdx.x;
+        if (i < w.rows) bias2[i] = load_f(bias, i) * kLog2e;
+    }
 }
 
 __device__ __forceinline__ float warp_add(float v) {
@@ -698,11 +840,12 @@ __device__ __forceinline__ float warp_add(float v) {
 constexpr int kRowLanes = 32, kRowSlices = 16;
 
 // Joins the statistics of 32 rows and forms their losses: lse2 (base 2) for
-// the backward pass, the loss per packed row, and per row where asked for.
+// the backward pass, the loss per packed row, and per row where asked for.  The
+// block that finishes last adds the losses of all rows, in their order.
 template <typename T>
 __global__ void __launch_bounds__(kRowLanes* kRowSlices)
-ce_rows_kernel(const T* x, const T* w, const T* bias, const int* index, const int* target, const Scalars* sc, const float2* part,
-               int parts, int64_t rows_pad, int64_t cols, float* lse2, float* loss, float* row_loss_out) {
+ce_rows_kernel(const T* x, const T* w, const T* bias, const int* index, const int* target, Scalars* sc, const float2* part,
+               int parts, int64_t rows_pad, int64_t cols, float* lse2, float* loss, int reduction, float* out) {
     pdl_wait();
     __shared__ float2 stat[kRowSlices][kRowLanes];
     __shared__ float hit[kRowLanes];
@@ -742,34 +885,51 @@ ce_rows_kernel(const T* x, const T* w, const T* bias, const int* index, const in
             const float v = l2 * kLn2 - hit[lane];
             lse2[m] = target[m] >= 0 ? l2 : NAN;
             loss[m] = v;
-            if (row_loss_out != nullptr) row_loss_out[index[m]] = v;
+            if (reduction == TK_REDUCE_NONE) out[index[m]] = v;
         }
         __syncthreads();
     }
-}
-
-// Sum or mean of the packed rows' losses, in a fixed order.
-__global__ void __launch_bounds__(1024) ce_loss_kernel(const float* loss, const Scalars* sc, bool mean, float* out) {
-    pdl_wait();
-    __shared__ double part[32];
-    const int rows = sc->count;
-    double s = 0.0;
-    for (int i = threadIdx.x; i < rows; i += 1024) s += loss[i];
-#pragma unroll
-    for (int m = 16; m > 0; m >>= 1) s += __shfl_xor_sync(0xFFFFFFFFu, s, m);
-    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = s;
+    if (reduction == TK_REDUCE_NONE) return;
+    __shared__ bool last;
+    __shared__ double total[kRowSlices];
+    __threadfence();
     __syncthreads();
-    if (threadIdx.x == 0) {
+    if (lane == 0 && slice == 0) last = atomicAdd(&sc->rows_done, 1u) == gridDim.x - 1;
+    __syncthreads();
+    if (!last) return;
+    __threadfence();
+    double s = 0.0;
+    for (int i = slice * kRowLanes + lane; i < rows; i += kRowLanes * kRowSlices) s += __ldcg(loss + i);
+#pragma unroll
+    for (int k = 16; k > 0; k >>= 1) s += __shfl_xor_sync(0xFFFFFFFFu, s, k);
+    if (lane == 0) total[slice] = s;
+    __syncthreads();
+    if (lane == 0 && slice == 0) {
         s = 0.0;
-        for (int i = 0; i < 32; ++i) s += part[i];
-        *out = static_cast<float>(mean ? s / rows : s);  // no rows: 0 / 0, as torch's mean
+        for (int i = 0; i < kRowSlices; ++i) s += total[i];
+        *out = static_cast<float>(reduction == TK_REDUCE_MEAN ? s / rows : s);  // no rows: 0 / 0, as torch's mean
     }
 }
 
-// g_i / max |g| per packed row, the maximum, and the gradients' scales.
+// Block 0: g_i / max |g| per packed row, the maximum, and the gradients'
+// scales.  The others: zero gradients for the ignored rows.
 __global__ void __launch_bounds__(1024)
-ce_grad_rows_kernel(const float* grad, int reduction, const int* index, Scalars* sc, float* grow, int planes) {
+ce_grad_rows_kernel(const float* grad, int reduction, const int* index, Scalars* sc, float* grow, int planes, const int64_t* target,
+                    int64_t ignore, int64_t all_rows, int64_t row_bytes, uint8_t* dx) {
     pdl_wait();
+    if (blockIdx.x > 0) {
+        const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+        for (int64_t r = (blockIdx.x - 1) * 32ll + warp; r < all_rows; r += (gridDim.x - 1) * 32ll) {
+            if (target[r] != ignore) continue;
+            uint8_t* o = dx + r * row_bytes;
+            if (((reinterpret_cast<uintptr_t>(o) | row_bytes) & 15) == 0) {
+                for (int64_t c = lane * 16; c < row_bytes; c += 32 * 16) *reinterpret_cast<uint4*>(o + c) = make_uint4(0, 0, 0, 0);
+            } else {
+                for (int64_t c = lane * 2; c < row_bytes; c += 32 * 2) *reinterpret_cast<uint16_t*>(o + c) = 0;
+            }
+        }
+        return;
+    }
     __shared__ unsigned warp_top[32];
     const int rows = sc->count;
     const float g1 = reduction == TK_REDUCE_NONE ? 0.0f : reduction == TK_REDUCE_MEAN ? grad[0] / static_cast<float>(rows) : grad[0];
@@ -791,19 +951,6 @@ ce_grad_rows_kernel(const float* grad, int reduction, const int* index, Scalars*
         sc->db_scale = unit;
         sc->dx_scale = planes == 2 ? unit / plane_scale(sc->amax_w) : unit;
         sc->dw_scale = planes == 2 ? unit / plane_scale(sc->amax_x) : unit;
-    }
-}
-
-// Zero gradients for the ignored rows.
-__global__ void __launch_bounds__(128) ce_ignored_rows_kernel(const int64_t* target, int64_t ignore, int64_t rows, int64_t row_bytes, uint8_t* dx) {
-    for (int64_t r = blockIdx.x; r < rows; r += gridDim.x) {
-        if (target[r] != ignore) continue;
-        uint8_t* o = dx + r * row_bytes;
-        if (((reinterpret_cast<uintptr_t>(o) | row_bytes) & 15) == 0) {
-            for (int64_t c = threadIdx.x * 16; c < row_bytes; c += 128 * 16) *reinterpret_cast<uint4*>(o + c) = make_uint4(0, 0, 0, 0);
-        } else {
-            for (int64_t c = threadIdx.x * 2; c < row_bytes; c += 128 * 2) *reinterpret_cast<uint16_t*>(o + c) = 0;
-        }
     }
 }
 
@@ -862,7 +1009,6 @@ ce_dbias_kernel(const float* partial, int chunks, int64_t dz_ld, int64_t cols, c
 // ---- host --------------------------------------------------------------------------
 
 constexpr int64_t kDzBytes = 512ll << 20;   // one piece's dz
-constexpr int kSplitUnitsPerSm = 2;
 constexpr int64_t kMaxSize = 0x7FFFFF00;
 
 size_t align(size_t v) { return round_up(v, 1024); }
@@ -874,12 +1020,13 @@ struct Plan {
     int64_t n_tiles;         // vocabulary tiles
     int64_t piece;           // vocabulary columns per piece (a multiple of BN)
     int64_t pieces;
+    int64_t acc_ld;
     int split_units;
     int db_chunks;
     // state: kept from the forward to the backward pass
-    size_t s_scalars, s_index, s_target, s_lse, state_bytes;
-    // workspace
-    size_t w_x, w_w, w_bias, w_part, w_loss, fwd_bytes;
+    size_t s_scalars, s_index, s_target, s_lse, s_x, s_w, s_bias, state_bytes;
+    // workspaces
+    size_t w_part, w_loss, fwd_bytes;
     size_t b_grow, b_dz, b_acc, b_split, b_db, bwd_bytes;
 };
 
@@ -904,7 +1051,8 @@ Plan make_plan(const tk_linear_ce_desc_t& d) {
     p.pieces = ceil_div(p.n_tiles, most);
     p.piece = ceil_div(p.n_tiles, p.pieces) * BN;
     p.pieces = ceil_div(p.n_tiles * BN, p.piece);
-    p.split_units = sm_count(current_device()) * kSplitUnitsPerSm;
+    p.acc_ld = static_cast<int64_t>(round_up(static_cast<size_t>(d.cols), 4));
+    p.split_units = sm_count(current_device());  // two per pair of CTAs
     p.db_chunks = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(ceil_div(d.rows, 64), ceil_div(4 * sm_count(current_device()), p.piece / 256))));
     size_t at = 0;
     auto take = [&](size_t bytes) {
@@ -916,19 +1064,18 @@ Plan make_plan(const tk_linear_ce_desc_t& d) {
     p.s_index = take(p.rows_pad * sizeof(int));
     p.s_target = take(p.rows_pad * sizeof(int));
     p.s_lse = take(p.rows_pad * sizeof(float));
+    p.s_x = take(static_cast<size_t>(p.planes) * p.rows_pad * p.ld * 2);
+    p.s_w = take(p.w_direct ? 0 : static_cast<size_t>(p.planes) * d.vocab * p.ld * 2);
+    p.s_bias = take(d.bias != nullptr ? static_cast<size_t>(d.vocab) * sizeof(float) : 0);
     p.state_bytes = at;
     at = 0;
-    p.w_x = take(static_cast<size_t>(p.planes) * p.rows_pad * p.ld * 2);
-    p.w_w = take(p.w_direct ? 0 : static_cast<size_t>(p.planes) * d.vocab * p.ld * 2);
-    p.w_bias = take(d.bias != nullptr ? static_cast<size_t>(d.vocab) * sizeof(float) : 0);
-    const size_t common = at;
     p.w_part = take(static_cast<size_t>(2 * p.n_tiles) * p.rows_pad * sizeof(float2));
     p.w_loss = take(p.rows_pad * sizeof(float));
     p.fwd_bytes = at + p.state_bytes;  // a call without a state keeps its own
-    at = common;
+    at = 0;
     p.b_grow = take(p.rows_pad * sizeof(float));
     p.b_dz = take(static_cast<size_t>(p.planes) * p.rows_pad * p.piece * 2);
-    p.b_acc = take(p.pieces > 1 ? static_cast<size_t>(p.rows_pad) * d.cols * sizeof(float) : 0);
+    p.b_acc = take(p.pieces > 1 ? static_cast<size_t>(p.rows_pad) * p.acc_ld * sizeof(float) : 0);
     p.b_split = take(static_cast<size_t>(p.split_units) * BM * BN * sizeof(float));
     p.b_db = take(d.bias != nullptr ? static_cast<size_t>(p.db_chunks) * p.piece * sizeof(float) : 0);
     p.bwd_bytes = at;
@@ -965,67 +1112,107 @@ int launch_chain(const char* what, void (*k)(K...), dim3 grid, dim3 block, size_
     return TK_OK;
 }
 
-template <int EPI>
-int gemm(const CUtensorMap& a, const CUtensorMap& b, const GemmParams& p, int64_t most_units, cudaStream_t s) {
-    TK_CUDA_TRY(cudaFuncSetAttribute(ce_gemm_kernel<EPI>, cudaFuncAttributeMaxDynamicSharedMemorySize, GEMM_SMEM));
-    const int64_t grid = std::max<int64_t>(1, std::min<int64_t>(sm_count(current_device()), most_units));
-    return launch_chain("cross entropy GEMM", ce_gemm_kernel<EPI>, dim3(static_cast<unsigned>(grid)), dim3(THREADS), GEMM_SMEM, s, a, b, p);
-}
+// K blocks per accumulator chunk: 16 steps of 16 where every output is
+// binary32, 64 for the loss of fp16 operands (measured at 4096 columns: the
+// loss 1e-6 off without chunks, and the same time).
+constexpr int kChunkF32 = 4, kChunkStats = 16;
 
-int blocks_for(int64_t rows) { return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(rows, 148 * 16))); }
-
-// Packed operands (x's listed rows; W unless it is read in place; the bias).
-template <typename T, int PLANES>
-int pack(const tk_linear_ce_desc_t& d, const Plan& p, uint8_t* ws, const int* index, Scalars* sc, bool scan, cudaStream_t s) {
-    const T* x = static_cast<const T*>(d.x);
-    const T* w = static_cast<const T*>(d.weight);
-    const bool xv = d.cols % 8 == 0 && (reinterpret_cast<uintptr_t>(x) & 15) == 0;
-    const bool wv = d.cols % 8 == 0 && (reinterpret_cast<uintptr_t>(w) & 15) == 0;
-    if constexpr (PLANES == 2) {
-        if (scan) {
-            CE_TRY(launch_chain("cross entropy amax", ce_amax_kernel, dim3(296, 2), dim3(256), 0, s, reinterpret_cast<const float*>(x),
-                                reinterpret_cast<const float*>(w), index, sc, d.cols, d.vocab));
-            CE_TRY(launch_chain("cross entropy scale", ce_scale_kernel, dim3(1), dim3(1), 0, s, sc));
-        }
+template <int EPI, bool CHUNKED>
+int gemm_launch(const CUtensorMap& a, const CUtensorMap& b, const GemmParams& p, int64_t most_units, cudaStream_t s) {
+    auto* kernel = ce_gemm_kernel<EPI, CHUNKED>;
+    static std::atomic<int> resident[64];  // pairs of CTAs each device holds at once; 0: not asked yet
+    const int device = current_device();
+    int pairs = device < 64 ? resident[device].load(std::memory_order_relaxed) : 0;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 2;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(2);
+    cfg.blockDim = dim3(THREADS);
+    cfg.dynamicSmemBytes = GEMM_SMEM;
+    cfg.stream = s;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    if (pairs == 0) {
+        TK_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, GEMM_SMEM));
+        TK_CUDA_TRY(cudaOccupancyMaxActiveClusters(&pairs, kernel, &cfg));
+        if (pairs < 1) TK_FAIL(TK_ERR_CUDA, "cross entropy GEMM: no pair of CTAs fits the GPU");
+        if (device < 64) resident[device].store(pairs, std::memory_order_relaxed);
     }
-    CE_TRY(launch_chain("cross entropy pack", ce_pack_kernel<T, PLANES>, dim3(blocks_for(p.rows_pad)), dim3(128), 0, s, x, index,
-                        static_cast<const Scalars*>(sc), d.rows, d.cols, reinterpret_cast<__half*>(ws + p.w_x), p.ld, p.rows_pad * p.ld, xv));
-    if (!p.w_direct)
-        CE_TRY(launch_chain("cross entropy pack", ce_pack_kernel<T, PLANES>, dim3(blocks_for(d.vocab)), dim3(128), 0, s, w,
-                            static_cast<const int*>(nullptr), static_cast<const Scalars*>(sc), d.vocab, d.cols,
-                            reinterpret_cast<__half*>(ws + p.w_w), p.ld, d.vocab * p.ld, wv));
-    if (d.bias != nullptr) {
-        ce_bias_kernel<T><<<static_cast<unsigned>(ceil_div(d.vocab, 256)), 256, 0, s>>>(static_cast<const T*>(d.bias), d.vocab,
-                                                                                       reinterpret_cast<float*>(ws + p.w_bias));
-        CE_TRY(launch_status("cross entropy bias"));
+    cfg.gridDim = dim3(static_cast<unsigned>(2 * std::max<int64_t>(1, std::min<int64_t>(pairs, most_units))));
+    cfg.numAttrs = 2;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, a, b, p);
+    if (e != cudaSuccess) {
+        cudaGetLastError();
+        TK_FAIL(TK_ERR_CUDA, "cross entropy GEMM launch failed: %s", cudaGetErrorString(e));
     }
     return TK_OK;
 }
 
-int pack_any(const tk_linear_ce_desc_t& d, const Plan& p, uint8_t* ws, const int* index, Scalars* sc, bool scan, cudaStream_t s) {
-    return p.f16 ? pack<__half, 1>(d, p, ws, index, sc, scan, s) : pack<float, 2>(d, p, ws, index, sc, scan, s);
+template <int EPI>
+int gemm(const CUtensorMap& a, const CUtensorMap& b, const GemmParams& p, int64_t most_units, cudaStream_t s) {
+    // a K loop no longer than a chunk needs no sum in registers
+    const bool one = p.chunk == 0 || (p.k_blocks >= 0 && p.k_blocks * p.pairs <= p.chunk);
+    return one ? gemm_launch<EPI, false>(a, b, p, most_units, s) : gemm_launch<EPI, true>(a, b, p, most_units, s);
 }
 
-struct Operands {
-    const void* w;
-    int64_t w_ld, w_plane;
+int blocks_for(int64_t rows) { return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(rows, 148 * 16))); }
+
+// The kept operands (x's listed rows; W unless it is read in place; the bias).
+template <typename T, int PLANES>
+int pack(const tk_linear_ce_desc_t& d, const Plan& p, uint8_t* st, cudaStream_t s) {
+    const T* x = static_cast<const T*>(d.x);
+    const T* w = static_cast<const T*>(d.weight);
+    Scalars* sc = reinterpret_cast<Scalars*>(st + p.s_scalars);
+    const int* index = reinterpret_cast<const int*>(st + p.s_index);
+    const bool eight = d.cols % 8 == 0;
+    if constexpr (PLANES == 2)
+        CE_TRY(launch_chain("cross entropy amax", ce_amax_kernel, dim3(296, 2), dim3(256), 0, s, x, w, index, sc, d.cols, d.vocab));
+    const PackJob<T> jx = {x, index, reinterpret_cast<__half*>(st + p.s_x), d.rows, d.cols, p.ld, p.rows_pad * p.ld,
+                           eight && (reinterpret_cast<uintptr_t>(x) & 15) == 0};
+    const PackJob<T> jw = {w, nullptr, reinterpret_cast<__half*>(st + p.s_w), d.vocab, d.cols, p.ld, d.vocab * p.ld,
+                           eight && (reinterpret_cast<uintptr_t>(w) & 15) == 0};
+    const int x_blocks = blocks_for(p.rows_pad), w_blocks = p.w_direct ? 0 : blocks_for(d.vocab);
+    const int64_t b_blocks = d.bias != nullptr ? ceil_div(d.vocab, kPackThreads) : 0;
+    return launch_chain("cross entropy pack", ce_pack_kernel<T, PLANES>, dim3(static_cast<unsigned>(x_blocks + w_blocks + b_blocks)), dim3(kPackThreads), 0,
+                        s, jx, jw, static_cast<const Scalars*>(sc), x_blocks, w_blocks, static_cast<const T*>(d.bias),
+                        reinterpret_cast<float*>(st + p.s_bias));
+}
+
+template <typename T>
+int rows_loss(const tk_linear_ce_desc_t& d, const Plan& p, uint8_t* st, uint8_t* ws, cudaStream_t s) {
+    const dim3 grid(static_cast<unsigned>(std::max<int64_t>(1, std::min<int64_t>(ceil_div(d.rows, kRowLanes), 148 * 4)))), block(kRowLanes, kRowSlices);
+    return launch_chain("cross entropy rows", ce_rows_kernel<T>, grid, block, 0, s, static_cast<const T*>(d.x), static_cast<const T*>(d.weight),
+                        static_cast<const T*>(d.bias), reinterpret_cast<const int*>(st + p.s_index), reinterpret_cast<const int*>(st + p.s_target),
+                        reinterpret_cast<Scalars*>(st + p.s_scalars), reinterpret_cast<const float2*>(ws + p.w_part), static_cast<int>(2 * p.n_tiles),
+                        p.rows_pad, d.cols, reinterpret_cast<float*>(st + p.s_lse), reinterpret_cast<float*>(ws + p.w_loss), static_cast<int>(d.reduction),
+                        d.loss);
+}
+
+struct Operand {
+    const uint8_t* base;
+    int64_t ld, plane;
 };
 
-Operands operands(const tk_linear_ce_desc_t& d, const Plan& p, uint8_t* ws) {
-    if (p.w_direct) return {d.weight, d.cols, d.vocab * d.cols};
-    return {ws + p.w_w, p.ld, d.vocab * p.ld};
+Operand weight_operand(const tk_linear_ce_desc_t& d, const Plan& p, const uint8_t* st) {
+    if (p.w_direct) return {static_cast<const uint8_t*>(d.weight), d.cols, d.vocab * d.cols};
+    return {st + p.s_w, p.ld, d.vocab * p.ld};
 }
 
-GemmParams base_params(const tk_linear_ce_desc_t& d, const Plan& p, uint8_t* ws, const Scalars* sc) {
+GemmParams base_params(const tk_linear_ce_desc_t& d, const Plan& p, const uint8_t* st) {
     GemmParams g = {};
-    g.sc = sc;
+    g.sc = reinterpret_cast<const Scalars*>(st + p.s_scalars);
     g.pairs = p.planes == 2 ? 3 : 1;
+    g.chunk = p.planes == 2 ? kChunkF32 : 0;
     g.m_tiles = -1;
     g.k_blocks = static_cast<int>(ceil_div(d.cols, BK));
-    g.group = 16;
+    g.group = 8;
     g.max_units = p.split_units;
     g.err = device_error_word(current_device());
-    g.bias2 = d.bias != nullptr ? reinterpret_cast<const float*>(ws + p.w_bias) : nullptr;
+    g.bias2 = d.bias != nullptr ? reinterpret_cast<const float*>(st + p.s_bias) : nullptr;
     g.vocab = d.vocab;
     g.rows_pad = p.rows_pad;
     return g;
@@ -1060,40 +1247,27 @@ int tk_linear_ce(const tk_linear_ce_desc_t* desc, void* workspace, size_t worksp
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     uint8_t* ws = static_cast<uint8_t*>(workspace);
     uint8_t* st = d.state != nullptr ? static_cast<uint8_t*>(d.state) : ws + (p.fwd_bytes - p.state_bytes);
-    Scalars* sc = reinterpret_cast<Scalars*>(st + p.s_scalars);
-    int* index = reinterpret_cast<int*>(st + p.s_index);
-    int* target = reinterpret_cast<int*>(st + p.s_target);
-    float* lse2 = reinterpret_cast<float*>(st + p.s_lse);
-    float* loss = reinterpret_cast<float*>(ws + p.w_loss);
-    float* per_row = d.reduction == TK_REDUCE_NONE ? d.loss : nullptr;
-    ce_index_kernel<<<1, kIndexThreads, 0, s>>>(d.target, d.rows, d.vocab, d.ignore_index, index, target, sc, per_row);
+    ce_index_kernel<<<1, kIndexThreads, 0, s>>>(d.target, d.rows, d.vocab, d.ignore_index, reinterpret_cast<int*>(st + p.s_index),
+                                                reinterpret_cast<int*>(st + p.s_target), reinterpret_cast<Scalars*>(st + p.s_scalars),
+                                                d.reduction == TK_REDUCE_NONE ? d.loss : nullptr);
     CE_TRY(launch_status("cross entropy index"));
     if (d.rows > 0) {
-        CE_TRY(pack_any(d, p, ws, index, sc, true, s));
-        const Operands o = operands(d, p, ws);
+        if (p.f16) {
+            CE_TRY((pack<__half, 1>(d, p, st, s)));
+        } else {
+            CE_TRY((pack<float, 2>(d, p, st, s)));
+        }
+        const Operand w = weight_operand(d, p, st);
         CUtensorMap tx, tw;
-        CE_TRY(make_map(&tx, ws + p.w_x, d.cols, p.rows_pad, p.planes, p.ld, p.rows_pad * p.ld, BM));
-        CE_TRY(make_map(&tw, o.w, d.cols, d.vocab, p.planes, o.w_ld, o.w_plane, BN));
-        GemmParams g = base_params(d, p, ws, sc);
+        CE_TRY(make_map(&tx, st + p.s_x, d.cols, p.rows_pad, p.planes, p.ld, p.rows_pad * p.ld, HM));
+        CE_TRY(make_map(&tw, w.base, d.cols, d.vocab, p.planes, w.ld, w.plane, HN));
+        GemmParams g = base_params(d, p, st);
+        if (g.chunk == 0) g.chunk = kChunkStats;
         g.n_tiles = static_cast<int>(p.n_tiles);
         g.part = reinterpret_cast<float2*>(ws + p.w_part);
         CE_TRY(gemm<kStats>(tx, tw, g, p.n_tiles * ceil_div(d.rows, BM), s));
-        const dim3 grid(static_cast<unsigned>(std::min<int64_t>(ceil_div(d.rows, kRowLanes), 148 * 4))), block(kRowLanes, kRowSlices);
-        const float2* part = g.part;
-        const int parts = static_cast<int>(2 * p.n_tiles);
-        if (p.f16) {
-            CE_TRY(launch_chain("cross entropy rows", ce_rows_kernel<__half>, grid, block, 0, s, static_cast<const __half*>(d.x),
-                                static_cast<const __half*>(d.weight), static_cast<const __half*>(d.bias), static_cast<const int*>(index),
-                                static_cast<const int*>(target), static_cast<const Scalars*>(sc), part, parts, p.rows_pad, d.cols, lse2, loss, per_row));
-        } else {
-            CE_TRY(launch_chain("cross entropy rows", ce_rows_kernel<float>, grid, block, 0, s, static_cast<const float*>(d.x),
-                                static_cast<const float*>(d.weight), static_cast<const float*>(d.bias), static_cast<const int*>(index),
-                                static_cast<const int*>(target), static_cast<const Scalars*>(sc), part, parts, p.rows_pad, d.cols, lse2, loss, per_row));
-        }
     }
-    if (d.reduction != TK_REDUCE_NONE)
-        CE_TRY(launch_chain("cross entropy loss", ce_loss_kernel, dim3(1), dim3(1024), 0, s, static_cast<const float*>(loss),
-                            static_cast<const Scalars*>(sc), d.reduction == TK_REDUCE_MEAN, d.loss));
+    if (d.rows > 0 || d.reduction != TK_REDUCE_NONE) CE_TRY(p.f16 ? rows_loss<__half>(d, p, st, ws, s) : rows_loss<float>(d, p, st, ws, s));
     return TK_OK;
 }
 
@@ -1126,31 +1300,27 @@ int tk_linear_ce_backward(const tk_linear_ce_grad_desc_t* desc, void* workspace,
     const int* index = reinterpret_cast<const int*>(st + p.s_index);
     float* grow = reinterpret_cast<float*>(ws + p.b_grow);
     __half* dz = reinterpret_cast<__half*>(ws + p.b_dz);
-    CE_TRY(pack_any(d, p, ws, index, sc, false, s));
-    CE_TRY(launch_chain("cross entropy gradient rows", ce_grad_rows_kernel, dim3(1), dim3(1024), 0, s, desc->grad_loss, static_cast<int>(d.reduction),
-                        index, sc, grow, p.planes));
-    if (desc->dx) {
-        ce_ignored_rows_kernel<<<blocks_for(d.rows), 128, 0, s>>>(d.target, d.ignore_index, d.rows, d.cols * static_cast<int64_t>(dtype_size(d.dtype)),
-                                                                  static_cast<uint8_t*>(desc->dx));
-        CE_TRY(launch_status("cross entropy ignored rows"));
-    }
-    const Operands o = operands(d, p, ws);
+    const size_t esz = dtype_size(d.dtype);
+    const int zero_blocks = desc->dx != nullptr ? static_cast<int>(std::min<int64_t>(ceil_div(d.rows, 32), 148 * 2)) : 0;
+    CE_TRY(launch_chain("cross entropy gradient rows", ce_grad_rows_kernel, dim3(static_cast<unsigned>(1 + zero_blocks)), dim3(1024), 0, s,
+                        desc->grad_loss, static_cast<int>(d.reduction), index, sc, grow, p.planes, d.target, d.ignore_index, d.rows,
+                        static_cast<int64_t>(d.cols * esz), static_cast<uint8_t*>(desc->dx)));
+    const Operand w = weight_operand(d, p, st);
     const int64_t x_plane = p.rows_pad * p.ld, dz_plane = p.rows_pad * p.piece;
     CUtensorMap tx, tx_mn;
-    CE_TRY(make_map(&tx, ws + p.w_x, d.cols, p.rows_pad, p.planes, p.ld, x_plane, BM));
-    CE_TRY(make_map(&tx_mn, ws + p.w_x, d.cols, p.rows_pad, p.planes, p.ld, x_plane, BK));
+    CE_TRY(make_map(&tx, st + p.s_x, d.cols, p.rows_pad, p.planes, p.ld, x_plane, HM));
+    CE_TRY(make_map(&tx_mn, st + p.s_x, d.cols, p.rows_pad, p.planes, p.ld, x_plane, BK));
     const int64_t row_tiles = ceil_div(d.rows, BM), col_tiles = ceil_div(d.cols, BN);
-    const size_t esz = dtype_size(d.dtype);
     const bool cols16 = d.cols * esz % 16 == 0;
     for (int64_t i = 0; i < p.pieces; ++i) {
         const int64_t v0 = i * p.piece, width = std::min(p.piece, d.vocab - v0);
-        const uint8_t* wbase = static_cast<const uint8_t*>(o.w) + v0 * o.w_ld * 2;
+        const uint8_t* wbase = w.base + v0 * w.ld * 2;
         CUtensorMap tw, tw_mn, tdz, tdz_mn;
-        CE_TRY(make_map(&tw, wbase, d.cols, width, p.planes, o.w_ld, o.w_plane, BN));
-        CE_TRY(make_map(&tw_mn, wbase, d.cols, width, p.planes, o.w_ld, o.w_plane, BK));
-        CE_TRY(make_map(&tdz, dz, width, p.rows_pad, p.planes, p.piece, dz_plane, BM));
+        CE_TRY(make_map(&tw, wbase, d.cols, width, p.planes, w.ld, w.plane, HN));
+        CE_TRY(make_map(&tw_mn, wbase, d.cols, width, p.planes, w.ld, w.plane, BK));
+        CE_TRY(make_map(&tdz, dz, width, p.rows_pad, p.planes, p.piece, dz_plane, HM));
         CE_TRY(make_map(&tdz_mn, dz, width, p.rows_pad, p.planes, p.piece, dz_plane, BK));
-        GemmParams g = base_params(d, p, ws, sc);
+        GemmParams g = base_params(d, p, st);
         g.n_tiles = static_cast<int>(ceil_div(width, BN));
         g.vocab0 = v0;
         g.lse2 = reinterpret_cast<const float*>(st + p.s_lse);
@@ -1160,7 +1330,7 @@ int tk_linear_ce_backward(const tk_linear_ce_grad_desc_t* desc, void* workspace,
         g.dz_ld = p.piece;
         g.dz_plane = p.planes == 2 ? dz_plane : 0;
         CE_TRY(gemm<kDlogits>(tx, tw, g, row_tiles * g.n_tiles, s));
-        GemmParams r = base_params(d, p, ws, sc);
+        GemmParams r = base_params(d, p, st);
         r.out_cols = d.cols;
         r.out_f32 = p.f16 ? 0 : 1;
         r.n_tiles = static_cast<int>(col_tiles);
@@ -1171,10 +1341,11 @@ int tk_linear_ce_backward(const tk_linear_ce_grad_desc_t* desc, void* workspace,
             r.out_vec = cols16 && (reinterpret_cast<uintptr_t>(desc->dx) & 15) == 0;
             r.index = index;
             r.acc = reinterpret_cast<float*>(ws + p.b_acc);
+            r.acc_ld = p.acc_ld;
             r.first = i == 0;
             r.last = i + 1 == p.pieces;
             CE_TRY(gemm<kGradX>(tdz, tw_mn, r, std::max<int64_t>(row_tiles * col_tiles, p.split_units), s));
-            CE_TRY(launch_chain("cross entropy split", ce_split_kernel<kGradX>, dim3(static_cast<unsigned>(p.split_units) * 4), dim3(64), 0, s, r));
+            CE_TRY(launch_chain("cross entropy split", ce_split_kernel<kGradX>, dim3(static_cast<unsigned>(p.split_units) * 8), dim3(256), 0, s, r));
         }
         if (desc->dweight) {
             r.m_tiles = static_cast<int>(ceil_div(width, BM));
@@ -1183,8 +1354,8 @@ int tk_linear_ce_backward(const tk_linear_ce_grad_desc_t* desc, void* workspace,
             r.out_vec = cols16 && (reinterpret_cast<uintptr_t>(r.out) & 15) == 0;
             r.out_rows = width;
             CE_TRY(gemm<kGradW>(tdz_mn, tx_mn, r, std::max<int64_t>(r.m_tiles * col_tiles, p.split_units), s));
-            if (2 * r.m_tiles * col_tiles <= p.split_units)
-                CE_TRY(launch_chain("cross entropy split", ce_split_kernel<kGradW>, dim3(static_cast<unsigned>(p.split_units) * 4), dim3(64), 0, s, r));
+            if (2 * r.m_tiles * col_tiles <= p.split_units)  // else no tile is split
+                CE_TRY(launch_chain("cross entropy split", ce_split_kernel<kGradW>, dim3(static_cast<unsigned>(p.split_units) * 8), dim3(256), 0, s, r));
         }
         if (desc->dbias) {
             float* part = reinterpret_cast<float*>(ws + p.b_db);
