@@ -23,14 +23,17 @@
 //
 // HBM bounds both directions: 4 tensors forward, 6 backward (5 without a post
 // norm and a gate, which need f).  A group of W warps holds a row in
-// registers, 8 * NV columns per thread; a CTA runs several groups when rows
-// are short, and a cluster of CTAs shares a row past 8192 (fp16) or 4096
-// (fp32) columns, its sums exchanged through distributed shared memory.  Each
-// thread copies its own columns of the next rows into its own shared-memory
-// slots (cp.async), so loads stay in flight without registers or barriers.
-// CTAs own contiguous rows; column sums stay in registers until a CTA's rows
-// end, and a second kernel adds the CTAs' partial sums in a fixed order, so
-// no gradient depends on timing.
+// registers, 8 * NV columns per thread, as pairs for the two-wide binary32
+// instructions (one per element made the kernels issue-bound: 8192 x 4096 with
+// both norms took 93 us forward, 2.4 TB/s, at 63 % issue); a CTA runs several
+// groups when rows are short, and a cluster of CTAs shares a row that one CTA
+// cannot hold, its sums exchanged through distributed shared memory.  The next
+// rows are copied to shared memory (cp.async) while a row is worked on: each
+// thread its own columns where rows are 16-byte aligned, which needs no
+// barrier, otherwise the group the 16-byte vectors that cover the row.  CTAs
+// own contiguous rows; column sums stay in registers until a CTA's rows end,
+// and a second kernel adds the CTAs' partial sums in a fixed order, so no
+// gradient depends on timing.
 #include <cuda_fp16.h>
 
 #include <algorithm>
@@ -69,44 +72,38 @@ __device__ __forceinline__ int64_t unit_of(int64_t r, int64_t rows, int64_t unit
     return ((r + 1) * units - 1) / rows;
 }
 
-__device__ __forceinline__ float to_f(__half v) { return __half2float(v); }
-__device__ __forceinline__ float to_f(float v) { return v; }
 template <typename T> __device__ __forceinline__ T from_f(float v);
 template <> __device__ __forceinline__ __half from_f<__half>(float v) { return __float2half_rn(v); }
 template <> __device__ __forceinline__ float from_f<float>(float v) { return v; }
 
-__device__ __forceinline__ void unpack8(const uint4 (&u)[1], float* o) {
-    const __half2* h = reinterpret_cast<const __half2*>(&u[0]);
-#pragma unroll
-    for (int t = 0; t < 4; ++t) {
-        const float2 f = __half22float2(h[t]);
-        o[2 * t] = f.x;
-        o[2 * t + 1] = f.y;
-    }
+// Two-wide binary32 arithmetic (one instruction for a pair).
+union Pair {
+    float2 f;
+    unsigned long long u;
+};
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    Pair x{a}, y{b}, z{c}, r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.u) : "l"(x.u), "l"(y.u), "l"(z.u));
+    return r.f;
 }
-__device__ __forceinline__ void unpack8(const uint4 (&u)[2], float* o) {
-#pragma unroll
-    for (int t = 0; t < 2; ++t) {
-        o[4 * t] = __uint_as_float(u[t].x);
-        o[4 * t + 1] = __uint_as_float(u[t].y);
-        o[4 * t + 2] = __uint_as_float(u[t].z);
-        o[4 * t + 3] = __uint_as_float(u[t].w);
-    }
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    Pair x{a}, y{b}, r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.u) : "l"(x.u), "l"(y.u));
+    return r.f;
 }
-__device__ __forceinline__ void store8(__half* p, const float* v) {
-    uint4 u;
-    __half2* h = reinterpret_cast<__half2*>(&u);
-#pragma unroll
-    for (int t = 0; t < 4; ++t) h[t] = __floats2half2_rn(v[2 * t], v[2 * t + 1]);
-    *reinterpret_cast<uint4*>(p) = u;
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    Pair x{a}, y{b}, r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.u) : "l"(x.u), "l"(y.u));
+    return r.f;
 }
-__device__ __forceinline__ void store8(float* p, const float* v) {
-    *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
-    *reinterpret_cast<float4*>(p + 4) = make_float4(v[4], v[5], v[6], v[7]);
-}
+__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+// The first `bytes` of a 16-byte vector, zeros after them.
+__device__ __forceinline__ void cp_async16_part(uint32_t dst, const void* src, int bytes) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 // Waits until at most `pending` of this thread's copy groups are in flight.
@@ -120,112 +117,192 @@ __device__ __forceinline__ void cp_async_wait(int pending) {
     }
 }
 
-// One thread's share of a row: which columns it holds, its shared-memory
-// slots, and the sums over the threads that hold the rest of the row.
+// E values of type T in registers, as stored (two binary16 to a word).
+template <typename T, int E>
+struct Raw {
+    uint32_t r[E * sizeof(T) / 4];
+    __device__ __forceinline__ float2 pair(int i) const {
+        if constexpr (sizeof(T) == 2) {
+            return __half22float2(*reinterpret_cast<const __half2*>(&r[i]));
+        } else {
+            return make_float2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1]));
+        }
+    }
+    __device__ __forceinline__ void set(int e, T v) {
+        if constexpr (sizeof(T) == 2) {
+            const uint32_t b = __half_as_ushort(v);
+            r[e / 2] = e % 2 ? (r[e / 2] & 0xFFFFu) | b << 16 : b;
+        } else {
+            r[e] = __float_as_uint(v);
+        }
+    }
+    __device__ __forceinline__ void vec(int i, uint4 v) { r[4 * i] = v.x, r[4 * i + 1] = v.y, r[4 * i + 2] = v.z, r[4 * i + 3] = v.w; }
+};
+
+constexpr int kTailPad = 32;  // bytes of a row's copy beyond the row: both 16-byte roundings
+
+// One thread's share of a row: which columns it holds, the copies of the rows
+// to come, and the sums over the threads that hold the rest of the row.
 //
 // VEC: octets of 8 consecutive columns, 16-byte accesses (every pointer
 // 16-byte aligned, cols a multiple of 8).  Otherwise single columns, one
 // row's width of threads apart.
 template <typename T, int NV, bool VEC>
 struct Lane {
-    static constexpr int E = 8 * NV;
-    static constexpr int PARTS = sizeof(T) / 2;  // 16-byte vectors of an octet
-    int t, lane, warp, group, gthreads, rank;
-    int64_t col0;  // first column of the CTA's slice
-    uint32_t ring;
+    static constexpr int E = 8 * NV, P = E / 2;
+    [[maybe_unused]] static constexpr int PARTS = sizeof(T) / 2;  // 16-byte vectors of an octet
+    int t, lane, warp, group, gthreads, rank, tensors;
+    int col0, cols;  // first column of the CTA's slice, columns of a row
+    uint32_t ring;   // this thread's (VEC) or this group's copies
+    uint32_t image;  // bytes of one row's copy (not VEC)
     float2* red;
     int red_stride, red_n, parity;
+    bool full;       // every column of the slice is in the row
     const RnParams& p;
 
-    __device__ Lane(const RnParams& pr, uint8_t* smem) : p(pr) {
+    __device__ Lane(const RnParams& pr, uint8_t* smem, int tensors_) : tensors(tensors_), p(pr) {
         gthreads = p.warps * 32;
         group = threadIdx.x / gthreads;
         t = threadIdx.x - group * gthreads;
         lane = threadIdx.x & 31;
         warp = t >> 5;
         rank = p.cluster > 1 ? static_cast<int>(cluster_ctarank()) : 0;
-        col0 = static_cast<int64_t>(rank) * gthreads * E;
+        col0 = rank * gthreads * E;
+        cols = static_cast<int>(p.cols);
+        full = col0 + gthreads * E <= cols;
         red = reinterpret_cast<float2*>(smem);
         red_n = p.warps * p.cluster;
         red_stride = red_n * p.groups;
         parity = 0;
-        ring = smem_u32(smem + 2 * sizeof(float2) * ((red_stride + 1) & ~1)) + threadIdx.x * 16;
+        ring = smem_u32(smem + 2 * sizeof(float2) * ((red_stride + 1) & ~1));
+        image = static_cast<uint32_t>(gthreads * E * sizeof(T) + kTailPad);
+        if constexpr (VEC) {
+            ring += threadIdx.x * 16;
+        } else {
+            ring += static_cast<uint32_t>(group * p.stages * tensors) * image;
+        }
         if (p.cluster > 1) cluster_sync_all();  // every CTA runs before its memory is written
     }
-    __device__ __forceinline__ int64_t col(int e) const {
-        return VEC ? col0 + (static_cast<int64_t>(e / 8) * gthreads + t) * 8 + e % 8
-                   : col0 + static_cast<int64_t>(e) * gthreads + t;
-    }
-    __device__ __forceinline__ bool has(int e) const { return col(e) < p.cols; }
+    __device__ __forceinline__ int col(int e) const { return VEC ? col0 + (e / 8 * gthreads + t) * 8 + e % 8 : col0 + e * gthreads + t; }
+    __device__ __forceinline__ bool has(int e) const { return VEC ? full || col(e & ~7) < cols : full || col(e) < cols; }
 
-    // Begins the copy of tensor `k` (of `tensors`) of a row into `stage`.
-    __device__ __forceinline__ void fetch(const void* base, int64_t row, int stage, int k, int tensors) const {
+    // Begins the copy of tensor k's row into `stage`.  base points at the row's
+    // first column of this thread (VEC) or of the slice.
+    __device__ __forceinline__ void fetch(const void* tensor, int64_t row, int stage, int k) const {
         if constexpr (VEC) {
+            const T* src = static_cast<const T*>(tensor) + row * p.cols;
+            const uint32_t slot = ring + static_cast<uint32_t>((stage * tensors + k) * NV * PARTS) * blockDim.x * 16;
 #pragma unroll
             for (int v = 0; v < NV; ++v) {
                 if (!has(8 * v)) continue;
-                const T* src = static_cast<const T*>(base) + row * p.cols + col(8 * v);
-                const uint32_t slot = ring + static_cast<uint32_t>(((stage * tensors + k) * NV + v) * PARTS) * blockDim.x * 16;
 #pragma unroll
-                for (int i = 0; i < PARTS; ++i) cp_async16(slot + i * blockDim.x * 16, reinterpret_cast<const uint4*>(src) + i);
-            }
-        }
-    }
-    __device__ __forceinline__ void row_values(const void* base, int64_t row, int stage, int k, int tensors, float (&o)[E]) const {
-        if constexpr (VEC) {
-#pragma unroll
-            for (int v = 0; v < NV; ++v) {
-                uint4 u[PARTS];
-                const uint32_t slot = ring + static_cast<uint32_t>(((stage * tensors + k) * NV + v) * PARTS) * blockDim.x * 16;
-#pragma unroll
-                for (int i = 0; i < PARTS; ++i) {
-                    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
-                                 : "=r"(u[i].x), "=r"(u[i].y), "=r"(u[i].z), "=r"(u[i].w)
-                                 : "r"(slot + i * blockDim.x * 16)
-                                 : "memory");
-                }
-                unpack8(u, &o[8 * v]);
-                if (!has(8 * v)) {
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) o[8 * v + j] = 0.0f;
-                }
+                for (int i = 0; i < PARTS; ++i) cp_async16(slot + (v * PARTS + i) * blockDim.x * 16, reinterpret_cast<const uint4*>(src + col(8 * v)) + i);
             }
         } else {
-#pragma unroll
-            for (int e = 0; e < E; ++e) o[e] = has(e) ? to_f(static_cast<const T*>(base)[row * p.cols + col(e)]) : 0.0f;
+            const int width = min(cols - col0, gthreads * E);
+            if (width <= 0) return;
+            const uintptr_t at = reinterpret_cast<uintptr_t>(static_cast<const T*>(tensor) + row * p.cols + col0);
+            const uintptr_t from = at & ~static_cast<uintptr_t>(15);
+            const uintptr_t end = reinterpret_cast<uintptr_t>(static_cast<const T*>(tensor) + p.rows * p.cols);
+            const uint32_t slot = ring + static_cast<uint32_t>(stage * tensors + k) * image;
+            const int vectors = static_cast<int>((at + width * sizeof(T) - from + 15) / 16);
+            for (int i = t; i < vectors; i += gthreads) {
+                const uintptr_t v = from + 16 * static_cast<uintptr_t>(i);
+                if (v >= reinterpret_cast<uintptr_t>(tensor)) {
+                    cp_async16_part(slot + 16 * i, reinterpret_cast<const void*>(v), static_cast<int>(min(static_cast<uintptr_t>(16), end - v)));
+                } else {  // the tensor begins inside this vector
+                    for (uintptr_t a = reinterpret_cast<uintptr_t>(tensor); a < v + 16 && a < end; a += 2)
+                        asm volatile("st.shared.u16 [%0], %1;" ::"r"(slot + static_cast<uint32_t>(a - from)), "h"(*reinterpret_cast<const uint16_t*>(a)) : "memory");
+                }
+            }
         }
     }
-    // This thread's columns of a [cols] vector, `absent` where it is NULL.
-    __device__ __forceinline__ void vector(const void* base, float absent, float (&o)[E]) const {
+    // Threads of the group wait for one another.
+    __device__ __forceinline__ void group_sync() const {
+        if (p.warps == 1) {
+            __syncwarp();
+        } else {
+            named_barrier_sync(1 + group, gthreads);
+        }
+    }
+    __device__ __forceinline__ void row_values(const void* tensor, int64_t row, int stage, int k, float2 (&o)[P]) const {
+        Raw<T, E> w;
+        if constexpr (VEC) {
+            const uint32_t slot = ring + static_cast<uint32_t>((stage * tensors + k) * NV * PARTS) * blockDim.x * 16;
+#pragma unroll
+            for (int v = 0; v < NV * PARTS; ++v) {
+                uint4 u;
+                asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(u.x), "=r"(u.y), "=r"(u.z), "=r"(u.w) : "r"(slot + v * blockDim.x * 16) : "memory");
+                w.vec(v, u);
+            }
+            if (!full) {  // octets past the row were not copied
+#pragma unroll
+                for (int v = 0; v < NV * PARTS; ++v)
+                    if (!has(8 * (v / PARTS))) w.vec(v, make_uint4(0, 0, 0, 0));
+            }
+        } else {
+            const uintptr_t at = reinterpret_cast<uintptr_t>(static_cast<const T*>(tensor) + row * p.cols + col0);
+            const uint32_t slot = ring + static_cast<uint32_t>(stage * tensors + k) * image + static_cast<uint32_t>(at & 15);
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                const uint32_t a = slot + static_cast<uint32_t>(e * gthreads + t) * sizeof(T);
+                if constexpr (sizeof(T) == 2) {
+                    uint16_t v = 0;
+                    if (has(e)) asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(a) : "memory");
+                    w.set(e, __ushort_as_half(v));
+                } else {
+                    uint32_t v = 0;
+                    if (has(e)) asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
+                    w.r[e] = v;
+                }
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < P; ++i) o[i] = w.pair(i);
+    }
+    // This thread's columns of a [cols] vector: `absent` where it is NULL, 0
+    // past the row.
+    __device__ __forceinline__ void vector(const void* base, float absent, Raw<T, E>& w) const {
         const T* b = static_cast<const T*>(base);
         if constexpr (VEC) {
 #pragma unroll
             for (int v = 0; v < NV; ++v) {
                 if (b != nullptr && has(8 * v)) {
-                    uint4 u[PARTS];
 #pragma unroll
-                    for (int i = 0; i < PARTS; ++i) u[i] = __ldg(reinterpret_cast<const uint4*>(b + col(8 * v)) + i);
-                    unpack8(u, &o[8 * v]);
+                    for (int i = 0; i < PARTS; ++i) w.vec(v * PARTS + i, __ldg(reinterpret_cast<const uint4*>(b + col(8 * v)) + i));
                 } else {
+                    const T one = from_f<T>(has(8 * v) ? absent : 0.0f);
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) o[8 * v + j] = absent;
+                    for (int e = 8 * v; e < 8 * v + 8; ++e) w.set(e, one);
                 }
             }
         } else {
 #pragma unroll
-            for (int e = 0; e < E; ++e) o[e] = b != nullptr && has(e) ? to_f(b[col(e)]) : absent;
+            for (int e = 0; e < E; ++e) w.set(e, !has(e) ? from_f<T>(0.0f) : b != nullptr ? b[col(e)] : from_f<T>(absent));
         }
     }
-    __device__ __forceinline__ void store(void* base, int64_t row, const float (&v)[E]) const {
-        T* b = static_cast<T*>(base) + row * p.cols;
+    __device__ __forceinline__ void store(void* tensor, int64_t row, const float2 (&v)[P]) const {
+        T* b = static_cast<T*>(tensor) + row * p.cols;
         if constexpr (VEC) {
 #pragma unroll
-            for (int k = 0; k < NV; ++k)
-                if (has(8 * k)) store8(b + col(8 * k), &v[8 * k]);
+            for (int k = 0; k < NV; ++k) {
+                if (!has(8 * k)) continue;
+                if constexpr (sizeof(T) == 2) {
+                    uint4 u;
+                    __half2* h = reinterpret_cast<__half2*>(&u);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) h[i] = __float22half2_rn(v[4 * k + i]);
+                    *reinterpret_cast<uint4*>(b + col(8 * k)) = u;
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 2; ++i)
+                        reinterpret_cast<float4*>(b + col(8 * k))[i] = make_float4(v[4 * k + 2 * i].x, v[4 * k + 2 * i].y, v[4 * k + 2 * i + 1].x, v[4 * k + 2 * i + 1].y);
+                }
+            }
         } else {
 #pragma unroll
             for (int e = 0; e < E; ++e)
-                if (has(e)) b[col(e)] = from_f<T>(v[e]);
+                if (has(e)) b[col(e)] = from_f<T>(e % 2 ? v[e / 2].y : v[e / 2].x);
         }
     }
     // Keep bits of this thread's columns of a row (bit e).
@@ -233,22 +310,40 @@ struct Lane {
         uint32_t m = 0;
         if constexpr (VEC) {
 #pragma unroll
-            for (int v = 0; v < NV; ++v)
-                m |= dropout_keep8(p.dropout, static_cast<uint64_t>(row * p.cols + col(8 * v)) / 8) << (8 * v);
+            for (int v = 0; v < NV; ++v) m |= dropout_keep8(p.dropout, static_cast<uint64_t>(row * p.cols + col(8 * v)) / 8) << (8 * v);
         } else {
+            // Columns e of the warp's lanes are 32 consecutive elements, 4 *
+            // block + shift on: eight blocks of four, a ninth where shift > 0.
+            // Lane 4 q + r works out block q for the columns e = r mod 4, lane
+            // e the ninth of column e; each lane then fetches the four keep
+            // bits of its own block.
+            const uint64_t first = static_cast<uint64_t>(row * p.cols + col0 + warp * 32);
+            const uint32_t shift = static_cast<uint32_t>(first) & 3u;
+            const uint32_t q = (shift + lane) >> 2, bit = (shift + lane) & 3u;
+            uint32_t mine = 0, ninth = 0;  // four keep bits each
 #pragma unroll
-            for (int e = 0; e < E; ++e) m |= (dropout_keep1(p.dropout, row * p.cols + col(e)) ? 1u : 0u) << e;
+            for (int a = 0; a < E / 4; ++a)
+                mine |= dropout_keep4(p.dropout, (first + static_cast<uint64_t>(4 * a + (lane & 3)) * gthreads) / 4 + (lane >> 2)) << (4 * (a % 8));
+            if (shift != 0) ninth = dropout_keep4(p.dropout, (first + static_cast<uint64_t>(lane % E) * gthreads) / 4 + 8);
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                uint32_t four = __shfl_sync(0xFFFFFFFFu, mine, (q & 7) * 4 + e % 4) >> (4 * (e / 4));
+                const uint32_t edge = __shfl_sync(0xFFFFFFFFu, ninth, e);
+                if (q == 8) four = edge;
+                m |= ((four >> bit) & 1u) << e;
+            }
         }
         return m;
     }
-    // Sums of a and b over the row's threads; every thread gets the same bits.
+    // Sums over the row's threads of N values; every thread gets the same bits.
     // One exchange buffer is read while the next sum fills the other, so one
     // barrier per sum is enough.
+    template <int N>
     __device__ __forceinline__ void row_sum(float& a, float& b) {
 #pragma unroll
         for (int m = 16; m > 0; m >>= 1) {
             a += __shfl_xor_sync(0xFFFFFFFFu, a, m);
-            b += __shfl_xor_sync(0xFFFFFFFFu, b, m);
+            if (N == 2) b += __shfl_xor_sync(0xFFFFFFFFu, b, m);
         }
         if (red_n == 1) return;
         float2* buf = red + parity * red_stride + group * red_n;
@@ -266,142 +361,179 @@ struct Lane {
             __syncwarp();
             cluster_sync_all();
         }
-        a = 0.0f;
-        b = 0.0f;
-        if (red_n <= 4) {
-            for (int i = 0; i < red_n; ++i) {
-                a += buf[i].x;
-                b += buf[i].y;
-            }
+        if (red_n <= 16) {
+            float2 s = buf[0];
+            for (int i = 1; i < red_n; ++i) s = add2(s, buf[i]);
+            a = s.x;
+            b = s.y;
         } else {
-            for (int i = lane; i < red_n; i += 32) {
-                a += buf[i].x;
-                b += buf[i].y;
-            }
+            float2 s = make_float2(0.0f, 0.0f);
+            for (int i = lane; i < red_n; i += 32) s = add2(s, buf[i]);
 #pragma unroll
             for (int m = 16; m > 0; m >>= 1) {
-                a += __shfl_xor_sync(0xFFFFFFFFu, a, m);
-                b += __shfl_xor_sync(0xFFFFFFFFu, b, m);
+                s.x += __shfl_xor_sync(0xFFFFFFFFu, s.x, m);
+                if (N == 2) s.y += __shfl_xor_sync(0xFFFFFFFFu, s.y, m);
             }
+            a = s.x;
+            b = s.y;
         }
     }
     // mean and rstd of v over the row (mean 0 for an rms norm); the mean
-    // square is taken about the mean, as values held in registers.
-    __device__ __forceinline__ void moments(const float (&v)[E], float& mean, float& rstd) {
+    // square is taken about the mean, of values held in registers.
+    __device__ __forceinline__ void moments(const float2 (&v)[P], float& mean, float& rstd) {
         mean = 0.0f;
         float unused = 0.0f;
         if (p.layer) {
-            float s = 0.0f;
+            float2 s = v[0];
 #pragma unroll
-            for (int e = 0; e < E; ++e) s += v[e];
-            row_sum(s, unused);
-            mean = s * p.inv_cols;
+            for (int i = 1; i < P; ++i) s = add2(s, v[i]);
+            float sum = s.x + s.y;
+            row_sum<1>(sum, unused);
+            mean = sum * p.inv_cols;
         }
-        float q = 0.0f;
+        const float2 shift = both(-mean);
+        float2 s = make_float2(0.0f, 0.0f);
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
-            const float c = v[e] - mean;
-            if (has(e)) q += c * c;
+        for (int i = 0; i < P; ++i) {
+            const float2 c = add2(v[i], shift);
+            if constexpr (VEC) {
+                if (has(2 * i)) s = fma2(c, c, s);
+            } else {
+                if (has(2 * i)) s.x = fmaf(c.x, c.x, s.x);
+                if (has(2 * i + 1)) s.y = fmaf(c.y, c.y, s.y);
+            }
         }
-        unused = 0.0f;
-        row_sum(q, unused);
+        float q = s.x + s.y;
+        row_sum<1>(q, unused);
         rstd = rsqrtf(q * p.inv_cols + p.eps);
     }
-};
-
-template <typename T, int NV, bool VEC, bool POST>
-__global__ void __launch_bounds__(kMaxThreads) residual_norm_kernel(const RnParams p) {
-    extern __shared__ __align__(16) uint8_t smem[];
-    using L = Lane<T, NV, VEC>;
-    constexpr int E = L::E;
-    L ln(p, smem);
-    const int64_t unit = blockIdx.x / p.cluster;
-    const int64_t end = unit_begin(unit + 1, p.rows, p.units);
-    const int64_t begin = unit_begin(unit, p.rows, p.units) + ln.group;
-    const int ahead = VEC ? p.stages - 1 : 0;
-    if constexpr (VEC) {
-        for (int i = 0; i < ahead; ++i) {
-            const int64_t r = begin + static_cast<int64_t>(i) * p.groups;
-            if (r < end) {
-                ln.fetch(p.x, r, i, 0, 2);
-                ln.fetch(p.f, r, i, 1, 2);
-            }
-            cp_async_commit();
+    __device__ __forceinline__ void drop(uint32_t keep, float2 (&v)[P]) const {
+        const float2 s = both(p.dropout.scale);
+#pragma unroll
+        for (int i = 0; i < P; ++i) {
+            v[i] = mul2(v[i], s);
+            if (!((keep >> (2 * i)) & 1u)) v[i].x = 0.0f;
+            if (!((keep >> (2 * i + 1)) & 1u)) v[i].y = 0.0f;
         }
     }
-    int stage = 0;
-    for (int64_t r = begin; r < end; r += p.groups) {
-        if constexpr (VEC) {
+    // Runs f(row, stage) over the group's rows [begin, end), a step of `groups`
+    // apart, with the copies of the rows ahead under way.
+    template <typename Fetch, typename F>
+    __device__ __forceinline__ void rows(int64_t begin, int64_t end, Fetch fetch_row, F f) const {
+        const int ahead = p.stages - 1;
+        for (int i = 0; i < ahead; ++i) {
+            const int64_t r = begin + static_cast<int64_t>(i) * p.groups;
+            if (r < end) fetch_row(r, i);
+            cp_async_commit();
+        }
+        int stage = 0;
+        for (int64_t r = begin; r < end; r += p.groups) {
             const int64_t next = r + static_cast<int64_t>(ahead) * p.groups;
             int ns = stage + ahead;
             if (ns >= p.stages) ns -= p.stages;
-            if (next < end) {
-                ln.fetch(p.x, next, ns, 0, 2);
-                ln.fetch(p.f, next, ns, 1, 2);
+            if constexpr (VEC) {
+                if (next < end) fetch_row(next, ns);
+                cp_async_commit();
+                cp_async_wait(ahead);
+            } else {
+                // the group's copies of this row are in, and its last row's
+                // are read, before that stage is filled again (stages >= 2)
+                cp_async_wait(ahead - 1);
+                group_sync();
+                if (next < end) fetch_row(next, ns);
+                cp_async_commit();
             }
-            cp_async_commit();
+            f(r, stage);
+            if (++stage == p.stages) stage = 0;
         }
-        const uint32_t keep = p.drop ? ln.keep(r) : 0u;
-        if constexpr (VEC) cp_async_wait(ahead);
-        float u[E], v[E];
-        ln.row_values(p.f, r, stage, 1, 2, u);
-        float4 st = make_float4(0.f, 0.f, 0.f, 0.f);
-        if constexpr (POST) {
-            ln.moments(u, st.x, st.y);
-            ln.vector(p.post_weight, 1.0f, v);
-#pragma unroll
-            for (int e = 0; e < E; ++e) u[e] = (u[e] - st.x) * st.y * v[e];
-            if (p.post_bias != nullptr) {
-                ln.vector(p.post_bias, 0.0f, v);
-#pragma unroll
-                for (int e = 0; e < E; ++e) u[e] += v[e];
-            }
-        }
-        if (p.drop) {
-#pragma unroll
-            for (int e = 0; e < E; ++e) u[e] = (keep >> e) & 1u ? u[e] * p.dropout.scale : 0.0f;
-        }
-        if (p.gate != nullptr) {
-            ln.vector(static_cast<const T*>(p.gate) + r / p.gate_period * p.cols, 0.0f, v);
-#pragma unroll
-            for (int e = 0; e < E; ++e) u[e] *= v[e];
-        }
-        ln.row_values(p.x, r, stage, 0, 2, v);
-#pragma unroll
-        for (int e = 0; e < E; ++e) u[e] = fmaf(p.a, v[e], u[e]);
-        if constexpr (POST) {  // a vector's columns past the row hold its bias there
-#pragma unroll
-            for (int e = 0; e < E; ++e)
-                if (!ln.has(e)) u[e] = 0.0f;
-        }
-        ln.store(p.x_new, r, u);
-        ln.moments(u, st.z, st.w);
-        ln.vector(p.weight, 1.0f, v);
-#pragma unroll
-        for (int e = 0; e < E; ++e) u[e] = (u[e] - st.z) * st.w * v[e];
-        if (p.bias != nullptr) {
-            ln.vector(p.bias, 0.0f, v);
-#pragma unroll
-            for (int e = 0; e < E; ++e) u[e] += v[e];
-        }
-        ln.store(p.h, r, u);
-        if (p.stats != nullptr && ln.t == 0 && ln.rank == 0) p.stats[r] = st;
-        if (++stage == p.stages) stage = 0;
+        cp_async_wait(0);
     }
+};
+
+// Parameter vectors stay in registers for up to 24 columns per thread; wider
+// shares read them again for each row (from L1).
+template <typename T, int NV, bool VEC, bool POST>
+__global__ void __launch_bounds__(kMaxThreads, 1) residual_norm_kernel(const RnParams p) {
+    extern __shared__ __align__(16) uint8_t smem[];
+    using L = Lane<T, NV, VEC>;
+    constexpr int P = L::P;
+    constexpr bool KEPT = NV <= 3;
+    L ln(p, smem, 2);
+    const int64_t unit = blockIdx.x / p.cluster;
+    const int64_t end = unit_begin(unit + 1, p.rows, p.units);
+    const int64_t begin = unit_begin(unit, p.rows, p.units) + ln.group;
+    Raw<T, L::E> w, b, pw, pb, gate;
+    int64_t gate_row = -1;
+    if constexpr (KEPT) {
+        ln.vector(p.weight, 1.0f, w);
+        if (p.bias != nullptr) ln.vector(p.bias, 0.0f, b);
+        if constexpr (POST) {
+            ln.vector(p.post_weight, 1.0f, pw);
+            if (p.post_bias != nullptr) ln.vector(p.post_bias, 0.0f, pb);
+        }
+    }
+    ln.rows(
+        begin, end,
+        [&](int64_t r, int stage) {
+            ln.fetch(p.x, r, stage, 0);
+            ln.fetch(p.f, r, stage, 1);
+        },
+        [&](int64_t r, int stage) {
+            float2 u[P], x[P];
+            ln.row_values(p.f, r, stage, 1, u);
+            float4 st = make_float4(0.f, 0.f, 0.f, 0.f);
+            if constexpr (POST) {
+                ln.moments(u, st.x, st.y);
+                if constexpr (!KEPT) ln.vector(p.post_weight, 1.0f, pw);
+                const float2 s = both(st.y), c = both(-st.x);
+#pragma unroll
+                for (int i = 0; i < P; ++i) u[i] = mul2(mul2(add2(u[i], c), s), pw.pair(i));
+                if (p.post_bias != nullptr) {
+                    if constexpr (!KEPT) ln.vector(p.post_bias, 0.0f, pb);
+#pragma unroll
+                    for (int i = 0; i < P; ++i) u[i] = add2(u[i], pb.pair(i));
+                }
+            }
+            if (p.drop) ln.drop(ln.keep(r), u);
+            if (p.gate != nullptr) {
+                const int64_t g = p.gate_period == p.rows ? 0 : r / p.gate_period;
+                if (!KEPT || g != gate_row) ln.vector(static_cast<const T*>(p.gate) + g * p.cols, 0.0f, gate);
+                gate_row = g;
+#pragma unroll
+                for (int i = 0; i < P; ++i) u[i] = mul2(u[i], gate.pair(i));
+            }
+            ln.row_values(p.x, r, stage, 0, x);
+            const float2 a = both(p.a);
+#pragma unroll
+            for (int i = 0; i < P; ++i) u[i] = fma2(a, x[i], u[i]);
+            ln.store(p.x_new, r, u);
+            ln.moments(u, st.z, st.w);
+            if constexpr (!KEPT) ln.vector(p.weight, 1.0f, w);
+            const float2 s = both(st.w), c = both(-st.z);
+#pragma unroll
+            for (int i = 0; i < P; ++i) u[i] = mul2(mul2(add2(u[i], c), s), w.pair(i));
+            if (p.bias != nullptr) {
+                if constexpr (!KEPT) ln.vector(p.bias, 0.0f, b);
+#pragma unroll
+                for (int i = 0; i < P; ++i) u[i] = add2(u[i], b.pair(i));
+            }
+            ln.store(p.h, r, u);
+            if (p.stats != nullptr && ln.t == 0 && ln.rank == 0) p.stats[r] = st;
+        });
 }
 
 // Adds `acc` over the CTA's groups and writes the CTA's columns, as fp32
 // partial sums or (to_final) as the finished gradient.  Every thread of the
 // CTA takes part; `buf` is the ring's memory, idle at this point.
 template <typename T, int NV, bool VEC>
-__device__ __forceinline__ void flush_columns(const Lane<T, NV, VEC>& ln, float* buf, const float (&acc)[8 * NV],
+__device__ __forceinline__ void flush_columns(const Lane<T, NV, VEC>& ln, float* buf, const float2 (&acc)[4 * NV],
                                               float* partial, T* final_row) {
     const RnParams& p = ln.p;
     const int width = ln.gthreads * 8 * NV;
     if (p.groups > 1) {
         __syncthreads();
 #pragma unroll
-        for (int e = 0; e < 8 * NV; ++e) buf[ln.group * width + (ln.col(e) - ln.col0)] = acc[e];
+        for (int e = 0; e < 8 * NV; ++e) buf[ln.group * width + (ln.col(e) - ln.col0)] = e % 2 ? acc[e / 2].y : acc[e / 2].x;
         __syncthreads();
         for (int c = threadIdx.x; c < width && ln.col0 + c < p.cols; c += blockDim.x) {
             float s = 0.0f;
@@ -417,180 +549,168 @@ __device__ __forceinline__ void flush_columns(const Lane<T, NV, VEC>& ln, float*
 #pragma unroll
         for (int e = 0; e < 8 * NV; ++e) {
             if (!ln.has(e)) continue;
+            const float v = e % 2 ? acc[e / 2].y : acc[e / 2].x;
             if (final_row != nullptr) {
-                final_row[ln.col(e)] = from_f<T>(acc[e]);
+                final_row[ln.col(e)] = from_f<T>(v);
             } else {
-                partial[ln.col(e)] = acc[e];
+                partial[ln.col(e)] = v;
             }
         }
     }
 }
 
 template <typename T, int NV, bool VEC, bool POST, bool GATE>
-__global__ void __launch_bounds__(kMaxThreads) residual_norm_backward_kernel(const RnParams p) {
+__global__ void __launch_bounds__(kMaxThreads, 1) residual_norm_backward_kernel(const RnParams p) {
     extern __shared__ __align__(16) uint8_t smem[];
     using L = Lane<T, NV, VEC>;
-    constexpr int E = L::E;
+    constexpr int P = L::P;
     constexpr bool NEED_F = POST || GATE;
-    constexpr int TENSORS = NEED_F ? 4 : 3;
-    L ln(p, smem);
+    L ln(p, smem, NEED_F ? 4 : 3);
     float* const buf = reinterpret_cast<float*>(smem + 2 * sizeof(float2) * ((ln.red_stride + 1) & ~1));
     const int64_t unit = blockIdx.x / p.cluster;
     const int64_t unit_lo = unit_begin(unit, p.rows, p.units), unit_hi = unit_begin(unit + 1, p.rows, p.units);
-    const int ahead = VEC ? p.stages - 1 : 0;
     const bool gate_sums = GATE && p.gate_period > 1;  // else each row writes its own gradient
-    float dw[E], db[E], dpw[POST ? E : 1], dpb[POST ? E : 1], dgt[GATE ? E : 1];
+    Raw<T, L::E> w, pw, gate;
+    ln.vector(p.weight, 1.0f, w);
+    if constexpr (POST) ln.vector(p.post_weight, 1.0f, pw);
+    float2 dw[P], db[P], dpw[POST ? P : 1], dpb[POST ? P : 1], dgt[GATE ? P : 1];
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-        dw[e] = 0.0f;
-        db[e] = 0.0f;
-        if constexpr (POST) dpw[e] = dpb[e] = 0.0f;
+    for (int i = 0; i < P; ++i) {
+        dw[i] = db[i] = make_float2(0.0f, 0.0f);
+        if constexpr (POST) dpw[i] = dpb[i] = make_float2(0.0f, 0.0f);
     }
-    auto fetch = [&](int64_t r, int stage) {
-        if (p.gx != nullptr) ln.fetch(p.gx, r, stage, 0, TENSORS);
-        if (p.gh != nullptr) ln.fetch(p.gh, r, stage, 1, TENSORS);
-        ln.fetch(p.x_new, r, stage, 2, TENSORS);
-        if constexpr (NEED_F) ln.fetch(p.f, r, stage, 3, TENSORS);
-    };
+    int64_t gate_row = -1;
     // a segment: the rows of this unit that share a gate row (all of them
     // where no sum of the gate's gradient is kept)
     int64_t seg_lo = unit_lo;
     while (seg_lo < unit_hi) {
-        const int64_t gate_row = gate_sums ? seg_lo / p.gate_period : 0;
-        const int64_t seg_hi = gate_sums ? min(unit_hi, (gate_row + 1) * p.gate_period) : unit_hi;
+        const int64_t seg_gate = gate_sums ? seg_lo / p.gate_period : 0;
+        const int64_t seg_hi = gate_sums ? min(unit_hi, (seg_gate + 1) * p.gate_period) : unit_hi;
         if constexpr (GATE) {
 #pragma unroll
-            for (int e = 0; e < E; ++e) dgt[e] = 0.0f;
+            for (int i = 0; i < P; ++i) dgt[i] = make_float2(0.0f, 0.0f);
         }
-        const int64_t begin = seg_lo + ln.group;
-        if constexpr (VEC) {
-            for (int i = 0; i < ahead; ++i) {
-                const int64_t r = begin + static_cast<int64_t>(i) * p.groups;
-                if (r < seg_hi) fetch(r, i);
-                cp_async_commit();
-            }
-        }
-        int stage = 0;
-        for (int64_t r = begin; r < seg_hi; r += p.groups) {
-            if constexpr (VEC) {
-                const int64_t next = r + static_cast<int64_t>(ahead) * p.groups;
-                int ns = stage + ahead;
-                if (ns >= p.stages) ns -= p.stages;
-                if (next < seg_hi) fetch(next, ns);
-                cp_async_commit();
-            }
-            const float4 st = p.stats[r];
-            const uint32_t keep = p.drop ? ln.keep(r) : 0u;
-            if constexpr (VEC) cp_async_wait(ahead);
-            float g[E], n[E], t[E];
-            if (p.gh != nullptr) {
-                float wv[E];
-                ln.row_values(p.x_new, r, stage, 2, TENSORS, n);
-                ln.row_values(p.gh, r, stage, 1, TENSORS, t);
-                ln.vector(p.weight, 1.0f, wv);
-                float c1 = 0.0f, c2 = 0.0f;
+        ln.rows(
+            seg_lo + ln.group, seg_hi,
+            [&](int64_t r, int stage) {
+                if (p.gx != nullptr) ln.fetch(p.gx, r, stage, 0);
+                if (p.gh != nullptr) ln.fetch(p.gh, r, stage, 1);
+                ln.fetch(p.x_new, r, stage, 2);
+                if constexpr (NEED_F) ln.fetch(p.f, r, stage, 3);
+            },
+            [&](int64_t r, int stage) {
+                const float4 st = p.stats[r];
+                float2 g[P];
+                if (p.gh != nullptr) {
+                    float2 n[P], h[P];
+                    ln.row_values(p.x_new, r, stage, 2, n);
+                    ln.row_values(p.gh, r, stage, 1, h);
+                    const float2 s = both(st.w), c = both(-st.z);
+                    float2 s1 = make_float2(0.0f, 0.0f), s2 = s1;
 #pragma unroll
-                for (int e = 0; e < E; ++e) {
-                    n[e] = ln.has(e) ? (n[e] - st.z) * st.w : 0.0f;
-                    dw[e] += t[e] * n[e];
-                    db[e] += t[e];
-                    t[e] *= wv[e];
-                    c1 += t[e];
-                    c2 += t[e] * n[e];
-                }
-                ln.row_sum(c1, c2);
-                c1 = p.layer ? c1 * p.inv_cols : 0.0f;
-                c2 *= p.inv_cols;
-                if (p.gx != nullptr) {
-                    ln.row_values(p.gx, r, stage, 0, TENSORS, g);
-                } else {
+                    for (int i = 0; i < P; ++i) {
+                        n[i] = mul2(add2(n[i], c), s);
+                        dw[i] = fma2(h[i], n[i], dw[i]);
+                        db[i] = add2(db[i], h[i]);
+                        h[i] = mul2(h[i], w.pair(i));  // 0 past the row
+                        s1 = add2(s1, h[i]);
+                        s2 = fma2(h[i], n[i], s2);
+                    }
+                    float c1 = s1.x + s1.y, c2 = s2.x + s2.y;
+                    ln.template row_sum<2>(c1, c2);
+                    const float2 m1 = both(p.layer ? -c1 * p.inv_cols : 0.0f), m2 = both(-c2 * p.inv_cols);
 #pragma unroll
-                    for (int e = 0; e < E; ++e) g[e] = 0.0f;
-                }
+                    for (int i = 0; i < P; ++i) h[i] = add2(fma2(n[i], m2, h[i]), m1);
+                    if (p.gx != nullptr) {
+                        ln.row_values(p.gx, r, stage, 0, g);
 #pragma unroll
-                for (int e = 0; e < E; ++e) g[e] += st.w * (t[e] - c1 - n[e] * c2);
-            } else {
-                ln.row_values(p.gx, r, stage, 0, TENSORS, g);
-            }
-            if (p.dx != nullptr) {
+                        for (int i = 0; i < P; ++i) g[i] = fma2(h[i], s, g[i]);
+                    } else {
 #pragma unroll
-                for (int e = 0; e < E; ++e) t[e] = p.a * g[e];
-                ln.store(p.dx, r, t);
-            }
-            if constexpr (NEED_F) {  // n: q = Norm(f) with a post norm, else f
-                ln.row_values(p.f, r, stage, 3, TENSORS, n);
-                if constexpr (POST) {
-#pragma unroll
-                    for (int e = 0; e < E; ++e) n[e] = ln.has(e) ? (n[e] - st.x) * st.y : 0.0f;
-                }
-            }
-            if constexpr (GATE) {
-                float u[E];
-                if constexpr (POST) {
-                    ln.vector(p.post_weight, 1.0f, u);
-#pragma unroll
-                    for (int e = 0; e < E; ++e) u[e] *= n[e];
-                    if (p.post_bias != nullptr) {
-                        ln.vector(p.post_bias, 0.0f, t);
-#pragma unroll
-                        for (int e = 0; e < E; ++e) u[e] += t[e];
+                        for (int i = 0; i < P; ++i) g[i] = mul2(h[i], s);
                     }
                 } else {
-#pragma unroll
-                    for (int e = 0; e < E; ++e) u[e] = n[e];
+                    ln.row_values(p.gx, r, stage, 0, g);
                 }
-                if (p.drop) {
+                if (p.dx != nullptr) {
+                    float2 o[P];
+                    const float2 a = both(p.a);
 #pragma unroll
-                    for (int e = 0; e < E; ++e) u[e] = (keep >> e) & 1u ? u[e] * p.dropout.scale : 0.0f;
+                    for (int i = 0; i < P; ++i) o[i] = mul2(a, g[i]);
+                    ln.store(p.dx, r, o);
                 }
+                const uint32_t keep = p.drop ? ln.keep(r) : 0u;
+                float2 q[NEED_F ? P : 1];  // Norm(f) with a post norm, else f
+                if constexpr (NEED_F) {
+                    ln.row_values(p.f, r, stage, 3, q);
+                    if constexpr (POST) {
+                        const float2 s = both(st.y), c = both(-st.x);
 #pragma unroll
-                for (int e = 0; e < E; ++e) u[e] *= g[e];
-                if (gate_sums) {
-#pragma unroll
-                    for (int e = 0; e < E; ++e) dgt[e] += u[e];
-                } else if (p.dgate != nullptr) {
-                    ln.store(p.dgate, r, u);
+                        for (int i = 0; i < P; ++i) q[i] = mul2(add2(q[i], c), s);
+                    }
                 }
-                ln.vector(static_cast<const T*>(p.gate) + r / p.gate_period * p.cols, 0.0f, u);
+                if constexpr (GATE) {
+                    float2 u[P];
+                    if constexpr (POST) {
 #pragma unroll
-                for (int e = 0; e < E; ++e) g[e] *= u[e];
-            }
-            if (p.drop) {
+                        for (int i = 0; i < P; ++i) u[i] = mul2(q[i], pw.pair(i));
+                        if (p.post_bias != nullptr) {
+                            Raw<T, L::E> pb;
+                            ln.vector(p.post_bias, 0.0f, pb);
 #pragma unroll
-                for (int e = 0; e < E; ++e) g[e] = (keep >> e) & 1u ? g[e] * p.dropout.scale : 0.0f;
-            }
-            if constexpr (POST) {
-                ln.vector(p.post_weight, 1.0f, t);
-                float c3 = 0.0f, c4 = 0.0f;
+                            for (int i = 0; i < P; ++i) u[i] = add2(u[i], pb.pair(i));
+                        }
+                    } else {
 #pragma unroll
-                for (int e = 0; e < E; ++e) {
-                    if (!ln.has(e)) g[e] = 0.0f;
-                    dpw[e] += g[e] * n[e];
-                    dpb[e] += g[e];
-                    g[e] *= t[e];
-                    c3 += g[e];
-                    c4 += g[e] * n[e];
+                        for (int i = 0; i < P; ++i) u[i] = q[i];
+                    }
+                    if (p.drop) ln.drop(keep, u);
+                    if (gate_sums) {
+#pragma unroll
+                        for (int i = 0; i < P; ++i) dgt[i] = fma2(u[i], g[i], dgt[i]);
+                    } else if (p.dgate != nullptr) {
+#pragma unroll
+                        for (int i = 0; i < P; ++i) u[i] = mul2(u[i], g[i]);
+                        ln.store(p.dgate, r, u);
+                    }
+                    const int64_t k = p.gate_period == p.rows ? 0 : r / p.gate_period;
+                    if (k != gate_row) ln.vector(static_cast<const T*>(p.gate) + k * p.cols, 0.0f, gate);
+                    gate_row = k;
+#pragma unroll
+                    for (int i = 0; i < P; ++i) g[i] = mul2(g[i], gate.pair(i));
                 }
-                ln.row_sum(c3, c4);
-                c3 = p.layer ? c3 * p.inv_cols : 0.0f;
-                c4 *= p.inv_cols;
+                if (p.drop) ln.drop(keep, g);
+                if constexpr (POST) {
+                    float2 s3 = make_float2(0.0f, 0.0f), s4 = s3;
 #pragma unroll
-                for (int e = 0; e < E; ++e) g[e] = st.y * (g[e] - c3 - n[e] * c4);
-            }
-            if (p.df != nullptr) ln.store(p.df, r, g);
-            if (++stage == p.stages) stage = 0;
-        }
-        if constexpr (VEC) cp_async_wait(0);
+                    for (int i = 0; i < P; ++i) {
+                        dpw[i] = fma2(g[i], q[i], dpw[i]);
+                        dpb[i] = add2(dpb[i], g[i]);
+                        g[i] = mul2(g[i], pw.pair(i));  // 0 past the row
+                        s3 = add2(s3, g[i]);
+                        s4 = fma2(g[i], q[i], s4);
+                    }
+                    float c3 = s3.x + s3.y, c4 = s4.x + s4.y;
+                    ln.template row_sum<2>(c3, c4);
+                    const float2 s = both(st.y), m3 = both(p.layer ? -c3 * p.inv_cols : 0.0f), m4 = both(-c4 * p.inv_cols);
+#pragma unroll
+                    for (int i = 0; i < P; ++i) g[i] = mul2(s, add2(fma2(q[i], m4, g[i]), m3));
+                }
+                if (p.df != nullptr) ln.store(p.df, r, g);
+            });
         if constexpr (GATE) {
             if (gate_sums && p.dgate != nullptr) {
                 // whole segments are finished here; one that other units share
                 // goes to the unit's first or last slot
-                const bool whole = seg_lo == gate_row * p.gate_period && seg_hi == (gate_row + 1) * p.gate_period;
+                const bool whole = seg_lo == seg_gate * p.gate_period && seg_hi == (seg_gate + 1) * p.gate_period;
                 float* slot = p.partial + (4 * static_cast<int64_t>(p.units) + 2 * unit + (seg_lo == unit_lo ? 0 : 1)) * p.cols;
-                flush_columns<T, NV, VEC>(ln, buf, dgt, slot, whole ? static_cast<T*>(p.dgate) + gate_row * p.cols : nullptr);
+                flush_columns<T, NV, VEC>(ln, buf, dgt, slot, whole ? static_cast<T*>(p.dgate) + seg_gate * p.cols : nullptr);
             }
         }
         seg_lo = seg_hi;
+        if constexpr (!VEC) {
+            if (seg_lo < unit_hi) ln.group_sync();  // the segment's copies are read before the next one's begin
+        }
     }
     const int64_t plane = static_cast<int64_t>(p.units) * p.cols;
     flush_columns<T, NV, VEC>(ln, buf, dw, p.partial + unit * p.cols, nullptr);
@@ -601,14 +721,15 @@ __global__ void __launch_bounds__(kMaxThreads) residual_norm_backward_kernel(con
     }
 }
 
-constexpr int kColLanes = 32, kColRows = 16;
+constexpr int kColLanes = 32, kColRows = 32;
 
-// The units' partial sums added in their order, rounded once.  Items 0..3 are
-// the parameter vectors; item 4 + c finishes the gate row that unit c ends
-// and unit c + 1 (and more) continues.
+// The units' partial sums added in a fixed order, rounded once.  Items 0..3 are
+// the parameter vectors; the others finish gate rows that several units share:
+// item 4 + g gate row g, or (by_unit, fewer units than gate rows) item 4 + c
+// the gate row that unit c ends and unit c + 1 continues.
 template <typename T>
 __global__ void __launch_bounds__(kColLanes* kColRows)
-residual_norm_columns_kernel(const RnParams p, T* d0, T* d1, T* d2, T* d3, int col_blocks) {
+residual_norm_columns_kernel(const RnParams p, T* d0, T* d1, T* d2, T* d3, int col_blocks, bool by_unit) {
     pdl_wait();
     __shared__ float part[kColRows][kColLanes + 1];
     const int item = static_cast<int>(blockIdx.x) / col_blocks;
@@ -620,18 +741,26 @@ residual_norm_columns_kernel(const RnParams p, T* d0, T* d1, T* d2, T* d3, int c
         if (out == nullptr) return;
         if (c < p.cols) {
             const float* src = p.partial + static_cast<int64_t>(item) * p.units * p.cols + c;
+#pragma unroll 4
             for (int u = threadIdx.y; u < p.units; u += kColRows) s += src[static_cast<int64_t>(u) * p.cols];
         }
     } else {
-        const int64_t next = item - 4 + 1;  // a unit whose start may cut a gate row
-        const int64_t start = unit_begin(next, p.rows, p.units);
-        const int64_t row = start / p.gate_period;
-        if (start % p.gate_period == 0 || unit_of(row * p.gate_period, p.rows, p.units) != next - 1) return;
+        int64_t row = item - 4, first;
+        if (by_unit) {
+            const int64_t start = unit_begin(item - 4 + 1, p.rows, p.units);
+            row = start / p.gate_period;
+            first = unit_of(row * p.gate_period, p.rows, p.units);
+            if (start % p.gate_period == 0 || first != item - 4) return;
+        } else {
+            first = unit_of(row * p.gate_period, p.rows, p.units);
+        }
         const int64_t last = unit_of((row + 1) * p.gate_period - 1, p.rows, p.units);
+        if (first == last) return;  // one unit held the row and finished it
         out = static_cast<T*>(p.dgate) + row * p.cols;
         if (c < p.cols) {
             const float* src = p.partial + 4 * static_cast<int64_t>(p.units) * p.cols + c;
-            for (int64_t u = next - 1 + threadIdx.y; u <= last; u += kColRows) {
+#pragma unroll 4
+            for (int64_t u = first + threadIdx.y; u <= last; u += kColRows) {
                 const int64_t slot = 2 * u + (unit_begin(u, p.rows, p.units) / p.gate_period == row ? 0 : 1);
                 s += src[slot * p.cols];
             }
@@ -641,6 +770,7 @@ residual_norm_columns_kernel(const RnParams p, T* d0, T* d1, T* d2, T* d3, int c
     __syncthreads();
     if (threadIdx.y == 0 && c < p.cols) {
         s = 0.0f;
+#pragma unroll
         for (int i = 0; i < kColRows; ++i) s += part[i][threadIdx.x];
         out[c] = from_f<T>(s);
     }
@@ -650,18 +780,19 @@ residual_norm_columns_kernel(const RnParams p, T* d0, T* d1, T* d2, T* d3, int c
 
 // NV octets per thread, W warps per row and CTA, CTAs per row: the cover of
 // the row with the least idle columns, more octets per thread where equal
-// (fewer warps to sum over).  NV 3 holds 768 columns in one warp; the
-// backward pass with a post norm or a gate keeps up to five sums per column
-// in registers and stays at 2.  fp32 doubles the bytes of a slot and takes 1.
+// (fewer warps to sum over).  NV 3 holds 768 columns in one warp, NV 4 up to
+// 16384 in one CTA (forward only: the backward pass keeps two to five sums per
+// column in registers).  fp32 doubles the bytes of a slot and takes 1.
 struct Geometry {
     int nv, warps, cluster, groups;
 };
 
-Geometry geometry(const RnParams& p, bool f16, bool vec, bool sums5) {
+Geometry geometry(const RnParams& p, bool f16, bool vec, bool backward, bool sums5) {
     Geometry best = {1, 1, 1, 1};
     int64_t best_cover = INT64_MAX;
-    const int nv_max = f16 ? (sums5 || !vec ? 2 : 3) : 1;
+    const int nv_max = !f16 ? 1 : !vec ? 2 : !backward ? 4 : sums5 ? 2 : 3;
     for (int nv = nv_max; nv >= 1; --nv) {
+        if (nv == 4 && p.cols <= 8192) continue;
         const int64_t per_warp = 256 * nv;
         const int max_warps = nv == 3 ? 8 : kMaxThreads / 32;
         const int64_t need = ceil_div(p.cols, per_warp);
@@ -669,9 +800,9 @@ Geometry geometry(const RnParams& p, bool f16, bool vec, bool sums5) {
         while (cluster * max_warps < need && cluster < kMaxCluster) cluster *= 2;
         const int64_t warps = ceil_div(need, cluster);
         if (warps > max_warps) continue;
-        const int64_t cover = warps * cluster * per_warp;
-        if (cover * (cluster > 1 ? 2 : 1) < best_cover) {
-            best_cover = cover * (cluster > 1 ? 2 : 1);
+        const int64_t cover = warps * cluster * per_warp * (cluster > 1 ? 2 : 1);
+        if (cover < best_cover) {
+            best_cover = cover;
             best = {nv, static_cast<int>(warps), cluster, 1};
         }
     }
@@ -684,6 +815,7 @@ using Kernel = void (*)(RnParams);
 template <typename T, bool VEC>
 Kernel forward_kernel(int nv, bool post) {
     if constexpr (VEC && sizeof(T) == 2) {
+        if (nv == 4) return post ? residual_norm_kernel<T, 4, VEC, true> : residual_norm_kernel<T, 4, VEC, false>;
         if (nv == 3) return post ? residual_norm_kernel<T, 3, VEC, true> : residual_norm_kernel<T, 3, VEC, false>;
     }
     if constexpr (sizeof(T) == 2) {
@@ -768,8 +900,9 @@ int max_units(int device, int64_t rows, const Geometry& g, int per_sm) {
 
 constexpr size_t kSmemPerSm = 220 * 1024;
 
-size_t stage_bytes(const Geometry& g, bool f16, int tensors) {
-    return static_cast<size_t>(g.warps) * 32 * g.groups * g.nv * (f16 ? 16 : 32) * tensors;
+size_t stage_bytes(const Geometry& g, bool f16, bool vec, int tensors) {
+    const size_t row = static_cast<size_t>(g.warps) * 32 * g.nv * (f16 ? 16 : 32);
+    return (row + (vec ? 0 : kTailPad)) * g.groups * tensors;
 }
 
 // The launch's shape and its dynamic shared memory: a ring of three rows per
@@ -779,15 +912,12 @@ size_t configure(RnParams& p, const Geometry& g, bool f16, bool vec, int tensors
     p.cluster = g.cluster;
     p.warps = g.warps;
     p.groups = g.groups;
-    const size_t one = stage_bytes(g, f16, tensors);
+    const size_t one = stage_bytes(g, f16, vec, tensors);
     const size_t fold = backward && g.groups > 1 ? static_cast<size_t>(g.warps) * 32 * g.groups * 8 * g.nv * sizeof(float) : 0;
     const int resident = std::max(1, 512 / (g.warps * 32 * g.groups));  // CTAs that registers admit
-    p.stages = 1;
-    if (vec) {
-        p.stages = 3;
-        while (p.stages > 1 && (red_bytes(g) + p.stages * one + 1024) * resident > kSmemPerSm) --p.stages;
-    }
-    return red_bytes(g) + std::max(vec ? p.stages * one : size_t(0), fold);
+    p.stages = 3;
+    while (p.stages > (vec ? 1 : 2) && (red_bytes(g) + p.stages * one + 1024) * resident > kSmemPerSm) --p.stages;
+    return red_bytes(g) + std::max(p.stages * one, fold);
 }
 
 int launch(Kernel k, const RnParams& p, size_t smem, cudaStream_t s, const char* what) {
@@ -824,10 +954,11 @@ constexpr int kBackwardPerSm = 2;
 template <typename T>
 int columns(const RnParams& p, const tk_residual_norm_grad_desc_t& g, bool gate_items, cudaStream_t s) {
     const int col_blocks = static_cast<int>(ceil_div(p.cols, kColLanes));
-    const int items = 4 + (gate_items ? p.units - 1 : 0);
+    const bool by_unit = gate_items && p.rows / p.gate_period > p.units;
+    const int items = 4 + (!gate_items ? 0 : by_unit ? p.units - 1 : static_cast<int>(p.rows / p.gate_period));
     cudaError_t e = launch_pdl(residual_norm_columns_kernel<T>, dim3(static_cast<unsigned>(items) * col_blocks), dim3(kColLanes, kColRows), 0, s,
                                p, static_cast<T*>(g.dweight), static_cast<T*>(g.dbias), static_cast<T*>(g.dpost_weight),
-                               static_cast<T*>(g.dpost_bias), col_blocks);
+                               static_cast<T*>(g.dpost_bias), col_blocks, by_unit);
     if (e != cudaSuccess) {
         cudaGetLastError();
         TK_FAIL(TK_ERR_CUDA, "residual norm columns launch failed: %s", cudaGetErrorString(e));
@@ -850,7 +981,7 @@ int tk_residual_norm(const tk_residual_norm_desc_t* desc, void* stream) {
     TK_CHECK_ARG(aligned16(d.stats), "tk_residual_norm: stats must be 16-byte aligned");
     RnParams p = params(d);
     const bool f16 = d.dtype == TK_DTYPE_F16, vec = vectorised(p);
-    const Geometry g = geometry(p, f16, vec, false);
+    const Geometry g = geometry(p, f16, vec, false, false);
     const size_t smem = configure(p, g, f16, vec, 2, false);
     const Kernel k = f16 ? (vec ? forward_kernel<__half, true>(g.nv, d.post_norm) : forward_kernel<__half, false>(g.nv, d.post_norm))
                          : (vec ? forward_kernel<float, true>(g.nv, d.post_norm) : forward_kernel<float, false>(g.nv, d.post_norm));
@@ -897,7 +1028,7 @@ int tk_residual_norm_backward(const tk_residual_norm_grad_desc_t* desc, void* wo
     const bool gate = d.gate != nullptr, post = d.post_norm != 0;
     if (!gate && !post) p.f = nullptr;
     const bool vec = vectorised(p);
-    const Geometry g = geometry(p, f16, vec, gate || post);
+    const Geometry g = geometry(p, f16, vec, true, gate || post);
     const size_t smem = configure(p, g, f16, vec, gate || post ? 4 : 3, true);
     const Kernel k = f16 ? (vec ? backward_kernel<__half, true>(g.nv, post, gate) : backward_kernel<__half, false>(g.nv, post, gate))
                          : (vec ? backward_kernel<float, true>(g.nv, post, gate) : backward_kernel<float, false>(g.nv, post, gate));

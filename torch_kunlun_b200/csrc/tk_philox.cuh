@@ -67,6 +67,16 @@ __device__ __forceinline__ uint32_t dropout_keep8(const DropoutParams& d, uint64
     return d.none_kept ? 0u : m;
 }
 
+// Keep bits of the 4 elements of one block.
+__device__ __forceinline__ uint32_t dropout_keep4(const DropoutParams& d, uint64_t block) {
+    uint32_t w[4];
+    philox4x32_10(block, d.offset, d.seed, w);
+    uint32_t m = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) m |= (w[j] >= d.threshold ? 1u : 0u) << j;
+    return d.none_kept ? 0u : m;
+}
+
 __device__ __forceinline__ bool dropout_keep1(const DropoutParams& d, uint64_t i) {
     uint32_t w[4];
     philox4x32_10(i >> 2, d.offset, d.seed, w);
