@@ -8,8 +8,8 @@
 // lists the others, their rows of x are packed, and every later kernel takes
 // its row count from that list on the device.
 //
-// Forward: one tcgen05 GEMM whose epilogue keeps, per row and 128 columns,
-// the maximum and the sum of exponentials (base 2); a small kernel joins them
+// Forward: one tcgen05 GEMM whose epilogue keeps, per row and 64 or 128
+// columns, the maximum and the sum of exponentials (base 2); a small kernel joins them
 // and computes the target's logit as a dot product of its own.  Backward: the
 // vocabulary is taken in pieces whose dz fits a workspace; per piece the
 // logits are computed again, the epilogue stores dz as binary16, and two
@@ -26,13 +26,13 @@
 // 2^15)), 22 bits or 2^-40 of the largest value, and a product is the sum
 // hi*hi + hi*lo + lo*hi: the K loop runs over three pairs of planes.
 //
-// GEMM kernel (persistent pairs of CTAs, one CTA per SM, 320 threads each):
+// GEMM kernel (persistent pairs of CTAs, one CTA per SM):
 // a pair computes 256 x 256 tiles, CTA r holding rows [128 r, + 128) of A and
 // of B in shared memory and of the result in TMEM, so each SM loads 32 KB per
 // 64 K values of a 256 x 256 tile.  Warp 0 of both CTAs loads its halves by
 // TMA (128-byte swizzle) onto the leader's barriers, warp 1 of the leader
 // issues tcgen05.mma cta_group::2 kind::f16 into two 256-column accumulators,
-// warps 2..9 of both CTAs run the epilogue of one while the other fills.
+// the other warps of both CTAs run the epilogue of one while the other fills.
 //
 // The tensor core adds each 16-deep step into a binary32 accumulator that it
 // cuts rather than rounds, a bias that grows with K.  Where outputs are
@@ -51,19 +51,26 @@ namespace {
 
 constexpr int BM = 256, BN = 256, BK = 64;     // a pair's tile
 constexpr int HM = BM / 2, HN = BN / 2;          // one CTA's operand rows
-constexpr int STAGES = 5;
 constexpr int A_BYTES = HM * BK * 2, B_BYTES = HN * BK * 2;
 constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
-constexpr int EPI_WARPS = 8;
-constexpr int THREADS = 64 + 32 * EPI_WARPS;
-// An epilogue warp turns 32 rows x 32 columns through its own 4.5 KB, so that
-// eight lanes store 128 consecutive bytes of a row (144-byte pitch: no bank
-// conflicts for 16-byte accesses).
-constexpr int PITCH = 36;
-constexpr int TURN_BYTES = EPI_WARPS * 32 * PITCH * 4;
-constexpr int GEMM_SMEM = STAGES * STAGE_BYTES + TURN_BYTES + 1024 + 256;
+// An epilogue warp turns 32 rows x 16 columns through its own 2.5 KB, so that
+// four lanes store whole sectors of a row (80-byte pitch: no bank conflicts for
+// 16-byte accesses).
+constexpr int TURN = 16;
+constexpr int PITCH = TURN + 4;
+// Sixteen epilogue warps keep up with short K loops; sums in registers (128
+// columns per thread) leave room for eight.
+template <bool CHUNKED>
+struct Config {
+    static constexpr int STAGES = CHUNKED ? 6 : 5;
+    static constexpr int EPI_WARPS = CHUNKED ? 8 : 16;
+    static constexpr int COLS = BN / (EPI_WARPS / 4);  // of a tile row, per warp
+    static constexpr int THREADS = 64 + 32 * EPI_WARPS;
+    static constexpr int TURN_BYTES = EPI_WARPS * 32 * PITCH * 4;
+    static constexpr int SMEM = STAGES * STAGE_BYTES + TURN_BYTES + 1024 + 256;
+    static_assert(SMEM <= 232448, "shared memory budget");
+};
 constexpr int TMEM_COLS = 512;
-static_assert(GEMM_SMEM <= 232448, "shared memory budget");
 
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kDzScale = 16384.0f;
@@ -94,8 +101,7 @@ struct GemmParams {
     unsigned* err;
     // kStats / kDlogits
     const float* bias2;  // bias * log2(e), or NULL
-    float2* part;           // [2 * n_tiles][rows_pad] maximum and sum
-    int64_t rows_pad;
+    float2* part;           // [rows][n_tiles][warps per tile row] maximum and sum
     const float* lse2;
     const float* grow;   // g_i / max |g|
     const int* target;
@@ -270,60 +276,69 @@ __device__ __forceinline__ void join(float& m, float& s, float m2, float s2) {
     m = top;
 }
 
-// The 32 x 32 block that the warp's lanes hold by rows (v: this lane's row),
-// handed out by columns: f(row, column, four values), eight lanes per row.
+// The 32 x 16 block that the warp's lanes hold by rows (v: this lane's row) in
+// shared memory, for its lanes to read by columns.
+__device__ __forceinline__ void turn_in(float* buf, int lane, const float* v) {
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < TURN; i += 4) *reinterpret_cast<float4*>(buf + lane * PITCH + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+    __syncwarp();
+}
+// Hands the block out as f(row, column, four values), four lanes per row.
 template <typename F>
-__device__ __forceinline__ void turn(float* buf, int lane, const float* v, F f) {
-    __syncwarp();
+__device__ __forceinline__ void turn_out4(const float* buf, int lane, F f) {
 #pragma unroll
-    for (int i = 0; i < 32; i += 4) *reinterpret_cast<float4*>(buf + lane * PITCH + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
-    __syncwarp();
-#pragma unroll
-    for (int r = 0; r < 32; r += 4) {
-        const int row = r + lane / 8, col = lane % 8 * 4;
+    for (int r = 0; r < 32; r += 8) {
+        const int row = r + lane / 4, col = lane % 4 * 4;
         f(row, col, *reinterpret_cast<const float4*>(buf + row * PITCH + col));
     }
 }
+// Hands it out as f(row, column, value), 16 lanes per row.
+template <typename F>
+__device__ __forceinline__ void turn_out1(const float* buf, int lane, F f) {
+#pragma unroll 4
+    for (int r = 0; r < 32; r += 2) f(r + lane / 16, lane % 16, buf[(r + lane / 16) * PITCH + lane % 16]);
+}
 
-// Four finished values of a gradient: joined with the earlier pieces' sum,
-// kept for the next piece, or scaled, rounded and stored.
-template <int EPI>
-__device__ __forceinline__ void finish4(const GemmParams& p, int64_t m, int64_t rows, int64_t col, float scale, float4 f) {
+// N (four or one) finished values of a gradient: joined with the
+// earlier pieces' sum, kept for the next piece, or scaled, rounded and stored.
+template <int EPI, int N>
+__device__ __forceinline__ void finish(const GemmParams& p, int64_t m, int64_t rows, int64_t col, float scale, float4 f) {
     if (m >= rows || col >= p.out_cols) return;
     float v[4] = {f.x, f.y, f.z, f.w};
-    const bool four = col + 4 <= p.out_cols;
     if (EPI == kGradX && !(p.first && p.last)) {
-        // rows of the sum are a multiple of four columns apart
-        float4* a = reinterpret_cast<float4*>(p.acc + m * p.acc_ld + col);
+        float* a = p.acc + m * p.acc_ld + col;  // acc_ld is a multiple of four
         if (!p.first) {
-            const float4 e = *a;
-            v[0] += e.x, v[1] += e.y, v[2] += e.z, v[3] += e.w;
+            if constexpr (N == 4) {
+                const float4 e = *reinterpret_cast<const float4*>(a);
+                v[0] += e.x, v[1] += e.y, v[2] += e.z, v[3] += e.w;
+            } else {
+                v[0] += *a;
+            }
         }
         if (!p.last) {
-            *a = make_float4(v[0], v[1], v[2], v[3]);
+            if constexpr (N == 4) {
+                *reinterpret_cast<float4*>(a) = make_float4(v[0], v[1], v[2], v[3]);
+            } else {
+                *a = v[0];
+            }
             return;
         }
     }
     const int64_t at = (EPI == kGradX ? p.index[m] : m) * p.out_cols + col;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] *= scale;
-    if (p.out_f32) {
-        float* o = static_cast<float*>(p.out) + at;
-        if (p.out_vec && four) {
-            *reinterpret_cast<float4*>(o) = make_float4(v[0], v[1], v[2], v[3]);
+    for (int i = 0; i < N; ++i) v[i] *= scale;
+    if constexpr (N == 4) {  // out_cols a multiple of 16 bytes, out 16-byte aligned
+        if (p.out_f32) {
+            *reinterpret_cast<float4*>(static_cast<float*>(p.out) + at) = make_float4(v[0], v[1], v[2], v[3]);
         } else {
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (col + i < p.out_cols) o[i] = v[i];
+            *reinterpret_cast<uint2*>(static_cast<__half*>(p.out) + at) = make_uint2(half2_bits(v[0], v[1]), half2_bits(v[2], v[3]));
         }
     } else {
-        __half* o = static_cast<__half*>(p.out) + at;
-        if (p.out_vec && four) {
-            *reinterpret_cast<uint2*>(o) = make_uint2(half2_bits(v[0], v[1]), half2_bits(v[2], v[3]));
+        if (p.out_f32) {
+            static_cast<float*>(p.out)[at] = v[0];
         } else {
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (col + i < p.out_cols) o[i] = __float2half_rn(v[i]);
+            static_cast<__half*>(p.out)[at] = __float2half_rn(v[0]);
         }
     }
 }
@@ -336,14 +351,16 @@ __device__ __forceinline__ float z_scale(const GemmParams& p) {
 // CHUNKED: the epilogue adds chunks of the K loop in registers (128 columns
 // of a row per thread).
 template <int EPI, bool CHUNKED>
-__global__ void __launch_bounds__(THREADS, 1)
+__global__ void __launch_bounds__(Config<CHUNKED>::THREADS, 1)
 ce_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const GemmParams p) {
     constexpr bool A_MN = EPI == kGradW, B_MN = EPI == kGradX || EPI == kGradW;
     constexpr uint32_t IDESC = idesc_f16(BM, BN, A_MN, B_MN);
+    using C = Config<CHUNKED>;
+    constexpr int STAGES = C::STAGES, EPI_WARPS = C::EPI_WARPS, COLS = C::COLS;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
     float* turn_buf = reinterpret_cast<float*>(smem + STAGES * STAGE_BYTES);
-    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + STAGES * STAGE_BYTES + TURN_BYTES);
+    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + STAGES * STAGE_BYTES + C::TURN_BYTES);
     uint64_t* full_bar = bars;               // [STAGES] both CTAs' TMA -> MMA (leader's)
     uint64_t* empty_bar = bars + STAGES;     // [STAGES] MMA -> TMA (each CTA's)
     uint64_t* acc_full = bars + 2 * STAGES;  // [2] MMA -> epilogue (each CTA's)
@@ -499,10 +516,10 @@ ce_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
             mbar_wait_bounded(smem_u32(drain_bar), 0, &no_abort, p.err, kDevErrWaitDrain);
         }
     } else {
-        // ---------------- epilogue (warps 2..9 of both CTAs) ----------------
+        // ---------------- epilogue (the other warps of both CTAs) ----------------
         // A warp reads TMEM lanes [32 * (warp % 4), + 32), one row per lane,
-        // and half of the tile's columns.
-        const int quarter = warp & 3, half = (warp - 2) >> 2;
+        // and COLS of the tile's columns.
+        const int quarter = warp & 3, share = (warp - 2) >> 2;
         float* const buf_turn = turn_buf + (warp - 2) * 32 * PITCH;
         const int rows = p.sc->count;
         float scale = 1.0f;
@@ -517,12 +534,15 @@ ce_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
             const int blocks = split_begin(sh, ks + 1) - split_begin(sh, ks);
             const int64_t m0 = static_cast<int64_t>(mt) * BM + rank * HM + quarter * 32;  // the warp's first row
             const int64_t m = m0 + lane;
-            const int64_t col0 = static_cast<int64_t>(nt) * BN + half * (BN / 2);
+            const int64_t col0 = static_cast<int64_t>(nt) * BN + share * COLS;
             float top = -INFINITY, sum = 0.0f;  // kStats
             const bool live = m < rows;         // kDlogits
             const float lse = EPI == kDlogits && live ? p.lse2[m] : 0.0f;
             const float g = EPI == kDlogits && live ? p.grow[m] * kDzScale : 0.0f;
             const int64_t hit = EPI == kDlogits && live ? p.target[m] - p.vocab0 : -1;
+            // rows that the warp works for: dz is read (as K) up to a multiple of BK
+            const int64_t limit = EPI == kGradW ? p.out_rows : EPI == kDlogits ? (rows + BK - 1) / BK * BK : rows;
+            const bool idle = m0 >= limit;
             // 32 columns of this lane's row, from column col0 + c of the tile
             auto take = [&](int c, const float* acc) {
                 const int64_t col = col0 + c;
@@ -547,32 +567,43 @@ ce_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
 #pragma unroll
                         for (int i = 0; i < 32; ++i) y[i] -= i == j ? g : 0.0f;
                     }
-                    turn(buf_turn, lane, y, [&](int r, int cc, float4 f) {
-                        __half* o = p.dz + (m0 + r) * p.dz_ld + col + cc;
-                        const uint2 hi = make_uint2(half2_bits(f.x, f.y), half2_bits(f.z, f.w));
-                        *reinterpret_cast<uint2*>(o) = hi;
-                        if (p.dz_plane != 0) {
-                            const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&hi.x));
-                            const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&hi.y));
-                            *reinterpret_cast<uint2*>(o + p.dz_plane) = make_uint2(half2_bits(f.x - a.x, f.y - a.y), half2_bits(f.z - b.x, f.w - b.y));
-                        }
-                    });
+#pragma unroll
+                    for (int h = 0; h < 32; h += TURN) {
+                        turn_in(buf_turn, lane, y + h);
+                        turn_out4(buf_turn, lane, [&](int r, int cc, float4 f) {
+                            __half* o = p.dz + (m0 + r) * p.dz_ld + col + h + cc;
+                            const uint2 hi = make_uint2(half2_bits(f.x, f.y), half2_bits(f.z, f.w));
+                            *reinterpret_cast<uint2*>(o) = hi;
+                            if (p.dz_plane != 0) {
+                                const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&hi.x));
+                                const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&hi.y));
+                                *reinterpret_cast<uint2*>(o + p.dz_plane) = make_uint2(half2_bits(f.x - a.x, f.y - a.y), half2_bits(f.z - b.x, f.w - b.y));
+                            }
+                        });
+                    }
                 } else {
-                    const int64_t limit = EPI == kGradX ? rows : p.out_rows;
-                    turn(buf_turn, lane, acc, [&](int r, int cc, float4 f) {
+#pragma unroll
+                    for (int h = 0; h < 32; h += TURN) {
+                        turn_in(buf_turn, lane, acc + h);
                         if (sh.splits > 1) {
-                            *reinterpret_cast<float4*>(p.split + (static_cast<int64_t>(u) * BM + rank * HM + quarter * 32 + r) * BN + half * (BN / 2) + c + cc) = f;
+                            turn_out4(buf_turn, lane, [&](int r, int cc, float4 f) {
+                                *reinterpret_cast<float4*>(p.split + (static_cast<int64_t>(u) * BM + rank * HM + quarter * 32 + r) * BN + share * COLS + c + h + cc) = f;
+                            });
+                        } else if (p.out_vec) {
+                            turn_out4(buf_turn, lane, [&](int r, int cc, float4 f) { finish<EPI, 4>(p, m0 + r, limit, col + h + cc, scale, f); });
                         } else {
-                            finish4<EPI>(p, m0 + r, limit, col + cc, scale, f);
+                            turn_out1(buf_turn, lane, [&](int r, int cc, float f) {
+                                finish<EPI, 1>(p, m0 + r, limit, col + h + cc, scale, make_float4(f, 0.0f, 0.0f, 0.0f));
+                            });
                         }
-                    });
+                    }
                 }
             };
             const int chunks = CHUNKED ? max(1, (blocks + p.chunk - 1) / p.chunk) : 1;
-            float v[CHUNKED ? BN / 2 : 32];
+            float v[CHUNKED ? COLS : 32];
             if constexpr (CHUNKED) {
 #pragma unroll
-                for (int i = 0; i < BN / 2; ++i) v[i] = 0.0f;
+                for (int i = 0; i < COLS; ++i) v[i] = 0.0f;
             }
             for (int k = 0; k < chunks; ++k, ++local) {
                 const int buf = local & 1;
@@ -581,10 +612,11 @@ ce_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
                     break;
                 }
                 tc_fence_after();
-                const uint32_t t0 = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + buf * BN + half * (BN / 2);
-                if constexpr (CHUNKED) {
+                const uint32_t t0 = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + buf * BN + share * COLS;
+                if (idle) {
+                } else if constexpr (CHUNKED) {
 #pragma unroll
-                    for (int c = 0; c < BN / 2; c += 32) {
+                    for (int c = 0; c < COLS; c += 32) {
                         uint32_t acc[32];
                         tmem_ld_32x32b_x32(t0 + c, acc);
                         tc_wait_ld();
@@ -593,7 +625,7 @@ ce_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
                     }
                 } else {
 #pragma unroll 1
-                    for (int c = 0; c < BN / 2; c += 32) {
+                    for (int c = 0; c < COLS; c += 32) {
                         uint32_t acc[32];
                         tmem_ld_32x32b_x32(t0 + c, acc);
                         tc_wait_ld();
@@ -607,11 +639,12 @@ ce_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
                 if (lane == 0) mbar_arrive_remote(mapa_shared(smem_u32(acc_empty + buf), 0));
             }
             if (!ok) break;
+            if (idle) continue;
             if constexpr (CHUNKED) {
 #pragma unroll
-                for (int c = 0; c < BN / 2; c += 32) take(c, v + c);
+                for (int c = 0; c < COLS; c += 32) take(c, v + c);
             }
-            if constexpr (EPI == kStats) p.part[(static_cast<int64_t>(nt) * 2 + half) * p.rows_pad + m] = make_float2(top, sum);
+            if constexpr (EPI == kStats) p.part[(m * p.n_tiles + nt) * (BN / COLS) + share] = make_float2(top, sum);
         }
     }
     tc_fence_before();
@@ -621,30 +654,52 @@ ce_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
     if (warp == 1) tmem_dealloc_pair(tmem_base, TMEM_COLS);
 }
 
-// Adds the K splits of the tiles in their order, four rows of a tile per block
-// of 256 threads, four columns per thread.
+// Adds the K splits of the tiles in a fixed order, 64 threads by four columns
+// to a row.  Few tiles have many splits: the block's four groups of 64 share
+// those of one row; otherwise each takes a row of its own.
 template <int EPI>
 __global__ void __launch_bounds__(256) ce_split_kernel(const GemmParams p) {
     pdl_wait();
+    __shared__ float4 part[4][64];
     const Shape sh = shape_of<EPI>(p);
     if (sh.splits <= 1) return;
     const int tiles = sh.m_tiles * p.n_tiles;
     const int64_t limit = EPI == kGradX ? p.sc->count : p.out_rows;
     const float scale = EPI == kGradX ? p.sc->dx_scale : p.sc->dw_scale;
-    for (int b = blockIdx.x; b < tiles * (BM / 4); b += gridDim.x) {
-        const int tile = b / (BM / 4);
-        const int row = b % (BM / 4) * 4 + static_cast<int>(threadIdx.x) / 64;
-        const int c = static_cast<int>(threadIdx.x % 64) * 4;
+    const int quad = threadIdx.x % 64, group = threadIdx.x / 64;
+    const int shares = sh.splits >= 16 ? 4 : 1, rows = 4 / shares;
+    const int share = shares == 4 ? group : 0;
+    const int k0 = share * sh.splits / shares, k1 = (share + 1) * sh.splits / shares;
+    for (int b = blockIdx.x; b < tiles * (BM / rows); b += gridDim.x) {
+        const int tile = b / (BM / rows), row = b % (BM / rows) * rows + (shares == 4 ? 0 : group);
         int mt, nt, ks;
         decode_unit(p, sh, tile, mt, nt, ks);
-        const int64_t m = static_cast<int64_t>(mt) * BM + row, col = static_cast<int64_t>(nt) * BN + c;
-        if (m >= limit || col >= p.out_cols) continue;
+        const int64_t m = static_cast<int64_t>(mt) * BM + row, col = static_cast<int64_t>(nt) * BN + quad * 4;
         float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        for (int k = 0; k < sh.splits; ++k) {
-            const float4 f = *reinterpret_cast<const float4*>(p.split + ((static_cast<int64_t>(k) * tiles + tile) * BM + row) * BN + c);
-            v.x += f.x, v.y += f.y, v.z += f.z, v.w += f.w;
+        if (m < limit) {
+#pragma unroll 4
+            for (int k = k0; k < k1; ++k) {
+                const float4 f = *reinterpret_cast<const float4*>(p.split + ((static_cast<int64_t>(k) * tiles + tile) * BM + row) * BN + quad * 4);
+                v.x += f.x, v.y += f.y, v.z += f.z, v.w += f.w;
+            }
         }
-        finish4<EPI>(p, m, limit, col, scale, v);
+        if (shares == 4) {
+            part[share][quad] = v;
+            __syncthreads();
+#pragma unroll
+            for (int i = 1; i < 4; ++i)
+                if (share == 0) v.x += part[i][quad].x, v.y += part[i][quad].y, v.z += part[i][quad].z, v.w += part[i][quad].w;
+            __syncthreads();
+        }
+        if (share != 0) continue;
+        if (p.out_vec) {
+            finish<EPI, 4>(p, m, limit, col, scale, v);
+        } else {
+            finish<EPI, 1>(p, m, limit, col, scale, make_float4(v.x, 0.0f, 0.0f, 0.0f));
+            finish<EPI, 1>(p, m, limit, col + 1, scale, make_float4(v.y, 0.0f, 0.0f, 0.0f));
+            finish<EPI, 1>(p, m, limit, col + 2, scale, make_float4(v.z, 0.0f, 0.0f, 0.0f));
+            finish<EPI, 1>(p, m, limit, col + 3, scale, make_float4(v.w, 0.0f, 0.0f, 0.0f));
+        }
     }
 }
 
@@ -653,41 +708,58 @@ __global__ void __launch_bounds__(256) ce_split_kernel(const GemmParams p) {
 __device__ __forceinline__ float load_f(const __half* p, int64_t i) { return __half2float(p[i]); }
 __device__ __forceinline__ float load_f(const float* p, int64_t i) { return p[i]; }
 
-constexpr int kIndexThreads = 1024;
+constexpr int kIndexThreads = 1024, kIndexRows = 8;  // rows per thread and step
 
 // Lists the rows that have a target (in order), their targets, and their
 // count; writes the ignored rows' losses (0) where there is one per row.
 __global__ void __launch_bounds__(kIndexThreads)
 ce_index_kernel(const int64_t* target, int64_t rows, int64_t vocab, int64_t ignore, int* index, int* packed_target, Scalars* sc,
                 float* row_loss_out) {
-    __shared__ int warp_sum[32];
+    __shared__ int before[kIndexRows][32];  // listed rows of a step before each warp's
     __shared__ int total;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     int base = 0;
-    for (int64_t r0 = 0; r0 < rows; r0 += kIndexThreads) {
-        const int64_t r = r0 + threadIdx.x;
-        const int64_t t = r < rows ? target[r] : ignore;
-        const bool used = r < rows && t != ignore;
-        const unsigned ballot = __ballot_sync(0xFFFFFFFFu, used);
-        if (lane == 0) warp_sum[warp] = __popc(ballot);
-        __syncthreads();
-        if (warp == 0) {
-            int v = warp_sum[lane], s = v;
+    for (int64_t r0 = 0; r0 < rows; r0 += kIndexThreads * kIndexRows) {
+        int64_t t[kIndexRows];
+        unsigned used[kIndexRows];
 #pragma unroll
-            for (int d = 1; d < 32; d <<= 1) {
-                const int o = __shfl_up_sync(0xFFFFFFFFu, s, d);
-                if (lane >= d) s += o;
-            }
-            warp_sum[lane] = s - v;
-            if (lane == 31) total = s;
+        for (int k = 0; k < kIndexRows; ++k) {
+            const int64_t r = r0 + k * kIndexThreads + threadIdx.x;
+            t[k] = r < rows ? target[r] : ignore;
+        }
+#pragma unroll
+        for (int k = 0; k < kIndexRows; ++k) {
+            used[k] = __ballot_sync(0xFFFFFFFFu, t[k] != ignore);
+            if (lane == 0) before[k][warp] = __popc(used[k]);
         }
         __syncthreads();
-        if (used) {
-            const int at = base + warp_sum[warp] + __popc(ballot & ((1u << lane) - 1u));
-            index[at] = static_cast<int>(r);
-            packed_target[at] = t >= 0 && t < vocab ? static_cast<int>(t) : -1;  // -1: the loss is NaN
-        } else if (r < rows && row_loss_out != nullptr) {
-            row_loss_out[r] = 0.0f;
+        if (warp == 0) {
+            int sum = 0;
+#pragma unroll
+            for (int k = 0; k < kIndexRows; ++k) {
+                const int v = before[k][lane];
+                int s = v;
+#pragma unroll
+                for (int d = 1; d < 32; d <<= 1) {
+                    const int o = __shfl_up_sync(0xFFFFFFFFu, s, d);
+                    if (lane >= d) s += o;
+                }
+                before[k][lane] = sum + s - v;
+                sum += __shfl_sync(0xFFFFFFFFu, s, 31);
+            }
+            if (lane == 0) total = sum;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < kIndexRows; ++k) {
+            const int64_t r = r0 + k * kIndexThreads + threadIdx.x;
+            if ((used[k] >> lane) & 1u) {
+                const int at = base + before[k][warp] + __popc(used[k] & ((1u << lane) - 1u));
+                index[at] = static_cast<int>(r);
+                packed_target[at] = t[k] >= 0 && t[k] < vocab ? static_cast<int>(t[k]) : -1;  // -1: the loss is NaN
+            } else if (r < rows && row_loss_out != nullptr) {
+                row_loss_out[r] = 0.0f;
+            }
         }
         base += total;
         __syncthreads();
@@ -700,18 +772,47 @@ ce_index_kernel(const int64_t* target, int64_t rows, int64_t vocab, int64_t igno
     }
 }
 
+__device__ __forceinline__ unsigned finite_magnitude(float v) {
+    const unsigned b = __float_as_uint(v) & 0x7FFFFFFFu;
+    return b < 0x7F800000u ? b : 0u;
+}
+
+// Largest finite |v| of n consecutive values, shared out over `of` blocks.
+__device__ __forceinline__ unsigned amax_span(const float* p, int64_t n, int64_t block, int64_t of) {
+    unsigned top = 0;
+    const int64_t head = min(n, static_cast<int64_t>((16 - (reinterpret_cast<uintptr_t>(p) & 15)) / 4 % 4));  // up to a 16-byte boundary
+    const int64_t quads = (n - head) / 4, tail = head + quads * 4;
+    if (block == 0) {
+        if (threadIdx.x < head) top = finite_magnitude(p[threadIdx.x]);
+        if (tail + threadIdx.x < n) top = max(top, finite_magnitude(p[tail + threadIdx.x]));
+    }
+    const float4* q = reinterpret_cast<const float4*>(p + head);
+    const int64_t step = of * blockDim.x;
+    int64_t i = block * blockDim.x + threadIdx.x;
+    for (; i + 3 * step < quads; i += 4 * step) {
+        float4 f[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) f[k] = __ldg(q + i + k * step);
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            top = max(max(top, max(finite_magnitude(f[k].x), finite_magnitude(f[k].y))), max(finite_magnitude(f[k].z), finite_magnitude(f[k].w)));
+    }
+    for (; i < quads; i += step) {
+        const float4 f = __ldg(q + i);
+        top = max(max(top, max(finite_magnitude(f.x), finite_magnitude(f.y))), max(finite_magnitude(f.z), finite_magnitude(f.w)));
+    }
+    return top;
+}
+
 // Largest finite |v| of x's listed rows (blockIdx.y 0) and of W (1).
 __global__ void __launch_bounds__(256) ce_amax_kernel(const float* x, const float* w, const int* index, Scalars* sc, int64_t cols, int64_t vocab) {
     pdl_wait();
     const bool is_w = blockIdx.y == 1;
-    const int64_t rows = is_w ? vocab : sc->count;
     unsigned top = 0;
-    for (int64_t r = blockIdx.x; r < rows; r += gridDim.x) {
-        const float* src = is_w ? w + r * cols : x + static_cast<int64_t>(index[r]) * cols;
-        for (int64_t c = threadIdx.x; c < cols; c += 256) {
-            const unsigned b = __float_as_uint(src[c]) & 0x7FFFFFFFu;
-            if (b < 0x7F800000u) top = max(top, b);
-        }
+    if (is_w) {
+        top = amax_span(w, vocab * cols, blockIdx.x, gridDim.x);
+    } else {
+        for (int64_t r = blockIdx.x; r < sc->count; r += gridDim.x) top = max(top, amax_span(x + static_cast<int64_t>(index[r]) * cols, cols, 0, 1));
     }
     top = __reduce_max_sync(0xFFFFFFFFu, top);
     if ((threadIdx.x & 31) == 0 && top != 0) atomicMax(is_w ? &sc->amax_w : &sc->amax_x, top);
@@ -831,82 +932,85 @@ ce_pack_kernel(const PackJob<T> x, const PackJob<T> w, const Scalars* sc, int x_
     }
 }
 
-__device__ __forceinline__ float warp_add(float v) {
+// This lane's part of the dot product of two rows, in one order however the
+// rows are aligned.
+template <typename T>
+__device__ __forceinline__ float dot_lane(const T* a, const T* b, int64_t n, int lane, bool vec) {
+    constexpr int V = 16 / sizeof(T);
+    float s[4] = {};
+#pragma unroll 4
+    for (int64_t c = lane * V; c < n; c += 32 * V) {
+        alignas(16) T x[V];
+        alignas(16) T y[V];
+        if (vec) {  // both rows 16-byte aligned, n a multiple of V
+            *reinterpret_cast<uint4*>(x) = *reinterpret_cast<const uint4*>(a + c);
+            *reinterpret_cast<uint4*>(y) = *reinterpret_cast<const uint4*>(b + c);
+        } else {
 #pragma unroll
-    for (int m = 16; m > 0; m >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, m);
-    return v;
+            for (int i = 0; i < V; ++i) {
+                x[i] = c + i < n ? a[c + i] : T(0.0f);
+                y[i] = c + i < n ? b[c + i] : T(0.0f);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < V; ++i) s[i % 4] = fmaf(load_f(x, i), load_f(y, i), s[i % 4]);
+    }
+    return (s[0] + s[1]) + (s[2] + s[3]);
 }
 
-constexpr int kRowLanes = 32, kRowSlices = 16;
+constexpr int kRowWarps = 8;
 
-// Joins the statistics of 32 rows and forms their losses: lse2 (base 2) for
-// the backward pass, the loss per packed row, and per row where asked for.  The
-// block that finishes last adds the losses of all rows, in their order.
+// A warp joins the statistics of a row, computes its target's logit and forms
+// its loss: lse2 (base 2) for the backward pass, the loss per packed row, and
+// per row where asked for.  The block that finishes last adds the losses of
+// all rows, in a fixed order.
 template <typename T>
-__global__ void __launch_bounds__(kRowLanes* kRowSlices)
+__global__ void __launch_bounds__(32 * kRowWarps)
 ce_rows_kernel(const T* x, const T* w, const T* bias, const int* index, const int* target, Scalars* sc, const float2* part,
-               int parts, int64_t rows_pad, int64_t cols, float* lse2, float* loss, int reduction, float* out) {
+               int parts, int64_t cols, bool vec, float* lse2, float* loss, int reduction, float* out) {
     pdl_wait();
-    __shared__ float2 stat[kRowSlices][kRowLanes];
-    __shared__ float hit[kRowLanes];
     const int rows = sc->count;
-    const int lane = threadIdx.x, slice = threadIdx.y;
-    for (int r0 = blockIdx.x * kRowLanes; r0 < rows; r0 += gridDim.x * kRowLanes) {
-        const int m = r0 + lane;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    for (int m = blockIdx.x * kRowWarps + warp; m < rows; m += gridDim.x * kRowWarps) {
+        const int t = target[m], r = index[m];
         float top = -INFINITY, sum = 0.0f;
-        for (int i = slice; i < parts; i += kRowSlices) {
-            const float2 v = part[static_cast<int64_t>(i) * rows_pad + m];
-            join(top, sum, v.x, v.y);
+        const float2* row = part + static_cast<int64_t>(m) * parts;
+#pragma unroll 4
+        for (int i = lane; i < parts; i += 32) join(top, sum, row[i].x, row[i].y);
+        float hit = t >= 0 ? dot_lane(x + r * cols, w + t * cols, cols, lane, vec) : 0.0f;
+#pragma unroll
+        for (int k = 16; k > 0; k >>= 1) {
+            join(top, sum, __shfl_xor_sync(0xFFFFFFFFu, top, k), __shfl_xor_sync(0xFFFFFFFFu, sum, k));
+            hit += __shfl_xor_sync(0xFFFFFFFFu, hit, k);
         }
-        stat[slice][lane] = make_float2(top, sum);
-        for (int k = slice; k < kRowLanes; k += kRowSlices) {  // a warp takes one row's target logit
-            const int r = r0 + k;
-            const int t = r < rows ? target[r] : -1;
-            float dot = 0.0f;
-            if (t >= 0) {
-                const T* xr = x + static_cast<int64_t>(index[r]) * cols;
-                const T* wr = w + static_cast<int64_t>(t) * cols;
-                float d2 = 0.0f;
-                int64_t c = lane;
-                for (; c + 32 < cols; c += 64) {
-                    dot = fmaf(load_f(xr, c), load_f(wr, c), dot);
-                    d2 = fmaf(load_f(xr, c + 32), load_f(wr, c + 32), d2);
-                }
-                if (c < cols) dot = fmaf(load_f(xr, c), load_f(wr, c), dot);
-                dot = warp_add(dot + d2);
-                if (bias != nullptr) dot += load_f(bias, t);
-            }
-            if (lane == 0) hit[k] = t >= 0 ? dot : NAN;
-        }
-        __syncthreads();
-        if (slice == 0 && m < rows) {
-            for (int i = 1; i < kRowSlices; ++i) join(top, sum, stat[i][lane].x, stat[i][lane].y);
+        if (lane == 0) {
+            if (bias != nullptr && t >= 0) hit += load_f(bias, t);
             const float l2 = top + log2f(sum);
-            const float v = l2 * kLn2 - hit[lane];
-            lse2[m] = target[m] >= 0 ? l2 : NAN;
+            const float v = t >= 0 ? l2 * kLn2 - hit : NAN;
+            lse2[m] = t >= 0 ? l2 : NAN;
             loss[m] = v;
-            if (reduction == TK_REDUCE_NONE) out[index[m]] = v;
+            if (reduction == TK_REDUCE_NONE) out[r] = v;
         }
-        __syncthreads();
     }
     if (reduction == TK_REDUCE_NONE) return;
     __shared__ bool last;
-    __shared__ double total[kRowSlices];
+    __shared__ double total[kRowWarps];
     __threadfence();
     __syncthreads();
-    if (lane == 0 && slice == 0) last = atomicAdd(&sc->rows_done, 1u) == gridDim.x - 1;
+    if (threadIdx.x == 0) last = atomicAdd(&sc->rows_done, 1u) == gridDim.x - 1;
     __syncthreads();
     if (!last) return;
     __threadfence();
     double s = 0.0;
-    for (int i = slice * kRowLanes + lane; i < rows; i += kRowLanes * kRowSlices) s += __ldcg(loss + i);
+#pragma unroll 4
+    for (int i = threadIdx.x; i < rows; i += 32 * kRowWarps) s += __ldcg(loss + i);
 #pragma unroll
     for (int k = 16; k > 0; k >>= 1) s += __shfl_xor_sync(0xFFFFFFFFu, s, k);
-    if (lane == 0) total[slice] = s;
+    if (lane == 0) total[warp] = s;
     __syncthreads();
-    if (lane == 0 && slice == 0) {
+    if (threadIdx.x == 0) {
         s = 0.0;
-        for (int i = 0; i < kRowSlices; ++i) s += total[i];
+        for (int i = 0; i < kRowWarps; ++i) s += total[i];
         *out = static_cast<float>(reduction == TK_REDUCE_MEAN ? s / rows : s);  // no rows: 0 / 0, as torch's mean
     }
 }
@@ -968,18 +1072,24 @@ ce_dbias_part_kernel(const __half* dz, int64_t dz_ld, int64_t dz_plane, const Sc
     const int lo = static_cast<int>(static_cast<int64_t>(blockIdx.y) * rows / gridDim.y);
     const int hi = static_cast<int>(static_cast<int64_t>(blockIdx.y + 1) * rows / gridDim.y);
     float s[8] = {};
-    for (int r = lo + warp; r < hi; r += 8) {
-        for (int64_t off = 0;; off = dz_plane) {
-            const uint4 u = *reinterpret_cast<const uint4*>(dz + off + r * dz_ld + col);
-            const __half2* h = reinterpret_cast<const __half2*>(&u);
+    for (int64_t off = 0;; off = dz_plane) {
+        const __half* d = dz + off + col;
+        for (int r = lo + warp; r < hi; r += 32) {
+            uint4 u[4];
 #pragma unroll
-            for (int t = 0; t < 4; ++t) {
-                const float2 f = __half22float2(h[t]);
-                s[2 * t] += f.x;
-                s[2 * t + 1] += f.y;
+            for (int k = 0; k < 4; ++k) u[k] = r + 8 * k < hi ? *reinterpret_cast<const uint4*>(d + (r + 8 * k) * dz_ld) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const __half2* h = reinterpret_cast<const __half2*>(&u[k]);
+#pragma unroll
+                for (int t = 0; t < 4; ++t) {
+                    const float2 f = __half22float2(h[t]);
+                    s[2 * t] += f.x;
+                    s[2 * t + 1] += f.y;
+                }
             }
-            if (off == dz_plane) break;
         }
+        if (off == dz_plane) break;
     }
 #pragma unroll
     for (int i = 0; i < 8; ++i) sums[warp][lane][i] = s[i];
@@ -1021,6 +1131,7 @@ struct Plan {
     int64_t piece;           // vocabulary columns per piece (a multiple of BN)
     int64_t pieces;
     int64_t acc_ld;
+    int64_t parts;           // statistics per row
     int split_units;
     int db_chunks;
     // state: kept from the forward to the backward pass
@@ -1036,6 +1147,18 @@ int check(const char* who, const tk_linear_ce_desc_t& d) {
     TK_CHECK_ARG(d.rows >= 0 && d.cols >= 1 && d.vocab >= 1, "%s: rows must not be negative, cols and vocab must be positive", who);
     if (d.rows > kMaxSize || d.cols > kMaxSize || d.vocab > kMaxSize) TK_FAIL(TK_ERR_UNSUPPORTED, "%s: sizes must be below 2^31 - 256", who);
     return TK_OK;
+}
+
+// K blocks per accumulator chunk: 16 steps of 16 where every output is
+// binary32, 64 for the loss of fp16 operands (measured at 4096 columns: the
+// loss 1e-6 off without chunks, and the same time).  A K loop no longer than a
+// chunk needs no sum in registers.
+constexpr int kChunkF32 = 4, kChunkStats = 16;
+
+bool chunked(int64_t k_blocks, int pairs, int chunk) { return chunk != 0 && (k_blocks < 0 || k_blocks * pairs > chunk); }
+
+bool stats_chunked(const Plan& p, const tk_linear_ce_desc_t& d) {
+    return chunked(ceil_div(d.cols, BK), p.f16 ? 1 : 3, p.f16 ? kChunkStats : kChunkF32);
 }
 
 Plan make_plan(const tk_linear_ce_desc_t& d) {
@@ -1069,7 +1192,8 @@ Plan make_plan(const tk_linear_ce_desc_t& d) {
     p.s_bias = take(d.bias != nullptr ? static_cast<size_t>(d.vocab) * sizeof(float) : 0);
     p.state_bytes = at;
     at = 0;
-    p.w_part = take(static_cast<size_t>(2 * p.n_tiles) * p.rows_pad * sizeof(float2));
+    p.parts = p.n_tiles * (stats_chunked(p, d) ? BN / Config<true>::COLS : BN / Config<false>::COLS);
+    p.w_part = take(static_cast<size_t>(p.parts) * p.rows_pad * sizeof(float2));
     p.w_loss = take(p.rows_pad * sizeof(float));
     p.fwd_bytes = at + p.state_bytes;  // a call without a state keeps its own
     at = 0;
@@ -1112,11 +1236,6 @@ int launch_chain(const char* what, void (*k)(K...), dim3 grid, dim3 block, size_
     return TK_OK;
 }
 
-// K blocks per accumulator chunk: 16 steps of 16 where every output is
-// binary32, 64 for the loss of fp16 operands (measured at 4096 columns: the
-// loss 1e-6 off without chunks, and the same time).
-constexpr int kChunkF32 = 4, kChunkStats = 16;
-
 template <int EPI, bool CHUNKED>
 int gemm_launch(const CUtensorMap& a, const CUtensorMap& b, const GemmParams& p, int64_t most_units, cudaStream_t s) {
     auto* kernel = ce_gemm_kernel<EPI, CHUNKED>;
@@ -1131,13 +1250,13 @@ int gemm_launch(const CUtensorMap& a, const CUtensorMap& b, const GemmParams& p,
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(2);
-    cfg.blockDim = dim3(THREADS);
-    cfg.dynamicSmemBytes = GEMM_SMEM;
+    cfg.blockDim = dim3(Config<CHUNKED>::THREADS);
+    cfg.dynamicSmemBytes = Config<CHUNKED>::SMEM;
     cfg.stream = s;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
     if (pairs == 0) {
-        TK_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, GEMM_SMEM));
+        TK_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Config<CHUNKED>::SMEM));
         TK_CUDA_TRY(cudaOccupancyMaxActiveClusters(&pairs, kernel, &cfg));
         if (pairs < 1) TK_FAIL(TK_ERR_CUDA, "cross entropy GEMM: no pair of CTAs fits the GPU");
         if (device < 64) resident[device].store(pairs, std::memory_order_relaxed);
@@ -1154,9 +1273,7 @@ int gemm_launch(const CUtensorMap& a, const CUtensorMap& b, const GemmParams& p,
 
 template <int EPI>
 int gemm(const CUtensorMap& a, const CUtensorMap& b, const GemmParams& p, int64_t most_units, cudaStream_t s) {
-    // a K loop no longer than a chunk needs no sum in registers
-    const bool one = p.chunk == 0 || (p.k_blocks >= 0 && p.k_blocks * p.pairs <= p.chunk);
-    return one ? gemm_launch<EPI, false>(a, b, p, most_units, s) : gemm_launch<EPI, true>(a, b, p, most_units, s);
+    return chunked(p.k_blocks, p.pairs, p.chunk) ? gemm_launch<EPI, true>(a, b, p, most_units, s) : gemm_launch<EPI, false>(a, b, p, most_units, s);
 }
 
 int blocks_for(int64_t rows) { return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(rows, 148 * 16))); }
@@ -1170,7 +1287,7 @@ int pack(const tk_linear_ce_desc_t& d, const Plan& p, uint8_t* st, cudaStream_t 
     const int* index = reinterpret_cast<const int*>(st + p.s_index);
     const bool eight = d.cols % 8 == 0;
     if constexpr (PLANES == 2)
-        CE_TRY(launch_chain("cross entropy amax", ce_amax_kernel, dim3(296, 2), dim3(256), 0, s, x, w, index, sc, d.cols, d.vocab));
+        CE_TRY(launch_chain("cross entropy amax", ce_amax_kernel, dim3(148 * 4, 2), dim3(256), 0, s, x, w, index, sc, d.cols, d.vocab));
     const PackJob<T> jx = {x, index, reinterpret_cast<__half*>(st + p.s_x), d.rows, d.cols, p.ld, p.rows_pad * p.ld,
                            eight && (reinterpret_cast<uintptr_t>(x) & 15) == 0};
     const PackJob<T> jw = {w, nullptr, reinterpret_cast<__half*>(st + p.s_w), d.vocab, d.cols, p.ld, d.vocab * p.ld,
@@ -1184,12 +1301,13 @@ int pack(const tk_linear_ce_desc_t& d, const Plan& p, uint8_t* st, cudaStream_t 
 
 template <typename T>
 int rows_loss(const tk_linear_ce_desc_t& d, const Plan& p, uint8_t* st, uint8_t* ws, cudaStream_t s) {
-    const dim3 grid(static_cast<unsigned>(std::max<int64_t>(1, std::min<int64_t>(ceil_div(d.rows, kRowLanes), 148 * 4)))), block(kRowLanes, kRowSlices);
-    return launch_chain("cross entropy rows", ce_rows_kernel<T>, grid, block, 0, s, static_cast<const T*>(d.x), static_cast<const T*>(d.weight),
-                        static_cast<const T*>(d.bias), reinterpret_cast<const int*>(st + p.s_index), reinterpret_cast<const int*>(st + p.s_target),
-                        reinterpret_cast<Scalars*>(st + p.s_scalars), reinterpret_cast<const float2*>(ws + p.w_part), static_cast<int>(2 * p.n_tiles),
-                        p.rows_pad, d.cols, reinterpret_cast<float*>(st + p.s_lse), reinterpret_cast<float*>(ws + p.w_loss), static_cast<int>(d.reduction),
-                        d.loss);
+    const int grid = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(ceil_div(d.rows, kRowWarps), 148 * 8)));
+    const bool vec = d.cols * sizeof(T) % 16 == 0 && ((reinterpret_cast<uintptr_t>(d.x) | reinterpret_cast<uintptr_t>(d.weight)) & 15) == 0;
+    return launch_chain("cross entropy rows", ce_rows_kernel<T>, dim3(grid), dim3(32 * kRowWarps), 0, s, static_cast<const T*>(d.x),
+                        static_cast<const T*>(d.weight), static_cast<const T*>(d.bias), reinterpret_cast<const int*>(st + p.s_index),
+                        reinterpret_cast<const int*>(st + p.s_target), reinterpret_cast<Scalars*>(st + p.s_scalars),
+                        reinterpret_cast<const float2*>(ws + p.w_part), static_cast<int>(p.parts), d.cols, vec,
+                        reinterpret_cast<float*>(st + p.s_lse), reinterpret_cast<float*>(ws + p.w_loss), static_cast<int>(d.reduction), d.loss);
 }
 
 struct Operand {
@@ -1214,7 +1332,6 @@ GemmParams base_params(const tk_linear_ce_desc_t& d, const Plan& p, const uint8_
     g.err = device_error_word(current_device());
     g.bias2 = d.bias != nullptr ? reinterpret_cast<const float*>(st + p.s_bias) : nullptr;
     g.vocab = d.vocab;
-    g.rows_pad = p.rows_pad;
     return g;
 }
 
