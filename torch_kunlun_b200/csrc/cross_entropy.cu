@@ -8,8 +8,8 @@
 // lists the others, their rows of x are packed, and every later kernel takes
 // its row count from that list on the device.
 //
-// Forward: one tcgen05 GEMM whose epilogue keeps, per row and 64 or 128
-// columns, the maximum and the sum of exponentials (base 2); a small kernel joins them
+// Forward: one tcgen05 GEMM whose epilogue keeps, per row and 128 columns,
+// the maximum and the sum of exponentials (base 2); a small kernel joins them
 // and computes the target's logit as a dot product of its own.  Backward: the
 // vocabulary is taken in pieces whose dz fits a workspace; per piece the
 // logits are computed again, the epilogue stores dz as binary16, and two
@@ -58,18 +58,24 @@ constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
 // 16-byte accesses).
 constexpr int TURN = 16;
 constexpr int PITCH = TURN + 4;
-// Sixteen epilogue warps keep up with short K loops; sums in registers (128
-// columns per thread) leave room for eight.
-template <bool CHUNKED>
+// kPlain: eight epilogue warps, six stages.  kWide: sixteen warps for dz where
+// the K loop is short (the logits of 2384 rows by 30011 words at 768 columns,
+// 12 K blocks: 177 -> 166 us; at 64 K blocks five stages cost 3 %).  kChunked:
+// sums in registers, 128 columns per thread.
+enum Mode { kPlain, kWide, kChunked };
+constexpr int kWideBlocks = 24;  // K blocks up to which kWide is taken
+
+template <int MODE>
 struct Config {
-    static constexpr int STAGES = CHUNKED ? 6 : 5;
-    static constexpr int EPI_WARPS = CHUNKED ? 8 : 16;
+    static constexpr int STAGES = MODE == kWide ? 5 : 6;
+    static constexpr int EPI_WARPS = MODE == kWide ? 16 : 8;
     static constexpr int COLS = BN / (EPI_WARPS / 4);  // of a tile row, per warp
     static constexpr int THREADS = 64 + 32 * EPI_WARPS;
     static constexpr int TURN_BYTES = EPI_WARPS * 32 * PITCH * 4;
     static constexpr int SMEM = STAGES * STAGE_BYTES + TURN_BYTES + 1024 + 256;
     static_assert(SMEM <= 232448, "shared memory budget");
 };
+constexpr int kParts = BN / Config<kPlain>::COLS;  // statistics per row of a tile
 constexpr int TMEM_COLS = 512;
 
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
@@ -101,7 +107,7 @@ struct GemmParams {
     unsigned* err;
     // kStats / kDlogits
     const float* bias2;  // bias * log2(e), or NULL
-    float2* part;           // [rows][n_tiles][warps per tile row] maximum and sum
+    float2* part;           // [rows][n_tiles][kParts] maximum and sum
     const float* lse2;
     const float* grow;   // g_i / max |g|
     const int* target;
@@ -348,14 +354,14 @@ __device__ __forceinline__ float z_scale(const GemmParams& p) {
     return p.pairs == 1 ? kLog2e : kLog2e / plane_scale(p.sc->amax_x) / plane_scale(p.sc->amax_w);
 }
 
-// CHUNKED: the epilogue adds chunks of the K loop in registers (128 columns
-// of a row per thread).
-template <int EPI, bool CHUNKED>
-__global__ void __launch_bounds__(Config<CHUNKED>::THREADS, 1)
+template <int EPI, int MODE>
+__global__ void __launch_bounds__(Config<MODE>::THREADS, 1)
 ce_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const GemmParams p) {
     constexpr bool A_MN = EPI == kGradW, B_MN = EPI == kGradX || EPI == kGradW;
     constexpr uint32_t IDESC = idesc_f16(BM, BN, A_MN, B_MN);
-    using C = Config<CHUNKED>;
+    using C = Config<MODE>;
+    constexpr bool CHUNKED = MODE == kChunked;
+    static_assert(MODE != kWide || EPI == kDlogits, "wide epilogues are for dz");
     constexpr int STAGES = C::STAGES, EPI_WARPS = C::EPI_WARPS, COLS = C::COLS;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
@@ -644,7 +650,7 @@ ce_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
 #pragma unroll
                 for (int c = 0; c < COLS; c += 32) take(c, v + c);
             }
-            if constexpr (EPI == kStats) p.part[(m * p.n_tiles + nt) * (BN / COLS) + share] = make_float2(top, sum);
+            if constexpr (EPI == kStats) p.part[(m * p.n_tiles + nt) * kParts + share] = make_float2(top, sum);
         }
     }
     tc_fence_before();
@@ -708,10 +714,13 @@ __global__ void __launch_bounds__(256) ce_split_kernel(const GemmParams p) {
 __device__ __forceinline__ float load_f(const __half* p, int64_t i) { return __half2float(p[i]); }
 __device__ __forceinline__ float load_f(const float* p, int64_t i) { return p[i]; }
 
-constexpr int kIndexThreads = 1024, kIndexRows = 8;  // rows per thread and step
+constexpr int kIndexThreads = 1024;
 
 // Lists the rows that have a target (in order), their targets, and their
 // count; writes the ignored rows' losses (0) where there is one per row.
+// kIndexRows: rows per thread and step (16384 rows: 23 us with one, 11 us with
+// eight; up to 1024 rows 1.8 us with one).
+template <int kIndexRows>
 __global__ void __launch_bounds__(kIndexThreads)
 ce_index_kernel(const int64_t* target, int64_t rows, int64_t vocab, int64_t ignore, int* index, int* packed_target, Scalars* sc,
                 float* row_loss_out) {
@@ -1131,7 +1140,6 @@ struct Plan {
     int64_t piece;           // vocabulary columns per piece (a multiple of BN)
     int64_t pieces;
     int64_t acc_ld;
-    int64_t parts;           // statistics per row
     int split_units;
     int db_chunks;
     // state: kept from the forward to the backward pass
@@ -1154,12 +1162,6 @@ int check(const char* who, const tk_linear_ce_desc_t& d) {
 // loss 1e-6 off without chunks, and the same time).  A K loop no longer than a
 // chunk needs no sum in registers.
 constexpr int kChunkF32 = 4, kChunkStats = 16;
-
-bool chunked(int64_t k_blocks, int pairs, int chunk) { return chunk != 0 && (k_blocks < 0 || k_blocks * pairs > chunk); }
-
-bool stats_chunked(const Plan& p, const tk_linear_ce_desc_t& d) {
-    return chunked(ceil_div(d.cols, BK), p.f16 ? 1 : 3, p.f16 ? kChunkStats : kChunkF32);
-}
 
 Plan make_plan(const tk_linear_ce_desc_t& d) {
     Plan p = {};
@@ -1192,8 +1194,7 @@ Plan make_plan(const tk_linear_ce_desc_t& d) {
     p.s_bias = take(d.bias != nullptr ? static_cast<size_t>(d.vocab) * sizeof(float) : 0);
     p.state_bytes = at;
     at = 0;
-    p.parts = p.n_tiles * (stats_chunked(p, d) ? BN / Config<true>::COLS : BN / Config<false>::COLS);
-    p.w_part = take(static_cast<size_t>(p.parts) * p.rows_pad * sizeof(float2));
+    p.w_part = take(static_cast<size_t>(kParts * p.n_tiles) * p.rows_pad * sizeof(float2));
     p.w_loss = take(p.rows_pad * sizeof(float));
     p.fwd_bytes = at + p.state_bytes;  // a call without a state keeps its own
     at = 0;
@@ -1236,9 +1237,9 @@ int launch_chain(const char* what, void (*k)(K...), dim3 grid, dim3 block, size_
     return TK_OK;
 }
 
-template <int EPI, bool CHUNKED>
+template <int EPI, int MODE>
 int gemm_launch(const CUtensorMap& a, const CUtensorMap& b, const GemmParams& p, int64_t most_units, cudaStream_t s) {
-    auto* kernel = ce_gemm_kernel<EPI, CHUNKED>;
+    auto* kernel = ce_gemm_kernel<EPI, MODE>;
     static std::atomic<int> resident[64];  // pairs of CTAs each device holds at once; 0: not asked yet
     const int device = current_device();
     int pairs = device < 64 ? resident[device].load(std::memory_order_relaxed) : 0;
@@ -1250,13 +1251,13 @@ int gemm_launch(const CUtensorMap& a, const CUtensorMap& b, const GemmParams& p,
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(2);
-    cfg.blockDim = dim3(Config<CHUNKED>::THREADS);
-    cfg.dynamicSmemBytes = Config<CHUNKED>::SMEM;
+    cfg.blockDim = dim3(Config<MODE>::THREADS);
+    cfg.dynamicSmemBytes = Config<MODE>::SMEM;
     cfg.stream = s;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
     if (pairs == 0) {
-        TK_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Config<CHUNKED>::SMEM));
+        TK_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Config<MODE>::SMEM));
         TK_CUDA_TRY(cudaOccupancyMaxActiveClusters(&pairs, kernel, &cfg));
         if (pairs < 1) TK_FAIL(TK_ERR_CUDA, "cross entropy GEMM: no pair of CTAs fits the GPU");
         if (device < 64) resident[device].store(pairs, std::memory_order_relaxed);
@@ -1273,7 +1274,12 @@ int gemm_launch(const CUtensorMap& a, const CUtensorMap& b, const GemmParams& p,
 
 template <int EPI>
 int gemm(const CUtensorMap& a, const CUtensorMap& b, const GemmParams& p, int64_t most_units, cudaStream_t s) {
-    return chunked(p.k_blocks, p.pairs, p.chunk) ? gemm_launch<EPI, true>(a, b, p, most_units, s) : gemm_launch<EPI, false>(a, b, p, most_units, s);
+    const int64_t blocks = p.k_blocks < 0 ? INT64_MAX : static_cast<int64_t>(p.k_blocks) * p.pairs;
+    if (p.chunk != 0 && blocks > p.chunk) return gemm_launch<EPI, kChunked>(a, b, p, most_units, s);
+    if constexpr (EPI == kDlogits) {
+        if (blocks <= kWideBlocks) return gemm_launch<EPI, kWide>(a, b, p, most_units, s);
+    }
+    return gemm_launch<EPI, kPlain>(a, b, p, most_units, s);
 }
 
 int blocks_for(int64_t rows) { return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(rows, 148 * 16))); }
@@ -1306,7 +1312,7 @@ int rows_loss(const tk_linear_ce_desc_t& d, const Plan& p, uint8_t* st, uint8_t*
     return launch_chain("cross entropy rows", ce_rows_kernel<T>, dim3(grid), dim3(32 * kRowWarps), 0, s, static_cast<const T*>(d.x),
                         static_cast<const T*>(d.weight), static_cast<const T*>(d.bias), reinterpret_cast<const int*>(st + p.s_index),
                         reinterpret_cast<const int*>(st + p.s_target), reinterpret_cast<Scalars*>(st + p.s_scalars),
-                        reinterpret_cast<const float2*>(ws + p.w_part), static_cast<int>(p.parts), d.cols, vec,
+                        reinterpret_cast<const float2*>(ws + p.w_part), static_cast<int>(kParts * p.n_tiles), d.cols, vec,
                         reinterpret_cast<float*>(st + p.s_lse), reinterpret_cast<float*>(ws + p.w_loss), static_cast<int>(d.reduction), d.loss);
 }
 
@@ -1364,7 +1370,8 @@ int tk_linear_ce(const tk_linear_ce_desc_t* desc, void* workspace, size_t worksp
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     uint8_t* ws = static_cast<uint8_t*>(workspace);
     uint8_t* st = d.state != nullptr ? static_cast<uint8_t*>(d.state) : ws + (p.fwd_bytes - p.state_bytes);
-    ce_index_kernel<<<1, kIndexThreads, 0, s>>>(d.target, d.rows, d.vocab, d.ignore_index, reinterpret_cast<int*>(st + p.s_index),
+    auto* index = d.rows <= kIndexThreads ? ce_index_kernel<1> : ce_index_kernel<8>;
+    index<<<1, kIndexThreads, 0, s>>>(d.target, d.rows, d.vocab, d.ignore_index, reinterpret_cast<int*>(st + p.s_index),
                                                 reinterpret_cast<int*>(st + p.s_target), reinterpret_cast<Scalars*>(st + p.s_scalars),
                                                 d.reduction == TK_REDUCE_NONE ? d.loss : nullptr);
     CE_TRY(launch_status("cross entropy index"));
@@ -1447,6 +1454,14 @@ int tk_linear_ce_backward(const tk_linear_ce_grad_desc_t* desc, void* workspace,
         g.dz_ld = p.piece;
         g.dz_plane = p.planes == 2 ? dz_plane : 0;
         CE_TRY(gemm<kDlogits>(tx, tw, g, row_tiles * g.n_tiles, s));
+        if (desc->dbias) {
+            float* part = reinterpret_cast<float*>(ws + p.b_db);
+            CE_TRY(launch_chain("cross entropy bias sums", ce_dbias_part_kernel, dim3(static_cast<unsigned>(p.piece / 256), p.db_chunks), dim3(kDbThreads), 0, s,
+                                static_cast<const __half*>(dz), p.piece, g.dz_plane, static_cast<const Scalars*>(sc), part));
+            CE_TRY(launch_chain("cross entropy bias sums", ce_dbias_kernel, dim3(static_cast<unsigned>(ceil_div(width, 256))), dim3(256), 0, s,
+                                static_cast<const float*>(part), p.db_chunks, p.piece, width, static_cast<const Scalars*>(sc),
+                                static_cast<void*>(static_cast<uint8_t*>(desc->dbias) + v0 * esz), p.f16 ? 0 : 1));
+        }
         GemmParams r = base_params(d, p, st);
         r.out_cols = d.cols;
         r.out_f32 = p.f16 ? 0 : 1;
@@ -1473,14 +1488,6 @@ int tk_linear_ce_backward(const tk_linear_ce_grad_desc_t* desc, void* workspace,
             CE_TRY(gemm<kGradW>(tdz_mn, tx_mn, r, std::max<int64_t>(r.m_tiles * col_tiles, p.split_units), s));
             if (2 * r.m_tiles * col_tiles <= p.split_units)  // else no tile is split
                 CE_TRY(launch_chain("cross entropy split", ce_split_kernel<kGradW>, dim3(static_cast<unsigned>(p.split_units) * 8), dim3(256), 0, s, r));
-        }
-        if (desc->dbias) {
-            float* part = reinterpret_cast<float*>(ws + p.b_db);
-            CE_TRY(launch_chain("cross entropy bias sums", ce_dbias_part_kernel, dim3(static_cast<unsigned>(p.piece / 256), p.db_chunks), dim3(kDbThreads), 0, s,
-                                static_cast<const __half*>(dz), p.piece, g.dz_plane, static_cast<const Scalars*>(sc), part));
-            CE_TRY(launch_chain("cross entropy bias sums", ce_dbias_kernel, dim3(static_cast<unsigned>(ceil_div(width, 256))), dim3(256), 0, s,
-                                static_cast<const float*>(part), p.db_chunks, p.piece, width, static_cast<const Scalars*>(sc),
-                                static_cast<void*>(static_cast<uint8_t*>(desc->dbias) + v0 * esz), p.f16 ? 0 : 1));
         }
     }
     return TK_OK;

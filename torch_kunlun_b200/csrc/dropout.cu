@@ -30,32 +30,29 @@ struct Octet {  // 8 elements as one (fp16) or two (fp32) 16-byte vectors
     }
 };
 
-__device__ __forceinline__ uint32_t scale2(uint32_t pair, float s, uint32_t keep) {
+// Scales the octet's values whose word reaches the threshold, zeroes the rest.
+__device__ __forceinline__ uint32_t scale2(uint32_t pair, float s, uint32_t w0, uint32_t w1, uint32_t threshold) {
     const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&pair));
-    const __half2 h = __floats2half2_rn(f.x * s, f.y * s);
-    const uint32_t bits = *reinterpret_cast<const uint32_t*>(&h);
-    return bits & ((keep & 1u ? 0x0000FFFFu : 0u) | (keep & 2u ? 0xFFFF0000u : 0u));
+    const __half2 h = __floats2half2_rn(w0 >= threshold ? f.x * s : 0.0f, w1 >= threshold ? f.y * s : 0.0f);
+    return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-__device__ __forceinline__ void apply(Octet<__half>& o, float s, uint32_t keep) {
-    o.v[0].x = scale2(o.v[0].x, s, keep);
-    o.v[0].y = scale2(o.v[0].y, s, keep >> 2);
-    o.v[0].z = scale2(o.v[0].z, s, keep >> 4);
-    o.v[0].w = scale2(o.v[0].w, s, keep >> 6);
+__device__ __forceinline__ void apply(Octet<__half>& o, float s, const uint32_t (&a)[4], const uint32_t (&b)[4], uint32_t threshold) {
+    o.v[0].x = scale2(o.v[0].x, s, a[0], a[1], threshold);
+    o.v[0].y = scale2(o.v[0].y, s, a[2], a[3], threshold);
+    o.v[0].z = scale2(o.v[0].z, s, b[0], b[1], threshold);
+    o.v[0].w = scale2(o.v[0].w, s, b[2], b[3], threshold);
 }
 
-__device__ __forceinline__ uint32_t scale1(uint32_t bits, float s, uint32_t keep) {
-    return keep & 1u ? __float_as_uint(__uint_as_float(bits) * s) : 0u;
+__device__ __forceinline__ uint32_t scale1(uint32_t bits, float s, uint32_t w, uint32_t threshold) {
+    return w >= threshold ? __float_as_uint(__uint_as_float(bits) * s) : 0u;
 }
 
-__device__ __forceinline__ void apply(Octet<float>& o, float s, uint32_t keep) {
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        o.v[i].x = scale1(o.v[i].x, s, keep >> (4 * i));
-        o.v[i].y = scale1(o.v[i].y, s, keep >> (4 * i + 1));
-        o.v[i].z = scale1(o.v[i].z, s, keep >> (4 * i + 2));
-        o.v[i].w = scale1(o.v[i].w, s, keep >> (4 * i + 3));
-    }
+__device__ __forceinline__ void apply(Octet<float>& o, float s, const uint32_t (&a)[4], const uint32_t (&b)[4], uint32_t threshold) {
+    o.v[0] = make_uint4(scale1(o.v[0].x, s, a[0], threshold), scale1(o.v[0].y, s, a[1], threshold),
+                        scale1(o.v[0].z, s, a[2], threshold), scale1(o.v[0].w, s, a[3], threshold));
+    o.v[1] = make_uint4(scale1(o.v[1].x, s, b[0], threshold), scale1(o.v[1].y, s, b[1], threshold),
+                        scale1(o.v[1].z, s, b[2], threshold), scale1(o.v[1].w, s, b[3], threshold));
 }
 
 __device__ __forceinline__ float to_f(__half v) { return __half2float(v); }
@@ -80,7 +77,10 @@ __global__ void __launch_bounds__(kThreads) dropout_kernel(const T* x, T* y, int
     for (int u = 0; u < kUnroll; ++u) {
         const int64_t i = base + u * kThreads;
         if (i < octets) {
-            apply(o[u], d.scale, dropout_keep8(d, i));
+            uint32_t a[4], b[4];
+            philox4x32_10(2 * i, d.offset, d.seed, a);
+            philox4x32_10(2 * i + 1, d.offset, d.seed, b);
+            apply(o[u], d.scale, a, b, d.threshold);
             o[u].store(y + 8 * i);
         }
     }
@@ -101,7 +101,7 @@ __global__ void __launch_bounds__(kThreads) dropout_any_kernel(const T* x, T* y,
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
         const int64_t i = 4 * b + j;
-        if (i < n) from_f(w[j] >= d.threshold && !d.none_kept ? to_f(x[i]) * d.scale : 0.0f, y[i]);
+        if (i < n) from_f(w[j] >= d.threshold ? to_f(x[i]) * d.scale : 0.0f, y[i]);
     }
 }
 
@@ -134,6 +134,11 @@ extern "C" int tk_dropout(tk_dtype_t dtype, const void* x, void* y, int64_t n, d
     TK_CHECK_ARG(x != nullptr && y != nullptr, "tk_dropout: NULL pointer");
     const tk::DropoutParams d = tk::dropout_params(p, seed, offset);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (d.none_kept) {
+        TK_CHECK_ARG(n <= INT64_MAX / 4, "tk_dropout: too many elements");
+        TK_CUDA_TRY(cudaMemsetAsync(y, 0, static_cast<size_t>(n) * tk::dtype_size(dtype), s));
+        return TK_OK;
+    }
     return dtype == TK_DTYPE_F16 ? tk::dropout_launch<__half>(x, y, n, d, s)
                                  : tk::dropout_launch<float>(x, y, n, d, s);
 }
