@@ -426,7 +426,7 @@ TK_API int tk_dropout(tk_dtype_t dtype, const void* x, void* y, int64_t n, doubl
  * each sample; rows: one for each token).  Sums and statistics are fp32; each
  * output is rounded once.  stats (NULL or 16-byte aligned, [rows][4]) receives
  * mean and rstd of f (post norm only) and of x_new for the backward pass.
- * cols <= 32768.  Outputs must not overlap inputs.  Extends layer_norm
+ * cols <= 32768; with dropout rows * cols < 2^34.  Outputs must not overlap inputs.  Extends layer_norm
  * (csrc/ops_nn.cpp:85-130) and the adds around it (csrc/ops.cpp:117-149). */
 typedef enum { TK_NORM_LAYER = 0, TK_NORM_RMS = 1 } tk_norm_t;
 

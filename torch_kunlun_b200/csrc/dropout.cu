@@ -2,9 +2,10 @@
 // tk_philox.cuh, recomputed wherever it is needed and never stored; the
 // backward pass is the same call on the gradient.
 //
-// Two bytes per fp16 element each way bound it (4 bytes in all); the ten
-// Philox rounds of four elements cost 20 wide multiplies, which run while the
-// thread's loads are in flight.
+// The generator bounds it: ten Philox rounds of four elements are 18 wide
+// multiplies, which issue at a quarter of the rate of an add (75 % of the
+// multiplier's cycles busy at 36 % of HBM's, fp16); the loads are in flight
+// meanwhile.
 #include <cuda_fp16.h>
 
 #include "tk_internal.h"
@@ -66,7 +67,10 @@ template <typename T>
 __global__ void __launch_bounds__(kThreads) dropout_kernel(const T* x, T* y, int64_t n,
                                                            const DropoutParams d) {
     const int64_t octets = n / 8;
-    const int64_t base = static_cast<int64_t>(blockIdx.x) * kThreads * kUnroll + threadIdx.x;
+    // a block's 1024 Philox blocks share the counter's high word
+    static_assert((2 * kThreads * kUnroll & (2 * kThreads * kUnroll - 1)) == 0, "a power of two");
+    const int64_t first = static_cast<int64_t>(blockIdx.x) * kThreads * kUnroll, base = first + threadIdx.x;
+    const uint32_t hi = static_cast<uint32_t>(2 * first >> 32);
     Octet<T> o[kUnroll];
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) {
@@ -78,15 +82,20 @@ __global__ void __launch_bounds__(kThreads) dropout_kernel(const T* x, T* y, int
         const int64_t i = base + u * kThreads;
         if (i < octets) {
             uint32_t a[4], b[4];
-            philox4x32_10(2 * i, d.offset, d.seed, a);
-            philox4x32_10(2 * i + 1, d.offset, d.seed, b);
+            const uint32_t lo = static_cast<uint32_t>(2 * first) + 2 * (threadIdx.x + u * kThreads);
+            philox4x32_10(lo, hi, d.offset, d.seed, a);
+            philox4x32_10(lo + 1, hi, d.offset, d.seed, b);
             apply(o[u], d.scale, a, b, d.threshold);
             o[u].store(y + 8 * i);
         }
     }
     const int64_t tail = octets * 8 + threadIdx.x;
     if (blockIdx.x == gridDim.x - 1 && tail < n) {
-        from_f(dropout_keep1(d, tail) ? to_f(x[tail]) * d.scale : 0.0f, y[tail]);
+        uint32_t w[4];
+        philox4x32_10(static_cast<uint32_t>(tail >> 2), static_cast<uint32_t>(tail >> 34), d.offset, d.seed, w);
+        const uint32_t lane = static_cast<uint32_t>(tail) & 3u;
+        const uint32_t v = lane == 0 ? w[0] : lane == 1 ? w[1] : lane == 2 ? w[2] : w[3];
+        from_f(v >= d.threshold ? to_f(x[tail]) * d.scale : 0.0f, y[tail]);
     }
 }
 
@@ -97,7 +106,7 @@ __global__ void __launch_bounds__(kThreads) dropout_any_kernel(const T* x, T* y,
     const int64_t b = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
     if (4 * b >= n) return;
     uint32_t w[4];
-    philox4x32_10(b, d.offset, d.seed, w);
+    philox4x32_10(static_cast<uint32_t>(b), static_cast<uint32_t>(b >> 32), d.offset, d.seed, w);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
         const int64_t i = 4 * b + j;

@@ -311,7 +311,7 @@ struct Lane {
         uint32_t m = 0;
         if constexpr (VEC) {
 #pragma unroll
-            for (int v = 0; v < NV; ++v) m |= dropout_keep8(p.dropout, static_cast<uint64_t>(row + col(8 * v)) / 8) << (8 * v);
+            for (int v = 0; v < NV; ++v) m |= dropout_keep8(p.dropout, static_cast<uint32_t>((row + col(8 * v)) / 8)) << (8 * v);
         } else {
             // Columns e of the warp's lanes are 32 consecutive elements, 4 *
             // block + shift on: eight blocks of four, a ninth where shift > 0.
@@ -324,8 +324,8 @@ struct Lane {
             uint32_t mine = 0, ninth = 0;  // four keep bits each
 #pragma unroll
             for (int a = 0; a < E / 4; ++a)
-                mine |= dropout_keep4(p.dropout, (first + static_cast<uint64_t>(4 * a + (lane & 3)) * gthreads) / 4 + (lane >> 2)) << (4 * (a % 8));
-            if (shift != 0) ninth = dropout_keep4(p.dropout, (first + static_cast<uint64_t>(lane % E) * gthreads) / 4 + 8);
+                mine |= dropout_keep4(p.dropout, static_cast<uint32_t>((first + static_cast<uint64_t>(4 * a + (lane & 3)) * gthreads) / 4) + (lane >> 2)) << (4 * (a % 8));
+            if (shift != 0) ninth = dropout_keep4(p.dropout, static_cast<uint32_t>((first + static_cast<uint64_t>(lane % E) * gthreads) / 4) + 8);
 #pragma unroll
             for (int e = 0; e < E; ++e) {
                 uint32_t four = __shfl_sync(0xFFFFFFFFu, mine, (q & 7) * 4 + e % 4) >> (4 * (e / 4));
@@ -844,6 +844,7 @@ int check(const char* who, const tk_residual_norm_desc_t& d) {
     if (d.cols > kMaxCols) TK_FAIL(TK_ERR_UNSUPPORTED, "%s: at most %lld columns, got %lld", who, static_cast<long long>(kMaxCols), static_cast<long long>(d.cols));
     TK_CHECK_ARG(d.rows <= INT64_MAX / 8 / d.cols, "%s: too many elements", who);
     TK_CHECK_ARG(d.p >= 0.0 && d.p <= 1.0, "%s: p must be in [0, 1], got %g", who, d.p);
+    if (d.p > 0.0 && d.rows * d.cols >= (1ll << 34)) TK_FAIL(TK_ERR_UNSUPPORTED, "%s: dropout of 2^34 elements or more", who);
     TK_CHECK_ARG(d.post_norm || (d.post_weight == nullptr && d.post_bias == nullptr), "%s: post_weight and post_bias need post_norm", who);
     TK_CHECK_ARG(d.gate == nullptr || (d.gate_rows >= 1 && d.rows % d.gate_rows == 0), "%s: gate_rows must divide rows", who);
     return TK_OK;
