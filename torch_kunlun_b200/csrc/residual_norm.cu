@@ -404,6 +404,29 @@ struct Lane {
             if (!((keep >> (2 * i + 1)) & 1u)) v[i].y = 0.0f;
         }
     }
+    // The same straight from the generator's words, where no mask is needed.
+    __device__ __forceinline__ void drop_row(int64_t row, float2 (&v)[P]) const {
+        if constexpr (VEC) {
+            const float2 s = both(p.dropout.scale);
+            const uint32_t t32 = p.dropout.threshold;
+#pragma unroll
+            for (int o = 0; o < E / 4; ++o) {
+                uint32_t w[4];
+                philox4x32_10(static_cast<uint32_t>((row + col(4 * o)) / 4), 0, p.dropout.offset, p.dropout.seed, w);
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const float2 m = mul2(v[2 * o + i], s);
+                    v[2 * o + i] = make_float2(w[2 * i] >= t32 ? m.x : 0.0f, w[2 * i + 1] >= t32 ? m.y : 0.0f);
+                }
+            }
+            if (p.dropout.none_kept) {
+#pragma unroll
+                for (int i = 0; i < P; ++i) v[i] = make_float2(0.0f, 0.0f);
+            }
+        } else {
+            drop(keep(row), v);
+        }
+    }
     // Runs f(row, stage) over the group's rows [begin, end), a step of `groups`
     // apart, with the copies of the rows ahead under way.
     template <typename Fetch, typename F>
@@ -484,7 +507,7 @@ __global__ void __launch_bounds__(kMaxThreads, 1) residual_norm_kernel(const RnP
                     for (int i = 0; i < P; ++i) u[i] = add2(u[i], pb.pair(i));
                 }
             }
-            if (p.drop) ln.drop(ln.keep(at), u);
+            if (p.drop) ln.drop_row(at, u);
             if (p.gate != nullptr) {
                 const int64_t g = p.gate_period == p.rows ? 0 : r / p.gate_period;
                 if (!KEPT || g != gate_row) ln.vector(static_cast<const T*>(p.gate) + g * p.cols, 0.0f, gate);
@@ -633,7 +656,7 @@ __global__ void __launch_bounds__(kMaxThreads, 1) residual_norm_backward_kernel(
                     for (int i = 0; i < P; ++i) o[i] = mul2(a, g[i]);
                     ln.store(p.dx, at, o);
                 }
-                const uint32_t keep = p.drop ? ln.keep(at) : 0u;
+                const uint32_t keep = GATE && p.drop ? ln.keep(at) : 0u;
                 float2 q[NEED_F ? P : 1];  // Norm(f) with a post norm, else f
                 if constexpr (NEED_F) {
                     ln.row_values(p.f, at, stage, 3, q);
@@ -673,7 +696,13 @@ __global__ void __launch_bounds__(kMaxThreads, 1) residual_norm_backward_kernel(
 #pragma unroll
                     for (int i = 0; i < P; ++i) g[i] = mul2(g[i], gate.pair(i));
                 }
-                if (p.drop) ln.drop(keep, g);
+                if (p.drop) {
+                    if constexpr (GATE) {
+                        ln.drop(keep, g);
+                    } else {
+                        ln.drop_row(at, g);
+                    }
+                }
                 if constexpr (POST) {
                     float2 s3 = make_float2(0.0f, 0.0f), s4 = s3;
 #pragma unroll
@@ -944,7 +973,7 @@ int resident_ctas(Kernel k, const RnParams& p, size_t smem, int& per_sm) {
 }
 
 // CTAs per SM the backward pass may use: its partial sums are sized by it.
-constexpr int kBackwardPerSm = 2;
+constexpr int kBackwardPerSm = 4;
 
 template <typename T>
 int columns(const RnParams& p, const tk_residual_norm_grad_desc_t& g, bool gate_items, cudaStream_t s) {
