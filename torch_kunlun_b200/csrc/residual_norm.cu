@@ -33,7 +33,9 @@
 // barrier, otherwise the group the 16-byte vectors that cover the row.  CTAs
 // own contiguous rows; column sums stay in registers until a CTA's rows end,
 // and a second kernel adds the CTAs' partial sums in a fixed order, so no
-// gradient depends on timing.
+// gradient depends on timing.  Where a CTA cannot hold a row's columns and their
+// sums, a pass of its own adds the columns, from the row statistics and the two
+// row means that the first pass leaves.
 #include <cuda_fp16.h>
 
 #include <algorithm>
@@ -55,6 +57,7 @@ struct RnParams {
     const void *gx, *gh;  // backward: gradients of x_new and h
     void *dx, *df, *dgate;
     float4* stats;   // per row: mean and rstd of f (post), mean and rstd of x_new
+    float2* means;   // backward of wide rows: mean(t), mean(t * n) per row
     float* partial;  // backward: [4][units][cols], then the gate's [2 * units][cols]
     int64_t rows, cols, gate_period;  // row r uses gate row r / gate_period
     int units;                        // row ranges: clusters of `cluster` CTAs
@@ -139,14 +142,35 @@ struct Raw {
     __device__ __forceinline__ void vec(int i, uint4 v) { r[4 * i] = v.x, r[4 * i + 1] = v.y, r[4 * i + 2] = v.z, r[4 * i + 3] = v.w; }
 };
 
+// The W words that start `bytes` (0 to 15, even) into u, in u[0..W).
+template <int W>
+__device__ __forceinline__ void shift_words(uint32_t (&u)[W + 5], uint32_t bytes) {
+    u[W + 4] = 0;
+    if (bytes & 8u) {
+#pragma unroll
+        for (int i = 0; i < W + 2; ++i) u[i] = u[i + 2];
+    }
+    if (bytes & 4u) {
+#pragma unroll
+        for (int i = 0; i < W + 1; ++i) u[i] = u[i + 1];
+    }
+    if (bytes & 2u) {
+#pragma unroll
+        for (int i = 0; i < W; ++i) u[i] = __funnelshift_r(u[i], u[i + 1], 16);
+    }
+}
+
 constexpr int kTailPad = 32;  // bytes of a row's copy beyond the row: both 16-byte roundings
 
 // One thread's share of a row: which columns it holds, the copies of the rows
 // to come, and the sums over the threads that hold the rest of the row.
 //
-// VEC: octets of 8 consecutive columns, 16-byte accesses (every pointer
-// 16-byte aligned, cols a multiple of 8).  Otherwise single columns, one
-// row's width of threads apart.
+// A thread holds octets of 8 consecutive columns.  VEC: every row is 16-byte
+// aligned (pointers and cols * size), octets are 16-byte accesses.  Otherwise a
+// row starts anywhere in a 16-byte vector: its copy in shared memory keeps that
+// offset, an octet is shifted out of the vectors that cover it, and a lane
+// stores the whole vector that its octet and its neighbour's fill (the warp's
+// outer lanes and the row's end store element by element).
 template <typename T, int NV, bool VEC>
 struct Lane {
     static constexpr int E = 8 * NV, P = E / 2;
@@ -184,8 +208,10 @@ struct Lane {
         }
         if (p.cluster > 1) cluster_sync_all();  // every CTA runs before its memory is written
     }
-    __device__ __forceinline__ int col(int e) const { return VEC ? col0 + (e / 8 * gthreads + t) * 8 + e % 8 : col0 + e * gthreads + t; }
-    __device__ __forceinline__ bool has(int e) const { return VEC ? full || col(e & ~7) < cols : full || col(e) < cols; }
+    __device__ __forceinline__ int col(int e) const { return col0 + (e / 8 * gthreads + t) * 8 + e % 8; }
+    __device__ __forceinline__ bool has(int e) const { return full || col(VEC ? e & ~7 : e) < cols; }
+    // All of octet v is in the row (VEC: or none of it).
+    __device__ __forceinline__ bool whole(int v) const { return full || col(8 * v) + (VEC ? 0 : 7) < cols; }
 
     // Begins the copy of tensor k's row into `stage`; `row` is the element at
     // which the row starts.
@@ -242,20 +268,32 @@ struct Lane {
                     if (!has(8 * (v / PARTS))) w.vec(v, make_uint4(0, 0, 0, 0));
             }
         } else {
-            const uintptr_t at = reinterpret_cast<uintptr_t>(static_cast<const T*>(tensor) + row + col0);
-            const uint32_t slot = ring + static_cast<uint32_t>(stage * tensors + k) * image + static_cast<uint32_t>(at & 15);
+            const uint32_t at = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(static_cast<const T*>(tensor) + row + col0)) & 15u;
+            const uint32_t slot = ring + static_cast<uint32_t>(stage * tensors + k) * image;
 #pragma unroll
-            for (int e = 0; e < E; ++e) {
-                const uint32_t a = slot + static_cast<uint32_t>(e * gthreads + t) * sizeof(T);
-                if constexpr (sizeof(T) == 2) {
-                    uint16_t v = 0;
-                    if (has(e)) asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(a) : "memory");
-                    w.set(e, __ushort_as_half(v));
-                } else {
-                    uint32_t v = 0;
-                    if (has(e)) asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
-                    w.r[e] = v;
+            for (int v = 0; v < NV; ++v) {
+                constexpr int W = 4 * PARTS;  // words of an octet
+                uint32_t u[W + 5];
+#pragma unroll
+                for (int i = 0; i <= PARTS; ++i)
+                    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                                 : "=r"(u[4 * i]), "=r"(u[4 * i + 1]), "=r"(u[4 * i + 2]), "=r"(u[4 * i + 3])
+                                 : "r"(slot + static_cast<uint32_t>((v * gthreads + t) * PARTS + i) * 16)
+                                 : "memory");
+                shift_words<W>(u, at);
+                if (!whole(v)) {  // what lies past the row reads as zero
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        if (has(8 * v + e)) continue;
+                        if constexpr (sizeof(T) == 2) {
+                            u[e / 2] &= e % 2 ? 0x0000FFFFu : 0xFFFF0000u;
+                        } else {
+                            u[e] = 0;
+                        }
+                    }
                 }
+#pragma unroll
+                for (int i = 0; i < W; ++i) w.r[v * W + i] = u[i];
             }
         }
 #pragma unroll
@@ -265,45 +303,79 @@ struct Lane {
     // past the row.
     __device__ __forceinline__ void vector(const void* base, float absent, Raw<T, E>& w) const {
         const T* b = static_cast<const T*>(base);
-        if constexpr (VEC) {
+        const bool vec = VEC || (reinterpret_cast<uintptr_t>(b) & 15) == 0;
 #pragma unroll
-            for (int v = 0; v < NV; ++v) {
-                if (b != nullptr && has(8 * v)) {
+        for (int v = 0; v < NV; ++v) {
+            if (b != nullptr && vec && whole(v) && has(8 * v)) {
 #pragma unroll
-                    for (int i = 0; i < PARTS; ++i) w.vec(v * PARTS + i, __ldg(reinterpret_cast<const uint4*>(b + col(8 * v)) + i));
-                } else {
-                    const T one = from_f<T>(has(8 * v) ? absent : 0.0f);
+                for (int i = 0; i < PARTS; ++i) w.vec(v * PARTS + i, __ldg(reinterpret_cast<const uint4*>(b + col(8 * v)) + i));
+            } else {
 #pragma unroll
-                    for (int e = 8 * v; e < 8 * v + 8; ++e) w.set(e, one);
-                }
+                for (int e = 8 * v; e < 8 * v + 8; ++e) w.set(e, !has(e) ? from_f<T>(0.0f) : b != nullptr ? b[col(e)] : from_f<T>(absent));
             }
-        } else {
-#pragma unroll
-            for (int e = 0; e < E; ++e) w.set(e, !has(e) ? from_f<T>(0.0f) : b != nullptr ? b[col(e)] : from_f<T>(absent));
         }
     }
     __device__ __forceinline__ void store(void* tensor, int64_t row, const float2 (&v)[P]) const {
         T* b = static_cast<T*>(tensor) + row;
-        if constexpr (VEC) {
 #pragma unroll
-            for (int k = 0; k < NV; ++k) {
+        for (int k = 0; k < NV; ++k) {
+            constexpr int W = 4 * PARTS;
+            uint32_t o[W];
+            if constexpr (sizeof(T) == 2) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const __half2 h = __float22half2_rn(v[4 * k + i]);
+                    o[i] = *reinterpret_cast<const uint32_t*>(&h);
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) o[i] = __float_as_uint(i % 2 ? v[4 * k + i / 2].y : v[4 * k + i / 2].x);
+            }
+            T* to = b + col(8 * k);
+            if constexpr (VEC) {
                 if (!has(8 * k)) continue;
-                if constexpr (sizeof(T) == 2) {
-                    uint4 u;
-                    __half2* h = reinterpret_cast<__half2*>(&u);
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) h[i] = __float22half2_rn(v[4 * k + i]);
-                    *reinterpret_cast<uint4*>(b + col(8 * k)) = u;
+                for (int i = 0; i < PARTS; ++i) reinterpret_cast<uint4*>(to)[i] = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+            } else {
+                // `off` bytes of the octet's first vector belong to the octet before
+                const uint32_t off = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(to)) & 15u;
+                uint32_t u[W + 5];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) u[i] = __shfl_up_sync(0xFFFFFFFFu, o[W - 4 + i], 1);
+#pragma unroll
+                for (int i = 0; i < W; ++i) u[4 + i] = o[i];
+                if (off == 0) {
+#pragma unroll
+                    for (int i = 0; i < W; ++i) u[i] = o[i];
                 } else {
+                    shift_words<W>(u, 16u - off);
+                }
+                const bool me = whole(k) && has(8 * k);
+                if (me && (lane > 0 || off == 0)) {
+                    uint4* q = reinterpret_cast<uint4*>(reinterpret_cast<uintptr_t>(to) - off);
 #pragma unroll
-                    for (int i = 0; i < 2; ++i)
-                        reinterpret_cast<float4*>(b + col(8 * k))[i] = make_float4(v[4 * k + 2 * i].x, v[4 * k + 2 * i].y, v[4 * k + 2 * i + 1].x, v[4 * k + 2 * i + 1].y);
+                    for (int i = 0; i < PARTS; ++i) q[i] = make_uint4(u[4 * i], u[4 * i + 1], u[4 * i + 2], u[4 * i + 3]);
+                }
+                // what no whole store covers: the head of a first or partial
+                // octet, the tail where the next lane stores no whole vector
+                const bool next = lane < 31 && (full || col(8 * k) + 15 < cols);
+                const int count = full ? 8 : min(8, max(0, cols - col(8 * k)));        // elements of the octet in the row
+                const int split = static_cast<int>((16u * PARTS - off) / sizeof(T));  // elements in its own vectors
+                const uint32_t head = (1u << min(split, 8)) - 1u;
+                uint32_t need = me && (lane > 0 || off == 0) ? 0u : head;
+                if (off != 0 && !next) need |= ~head;
+                need &= (1u << count) - 1u;
+                if (need != 0) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        if constexpr (sizeof(T) == 2) {
+                            if ((need >> e) & 1u) reinterpret_cast<uint16_t*>(to)[e] = static_cast<uint16_t>(e % 2 ? o[e / 2] >> 16 : o[e / 2]);
+                        } else {
+                            if ((need >> e) & 1u) reinterpret_cast<uint32_t*>(to)[e] = o[e];
+                        }
+                    }
                 }
             }
-        } else {
-#pragma unroll
-            for (int e = 0; e < E; ++e)
-                if (has(e)) b[col(e)] = from_f<T>(e % 2 ? v[e / 2].y : v[e / 2].x);
         }
     }
     // Keep bits of this thread's columns of the row that starts at an element.
@@ -313,25 +385,13 @@ struct Lane {
 #pragma unroll
             for (int v = 0; v < NV; ++v) m |= dropout_keep8(p.dropout, static_cast<uint32_t>((row + col(8 * v)) / 8)) << (8 * v);
         } else {
-            // Columns e of the warp's lanes are 32 consecutive elements, 4 *
-            // block + shift on: eight blocks of four, a ninth where shift > 0.
-            // Lane 4 q + r works out block q for the columns e = r mod 4, lane
-            // e the ninth of column e; each lane then fetches the four keep
-            // bits of its own block.
-            const uint64_t first = static_cast<uint64_t>(row + col0 + warp * 32);
-            const uint32_t shift = static_cast<uint32_t>(first) & 3u;
-            const uint32_t q = (shift + lane) >> 2, bit = (shift + lane) & 3u;
-            uint32_t mine = 0, ninth = 0;  // four keep bits each
+            // the octet's elements begin `shift` into a block of four
+            const uint32_t shift = static_cast<uint32_t>(row) & 3u;
 #pragma unroll
-            for (int a = 0; a < E / 4; ++a)
-                mine |= dropout_keep4(p.dropout, static_cast<uint32_t>((first + static_cast<uint64_t>(4 * a + (lane & 3)) * gthreads) / 4) + (lane >> 2)) << (4 * (a % 8));
-            if (shift != 0) ninth = dropout_keep4(p.dropout, static_cast<uint32_t>((first + static_cast<uint64_t>(lane % E) * gthreads) / 4) + 8);
-#pragma unroll
-            for (int e = 0; e < E; ++e) {
-                uint32_t four = __shfl_sync(0xFFFFFFFFu, mine, (q & 7) * 4 + e % 4) >> (4 * (e / 4));
-                const uint32_t edge = __shfl_sync(0xFFFFFFFFu, ninth, e);
-                if (q == 8) four = edge;
-                m |= ((four >> bit) & 1u) << e;
+            for (int v = 0; v < NV; ++v) {
+                const uint32_t block = static_cast<uint32_t>((row + col(8 * v)) / 4);
+                const uint32_t bits = dropout_keep4(p.dropout, block) | dropout_keep4(p.dropout, block + 1) << 4 | dropout_keep4(p.dropout, block + 2) << 8;
+                m |= ((bits >> shift) & 0xFFu) << (8 * v);
             }
         }
         return m;
@@ -384,13 +444,20 @@ struct Lane {
         const float2 shift = both(-mean);
         float2 s = make_float2(0.0f, 0.0f);
 #pragma unroll
-        for (int i = 0; i < P; ++i) {
-            const float2 c = add2(v[i], shift);
-            if constexpr (VEC) {
-                if (has(2 * i)) s = fma2(c, c, s);
-            } else {
-                if (has(2 * i)) s.x = fmaf(c.x, c.x, s.x);
-                if (has(2 * i + 1)) s.y = fmaf(c.y, c.y, s.y);
+        for (int o = 0; o < NV; ++o) {
+            if (VEC ? has(8 * o) : whole(o)) {
+#pragma unroll
+                for (int i = 4 * o; i < 4 * o + 4; ++i) {
+                    const float2 c = add2(v[i], shift);
+                    s = fma2(c, c, s);
+                }
+            } else if constexpr (!VEC) {
+#pragma unroll
+                for (int i = 4 * o; i < 4 * o + 4; ++i) {
+                    const float2 c = add2(v[i], shift);
+                    if (has(2 * i)) s.x = fmaf(c.x, c.x, s.x);
+                    if (has(2 * i + 1)) s.y = fmaf(c.y, c.y, s.y);
+                }
             }
         }
         rstd = rsqrtf(row_sum<1>(make_float2(s.x + s.y, 0.0f)).x * p.inv_cols + p.eps);
@@ -572,7 +639,8 @@ __device__ __forceinline__ void flush_columns(const Lane<T, NV, VEC>& ln, float*
     }
 }
 
-template <typename T, int NV, bool VEC, bool POST, bool GATE>
+// SUMS: keeps the column sums; otherwise leaves p.means for the column pass.
+template <typename T, int NV, bool VEC, bool POST, bool GATE, bool SUMS>
 __global__ void __launch_bounds__(kMaxThreads, 1) residual_norm_backward_kernel(const RnParams p) {
     extern __shared__ __align__(16) uint8_t smem[];
     using L = Lane<T, NV, VEC>;
@@ -582,15 +650,17 @@ __global__ void __launch_bounds__(kMaxThreads, 1) residual_norm_backward_kernel(
     float* const buf = reinterpret_cast<float*>(smem + 2 * sizeof(float2) * ((ln.red_stride + 1) & ~1));
     const int64_t unit = blockIdx.x / p.cluster;
     const int64_t unit_lo = unit_begin(unit, p.rows, p.units), unit_hi = unit_begin(unit + 1, p.rows, p.units);
-    const bool gate_sums = GATE && p.gate_period > 1;  // else each row writes its own gradient
+    const bool gate_sums = GATE && SUMS && p.gate_period > 1;  // else each row writes its own gradient
     Raw<T, L::E> w, pw, gate;
     ln.vector(p.weight, 1.0f, w);
     if constexpr (POST) ln.vector(p.post_weight, 1.0f, pw);
-    float2 dw[P], db[P], dpw[POST ? P : 1], dpb[POST ? P : 1], dgt[GATE ? P : 1];
+    float2 dw[SUMS ? P : 1], db[SUMS ? P : 1], dpw[POST && SUMS ? P : 1], dpb[POST && SUMS ? P : 1], dgt[GATE && SUMS ? P : 1];
+    if constexpr (SUMS) {
 #pragma unroll
-    for (int i = 0; i < P; ++i) {
-        dw[i] = db[i] = make_float2(0.0f, 0.0f);
-        if constexpr (POST) dpw[i] = dpb[i] = make_float2(0.0f, 0.0f);
+        for (int i = 0; i < P; ++i) {
+            dw[i] = db[i] = make_float2(0.0f, 0.0f);
+            if constexpr (POST) dpw[i] = dpb[i] = make_float2(0.0f, 0.0f);
+        }
     }
     int64_t gate_row = -1;
     // a segment: the rows of this unit that share a gate row (all of them
@@ -599,7 +669,7 @@ __global__ void __launch_bounds__(kMaxThreads, 1) residual_norm_backward_kernel(
     while (seg_lo < unit_hi) {
         const int64_t seg_gate = gate_sums ? seg_lo / p.gate_period : 0;
         const int64_t seg_hi = gate_sums ? min(unit_hi, (seg_gate + 1) * p.gate_period) : unit_hi;
-        if constexpr (GATE) {
+        if constexpr (GATE && SUMS) {
 #pragma unroll
             for (int i = 0; i < P; ++i) dgt[i] = make_float2(0.0f, 0.0f);
         }
@@ -628,14 +698,17 @@ __global__ void __launch_bounds__(kMaxThreads, 1) residual_norm_backward_kernel(
 #pragma unroll
                     for (int i = 0; i < P; ++i) {
                         n[i] = mul2(add2(n[i], c), s);
-                        dw[i] = fma2(h[i], n[i], dw[i]);
-                        db[i] = add2(db[i], h[i]);
+                        if constexpr (SUMS) {
+                            dw[i] = fma2(h[i], n[i], dw[i]);
+                            db[i] = add2(db[i], h[i]);
+                        }
                         h[i] = mul2(h[i], w.pair(i));  // 0 past the row
                         s1 = add2(s1, h[i]);
                         s2 = fma2(h[i], n[i], s2);
                     }
                     s1 = ln.template row_sum<2>(make_float2(s1.x + s1.y, s2.x + s2.y));
                     const float2 m1 = both(p.layer ? -s1.x * p.inv_cols : 0.0f), m2 = both(-s1.y * p.inv_cols);
+                    if (!SUMS && ln.t == 0 && ln.rank == 0) p.means[r] = make_float2(-m1.x, -m2.x);
 #pragma unroll
                     for (int i = 0; i < P; ++i) h[i] = add2(fma2(n[i], m2, h[i]), m1);
                     if (p.gx != nullptr) {
@@ -667,28 +740,32 @@ __global__ void __launch_bounds__(kMaxThreads, 1) residual_norm_backward_kernel(
                     }
                 }
                 if constexpr (GATE) {
-                    float2 u[P];
-                    if constexpr (POST) {
+                    if (SUMS || (p.gate_period == 1 && p.dgate != nullptr)) {
+                        float2 u[P];
+                        if constexpr (POST) {
 #pragma unroll
-                        for (int i = 0; i < P; ++i) u[i] = mul2(q[i], pw.pair(i));
-                        if (p.post_bias != nullptr) {
-                            Raw<T, L::E> pb;
-                            ln.vector(p.post_bias, 0.0f, pb);
+                            for (int i = 0; i < P; ++i) u[i] = mul2(q[i], pw.pair(i));
+                            if (p.post_bias != nullptr) {
+                                Raw<T, L::E> pb;
+                                ln.vector(p.post_bias, 0.0f, pb);
 #pragma unroll
-                            for (int i = 0; i < P; ++i) u[i] = add2(u[i], pb.pair(i));
+                                for (int i = 0; i < P; ++i) u[i] = add2(u[i], pb.pair(i));
+                            }
+                        } else {
+#pragma unroll
+                            for (int i = 0; i < P; ++i) u[i] = q[i];
                         }
-                    } else {
+                        if (p.drop) ln.drop(keep, u);
+                        if (gate_sums) {
+                            if constexpr (SUMS) {
 #pragma unroll
-                        for (int i = 0; i < P; ++i) u[i] = q[i];
-                    }
-                    if (p.drop) ln.drop(keep, u);
-                    if (gate_sums) {
+                                for (int i = 0; i < P; ++i) dgt[i] = fma2(u[i], g[i], dgt[i]);
+                            }
+                        } else if (p.dgate != nullptr) {
 #pragma unroll
-                        for (int i = 0; i < P; ++i) dgt[i] = fma2(u[i], g[i], dgt[i]);
-                    } else if (p.dgate != nullptr) {
-#pragma unroll
-                        for (int i = 0; i < P; ++i) u[i] = mul2(u[i], g[i]);
-                        ln.store(p.dgate, at, u);
+                            for (int i = 0; i < P; ++i) u[i] = mul2(u[i], g[i]);
+                            ln.store(p.dgate, at, u);
+                        }
                     }
                     const int64_t k = p.gate_period == p.rows ? 0 : r / p.gate_period;
                     if (k != gate_row) ln.vector(static_cast<const T*>(p.gate) + k * p.cols, 0.0f, gate);
@@ -707,8 +784,10 @@ __global__ void __launch_bounds__(kMaxThreads, 1) residual_norm_backward_kernel(
                     float2 s3 = make_float2(0.0f, 0.0f), s4 = s3;
 #pragma unroll
                     for (int i = 0; i < P; ++i) {
-                        dpw[i] = fma2(g[i], q[i], dpw[i]);
-                        dpb[i] = add2(dpb[i], g[i]);
+                        if constexpr (SUMS) {
+                            dpw[i] = fma2(g[i], q[i], dpw[i]);
+                            dpb[i] = add2(dpb[i], g[i]);
+                        }
                         g[i] = mul2(g[i], pw.pair(i));  // 0 past the row
                         s3 = add2(s3, g[i]);
                         s4 = fma2(g[i], q[i], s4);
@@ -720,7 +799,7 @@ __global__ void __launch_bounds__(kMaxThreads, 1) residual_norm_backward_kernel(
                 }
                 if (p.df != nullptr) ln.store(p.df, at, g);
             });
-        if constexpr (GATE) {
+        if constexpr (GATE && SUMS) {
             if (gate_sums && p.dgate != nullptr) {
                 // whole segments are finished here; one that other units share
                 // goes to the unit's first or last slot
@@ -734,6 +813,7 @@ __global__ void __launch_bounds__(kMaxThreads, 1) residual_norm_backward_kernel(
             if (seg_lo < unit_hi) ln.group_sync();  // the segment's copies are read before the next one's begin
         }
     }
+    if constexpr (SUMS) {
     const int64_t plane = static_cast<int64_t>(p.units) * p.cols;
     flush_columns<T, NV, VEC>(ln, buf, dw, p.partial + unit * p.cols, nullptr);
     flush_columns<T, NV, VEC>(ln, buf, db, p.partial + plane + unit * p.cols, nullptr);
@@ -741,38 +821,163 @@ __global__ void __launch_bounds__(kMaxThreads, 1) residual_norm_backward_kernel(
         flush_columns<T, NV, VEC>(ln, buf, dpw, p.partial + 2 * plane + unit * p.cols, nullptr);
         flush_columns<T, NV, VEC>(ln, buf, dpb, p.partial + 3 * plane + unit * p.cols, nullptr);
     }
+    }
 }
 
-constexpr int kColLanes = 32, kColRows = 32;
+// Column sums of wide rows: a block's threads take V columns each (8 where rows
+// are 16-byte aligned) over the rows of a unit, and leave partial sums, or
+// finished gate rows, as the kernel above does.
+constexpr int kPassThreads = 128;
 
-// The units' partial sums added in a fixed order, rounded once.  Items 0..3 are
-// the parameter vectors; the others finish gate rows that several units share:
-// item 4 + g gate row g, or (by_unit, fewer units than gate rows) item 4 + c
-// the gate row that unit c ends and unit c + 1 continues.
-template <typename T>
-__global__ void __launch_bounds__(kColLanes* kColRows)
-residual_norm_columns_kernel(const RnParams p, T* d0, T* d1, T* d2, T* d3, int col_blocks, bool by_unit) {
+template <typename T, int V, bool POST, bool GATE>
+__global__ void __launch_bounds__(kPassThreads) residual_norm_column_pass_kernel(const RnParams p) {
     pdl_wait();
-    __shared__ float part[kColRows][kColLanes + 1];
-    const int item = static_cast<int>(blockIdx.x) / col_blocks;
-    const int64_t c = static_cast<int64_t>(blockIdx.x - item * col_blocks) * kColLanes + threadIdx.x;
+    const int64_t c = (static_cast<int64_t>(blockIdx.x) * kPassThreads + threadIdx.x) * V;
+    if (c >= p.cols) return;
+    const int64_t unit = blockIdx.y;
+    const int64_t lo = unit_begin(unit, p.rows, p.units), hi = unit_begin(unit + 1, p.rows, p.units);
+    auto load = [&](const void* tensor, int64_t row, float (&o)[V]) {
+        const T* src = static_cast<const T*>(tensor) + row * p.cols + c;
+        if constexpr (V == 8) {
+            Raw<T, 8> w;
+#pragma unroll
+            for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i) w.vec(i, __ldg(reinterpret_cast<const uint4*>(src) + i));
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float2 f = w.pair(i);
+                o[2 * i] = f.x;
+                o[2 * i + 1] = f.y;
+            }
+        } else {
+            o[0] = static_cast<float>(src[0]);
+        }
+    };
+    float w[V], pw[V], pb[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) w[i] = pw[i] = 1.0f, pb[i] = 0.0f;
+    if (p.weight != nullptr) load(p.weight, 0, w);
+    if (POST && p.post_weight != nullptr) load(p.post_weight, 0, pw);
+    if (POST && p.post_bias != nullptr) load(p.post_bias, 0, pb);
+    float dw[V] = {}, db[V] = {}, dpw[V] = {}, dpb[V] = {};
+    const bool gate_sums = GATE && p.gate_period > 1 && p.dgate != nullptr;
+    int64_t seg_lo = lo;
+    while (seg_lo < hi) {
+        const int64_t gate_row = GATE ? seg_lo / p.gate_period : 0;
+        const int64_t seg_hi = GATE ? min(hi, (gate_row + 1) * p.gate_period) : hi;
+        float dgt[V] = {}, gate[V];
+        if (GATE) load(p.gate, gate_row, gate);
+#pragma unroll 2
+        for (int64_t r = seg_lo; r < seg_hi; ++r) {
+            const float4 st = p.stats[r];
+            float n[V], h[V], g[V], q[V];
+            float2 m = make_float2(0.0f, 0.0f);
+#pragma unroll
+            for (int i = 0; i < V; ++i) h[i] = g[i] = 0.0f;
+            load(p.x_new, r, n);
+            if (p.gh != nullptr) {
+                load(p.gh, r, h);
+                m = p.means[r];
+            }
+            if ((POST || GATE) && p.gx != nullptr) load(p.gx, r, g);
+            if (POST || GATE) load(p.f, r, q);
+            uint32_t keep = 0xFFu;
+            if ((POST || GATE) && p.drop) {
+                const uint64_t e = static_cast<uint64_t>(r * p.cols + c);
+                if constexpr (V == 8) {
+                    keep = dropout_keep8(p.dropout, static_cast<uint32_t>(e / 8));
+                } else {
+                    keep = dropout_keep4(p.dropout, static_cast<uint32_t>(e / 4)) >> (e & 3);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                n[i] = (n[i] - st.z) * st.w;
+                dw[i] = fmaf(h[i], n[i], dw[i]);
+                db[i] += h[i];
+                if constexpr (POST || GATE) {
+                    float u = POST ? (q[i] - st.x) * st.y : q[i];
+                    const float qn = u;
+                    if (POST) u = fmaf(u, pw[i], pb[i]);
+                    g[i] = fmaf(st.w, h[i] * w[i] - n[i] * m.y - m.x, g[i]);
+                    const bool kept = !p.drop || (keep >> i & 1u);
+                    const float s = p.drop ? p.dropout.scale : 1.0f;
+                    if (GATE) {
+                        dgt[i] += kept ? g[i] * u * s : 0.0f;
+                        g[i] *= gate[i];
+                    }
+                    if (POST) {
+                        g[i] = kept ? g[i] * s : 0.0f;
+                        dpw[i] = fmaf(g[i], qn, dpw[i]);
+                        dpb[i] += g[i];
+                    }
+                }
+            }
+        }
+        if (gate_sums) {
+            const bool whole = seg_lo == gate_row * p.gate_period && seg_hi == (gate_row + 1) * p.gate_period;
+            float* slot = p.partial + (4 * static_cast<int64_t>(p.units) + 2 * unit + (seg_lo == lo ? 0 : 1)) * p.cols + c;
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                if (whole) {
+                    static_cast<T*>(p.dgate)[gate_row * p.cols + c + i] = from_f<T>(dgt[i]);
+                } else {
+                    slot[i] = dgt[i];
+                }
+            }
+        }
+        seg_lo = seg_hi;
+    }
+    const int64_t plane = static_cast<int64_t>(p.units) * p.cols;
+    float* out = p.partial + unit * p.cols + c;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        out[i] = dw[i];
+        out[plane + i] = db[i];
+        if (POST) {
+            out[2 * plane + i] = dpw[i];
+            out[3 * plane + i] = dpb[i];
+        }
+    }
+}
+
+constexpr int kColLanes = 32;
+
+// The units' partial sums added in a fixed order, rounded once: blockDim.y
+// units at a time.  The first `vectors` items are the parameter vectors asked
+// for (plane[i] of the partial sums to out[i]); the others finish gate rows
+// that several units share: item vectors + g gate row g, or (by_unit, fewer
+// units than gate rows) item vectors + c the gate row that unit c ends and unit
+// c + 1 continues.
+struct ColumnJobs {
+    void* out[4];
+    int plane[4];
+    int vectors, col_blocks;
+    bool by_unit;
+};
+
+template <typename T>
+__global__ void __launch_bounds__(1024) residual_norm_columns_kernel(const RnParams p, const __grid_constant__ ColumnJobs j) {
+    pdl_wait();
+    __shared__ float part[32][kColLanes + 1];
+    const int item = static_cast<int>(blockIdx.x) / j.col_blocks;
+    const int64_t c = static_cast<int64_t>(blockIdx.x - item * j.col_blocks) * kColLanes + threadIdx.x;
+    const int step = static_cast<int>(blockDim.y);
     float s = 0.0f;
     T* out;
-    if (item < 4) {
-        out = item == 0 ? d0 : item == 1 ? d1 : item == 2 ? d2 : d3;
-        if (out == nullptr) return;
+    if (item < j.vectors) {
+        out = static_cast<T*>(j.out[item]);
         if (c < p.cols) {
-            const float* src = p.partial + static_cast<int64_t>(item) * p.units * p.cols + c;
+            const float* src = p.partial + static_cast<int64_t>(j.plane[item]) * p.units * p.cols + c;
 #pragma unroll 4
-            for (int u = threadIdx.y; u < p.units; u += kColRows) s += src[static_cast<int64_t>(u) * p.cols];
+            for (int u = threadIdx.y; u < p.units; u += step) s += src[static_cast<int64_t>(u) * p.cols];
         }
     } else {
-        int64_t row = item - 4, first;
-        if (by_unit) {
-            const int64_t start = unit_begin(item - 4 + 1, p.rows, p.units);
+        int64_t row = item - j.vectors, first;
+        if (j.by_unit) {
+            const int64_t start = unit_begin(row + 1, p.rows, p.units);
+            first = unit_of(start / p.gate_period * p.gate_period, p.rows, p.units);
+            if (start % p.gate_period == 0 || first != row) return;
             row = start / p.gate_period;
-            first = unit_of(row * p.gate_period, p.rows, p.units);
-            if (start % p.gate_period == 0 || first != item - 4) return;
         } else {
             first = unit_of(row * p.gate_period, p.rows, p.units);
         }
@@ -782,7 +987,7 @@ residual_norm_columns_kernel(const RnParams p, T* d0, T* d1, T* d2, T* d3, int c
         if (c < p.cols) {
             const float* src = p.partial + 4 * static_cast<int64_t>(p.units) * p.cols + c;
 #pragma unroll 4
-            for (int64_t u = first + threadIdx.y; u <= last; u += kColRows) {
+            for (int64_t u = first + threadIdx.y; u <= last; u += step) {
                 const int64_t slot = 2 * u + (unit_begin(u, p.rows, p.units) / p.gate_period == row ? 0 : 1);
                 s += src[slot * p.cols];
             }
@@ -792,40 +997,43 @@ residual_norm_columns_kernel(const RnParams p, T* d0, T* d1, T* d2, T* d3, int c
     __syncthreads();
     if (threadIdx.y == 0 && c < p.cols) {
         s = 0.0f;
-#pragma unroll
-        for (int i = 0; i < kColRows; ++i) s += part[i][threadIdx.x];
+        for (int i = 0; i < step; ++i) s += part[i][threadIdx.x];
         out[c] = from_f<T>(s);
     }
 }
 
 // ---- host ----------------------------------------------------------------------
 
-// NV octets per thread, W warps per row and CTA, CTAs per row: the cover of
-// the row with the least idle columns, more octets per thread where equal
-// (fewer warps to sum over).  NV 3 holds 768 columns in one warp, NV 4 up to
-// 16384 in one CTA (forward only: the backward pass keeps two to five sums per
-// column in registers: with a post norm or a gate NV 1, 153 us against 198 us
-// with NV 2 and its spills at 8192 x 4096).  fp32 doubles the bytes of a slot and takes 1.
+// NV octets per thread, W warps per row and CTA, CTAs per row.  A warp's work
+// for a row is about two octets' worth of sums and addresses and NV octets, so
+// the least W * (2 + NV) is taken (8192 x 4096 with both norms, forward: NV 1
+// 91 us, 2 58 us, 4 60 us).  Registers rule some out: NV 3 with a post norm
+// spills; the backward pass keeps two sums per column up to NV 2 (NV 3: 154
+// against 93 us), five at NV 1 (NV 2: 198 against 153 us).  fp32 doubles the
+// bytes of a row's copy: NV 1 (2331 x 1151 forward: 32 us, with NV 2 40 us),
+// and forward 2 where that spares a cluster.
+enum Pass { kForward, kSums2, kSums5, kNoSums };
+
 struct Geometry {
     int nv, warps, cluster, groups;
 };
 
-Geometry geometry(const RnParams& p, bool f16, bool vec, bool backward, bool sums5) {
+Geometry geometry(int64_t cols, bool f16, Pass pass, bool post) {
     Geometry best = {1, 1, 1, 1};
-    int64_t best_cover = INT64_MAX;
-    const int nv_max = !f16 ? 1 : !vec ? 2 : !backward ? 4 : sums5 ? 1 : 3;
+    int64_t best_cost = INT64_MAX;
+    const int nv_max = pass == kForward ? (f16 ? 4 : cols > 4096 ? 2 : 1) : pass == kSums5 || !f16 ? 1 : 2;
     for (int nv = nv_max; nv >= 1; --nv) {
-        if (nv == 4 && p.cols <= 8192) continue;
+        if (nv == 3 && post) continue;
         const int64_t per_warp = 256 * nv;
         const int max_warps = nv == 3 ? 8 : kMaxThreads / 32;
-        const int64_t need = ceil_div(p.cols, per_warp);
+        const int64_t need = ceil_div(cols, per_warp);
         int cluster = 1;
         while (cluster * max_warps < need && cluster < kMaxCluster) cluster *= 2;
         const int64_t warps = ceil_div(need, cluster);
         if (warps > max_warps) continue;
-        const int64_t cover = warps * cluster * per_warp * (cluster > 1 ? 2 : 1);
-        if (cover < best_cover) {
-            best_cover = cover;
+        const int64_t cost = warps * cluster * (2 + nv) * (cluster > 1 ? 2 : 1);
+        if (cost < best_cost) {
+            best_cost = cost;
             best = {nv, static_cast<int>(warps), cluster, 1};
         }
     }
@@ -837,31 +1045,32 @@ using Kernel = void (*)(RnParams);
 
 template <typename T, bool VEC>
 Kernel forward_kernel(int nv, bool post) {
-    if constexpr (VEC && sizeof(T) == 2) {
-        if (nv == 4) return post ? residual_norm_kernel<T, 4, VEC, true> : residual_norm_kernel<T, 4, VEC, false>;
-        if (nv == 3) return post ? residual_norm_kernel<T, 3, VEC, true> : residual_norm_kernel<T, 3, VEC, false>;
-    }
     if constexpr (sizeof(T) == 2) {
-        if (nv == 2) return post ? residual_norm_kernel<T, 2, VEC, true> : residual_norm_kernel<T, 2, VEC, false>;
+        if (nv == 4) return post ? residual_norm_kernel<T, 4, VEC, true> : residual_norm_kernel<T, 4, VEC, false>;
+        if (nv == 3) return residual_norm_kernel<T, 3, VEC, false>;
     }
+    if (nv == 2) return post ? residual_norm_kernel<T, 2, VEC, true> : residual_norm_kernel<T, 2, VEC, false>;
     return post ? residual_norm_kernel<T, 1, VEC, true> : residual_norm_kernel<T, 1, VEC, false>;
 }
 
-template <typename T, int NV, bool VEC>
-Kernel backward_kernel_nv(bool post, bool gate) {
-    if (post) return gate ? residual_norm_backward_kernel<T, NV, VEC, true, true> : residual_norm_backward_kernel<T, NV, VEC, true, false>;
-    return gate ? residual_norm_backward_kernel<T, NV, VEC, false, true> : residual_norm_backward_kernel<T, NV, VEC, false, false>;
+template <typename T, int NV, bool VEC, bool SUMS>
+Kernel backward_kernel_of(bool post, bool gate) {
+    if (post) return gate ? residual_norm_backward_kernel<T, NV, VEC, true, true, SUMS> : residual_norm_backward_kernel<T, NV, VEC, true, false, SUMS>;
+    return gate ? residual_norm_backward_kernel<T, NV, VEC, false, true, SUMS> : residual_norm_backward_kernel<T, NV, VEC, false, false, SUMS>;
 }
 
 template <typename T, bool VEC>
-Kernel backward_kernel(int nv, bool post, bool gate) {
-    if constexpr (VEC && sizeof(T) == 2) {
-        if (nv == 3) return residual_norm_backward_kernel<T, 3, VEC, false, false>;
-    }
+Kernel backward_kernel(int nv, bool post, bool gate, bool sums) {
     if constexpr (sizeof(T) == 2) {
-        if (nv == 2) return backward_kernel_nv<T, 2, VEC>(post, gate);
+        if (nv == 2) return sums ? residual_norm_backward_kernel<T, 2, VEC, false, false, true> : backward_kernel_of<T, 2, VEC, false>(post, gate);
     }
-    return backward_kernel_nv<T, 1, VEC>(post, gate);
+    return sums ? backward_kernel_of<T, 1, VEC, true>(post, gate) : backward_kernel_of<T, 1, VEC, false>(post, gate);
+}
+
+template <typename T, int V>
+Kernel column_pass_of(bool post, bool gate) {
+    if (post) return gate ? residual_norm_column_pass_kernel<T, V, true, true> : residual_norm_column_pass_kernel<T, V, true, false>;
+    return gate ? residual_norm_column_pass_kernel<T, V, false, true> : residual_norm_column_pass_kernel<T, V, false, false>;
 }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
@@ -923,6 +1132,7 @@ int max_units(int device, int64_t rows, const Geometry& g, int per_sm) {
 }
 
 constexpr size_t kSmemPerSm = 220 * 1024;
+constexpr int kSmemMost = 227 * 1024;
 
 size_t stage_bytes(const Geometry& g, bool f16, bool vec, int tensors) {
     const size_t row = static_cast<size_t>(g.warps) * 32 * g.nv * (f16 ? 16 : 32);
@@ -945,7 +1155,6 @@ size_t configure(RnParams& p, const Geometry& g, bool f16, bool vec, int tensors
 }
 
 int launch(Kernel k, const RnParams& p, size_t smem, cudaStream_t s, const char* what) {
-    TK_CUDA_TRY(cudaFuncSetAttribute(reinterpret_cast<const void*>(k), cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = p.cluster;
@@ -966,7 +1175,7 @@ int launch(Kernel k, const RnParams& p, size_t smem, cudaStream_t s, const char*
 }
 
 int resident_ctas(Kernel k, const RnParams& p, size_t smem, int& per_sm) {
-    TK_CUDA_TRY(cudaFuncSetAttribute(reinterpret_cast<const void*>(k), cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
+    TK_CUDA_TRY(cudaFuncSetAttribute(reinterpret_cast<const void*>(k), cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemMost));
     TK_CUDA_TRY(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, reinterpret_cast<const void*>(k), p.warps * 32 * p.groups, smem));
     if (per_sm < 1) TK_FAIL(TK_ERR_CUDA, "residual norm: the kernel does not fit an SM");
     return TK_OK;
@@ -975,14 +1184,33 @@ int resident_ctas(Kernel k, const RnParams& p, size_t smem, int& per_sm) {
 // CTAs per SM the backward pass may use: its partial sums are sized by it.
 constexpr int kBackwardPerSm = 4;
 
+// Rows that one CTA cannot hold together with their column sums.
+bool is_wide(const tk_residual_norm_desc_t& d) {
+    const bool sums5 = d.post_norm != 0 || d.gate != nullptr;
+    return d.cols > (sums5 || d.dtype == TK_DTYPE_F32 ? 1 : 2) * 256 * (kMaxThreads / 32);
+}
+
+// Row ranges of the column pass: about eight blocks per SM.
+int column_units(int device, int64_t rows, int64_t cols, bool vec) {
+    const int64_t blocks = ceil_div(cols, kPassThreads * (vec ? 8 : 1));
+    return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(rows, ceil_div(8 * sm_count(device), blocks))));
+}
+
 template <typename T>
 int columns(const RnParams& p, const tk_residual_norm_grad_desc_t& g, bool gate_items, cudaStream_t s) {
-    const int col_blocks = static_cast<int>(ceil_div(p.cols, kColLanes));
-    const bool by_unit = gate_items && p.rows / p.gate_period > p.units;
-    const int items = 4 + (!gate_items ? 0 : by_unit ? p.units - 1 : static_cast<int>(p.rows / p.gate_period));
-    cudaError_t e = launch_pdl(residual_norm_columns_kernel<T>, dim3(static_cast<unsigned>(items) * col_blocks), dim3(kColLanes, kColRows), 0, s,
-                               p, static_cast<T*>(g.dweight), static_cast<T*>(g.dbias), static_cast<T*>(g.dpost_weight),
-                               static_cast<T*>(g.dpost_bias), col_blocks, by_unit);
+    ColumnJobs j = {};
+    void* const outs[4] = {g.dweight, g.dbias, g.dpost_weight, g.dpost_bias};
+    for (int i = 0; i < 4; ++i) {
+        if (outs[i] == nullptr || (i >= 2 && !g.fwd.post_norm)) continue;
+        j.out[j.vectors] = outs[i];
+        j.plane[j.vectors++] = i;
+    }
+    j.col_blocks = static_cast<int>(ceil_div(p.cols, kColLanes));
+    j.by_unit = gate_items && p.rows / p.gate_period > p.units;
+    const int items = j.vectors + (!gate_items ? 0 : j.by_unit ? p.units - 1 : static_cast<int>(p.rows / p.gate_period));
+    if (items == 0) return TK_OK;
+    const int rows = std::max(1, std::min(32, (p.units + 3) / 4));  // about four partial sums per thread
+    cudaError_t e = launch_pdl(residual_norm_columns_kernel<T>, dim3(static_cast<unsigned>(items) * j.col_blocks), dim3(kColLanes, rows), 0, s, p, j);
     if (e != cudaSuccess) {
         cudaGetLastError();
         TK_FAIL(TK_ERR_CUDA, "residual norm columns launch failed: %s", cudaGetErrorString(e));
@@ -1005,7 +1233,7 @@ int tk_residual_norm(const tk_residual_norm_desc_t* desc, void* stream) {
     TK_CHECK_ARG(aligned16(d.stats), "tk_residual_norm: stats must be 16-byte aligned");
     RnParams p = params(d);
     const bool f16 = d.dtype == TK_DTYPE_F16, vec = vectorised(p);
-    const Geometry g = geometry(p, f16, vec, false, false);
+    const Geometry g = geometry(p.cols, f16, kForward, d.post_norm != 0);
     const size_t smem = configure(p, g, f16, vec, 2, false);
     const Kernel k = f16 ? (vec ? forward_kernel<__half, true>(g.nv, d.post_norm) : forward_kernel<__half, false>(g.nv, d.post_norm))
                          : (vec ? forward_kernel<float, true>(g.nv, d.post_norm) : forward_kernel<float, false>(g.nv, d.post_norm));
@@ -1018,9 +1246,13 @@ int tk_residual_norm(const tk_residual_norm_desc_t* desc, void* stream) {
 size_t tk_residual_norm_backward_workspace_size(const tk_residual_norm_grad_desc_t* desc) {
     using namespace tk;
     if (desc == nullptr || check("tk_residual_norm_backward", desc->fwd) != TK_OK) return 0;
-    // [4 + 2][units][cols] fp32 partial sums, `units` at its largest
-    const int64_t units = std::max<int64_t>(1, std::min<int64_t>(static_cast<int64_t>(sm_count(current_device())) * kBackwardPerSm, desc->fwd.rows));
-    return static_cast<size_t>(6 * units * desc->fwd.cols) * sizeof(float) + 256;
+    // [4 + 2][units][cols] fp32 partial sums, `units` at its largest, and two
+    // means per row where a pass of its own adds the columns
+    const tk_residual_norm_desc_t& d = desc->fwd;
+    const int device = current_device();
+    const int64_t units = is_wide(d) ? column_units(device, std::max<int64_t>(1, d.rows), d.cols, true)
+                                     : std::max<int64_t>(1, std::min<int64_t>(static_cast<int64_t>(sm_count(device)) * kBackwardPerSm, d.rows));
+    return static_cast<size_t>(6 * units * d.cols) * sizeof(float) + (is_wide(d) ? round_up(static_cast<size_t>(d.rows) * sizeof(float2), 16) : 0) + 256;
 }
 
 int tk_residual_norm_backward(const tk_residual_norm_grad_desc_t* desc, void* workspace, size_t workspace_bytes, void* stream) {
@@ -1052,20 +1284,34 @@ int tk_residual_norm_backward(const tk_residual_norm_grad_desc_t* desc, void* wo
     const bool gate = d.gate != nullptr, post = d.post_norm != 0;
     if (!gate && !post) p.f = nullptr;
     const bool vec = vectorised(p);
-    const Geometry g = geometry(p, f16, vec, true, gate || post);
-    const size_t smem = configure(p, g, f16, vec, gate || post ? 4 : 3, true);
-    const Kernel k = f16 ? (vec ? backward_kernel<__half, true>(g.nv, post, gate) : backward_kernel<__half, false>(g.nv, post, gate))
-                         : (vec ? backward_kernel<float, true>(g.nv, post, gate) : backward_kernel<float, false>(g.nv, post, gate));
+    const bool wide = is_wide(d);
+    const Geometry g = geometry(p.cols, f16, wide ? kNoSums : gate || post ? kSums5 : kSums2, post);
+    const size_t smem = configure(p, g, f16, vec, gate || post ? 4 : 3, !wide);
+    const Kernel k = f16 ? (vec ? backward_kernel<__half, true>(g.nv, post, gate, !wide) : backward_kernel<__half, false>(g.nv, post, gate, !wide))
+                         : (vec ? backward_kernel<float, true>(g.nv, post, gate, !wide) : backward_kernel<float, false>(g.nv, post, gate, !wide));
     int per_sm = 0;
     if (int rc = resident_ctas(k, p, smem, per_sm)) return rc;
     p.units = max_units(current_device(), p.rows, g, std::min(per_sm, kBackwardPerSm));
-    const size_t need = static_cast<size_t>(6) * p.units * p.cols * sizeof(float);
+    const int pass_units = column_units(current_device(), p.rows, p.cols, vec);
+    const size_t means = wide ? round_up(static_cast<size_t>(p.rows) * sizeof(float2), 16) : 0;
+    const size_t need = means + static_cast<size_t>(6) * (wide ? pass_units : p.units) * p.cols * sizeof(float);
     if (workspace == nullptr || workspace_bytes < need || !aligned16(workspace))
         TK_FAIL(TK_ERR_WORKSPACE, "tk_residual_norm_backward: 16-byte aligned workspace of %zu bytes needed, got %zu", need, workspace_bytes);
-    p.partial = static_cast<float*>(workspace);
+    p.means = static_cast<float2*>(workspace);
+    p.partial = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + means);
     if (int rc = launch(k, p, smem, s, "residual_norm_backward")) return rc;
+    const bool sums = desc->dweight || desc->dbias || desc->dpost_weight || desc->dpost_bias || (p.dgate != nullptr && p.gate_period > 1);
+    if (wide && sums) {
+        p.units = pass_units;
+        const Kernel pass = f16 ? (vec ? column_pass_of<__half, 8>(post, gate) : column_pass_of<__half, 1>(post, gate))
+                                : (vec ? column_pass_of<float, 8>(post, gate) : column_pass_of<float, 1>(post, gate));
+        const cudaError_t e = launch_pdl(pass, dim3(static_cast<unsigned>(ceil_div(p.cols, kPassThreads * (vec ? 8 : 1))), p.units), dim3(kPassThreads), 0, s, p);
+        if (e != cudaSuccess) {
+            cudaGetLastError();
+            TK_FAIL(TK_ERR_CUDA, "residual norm column pass launch failed: %s", cudaGetErrorString(e));
+        }
+    }
     const bool gate_items = p.dgate != nullptr && p.gate_period > 1;
-    if (!desc->dweight && !desc->dbias && !desc->dpost_weight && !desc->dpost_bias && !gate_items) return TK_OK;
     return f16 ? columns<__half>(p, *desc, gate_items, s) : columns<float>(p, *desc, gate_items, s);
 }
 
