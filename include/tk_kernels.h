@@ -453,10 +453,10 @@ typedef struct {
 
 TK_API int tk_residual_norm(const tk_residual_norm_desc_t* desc, void* stream);
 
-/* Its gradients.  fwd holds the forward call's sizes, parameters, x_new and
- * stats, and f where there is a post norm or a gate; its x, h and bias are not
- * read.  grad_x_new and grad_h are the gradients of the outputs (NULL: zero,
- * not both).  Each result may be NULL: dx, df [rows, cols], dweight, dbias,
+/* Its gradients.  fwd holds the forward call's sizes, inputs, parameters and
+ * stats; its x_new, h and bias are not read (x_new is formed again, unrounded).
+ * grad_x_new and grad_h are the gradients of the outputs (NULL: zero, not
+ * both).  Each result may be NULL: dx, df [rows, cols], dweight, dbias,
  * dpost_weight, dpost_bias [cols], dgate [gate_rows, cols].  Column sums are
  * fp32 in a fixed order (deterministic). */
 typedef struct {

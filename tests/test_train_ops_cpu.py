@@ -93,15 +93,16 @@ def test_residual_norm_refuses_bad_arguments_before_the_device(fields, status):
 def test_residual_norm_backward_needs_its_inputs():
     L = C.lib()
     g = C.ResidualNormGradDesc()
-    g.fwd = _norm_desc(x_new=16, stats=16)
+    g.fwd = _norm_desc(x=16, f=16, stats=16)
     assert L.tk_residual_norm_backward(ctypes.byref(g), None, 0, None) == 1
     assert b"no incoming gradient" in L.tk_last_error_string()
     g.grad_h = 16
-    g.fwd.post_norm = 1
-    assert L.tk_residual_norm_backward(ctypes.byref(g), None, 0, None) == 1
-    assert b"f is needed" in L.tk_last_error_string()
-    g.fwd.stats = 8
-    assert L.tk_residual_norm_backward(ctypes.byref(g), None, 0, None) == 1
+    for field, bad in (("f", None), ("x", None), ("stats", 8)):
+        kept = getattr(g.fwd, field)
+        setattr(g.fwd, field, bad)
+        assert L.tk_residual_norm_backward(ctypes.byref(g), None, 0, None) == 1
+        assert b"are needed" in L.tk_last_error_string()
+        setattr(g.fwd, field, kept)
     assert L.tk_residual_norm(ctypes.byref(_norm_desc(rows=0)), None) == 0
 
 

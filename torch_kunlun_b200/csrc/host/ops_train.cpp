@@ -6,6 +6,7 @@
 // (csrc/autograd.cpp) and at a forward layer_norm (csrc/ops_nn.cpp:85-130);
 // these ops follow its float16/float32 rules.  Their backward passes are not
 // differentiable themselves and say so.
+#include <ATen/EmptyTensor.h>
 #include <torch/csrc/autograd/custom_function.h>
 
 #include "kunlun.h"
@@ -57,15 +58,24 @@ void check_single_backward(const char* op) {
     TORCH_CHECK(!at::GradMode::is_enabled(), "kunlun ", op, ": gradients of its backward pass (create_graph=True) are not implemented");
 }
 
+// A contiguous tensor on the current device, allocated without a trip through
+// the dispatcher: these ops allocate up to nine tensors a call.
+at::Tensor fresh(at::IntArrayRef shape, at::ScalarType type) {
+    return at::detail::empty_generic(shape, get_allocator(), c10::DispatchKeySet(c10::DispatchKey::PrivateUse1), type,
+                                     std::nullopt);
+}
+
+at::Tensor scratch(size_t bytes) { return fresh({static_cast<int64_t>(bytes + 1024)}, at::kByte); }
+
 void* ptr(const at::Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 
 // ---- dropout --------------------------------------------------------------------
 
 at::Tensor dropout_run(const at::Tensor& x, double p, uint64_t seed, uint64_t offset) {
     at::Tensor xc = x.contiguous();
-    at::Tensor y = at::empty(xc.sizes(), xc.options());
     const int dev = xc.device().index();
     DeviceScope g(dev);
+    at::Tensor y = fresh(xc.sizes(), xc.scalar_type());
     check_tk(tk_dropout(tk_dtype(xc.scalar_type()), ptr(xc), ptr(y), xc.numel(), p, seed, offset, current_stream(dev)),
              "tk_dropout");
     return y;
@@ -122,7 +132,7 @@ std::tuple<at::Tensor, at::Tensor> norm_run(const at::Tensor& x, const at::Tenso
                                             const at::Tensor& stats) {
     const int dev = x.device().index();
     DeviceScope g(dev);
-    at::Tensor x_new = at::empty(x.sizes(), x.options()), h = at::empty(x.sizes(), x.options());
+    at::Tensor x_new = fresh(x.sizes(), x.scalar_type()), h = fresh(x.sizes(), x.scalar_type());
     tk_residual_norm_desc_t d = norm_desc(x, o, weight, post_weight, post_bias, gate);
     d.x = ptr(x);
     d.f = ptr(f);
@@ -145,11 +155,10 @@ struct ResidualNorm : torch::autograd::Function<ResidualNorm> {
         at::Tensor stats;
         {
             DeviceScope g(x.device().index());
-            stats = at::empty({rows, 4}, x.options().dtype(at::kFloat));
+            stats = fresh({rows, 4}, at::kFloat);
         }
         auto [x_new, h] = norm_run(x, f, weight, bias, post_weight, post_bias, gate, o, stats);
-        const bool need_f = o.post || gate.defined();
-        ctx->save_for_backward({x_new, need_f ? f : at::Tensor(), weight, post_weight, post_bias, gate, stats});
+        ctx->save_for_backward({x, f, weight, post_weight, post_bias, gate, stats});
         ctx->saved_data["flags"] = std::vector<bool>{o.rms,
                                                      o.post,
                                                      x.requires_grad(),
@@ -171,7 +180,7 @@ struct ResidualNorm : torch::autograd::Function<ResidualNorm> {
         at::Tensor gx = grads[0], gh = grads[1];
         if (!gx.defined() && !gh.defined()) return out;
         const variable_list saved = ctx->get_saved_variables();
-        const at::Tensor &x_new = saved[0], &f = saved[1], &weight = saved[2], &post_weight = saved[3],
+        const at::Tensor &x = saved[0], &f = saved[1], &weight = saved[2], &post_weight = saved[3],
                          &post_bias = saved[4], &gate = saved[5], &stats = saved[6];
         const auto flag = ctx->saved_data["flags"].toBoolList();
         const auto real = ctx->saved_data["reals"].toDoubleVector();
@@ -179,23 +188,21 @@ struct ResidualNorm : torch::autograd::Function<ResidualNorm> {
         const NormOptions o = {flag[0], flag[1], real[0], real[1], real[2], random[0], random[1]};
         if (gx.defined()) gx = gx.contiguous();
         if (gh.defined()) gh = gh.contiguous();
-        const int dev = x_new.device().index();
+        const int dev = x.device().index();
         DeviceScope g(dev);
-        auto fresh = [&](bool wanted, at::IntArrayRef shape) {
-            return wanted ? at::empty(shape, x_new.options()) : at::Tensor();
-        };
-        const int64_t cols = x_new.size(-1);
-        out[0] = fresh(flag[2], x_new.sizes());
-        out[1] = fresh(flag[3], x_new.sizes());
-        out[2] = fresh(flag[4], {cols});
-        out[3] = fresh(flag[5], {cols});
-        out[4] = fresh(flag[6], {cols});
-        out[5] = fresh(flag[7], {cols});
-        if (flag[8]) out[6] = at::empty(gate.sizes(), gate.options());
+        const at::ScalarType type = x.scalar_type();
+        const int64_t cols = x.size(-1);
+        if (flag[2]) out[0] = fresh(x.sizes(), type);
+        if (flag[3]) out[1] = fresh(x.sizes(), type);
+        if (flag[4]) out[2] = fresh({cols}, type);
+        if (flag[5]) out[3] = fresh({cols}, type);
+        if (flag[6]) out[4] = fresh({cols}, type);
+        if (flag[7]) out[5] = fresh({cols}, type);
+        if (flag[8]) out[6] = fresh(gate.sizes(), type);
         tk_residual_norm_grad_desc_t d = {};
-        d.fwd = norm_desc(x_new, o, weight, post_weight, post_bias, gate);
+        d.fwd = norm_desc(x, o, weight, post_weight, post_bias, gate);
+        d.fwd.x = ptr(x);
         d.fwd.f = ptr(f);
-        d.fwd.x_new = ptr(x_new);
         d.fwd.stats = stats.data_ptr<float>();
         d.grad_x_new = ptr(gx);
         d.grad_h = ptr(gh);
@@ -208,7 +215,7 @@ struct ResidualNorm : torch::autograd::Function<ResidualNorm> {
         d.dgate = ptr(out[6]);
         const size_t bytes = tk_residual_norm_backward_workspace_size(&d);
         TORCH_CHECK(bytes > 0, "kunlun residual_norm: ", tk_last_error_string());
-        at::Tensor ws = workspace(bytes, x_new.device());
+        at::Tensor ws = scratch(bytes);
         check_tk(tk_residual_norm_backward(&d, aligned_base(ws), bytes, current_stream(dev)), "tk_residual_norm_backward");
         return out;
     }
@@ -237,16 +244,15 @@ tk_linear_ce_desc_t ce_desc(const at::Tensor& x, const at::Tensor& weight, const
 at::Tensor ce_run(tk_linear_ce_desc_t d, const at::Tensor& x, at::Tensor* state) {
     const int dev = x.device().index();
     DeviceScope g(dev);
-    const auto f32 = x.options().dtype(at::kFloat);
-    at::Tensor loss = d.reduction == TK_REDUCE_NONE ? at::empty({d.rows}, f32) : at::empty({}, f32);
+    at::Tensor loss = d.reduction == TK_REDUCE_NONE ? fresh({d.rows}, at::kFloat) : fresh({}, at::kFloat);
     d.loss = d.reduction == TK_REDUCE_NONE && d.rows == 0 ? nullptr : loss.data_ptr<float>();
     const size_t bytes = tk_linear_ce_workspace_size(&d);
     TORCH_CHECK(bytes > 0, "kunlun linear_cross_entropy: ", tk_last_error_string());
     if (state != nullptr) {
-        *state = at::empty({static_cast<int64_t>(tk_linear_ce_state_size(&d))}, x.options().dtype(at::kByte));
+        *state = fresh({static_cast<int64_t>(tk_linear_ce_state_size(&d))}, at::kByte);
         d.state = state->data_ptr();
     }
-    at::Tensor ws = workspace(bytes, x.device());
+    at::Tensor ws = scratch(bytes);
     check_tk(tk_linear_ce(&d, aligned_base(ws), bytes, current_stream(dev)), "tk_linear_ce");
     return loss;
 }
@@ -274,9 +280,9 @@ struct LinearCrossEntropy : torch::autograd::Function<LinearCrossEntropy> {
         const int dev = x.device().index();
         DeviceScope g(dev);
         const at::Tensor grad = grads[0].contiguous();
-        if (ints[2]) out[0] = at::empty(x.sizes(), x.options());
-        if (ints[3]) out[1] = at::empty(weight.sizes(), weight.options());
-        if (ints[4]) out[3] = at::empty(bias.sizes(), bias.options());
+        if (ints[2]) out[0] = fresh(x.sizes(), x.scalar_type());
+        if (ints[3]) out[1] = fresh(weight.sizes(), x.scalar_type());
+        if (ints[4]) out[3] = fresh(bias.sizes(), x.scalar_type());
         tk_linear_ce_grad_desc_t d = {};
         d.fwd = ce_desc(x, weight, target, bias, ints[0], ints[1]);
         d.fwd.state = state.data_ptr();
@@ -286,7 +292,7 @@ struct LinearCrossEntropy : torch::autograd::Function<LinearCrossEntropy> {
         d.dbias = ptr(out[3]);
         const size_t bytes = tk_linear_ce_backward_workspace_size(&d);
         TORCH_CHECK(bytes > 0, "kunlun linear_cross_entropy: ", tk_last_error_string());
-        at::Tensor ws = workspace(bytes, x.device());
+        at::Tensor ws = scratch(bytes);
         check_tk(tk_linear_ce_backward(&d, aligned_base(ws), bytes, current_stream(dev)), "tk_linear_ce_backward");
         return out;
     }

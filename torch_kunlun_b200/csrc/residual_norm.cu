@@ -18,11 +18,11 @@
 //   dweight = sum gh * n, dbias = sum gh, dpost_weight = sum gu * q,
 //   dpost_bias = sum gu over the rows
 //
-// (an rms norm has no mean(t) terms).  x_new stands for x there, so neither x
-// nor h is read again.
+// (an rms norm has no mean(t) terms).  x_new is formed again from x and f, as
+// the forward pass had it before it was rounded: from the rounded x_new the
+// binary16 gradient of weight came out up to 1.5 times as far off.
 //
-// HBM bounds both directions: 4 tensors forward, 6 backward (5 without a post
-// norm and a gate, which need f).  A group of W warps holds a row in
+// HBM bounds both directions: 4 tensors forward, 6 backward.  A group of W warps holds a row in
 // registers, 8 * NV columns per thread, as pairs for the two-wide binary32
 // instructions (one per element made the kernels issue-bound: 8192 x 4096 with
 // both norms took 93 us forward, 2.4 TB/s, at 63 % issue); a CTA runs several
@@ -645,8 +645,7 @@ __global__ void __launch_bounds__(kMaxThreads, 1) residual_norm_backward_kernel(
     extern __shared__ __align__(16) uint8_t smem[];
     using L = Lane<T, NV, VEC>;
     constexpr int P = L::P;
-    constexpr bool NEED_F = POST || GATE;
-    L ln(p, smem, NEED_F ? 4 : 3);
+    L ln(p, smem, 4);
     float* const buf = reinterpret_cast<float*>(smem + 2 * sizeof(float2) * ((ln.red_stride + 1) & ~1));
     const int64_t unit = blockIdx.x / p.cluster;
     const int64_t unit_lo = unit_begin(unit, p.rows, p.units), unit_hi = unit_begin(unit + 1, p.rows, p.units);
@@ -680,19 +679,44 @@ __global__ void __launch_bounds__(kMaxThreads, 1) residual_norm_backward_kernel(
             [&](int64_t r, int stage) {
                 const int64_t at = r * p.cols;
                 if (p.gx != nullptr) ln.fetch(p.gx, at, stage, 0);
-                if (p.gh != nullptr) ln.fetch(p.gh, at, stage, 1);
-                ln.fetch(p.x_new, at, stage, 2);
-                if constexpr (NEED_F) ln.fetch(p.f, at, stage, 3);
+                if (p.gh != nullptr) {
+                    ln.fetch(p.gh, at, stage, 1);
+                    ln.fetch(p.x, at, stage, 2);
+                }
+                ln.fetch(p.f, at, stage, 3);
             },
             [&](int64_t r, int stage) {
                 const int64_t at = r * p.cols;
                 const float4 st = next_st;
                 if (r + p.groups < seg_hi) next_st = p.stats[r + p.groups];
+                const uint32_t keep = p.drop ? ln.keep(at) : 0u;
+                if constexpr (GATE) {
+                    const int64_t k = p.gate_period == p.rows ? 0 : r / p.gate_period;
+                    if (k != gate_row) ln.vector(static_cast<const T*>(p.gate) + k * p.cols, 0.0f, gate);
+                    gate_row = k;
+                }
+                float2 u[P];  // the block's dropped output
+                ln.row_values(p.f, at, stage, 3, u);
+                if constexpr (POST) {
+                    const float2 s = both(st.y), c = both(-st.x);
+#pragma unroll
+                    for (int i = 0; i < P; ++i) u[i] = mul2(mul2(add2(u[i], c), s), pw.pair(i));
+                    if (p.post_bias != nullptr) {
+                        Raw<T, L::E> pb;
+                        ln.vector(p.post_bias, 0.0f, pb);
+#pragma unroll
+                        for (int i = 0; i < P; ++i) u[i] = add2(u[i], pb.pair(i));
+                    }
+                }
+                if (p.drop) ln.drop(keep, u);
                 float2 g[P];
                 if (p.gh != nullptr) {
                     float2 n[P], h[P];
-                    ln.row_values(p.x_new, at, stage, 2, n);
+                    ln.row_values(p.x, at, stage, 2, n);
                     ln.row_values(p.gh, at, stage, 1, h);
+                    const float2 a = both(p.a);
+#pragma unroll
+                    for (int i = 0; i < P; ++i) n[i] = GATE ? fma2(a, n[i], mul2(u[i], gate.pair(i))) : fma2(a, n[i], u[i]);
                     const float2 s = both(st.w), c = both(-st.z);
                     float2 s1 = make_float2(0.0f, 0.0f), s2 = s1;
 #pragma unroll
@@ -729,56 +753,27 @@ __global__ void __launch_bounds__(kMaxThreads, 1) residual_norm_backward_kernel(
                     for (int i = 0; i < P; ++i) o[i] = mul2(a, g[i]);
                     ln.store(p.dx, at, o);
                 }
-                const uint32_t keep = GATE && p.drop ? ln.keep(at) : 0u;
-                float2 q[NEED_F ? P : 1];  // Norm(f) with a post norm, else f
-                if constexpr (NEED_F) {
-                    ln.row_values(p.f, at, stage, 3, q);
-                    if constexpr (POST) {
-                        const float2 s = both(st.y), c = both(-st.x);
-#pragma unroll
-                        for (int i = 0; i < P; ++i) q[i] = mul2(add2(q[i], c), s);
-                    }
-                }
                 if constexpr (GATE) {
-                    if (SUMS || (p.gate_period == 1 && p.dgate != nullptr)) {
-                        float2 u[P];
-                        if constexpr (POST) {
+                    if (gate_sums) {
+                        if constexpr (SUMS) {
 #pragma unroll
-                            for (int i = 0; i < P; ++i) u[i] = mul2(q[i], pw.pair(i));
-                            if (p.post_bias != nullptr) {
-                                Raw<T, L::E> pb;
-                                ln.vector(p.post_bias, 0.0f, pb);
-#pragma unroll
-                                for (int i = 0; i < P; ++i) u[i] = add2(u[i], pb.pair(i));
-                            }
-                        } else {
-#pragma unroll
-                            for (int i = 0; i < P; ++i) u[i] = q[i];
+                            for (int i = 0; i < P; ++i) dgt[i] = fma2(u[i], g[i], dgt[i]);
                         }
-                        if (p.drop) ln.drop(keep, u);
-                        if (gate_sums) {
-                            if constexpr (SUMS) {
+                    } else if (p.gate_period == 1 && p.dgate != nullptr) {
 #pragma unroll
-                                for (int i = 0; i < P; ++i) dgt[i] = fma2(u[i], g[i], dgt[i]);
-                            }
-                        } else if (p.dgate != nullptr) {
-#pragma unroll
-                            for (int i = 0; i < P; ++i) u[i] = mul2(u[i], g[i]);
-                            ln.store(p.dgate, at, u);
-                        }
+                        for (int i = 0; i < P; ++i) u[i] = mul2(u[i], g[i]);
+                        ln.store(p.dgate, at, u);
                     }
-                    const int64_t k = p.gate_period == p.rows ? 0 : r / p.gate_period;
-                    if (k != gate_row) ln.vector(static_cast<const T*>(p.gate) + k * p.cols, 0.0f, gate);
-                    gate_row = k;
 #pragma unroll
                     for (int i = 0; i < P; ++i) g[i] = mul2(g[i], gate.pair(i));
                 }
-                if (p.drop) {
-                    if constexpr (GATE) {
-                        ln.drop(keep, g);
-                    } else {
-                        ln.drop_row(at, g);
-                    }
+                if (p.drop) ln.drop(keep, g);
+                float2 q[POST ? P : 1];  // Norm(f)
+                if constexpr (POST) {
+                    ln.row_values(p.f, at, stage, 3, q);
+                    const float2 s = both(st.y), c = both(-st.x);
+#pragma unroll
+                    for (int i = 0; i < P; ++i) q[i] = mul2(add2(q[i], c), s);
                 }
                 if constexpr (POST) {
                     float2 s3 = make_float2(0.0f, 0.0f), s4 = s3;
@@ -872,16 +867,16 @@ __global__ void __launch_bounds__(kPassThreads) residual_norm_column_pass_kernel
             float n[V], h[V], g[V], q[V];
             float2 m = make_float2(0.0f, 0.0f);
 #pragma unroll
-            for (int i = 0; i < V; ++i) h[i] = g[i] = 0.0f;
-            load(p.x_new, r, n);
+            for (int i = 0; i < V; ++i) n[i] = h[i] = g[i] = 0.0f;
             if (p.gh != nullptr) {
+                load(p.x, r, n);
                 load(p.gh, r, h);
                 m = p.means[r];
             }
             if ((POST || GATE) && p.gx != nullptr) load(p.gx, r, g);
-            if (POST || GATE) load(p.f, r, q);
+            load(p.f, r, q);
             uint32_t keep = 0xFFu;
-            if ((POST || GATE) && p.drop) {
+            if (p.drop) {
                 const uint64_t e = static_cast<uint64_t>(r * p.cols + c);
                 if constexpr (V == 8) {
                     keep = dropout_keep8(p.dropout, static_cast<uint32_t>(e / 8));
@@ -891,18 +886,19 @@ __global__ void __launch_bounds__(kPassThreads) residual_norm_column_pass_kernel
             }
 #pragma unroll
             for (int i = 0; i < V; ++i) {
-                n[i] = (n[i] - st.z) * st.w;
+                float u = POST ? (q[i] - st.x) * st.y : q[i];
+                const float qn = u;
+                if (POST) u = fmaf(u, pw[i], pb[i]);
+                const bool kept = !p.drop || (keep >> i & 1u);
+                const float s = p.drop ? p.dropout.scale : 1.0f;
+                u = kept ? u * s : 0.0f;
+                n[i] = (fmaf(p.a, n[i], GATE ? u * gate[i] : u) - st.z) * st.w;
                 dw[i] = fmaf(h[i], n[i], dw[i]);
                 db[i] += h[i];
                 if constexpr (POST || GATE) {
-                    float u = POST ? (q[i] - st.x) * st.y : q[i];
-                    const float qn = u;
-                    if (POST) u = fmaf(u, pw[i], pb[i]);
                     g[i] = fmaf(st.w, h[i] * w[i] - n[i] * m.y - m.x, g[i]);
-                    const bool kept = !p.drop || (keep >> i & 1u);
-                    const float s = p.drop ? p.dropout.scale : 1.0f;
                     if (GATE) {
-                        dgt[i] += kept ? g[i] * u * s : 0.0f;
+                        dgt[i] = fmaf(g[i], u, dgt[i]);
                         g[i] *= gate[i];
                     }
                     if (POST) {
@@ -1269,11 +1265,10 @@ int tk_residual_norm_backward(const tk_residual_norm_grad_desc_t* desc, void* wo
         if (desc->dgate != nullptr && d.gate != nullptr) TK_CUDA_TRY(cudaMemsetAsync(desc->dgate, 0, row * d.gate_rows, s));
         return TK_OK;
     }
-    TK_CHECK_ARG(d.x_new && d.stats && aligned16(d.stats), "tk_residual_norm_backward: x_new and 16-byte aligned stats are needed");
+    TK_CHECK_ARG(d.x && d.f && d.stats && aligned16(d.stats), "tk_residual_norm_backward: x, f and 16-byte aligned stats are needed");
     TK_CHECK_ARG(desc->grad_x_new || desc->grad_h, "tk_residual_norm_backward: no incoming gradient");
-    TK_CHECK_ARG(d.f || !(d.post_norm || d.gate), "tk_residual_norm_backward: f is needed with a post norm or a gate");
     RnParams p = params(d);
-    p.x = nullptr;
+    p.x_new = nullptr;
     p.h = nullptr;
     p.bias = nullptr;
     p.gx = desc->grad_x_new;
@@ -1282,11 +1277,10 @@ int tk_residual_norm_backward(const tk_residual_norm_grad_desc_t* desc, void* wo
     p.df = desc->df;
     p.dgate = d.gate != nullptr ? desc->dgate : nullptr;
     const bool gate = d.gate != nullptr, post = d.post_norm != 0;
-    if (!gate && !post) p.f = nullptr;
     const bool vec = vectorised(p);
     const bool wide = is_wide(d);
     const Geometry g = geometry(p.cols, f16, wide ? kNoSums : gate || post ? kSums5 : kSums2, post);
-    const size_t smem = configure(p, g, f16, vec, gate || post ? 4 : 3, !wide);
+    const size_t smem = configure(p, g, f16, vec, 4, !wide);
     const Kernel k = f16 ? (vec ? backward_kernel<__half, true>(g.nv, post, gate, !wide) : backward_kernel<__half, false>(g.nv, post, gate, !wide))
                          : (vec ? backward_kernel<float, true>(g.nv, post, gate, !wide) : backward_kernel<float, false>(g.nv, post, gate, !wide));
     int per_sm = 0;

@@ -123,7 +123,7 @@ def residual_norm(x: torch.Tensor, f: torch.Tensor, weight: Optional[torch.Tenso
     ([B, 1, D] gates each sample).  All tensors share one dtype, float16 or
     float32; sums are fp32 (of the unrounded x_new for h) and each output is
     rounded once.  D is at most 32768.  Differentiable in every tensor; the
-    backward pass recomputes the mask and takes x_new as it was rounded."""
+    backward pass forms the mask and the unrounded x_new again from x and f."""
     if norm not in ("layer", "rms"):
         raise ValueError(f"norm must be 'layer' or 'rms', got {norm!r}")
     return _C.residual_norm(x, f, weight, bias, norm == "rms", bool(post_norm), post_weight, post_bias, gate,
