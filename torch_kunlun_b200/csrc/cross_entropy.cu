@@ -24,7 +24,8 @@
 // fp32 operands are split into two binary16 planes of a power-of-two multiple
 // (hi = rn(v s), lo = rn(v s - hi), the tensor's largest value in [2^14,
 // 2^15)), 22 bits or 2^-40 of the largest value, and a product is the sum
-// hi*hi + hi*lo + lo*hi: the K loop runs over three pairs of planes.
+// hi*hi + hi*lo + lo*hi: a K block takes two stages, one for each plane of both
+// operands, and three products.
 //
 // GEMM kernel (persistent pairs of CTAs, one CTA per SM):
 // a pair computes 256 x 256 tiles, CTA r holding rows [128 r, + 128) of A and
@@ -61,8 +62,9 @@ constexpr int PITCH = TURN + 4;
 // kPlain: eight epilogue warps, six stages.  kWide: sixteen warps for dz where
 // the K loop is short (the logits of 2384 rows by 30011 words at 768 columns,
 // 12 K blocks: 177 -> 166 us; at 64 K blocks five stages cost 3 %).  kChunked:
-// sums in registers, 128 columns per thread.
-enum Mode { kPlain, kWide, kChunked };
+// sums in registers, 128 columns per thread.  kPlanes: the same for fp32
+// operands.
+enum Mode { kPlain, kWide, kChunked, kPlanes };
 constexpr int kWideBlocks = 24;  // K blocks up to which kWide is taken
 
 template <int MODE>
@@ -80,7 +82,7 @@ constexpr int TMEM_COLS = 512;
 
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kDzScale = 16384.0f;
-constexpr int kRowPad = 256;  // packed rows are zero up to a multiple of this
+constexpr int kRowPad = 256;  // rows of a tile: packed rows have room up to a multiple of this
 
 // Device scalars of one call.
 struct Scalars {
@@ -98,8 +100,8 @@ struct GemmParams {
     const Scalars* sc;
     int n_tiles;
     int m_tiles;   // < 0: from sc->count
-    int k_blocks;  // per pair of planes; < 0: from sc->count
-    int pairs;     // 1 (fp16 operands) or 3 (two planes each)
+    int k_blocks;  // < 0: from sc->count
+    int planes;    // 1 (fp16 operands) or 2 (fp32)
     int chunk;     // K blocks per accumulator chunk
     int max_units; // tiles x K splits the workspace of a split reduction holds
     int64_t vocab0, vocab;  // the piece's first column, all columns
@@ -139,7 +141,7 @@ __device__ __forceinline__ Shape shape_of(const GemmParams& p) {
     const int count = p.sc->count;
     Shape s;
     s.m_tiles = p.m_tiles >= 0 ? p.m_tiles : (count + BM - 1) / BM;
-    s.blocks = (p.k_blocks >= 0 ? p.k_blocks : (count + BK - 1) / BK) * p.pairs;
+    s.blocks = p.k_blocks >= 0 ? p.k_blocks : (count + BK - 1) / BK;
     s.splits = EPI == kGradX || EPI == kGradW ? k_splits(p, s.m_tiles * p.n_tiles, s.blocks) : 1;
     s.units = s.m_tiles * p.n_tiles * s.splits;
     return s;
@@ -351,7 +353,7 @@ __device__ __forceinline__ void finish(const GemmParams& p, int64_t m, int64_t r
 
 // The scale that takes an accumulator to a base-2 logit.
 __device__ __forceinline__ float z_scale(const GemmParams& p) {
-    return p.pairs == 1 ? kLog2e : kLog2e / plane_scale(p.sc->amax_x) / plane_scale(p.sc->amax_w);
+    return p.planes == 1 ? kLog2e : kLog2e / plane_scale(p.sc->amax_x) / plane_scale(p.sc->amax_w);
 }
 
 template <int EPI, int MODE>
@@ -360,9 +362,11 @@ ce_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
     constexpr bool A_MN = EPI == kGradW, B_MN = EPI == kGradX || EPI == kGradW;
     constexpr uint32_t IDESC = idesc_f16(BM, BN, A_MN, B_MN);
     using C = Config<MODE>;
-    constexpr bool CHUNKED = MODE == kChunked;
+    constexpr bool CHUNKED = MODE == kChunked || MODE == kPlanes;
+    constexpr int PLANES = MODE == kPlanes ? 2 : 1;
     static_assert(MODE != kWide || EPI == kDlogits, "wide epilogues are for dz");
     constexpr int STAGES = C::STAGES, EPI_WARPS = C::EPI_WARPS, COLS = C::COLS;
+    static_assert(STAGES % PLANES == 0, "both planes' stages are neighbours");
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
     float* turn_buf = reinterpret_cast<float*>(smem + STAGES * STAGE_BYTES);
@@ -413,36 +417,34 @@ ce_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
             used[s] = false;
             last_phase[s] = 0;
         }
-        const int per_pair = sh.blocks / p.pairs;
         bool ok = true;
         for (int u = first_unit; u < sh.units && ok; u += unit_step) {
             int mt, nt, ks;
             decode_unit(p, sh, u, mt, nt, ks);
             const int kb1 = split_begin(sh, ks + 1);
             const int a0 = mt * BM + static_cast<int>(rank) * HM, b0 = nt * BN + static_cast<int>(rank) * HN;
-            for (int kb = split_begin(sh, ks); kb < kb1; ++kb) {
+            // a stage for each plane of each K block
+            for (int i = split_begin(sh, ks) * PLANES; i < kb1 * PLANES; ++i) {
                 if (!mbar_wait_bounded(smem_u32(empty_bar + stage), phase ^ 1u, abort_flag, p.err, kDevErrWaitEmpty)) {
                     ok = false;
                     break;
                 }
                 if (lane == 0) {
-                    const int pair = kb / per_pair;
-                    const int kx = (kb - pair * per_pair) * BK;
-                    const int pa = pair == 2 ? 1 : 0, pb = pair == 1 ? 1 : 0;
+                    const int kx = i / PLANES * BK, plane = i % PLANES;
                     if (leader) mbar_arrive_expect_tx(smem_u32(full_bar + stage), 2 * STAGE_BYTES);
                     const uint32_t fb = mapa_shared(smem_u32(full_bar + stage), 0);
                     const uint32_t sa = smem_u32(smem + stage * STAGE_BYTES);
                     if constexpr (A_MN) {
 #pragma unroll
-                        for (int i = 0; i < HM / 64; ++i) tma_load_3d_pair(sa + i * BK * 128, &tmA, fb, a0 + i * 64, kx, pa);
+                        for (int j = 0; j < HM / 64; ++j) tma_load_3d_pair(sa + j * BK * 128, &tmA, fb, a0 + j * 64, kx, plane);
                     } else {
-                        tma_load_3d_pair(sa, &tmA, fb, kx, a0, pa);
+                        tma_load_3d_pair(sa, &tmA, fb, kx, a0, plane);
                     }
                     if constexpr (B_MN) {
 #pragma unroll
-                        for (int i = 0; i < HN / 64; ++i) tma_load_3d_pair(sa + A_BYTES + i * BK * 128, &tmB, fb, b0 + i * 64, kx, pb);
+                        for (int j = 0; j < HN / 64; ++j) tma_load_3d_pair(sa + A_BYTES + j * BK * 128, &tmB, fb, b0 + j * 64, kx, plane);
                     } else {
-                        tma_load_3d_pair(sa + A_BYTES, &tmB, fb, kx, b0, pb);
+                        tma_load_3d_pair(sa + A_BYTES, &tmB, fb, kx, b0, plane);
                     }
                 }
                 __syncwarp();
@@ -486,25 +488,37 @@ ce_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
                     tc_fence_after();
                     const uint32_t acc = tmem_base + buf * BN;
                     for (; kb < c1; ++kb) {
-                        if (!mbar_wait_bounded(smem_u32(full_bar + stage), phase, abort_flag, p.err, kDevErrWaitFull)) {
-                            ok = false;
-                            break;
-                        }
+                        // PLANES divides STAGES: the planes' stages are neighbours
+                        for (int j = 0; j < PLANES && ok; ++j)
+                            ok = mbar_wait_bounded(smem_u32(full_bar + stage + j), phase, abort_flag, p.err, kDevErrWaitFull);
+                        if (!ok) break;
                         tc_fence_after();
                         if (lane == 0) {
                             const uint32_t sa = smem_u32(smem + stage * STAGE_BYTES);
-                            const uint64_t da = A_MN ? smem_desc_mnmajor_sw128(sa) : smem_desc_kmajor_sw128(sa);
-                            const uint64_t db = B_MN ? smem_desc_mnmajor_sw128(sa + A_BYTES) : smem_desc_kmajor_sw128(sa + A_BYTES);
+                            uint64_t da[PLANES], db[PLANES];
+#pragma unroll
+                            for (int j = 0; j < PLANES; ++j) {
+                                const uint32_t s = sa + j * STAGE_BYTES;
+                                da[j] = A_MN ? smem_desc_mnmajor_sw128(s) : smem_desc_kmajor_sw128(s);
+                                db[j] = B_MN ? smem_desc_mnmajor_sw128(s + A_BYTES) : smem_desc_kmajor_sw128(s + A_BYTES);
+                            }
                             // 16 K values on: 32 bytes inside the swizzled row of a
                             // K-major tile, two 1 KB atoms of an MN-major one
                             constexpr uint64_t step_a = (A_MN ? 2048 : 32) >> 4, step_b = (B_MN ? 2048 : 32) >> 4;
 #pragma unroll
-                            for (int kk = 0; kk < BK / 16; ++kk)
-                                tc_mma_f16_pair(acc, da + kk * step_a, db + kk * step_b, IDESC, kb > c0 || kk > 0 ? 1u : 0u);
-                            tc_commit_pair(smem_u32(empty_bar + stage));
+                            for (int kk = 0; kk < BK / 16; ++kk) {
+                                tc_mma_f16_pair(acc, da[0] + kk * step_a, db[0] + kk * step_b, IDESC, kb > c0 || kk > 0 ? 1u : 0u);
+                                if constexpr (PLANES == 2) {
+                                    tc_mma_f16_pair(acc, da[0] + kk * step_a, db[1] + kk * step_b, IDESC, 1u);
+                                    tc_mma_f16_pair(acc, da[1] + kk * step_a, db[0] + kk * step_b, IDESC, 1u);
+                                }
+                            }
+#pragma unroll
+                            for (int j = 0; j < PLANES; ++j) tc_commit_pair(smem_u32(empty_bar + stage + j));
                         }
                         __syncwarp();
-                        if (++stage == STAGES) {
+                        stage += PLANES;
+                        if (stage == STAGES) {
                             stage = 0;
                             phase ^= 1u;
                         }
@@ -922,7 +936,7 @@ __device__ __forceinline__ void pack_rows(const PackJob<T>& j, int64_t live, int
 
 constexpr int kPackThreads = 128;
 
-// Packs x's listed rows (zero rows after them up to a multiple of kRowPad), W
+// Packs x's listed rows (zero rows after them up to a multiple of BK), W
 // where it is not read in place, and the bias in base 2: blocks [0, x_blocks),
 // the next w_blocks, the rest.
 template <typename T, int PLANES>
@@ -932,7 +946,7 @@ ce_pack_kernel(const PackJob<T> x, const PackJob<T> w, const Scalars* sc, int x_
     const int b = static_cast<int>(blockIdx.x);
     if (b < x_blocks) {
         const int64_t live = sc->count;
-        pack_rows<T, PLANES>(x, live, (live + kRowPad - 1) / kRowPad * kRowPad, PLANES == 2 ? plane_scale(sc->amax_x) : 1.0f, b, x_blocks);
+        pack_rows<T, PLANES>(x, live, (live + BK - 1) / BK * BK, PLANES == 2 ? plane_scale(sc->amax_x) : 1.0f, b, x_blocks);
     } else if (b < x_blocks + w_blocks) {
         pack_rows<T, PLANES>(w, w.rows, w.rows, PLANES == 2 ? plane_scale(sc->amax_w) : 1.0f, b - x_blocks, w_blocks);
     } else {
@@ -1136,6 +1150,7 @@ struct Plan {
     bool f16, w_direct;
     int planes;
     int64_t rows_pad, ld;    // packed rows and their length
+    int64_t rows_read;       // rows that the products read; tiles end in zeros of their own
     int64_t n_tiles;         // vocabulary tiles
     int64_t piece;           // vocabulary columns per piece (a multiple of BN)
     int64_t pieces;
@@ -1157,17 +1172,18 @@ int check(const char* who, const tk_linear_ce_desc_t& d) {
     return TK_OK;
 }
 
-// K blocks per accumulator chunk: 16 steps of 16 where every output is
-// binary32, 64 for the loss of fp16 operands (measured at 4096 columns: the
-// loss 1e-6 off without chunks, and the same time).  A K loop no longer than a
-// chunk needs no sum in registers.
-constexpr int kChunkF32 = 4, kChunkStats = 16;
+// K blocks per accumulator chunk: 24 steps of 16 (two blocks, three products)
+// where every output is binary32, 64 for the loss of fp16 operands (measured at
+// 4096 columns: the loss 1e-6 off without chunks, and the same time).  A K loop
+// of fp16 no longer than a chunk needs no sum in registers.
+constexpr int kChunkF32 = 2, kChunkStats = 16;
 
 Plan make_plan(const tk_linear_ce_desc_t& d) {
     Plan p = {};
     p.f16 = d.dtype == TK_DTYPE_F16;
     p.planes = p.f16 ? 1 : 2;
     p.rows_pad = static_cast<int64_t>(round_up(static_cast<size_t>(std::max<int64_t>(d.rows, 1)), kRowPad));
+    p.rows_read = static_cast<int64_t>(round_up(static_cast<size_t>(std::max<int64_t>(d.rows, 1)), BK));
     p.ld = static_cast<int64_t>(round_up(static_cast<size_t>(d.cols), 8));
     p.w_direct = p.f16 && d.cols % 8 == 0 && (reinterpret_cast<uintptr_t>(d.weight) & 15) == 0;
     p.n_tiles = ceil_div(d.vocab, BN);
@@ -1274,8 +1290,11 @@ int gemm_launch(const CUtensorMap& a, const CUtensorMap& b, const GemmParams& p,
 
 template <int EPI>
 int gemm(const CUtensorMap& a, const CUtensorMap& b, const GemmParams& p, int64_t most_units, cudaStream_t s) {
-    const int64_t blocks = p.k_blocks < 0 ? INT64_MAX : static_cast<int64_t>(p.k_blocks) * p.pairs;
-    if (p.chunk != 0 && blocks > p.chunk) return gemm_launch<EPI, kChunked>(a, b, p, most_units, s);
+    if (p.planes == 2) return gemm_launch<EPI, kPlanes>(a, b, p, most_units, s);
+    const int64_t blocks = p.k_blocks < 0 ? INT64_MAX : p.k_blocks;
+    if constexpr (EPI == kStats) {
+        if (blocks > p.chunk) return gemm_launch<EPI, kChunked>(a, b, p, most_units, s);
+    }
     if constexpr (EPI == kDlogits) {
         if (blocks <= kWideBlocks) return gemm_launch<EPI, kWide>(a, b, p, most_units, s);
     }
@@ -1329,8 +1348,8 @@ Operand weight_operand(const tk_linear_ce_desc_t& d, const Plan& p, const uint8_
 GemmParams base_params(const tk_linear_ce_desc_t& d, const Plan& p, const uint8_t* st) {
     GemmParams g = {};
     g.sc = reinterpret_cast<const Scalars*>(st + p.s_scalars);
-    g.pairs = p.planes == 2 ? 3 : 1;
-    g.chunk = p.planes == 2 ? kChunkF32 : 0;
+    g.planes = p.planes;
+    g.chunk = p.planes == 2 ? kChunkF32 : kChunkStats;
     g.m_tiles = -1;
     g.k_blocks = static_cast<int>(ceil_div(d.cols, BK));
     g.group = 8;
@@ -1383,10 +1402,9 @@ int tk_linear_ce(const tk_linear_ce_desc_t* desc, void* workspace, size_t worksp
         }
         const Operand w = weight_operand(d, p, st);
         CUtensorMap tx, tw;
-        CE_TRY(make_map(&tx, st + p.s_x, d.cols, p.rows_pad, p.planes, p.ld, p.rows_pad * p.ld, HM));
+        CE_TRY(make_map(&tx, st + p.s_x, d.cols, p.rows_read, p.planes, p.ld, p.rows_pad * p.ld, HM));
         CE_TRY(make_map(&tw, w.base, d.cols, d.vocab, p.planes, w.ld, w.plane, HN));
         GemmParams g = base_params(d, p, st);
-        if (g.chunk == 0) g.chunk = kChunkStats;
         g.n_tiles = static_cast<int>(p.n_tiles);
         g.part = reinterpret_cast<float2*>(ws + p.w_part);
         CE_TRY(gemm<kStats>(tx, tw, g, p.n_tiles * ceil_div(d.rows, BM), s));
@@ -1432,8 +1450,8 @@ int tk_linear_ce_backward(const tk_linear_ce_grad_desc_t* desc, void* workspace,
     const Operand w = weight_operand(d, p, st);
     const int64_t x_plane = p.rows_pad * p.ld, dz_plane = p.rows_pad * p.piece;
     CUtensorMap tx, tx_mn;
-    CE_TRY(make_map(&tx, st + p.s_x, d.cols, p.rows_pad, p.planes, p.ld, x_plane, HM));
-    CE_TRY(make_map(&tx_mn, st + p.s_x, d.cols, p.rows_pad, p.planes, p.ld, x_plane, BK));
+    CE_TRY(make_map(&tx, st + p.s_x, d.cols, p.rows_read, p.planes, p.ld, x_plane, HM));
+    CE_TRY(make_map(&tx_mn, st + p.s_x, d.cols, p.rows_read, p.planes, p.ld, x_plane, BK));
     const int64_t row_tiles = ceil_div(d.rows, BM), col_tiles = ceil_div(d.cols, BN);
     const bool cols16 = d.cols * esz % 16 == 0;
     for (int64_t i = 0; i < p.pieces; ++i) {
@@ -1442,8 +1460,8 @@ int tk_linear_ce_backward(const tk_linear_ce_grad_desc_t* desc, void* workspace,
         CUtensorMap tw, tw_mn, tdz, tdz_mn;
         CE_TRY(make_map(&tw, wbase, d.cols, width, p.planes, w.ld, w.plane, HN));
         CE_TRY(make_map(&tw_mn, wbase, d.cols, width, p.planes, w.ld, w.plane, BK));
-        CE_TRY(make_map(&tdz, dz, width, p.rows_pad, p.planes, p.piece, dz_plane, HM));
-        CE_TRY(make_map(&tdz_mn, dz, width, p.rows_pad, p.planes, p.piece, dz_plane, BK));
+        CE_TRY(make_map(&tdz, dz, width, p.rows_read, p.planes, p.piece, dz_plane, HM));
+        CE_TRY(make_map(&tdz_mn, dz, width, p.rows_read, p.planes, p.piece, dz_plane, BK));
         GemmParams g = base_params(d, p, st);
         g.n_tiles = static_cast<int>(ceil_div(width, BN));
         g.vocab0 = v0;

@@ -819,105 +819,146 @@ __global__ void __launch_bounds__(kMaxThreads, 1) residual_norm_backward_kernel(
     }
 }
 
-// Column sums of wide rows: a block's threads take V columns each (8 where rows
-// are 16-byte aligned) over the rows of a unit, and leave partial sums, or
-// finished gate rows, as the kernel above does.
+// Column sums in a pass of their own: a thread takes 8 columns (aligned rows)
+// or one over the rows of a unit, the next row's values on their way while one
+// is added, and leaves partial sums, or finished gate rows, as the kernel above
+// does.
 constexpr int kPassThreads = 128;
 
-template <typename T, int V, bool POST, bool GATE>
-__global__ void __launch_bounds__(kPassThreads) residual_norm_column_pass_kernel(const RnParams p) {
+template <typename T, bool VEC, bool POST, bool GATE>
+__global__ void __launch_bounds__(kPassThreads, 4) residual_norm_column_pass_kernel(const RnParams p) {
     pdl_wait();
-    const int64_t c = (static_cast<int64_t>(blockIdx.x) * kPassThreads + threadIdx.x) * V;
+    constexpr int V = VEC ? 8 : 2;  // values held (one column uses the first)
+    constexpr int P = V / 2;
+    constexpr int STEP = VEC ? 8 : 1;
+    using R = Raw<T, V>;
+    const int64_t c = (static_cast<int64_t>(blockIdx.x) * kPassThreads + threadIdx.x) * STEP;
     if (c >= p.cols) return;
     const int64_t unit = blockIdx.y;
     const int64_t lo = unit_begin(unit, p.rows, p.units), hi = unit_begin(unit + 1, p.rows, p.units);
-    auto load = [&](const void* tensor, int64_t row, float (&o)[V]) {
-        const T* src = static_cast<const T*>(tensor) + row * p.cols + c;
-        if constexpr (V == 8) {
-            Raw<T, 8> w;
+    auto load = [&](const void* tensor, int64_t at, R& w) {
+        const T* src = static_cast<const T*>(tensor) + at + c;
+        if constexpr (VEC) {
 #pragma unroll
             for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i) w.vec(i, __ldg(reinterpret_cast<const uint4*>(src) + i));
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float2 f = w.pair(i);
-                o[2 * i] = f.x;
-                o[2 * i + 1] = f.y;
-            }
         } else {
-            o[0] = static_cast<float>(src[0]);
+            w.set(0, src[0]);
+            w.set(1, from_f<T>(0.0f));
         }
     };
-    float w[V], pw[V], pb[V];
+    auto fill = [&](R& w, float v) {
 #pragma unroll
-    for (int i = 0; i < V; ++i) w[i] = pw[i] = 1.0f, pb[i] = 0.0f;
+        for (int i = 0; i < V; ++i) w.set(i, from_f<T>(v));
+    };
+    struct Row {
+        R x, h, g, f;
+        float4 st;
+        float2 m;
+    };
+    auto fetch = [&](int64_t r, Row& w) {
+        const int64_t at = r * p.cols;
+        if (p.gh != nullptr) {
+            load(p.x, at, w.x);
+            load(p.gh, at, w.h);
+            w.m = p.means[r];
+        }
+        if ((POST || GATE) && p.gx != nullptr) load(p.gx, at, w.g);
+        load(p.f, at, w.f);
+        w.st = p.stats[r];
+    };
+    R w, pw, pb, gate;
+    fill(w, 1.0f);
+    fill(pw, 1.0f);
+    fill(pb, 0.0f);
+    fill(gate, 1.0f);
     if (p.weight != nullptr) load(p.weight, 0, w);
     if (POST && p.post_weight != nullptr) load(p.post_weight, 0, pw);
     if (POST && p.post_bias != nullptr) load(p.post_bias, 0, pb);
-    float dw[V] = {}, db[V] = {}, dpw[V] = {}, dpb[V] = {};
+    const float2 zero = make_float2(0.0f, 0.0f);
+    float2 dw[P], db[P], dpw[POST ? P : 1], dpb[POST ? P : 1];
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+        dw[i] = db[i] = zero;
+        if constexpr (POST) dpw[i] = dpb[i] = zero;
+    }
     const bool gate_sums = GATE && p.gate_period > 1 && p.dgate != nullptr;
+    const float2 a = both(p.a), drop_scale = both(p.drop ? p.dropout.scale : 1.0f);
+    Row next;
+    fill(next.x, 0.0f);
+    fill(next.h, 0.0f);
+    fill(next.g, 0.0f);
+    next.m = zero;
+    fetch(lo, next);
     int64_t seg_lo = lo;
     while (seg_lo < hi) {
         const int64_t gate_row = GATE ? seg_lo / p.gate_period : 0;
         const int64_t seg_hi = GATE ? min(hi, (gate_row + 1) * p.gate_period) : hi;
-        float dgt[V] = {}, gate[V];
-        if (GATE) load(p.gate, gate_row, gate);
-#pragma unroll 2
-        for (int64_t r = seg_lo; r < seg_hi; ++r) {
-            const float4 st = p.stats[r];
-            float n[V], h[V], g[V], q[V];
-            float2 m = make_float2(0.0f, 0.0f);
+        float2 dgt[GATE ? P : 1];
+        if constexpr (GATE) {
+            load(p.gate, gate_row * p.cols, gate);
 #pragma unroll
-            for (int i = 0; i < V; ++i) n[i] = h[i] = g[i] = 0.0f;
-            if (p.gh != nullptr) {
-                load(p.x, r, n);
-                load(p.gh, r, h);
-                m = p.means[r];
-            }
-            if ((POST || GATE) && p.gx != nullptr) load(p.gx, r, g);
-            load(p.f, r, q);
+            for (int i = 0; i < P; ++i) dgt[i] = zero;
+        }
+        for (int64_t r = seg_lo; r < seg_hi; ++r) {
+            const Row now = next;
+            if (r + 1 < hi) fetch(r + 1, next);
             uint32_t keep = 0xFFu;
             if (p.drop) {
                 const uint64_t e = static_cast<uint64_t>(r * p.cols + c);
-                if constexpr (V == 8) {
+                if constexpr (VEC) {
                     keep = dropout_keep8(p.dropout, static_cast<uint32_t>(e / 8));
                 } else {
                     keep = dropout_keep4(p.dropout, static_cast<uint32_t>(e / 4)) >> (e & 3);
                 }
             }
+            const float2 q_c = both(-now.st.x), q_s = both(now.st.y), n_c = both(-now.st.z), n_s = both(now.st.w);
+            const float2 m1 = both(-now.m.x), m2 = both(-now.m.y);
 #pragma unroll
-            for (int i = 0; i < V; ++i) {
-                float u = POST ? (q[i] - st.x) * st.y : q[i];
-                const float qn = u;
-                if (POST) u = fmaf(u, pw[i], pb[i]);
-                const bool kept = !p.drop || (keep >> i & 1u);
-                const float s = p.drop ? p.dropout.scale : 1.0f;
-                u = kept ? u * s : 0.0f;
-                n[i] = (fmaf(p.a, n[i], GATE ? u * gate[i] : u) - st.z) * st.w;
-                dw[i] = fmaf(h[i], n[i], dw[i]);
-                db[i] += h[i];
+            for (int i = 0; i < P; ++i) {
+                float2 u = now.f.pair(i), q = zero;
+                if constexpr (POST) {
+                    q = mul2(add2(u, q_c), q_s);
+                    u = fma2(q, pw.pair(i), pb.pair(i));
+                }
+                const bool k0 = (keep >> (2 * i)) & 1u, k1 = (keep >> (2 * i + 1)) & 1u;
+                if (p.drop) {
+                    u = mul2(u, drop_scale);
+                    u = make_float2(k0 ? u.x : 0.0f, k1 ? u.y : 0.0f);
+                }
+                const float2 h = now.h.pair(i);
+                float2 n = GATE ? mul2(u, gate.pair(i)) : u;
+                n = mul2(add2(fma2(a, now.x.pair(i), n), n_c), n_s);
+                dw[i] = fma2(h, n, dw[i]);
+                db[i] = add2(db[i], h);
                 if constexpr (POST || GATE) {
-                    g[i] = fmaf(st.w, h[i] * w[i] - n[i] * m.y - m.x, g[i]);
-                    if (GATE) {
-                        dgt[i] = fmaf(g[i], u, dgt[i]);
-                        g[i] *= gate[i];
+                    float2 g = fma2(add2(fma2(n, m2, mul2(h, w.pair(i))), m1), n_s, now.g.pair(i));
+                    if constexpr (GATE) {
+                        dgt[i] = fma2(g, u, dgt[i]);
+                        g = mul2(g, gate.pair(i));
                     }
-                    if (POST) {
-                        g[i] = kept ? g[i] * s : 0.0f;
-                        dpw[i] = fmaf(g[i], qn, dpw[i]);
-                        dpb[i] += g[i];
+                    if constexpr (POST) {
+                        if (p.drop) {
+                            g = mul2(g, drop_scale);
+                            g = make_float2(k0 ? g.x : 0.0f, k1 ? g.y : 0.0f);
+                        }
+                        dpw[i] = fma2(g, q, dpw[i]);
+                        dpb[i] = add2(dpb[i], g);
                     }
                 }
             }
         }
-        if (gate_sums) {
-            const bool whole = seg_lo == gate_row * p.gate_period && seg_hi == (gate_row + 1) * p.gate_period;
-            float* slot = p.partial + (4 * static_cast<int64_t>(p.units) + 2 * unit + (seg_lo == lo ? 0 : 1)) * p.cols + c;
+        if constexpr (GATE) {
+            if (gate_sums) {
+                const bool whole = seg_lo == gate_row * p.gate_period && seg_hi == (gate_row + 1) * p.gate_period;
+                float* slot = p.partial + (4 * static_cast<int64_t>(p.units) + 2 * unit + (seg_lo == lo ? 0 : 1)) * p.cols + c;
 #pragma unroll
-            for (int i = 0; i < V; ++i) {
-                if (whole) {
-                    static_cast<T*>(p.dgate)[gate_row * p.cols + c + i] = from_f<T>(dgt[i]);
-                } else {
-                    slot[i] = dgt[i];
+                for (int i = 0; i < STEP; ++i) {
+                    const float v = i % 2 ? dgt[i / 2].y : dgt[i / 2].x;
+                    if (whole) {
+                        static_cast<T*>(p.dgate)[gate_row * p.cols + c + i] = from_f<T>(v);
+                    } else {
+                        slot[i] = v;
+                    }
                 }
             }
         }
@@ -926,12 +967,12 @@ __global__ void __launch_bounds__(kPassThreads) residual_norm_column_pass_kernel
     const int64_t plane = static_cast<int64_t>(p.units) * p.cols;
     float* out = p.partial + unit * p.cols + c;
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-        out[i] = dw[i];
-        out[plane + i] = db[i];
-        if (POST) {
-            out[2 * plane + i] = dpw[i];
-            out[3 * plane + i] = dpb[i];
+    for (int i = 0; i < STEP; ++i) {
+        out[i] = i % 2 ? dw[i / 2].y : dw[i / 2].x;
+        out[plane + i] = i % 2 ? db[i / 2].y : db[i / 2].x;
+        if constexpr (POST) {
+            out[2 * plane + i] = i % 2 ? dpw[i / 2].y : dpw[i / 2].x;
+            out[3 * plane + i] = i % 2 ? dpb[i / 2].y : dpb[i / 2].x;
         }
     }
 }
@@ -1063,10 +1104,10 @@ Kernel backward_kernel(int nv, bool post, bool gate, bool sums) {
     return sums ? backward_kernel_of<T, 1, VEC, true>(post, gate) : backward_kernel_of<T, 1, VEC, false>(post, gate);
 }
 
-template <typename T, int V>
+template <typename T, bool VEC>
 Kernel column_pass_of(bool post, bool gate) {
-    if (post) return gate ? residual_norm_column_pass_kernel<T, V, true, true> : residual_norm_column_pass_kernel<T, V, true, false>;
-    return gate ? residual_norm_column_pass_kernel<T, V, false, true> : residual_norm_column_pass_kernel<T, V, false, false>;
+    if (post) return gate ? residual_norm_column_pass_kernel<T, VEC, true, true> : residual_norm_column_pass_kernel<T, VEC, true, false>;
+    return gate ? residual_norm_column_pass_kernel<T, VEC, false, true> : residual_norm_column_pass_kernel<T, VEC, false, false>;
 }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
@@ -1186,10 +1227,10 @@ bool is_wide(const tk_residual_norm_desc_t& d) {
     return d.cols > (sums5 || d.dtype == TK_DTYPE_F32 ? 1 : 2) * 256 * (kMaxThreads / 32);
 }
 
-// Row ranges of the column pass: about eight blocks per SM.
+// Row ranges of the column pass: one resident wave of four blocks per SM.
 int column_units(int device, int64_t rows, int64_t cols, bool vec) {
     const int64_t blocks = ceil_div(cols, kPassThreads * (vec ? 8 : 1));
-    return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(rows, ceil_div(8 * sm_count(device), blocks))));
+    return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(rows, 4 * sm_count(device) / blocks)));
 }
 
 template <typename T>
@@ -1297,8 +1338,8 @@ int tk_residual_norm_backward(const tk_residual_norm_grad_desc_t* desc, void* wo
     const bool sums = desc->dweight || desc->dbias || desc->dpost_weight || desc->dpost_bias || (p.dgate != nullptr && p.gate_period > 1);
     if (wide && sums) {
         p.units = pass_units;
-        const Kernel pass = f16 ? (vec ? column_pass_of<__half, 8>(post, gate) : column_pass_of<__half, 1>(post, gate))
-                                : (vec ? column_pass_of<float, 8>(post, gate) : column_pass_of<float, 1>(post, gate));
+        const Kernel pass = f16 ? (vec ? column_pass_of<__half, true>(post, gate) : column_pass_of<__half, false>(post, gate))
+                                : (vec ? column_pass_of<float, true>(post, gate) : column_pass_of<float, false>(post, gate));
         const cudaError_t e = launch_pdl(pass, dim3(static_cast<unsigned>(ceil_div(p.cols, kPassThreads * (vec ? 8 : 1))), p.units), dim3(kPassThreads), 0, s, p);
         if (e != cudaSuccess) {
             cudaGetLastError();
