@@ -171,7 +171,14 @@ def test_linear_ce_strided_and_misaligned_inputs():
     assert torch.equal(got, plain)
 
 
-@pytest.mark.parametrize("dtype,n,d,v", [(F16, 16384, 64, 20003), (F32, 9000, 40, 20003)])
+@pytest.mark.parametrize("n,d,v,ignored", [(2100, 512, 2300, 0), (2500, 1000, 2100, 900), (2050, 2048, 5003, 0), (4000, 1024, 2048, 3990)])
+def test_linear_ce_many_tiles(n, d, v, ignored):
+    # more tiles than pairs of SMs, and few, split along K
+    t, target = ce_inputs(n, d, v, F16, True, ignored, seed=n)
+    check_ce(t, target, "mean", torch.tensor(4096.0))
+
+
+@pytest.mark.parametrize("dtype,n,d,v", [(F16, 16384, 64, 20003), (F16, 14000, 512, 20003), (F32, 9000, 40, 20003)])
 def test_linear_ce_several_pieces_of_the_vocabulary(dtype, n, d, v):
     # dz of all columns is larger than one piece
     t, target = ce_inputs(n, d, v, dtype, True, n // 3, seed=12)
