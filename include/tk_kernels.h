@@ -485,8 +485,9 @@ TK_API int tk_residual_norm_backward(const tk_residual_norm_grad_desc_t* desc, v
  * and the gradients NaN.  reduction: one loss per row, or their mean over the
  * rows with a target (NaN without any) or sum.  Losses are fp32.  fp16
  * products are exact and summed in fp32; fp32 operands enter as two binary16
- * planes each (22 bits, or 2^-40 of the tensor's largest value).  The
- * counterpart in training of mse_loss (csrc/autograd.cpp). */
+ * planes each (22 bits, or 2^-40 of the tensor's largest value).  Sizes below
+ * 2^31 - 256, and no product of more than 2^30 tiles of 256 x 256.  A loss
+ * beside mse_loss; the reference has none of this kind. */
 typedef enum { TK_REDUCE_NONE = 0, TK_REDUCE_MEAN = 1, TK_REDUCE_SUM = 2 } tk_reduction_t;
 
 typedef struct {

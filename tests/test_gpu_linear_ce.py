@@ -1,6 +1,8 @@
 """The linear cross entropy against its 64-bit definition on the same rounded
 inputs (tests/_train_helpers.py derives the bounds), its gradients, masks and
 refusals, and the training operators in one step."""
+import ctypes
+
 import pytest
 import torch
 import torch.nn.functional as F
@@ -157,6 +159,63 @@ def test_linear_ce_other_ignore_index_and_leading_dimensions():
     assert loss.shape == (2, 3, 4) and loss.dtype == F32
     flat = run_ce(t, target, "none")["loss"]
     assert torch.equal(loss.cpu().view(-1), flat)
+
+
+def test_linear_ce_single_row_without_leading_dimensions():
+    t, target = ce_inputs(1, 40, 90, F16, True, seed=2)
+    x = t["x"][0].to(DEV).requires_grad_()
+    loss = ops.linear_cross_entropy(x, t["weight"].to(DEV), target[0].to(DEV), t["bias"].to(DEV), reduction="none")
+    assert loss.shape == ()
+    loss.backward()
+    want = R.linear_ce64(t["x"], t["weight"], target, t["bias"], reduction="none", grad=torch.ones(1))
+    R.assert_within(loss.detach().cpu()[None], *want["loss"], "loss")
+    R.assert_within(x.grad.cpu()[None], *want["x"], "x")
+
+
+def test_linear_ce_replayed_from_a_graph():
+    """The C entries captured into a CUDA graph and replayed on new values in the
+    same memory, twice, against ordinary calls."""
+    n, d, v = 300, 96, 1000
+    t, target = ce_inputs(n, d, v, F16, True, 40, seed=31)
+    cu = {k: u.cuda() for k, u in t.items()}
+    tg, g, loss = target.cuda(), torch.tensor([512.0], device="cuda"), torch.zeros(1, device="cuda")
+    out = {k: torch.empty_like(u) for k, u in cu.items()}
+    L, desc = _capi.lib(), _capi.LinearCeGradDesc()
+    f = desc.fwd
+    f.dtype, f.rows, f.cols, f.vocab, f.ignore_index, f.reduction = 0, n, d, v, -100, 1
+    f.x, f.weight, f.bias, f.target, f.loss = cu["x"].data_ptr(), cu["weight"].data_ptr(), cu["bias"].data_ptr(), tg.data_ptr(), loss.data_ptr()
+    desc.grad_loss, desc.dx, desc.dweight, desc.dbias = g.data_ptr(), out["x"].data_ptr(), out["weight"].data_ptr(), out["bias"].data_ptr()
+
+    def room(size):
+        b = torch.empty(size + 1024, dtype=torch.uint8, device="cuda")
+        return b, (b.data_ptr() + 1023) // 1024 * 1024
+
+    keep = [room(L.tk_linear_ce_state_size(ctypes.byref(f)))]
+    f.state = keep[0][1]
+    sizes = L.tk_linear_ce_workspace_size(ctypes.byref(f)), L.tk_linear_ce_backward_workspace_size(ctypes.byref(desc))
+    keep += [room(s) for s in sizes]
+
+    def call(stream):
+        _capi.check(L.tk_linear_ce(ctypes.byref(f), keep[1][1], sizes[0], stream), "tk_linear_ce")
+        _capi.check(L.tk_linear_ce_backward(ctypes.byref(desc), keep[2][1], sizes[1], stream), "tk_linear_ce_backward")
+
+    call(None)
+    torch.cuda.synchronize()
+    s = torch.cuda.Stream()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=s):
+        call(s.cuda_stream)
+    for seed in (32, 33):
+        t2, target2 = ce_inputs(n, d, v, F16, True, 10 * (seed - 30), seed=seed)
+        for k in cu:
+            cu[k].copy_(t2[k])
+        tg.copy_(target2)
+        graph.replay()
+        torch.cuda.synchronize()
+        plain = run_ce(t2, target2, "mean", torch.tensor(512.0))
+        assert torch.equal(loss.cpu()[0], plain["loss"])
+        for k in cu:
+            assert torch.equal(out[k].cpu(), plain[k]), k
 
 
 def test_linear_ce_strided_and_misaligned_inputs():

@@ -11,7 +11,7 @@ pytestmark = pytest.mark.gpu
 torch_kunlun = pytest.importorskip("torch_kunlun")
 kunlun = torch_kunlun.kunlun
 from tests import _train_helpers as R  # noqa: E402
-from torch_kunlun_b200 import ops  # noqa: E402
+from torch_kunlun_b200 import _capi as C, ops  # noqa: E402
 
 DEV = "kunlun"
 F16, F32 = torch.float16, torch.float32
@@ -67,16 +67,23 @@ def test_dropout_gradient_uses_the_same_mask():
     assert torch.equal(xd.grad.cpu(), dropout_reference(g, 0.25, 9, 2))
 
 
-def test_dropout_empty_and_large_index():
+def test_dropout_empty():
     assert ops.dropout(torch.empty(0, 5, dtype=F16).to(DEV), 0.5, 1).shape == (0, 5)
-    # element indices past 2^32: the block counter's high word is in use
-    n = (1 << 32) + 4096
-    if torch.cuda.mem_get_info()[0] < 24 << 30:
-        pytest.skip("needs 17 GB")
-    x = torch.empty(n, dtype=F16, device=DEV)
-    x.fill_(1.0)
-    tail = ops.dropout(x, 0.5, 21, 4)[-4096:].cpu()
-    words = np.concatenate([_block(i, 21, 4) for i in range((n - 4096) // 4, n // 4)])
+
+
+@pytest.mark.parametrize("n", [(1 << 32) + 4093, (1 << 34) + 4093])
+def test_dropout_large_index_in_place(n):
+    # element indices past 2^32, and past 2^34, where the block counter has a high word
+    if torch.cuda.mem_get_info()[0] < 2 * n + (8 << 30):
+        pytest.skip("needs the memory of one large tensor")
+    x = torch.ones(n, dtype=F16, device="cuda")
+    torch.cuda.synchronize()
+    C.check(C.lib().tk_dropout(0, x.data_ptr(), x.data_ptr(), n, 0.5, 21, 4, None), "tk_dropout")
+    torch.cuda.synchronize()
+    tail, first = x[-4096:].cpu(), n - 4096
+    del x
+    torch.cuda.empty_cache()
+    words = np.concatenate([_block(i, 21, 4) for i in range(first // 4, n // 4 + 1)])[first % 4:][:4096]
     assert torch.equal(tail, torch.from_numpy(np.where(words >= 1 << 31, 2.0, 0.0)).to(F16))
 
 
@@ -211,6 +218,58 @@ def test_residual_norm_strided_and_misaligned_inputs():
     want = R.residual_norm64(t["x"], t["f"], t["weight"], t["bias"], True, t["post_weight"], t["post_bias"], t["gate"])
     R.assert_within(x_new.cpu(), *want["x_new"], "x_new")
     R.assert_within(h.cpu(), *want["h"], "h")
+
+
+def test_residual_norm_vectors_shared_inputs_and_expanded_gates():
+    # one row without leading dimensions
+    t = {"x": rnd((70,), 1, F32), "f": rnd((70,), 2, F32), "weight": rnd((70,), 3, F32), "gate": rnd((70,), 4, F32)}
+    gx, gh = rnd((70,), 5, F32), rnd((70,), 6, F32)
+    got = run_norm(t, "layer", True, 1.0, 0.2, gx, gh)
+    one = lambda v: v[None]  # noqa: E731
+    want = R.residual_norm64(one(t["x"]), one(t["f"]), t["weight"], None, True, None, None, t["gate"], False, 1.0, 1e-5,
+                             R.keep_mask((1, 70), 0.2, 77, 5), 0.2, one(gx), one(gh))
+    for k, v in got.items():
+        R.assert_within(v, want[k][0].reshape(v.shape), want[k][1].expand_as(want[k][0]).reshape(v.shape), k)
+    # x and f one tensor: its gradient is the sum of both
+    x = rnd((3, 4, 32), 7, F32)
+    xd = x.to(DEV).requires_grad_()
+    y, _ = ops.residual_norm(xd, xd, residual_scale=2.0)
+    y.backward(torch.ones(3, 4, 32).to(DEV))
+    assert torch.equal(xd.grad.cpu(), torch.full((3, 4, 32), 3.0))
+    # a gate for all samples, with its leading ones
+    check_norm((3, 4, 32), F32, "rms", False, "none", t={"x": x, "f": rnd((3, 4, 32), 8, F32), "gate": rnd((1, 1, 32), 9, F32)})
+
+
+def test_train_ops_on_two_streams_at_once():
+    t = norm_inputs((4, 500, 512), F16, "rms", True, "sample", 5)
+    g = rnd((4, 500, 512), 6)
+    x, w = rnd((600, 128), 7), rnd((3000, 128), 8, F16, 0.1)
+    target = torch.randint(0, 3000, (600,), generator=torch.Generator().manual_seed(1)).to(DEV)
+
+    def both():
+        dev = {k: v.to(DEV).requires_grad_() for k, v in t.items()}
+        xd, wd = x.to(DEV).requires_grad_(), w.to(DEV).requires_grad_()
+        return dev, xd, wd
+
+    def work(dev, xd, wd):
+        y, h = ops.residual_norm(dev["x"], dev["f"], dev["weight"], norm="rms", post_norm=True, post_weight=dev["post_weight"], gate=dev["gate"], p=0.1, seed=3)
+        loss = ops.linear_cross_entropy(xd, wd, target)
+        return [y, h, loss] + list(torch.autograd.grad([y, h, loss], list(dev.values()) + [xd, wd], [gd, gd, one]))
+
+    gd, one = g.to(DEV), torch.tensor(64.0).to(DEV)
+    inputs = [both() for _ in range(4)]
+    kunlun.synchronize()
+    first = [v.detach().cpu() for v in work(*inputs[0])]
+    streams = [kunlun.Stream() for _ in range(2)]
+    results = []
+    for i in range(6):
+        with kunlun.stream(streams[i % 2]):
+            results.append(work(*inputs[1 + i % 3]))
+    for s in streams:
+        s.synchronize()
+    for r in results:
+        for a, b in zip(first, r):
+            assert torch.equal(a, b.detach().cpu())
 
 
 def test_residual_norm_non_finite_rows_stay_in_their_rows():

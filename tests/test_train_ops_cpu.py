@@ -97,6 +97,10 @@ def test_residual_norm_backward_needs_its_inputs():
     assert L.tk_residual_norm_backward(ctypes.byref(g), None, 0, None) == 1
     assert b"no incoming gradient" in L.tk_last_error_string()
     g.grad_h = 16
+    for field in ("dpost_weight", "dpost_bias", "dgate"):
+        setattr(g, field, 16)
+        assert L.tk_residual_norm_backward(ctypes.byref(g), None, 0, None) == 1, field
+        setattr(g, field, None)
     for field, bad in (("f", None), ("x", None), ("stats", 8)):
         kept = getattr(g.fwd, field)
         setattr(g.fwd, field, bad)
@@ -177,7 +181,7 @@ def _ce_desc(**kw):
 
 @pytest.mark.parametrize("fields,status", [
     (dict(dtype=3), 1), (dict(reduction=5), 1), (dict(rows=-1), 1), (dict(cols=0), 1), (dict(vocab=0), 1),
-    (dict(vocab=1 << 31), 2), (dict(rows=1 << 40), 2)])
+    (dict(vocab=1 << 31), 2), (dict(rows=1 << 40), 2), (dict(rows=1 << 30, vocab=1 << 20), 2), (dict(cols=1 << 30, vocab=1 << 20), 2)])
 def test_linear_ce_refuses_bad_arguments_before_the_device(fields, status):
     L = C.lib()
     d = _ce_desc(**fields)

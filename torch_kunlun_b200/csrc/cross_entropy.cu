@@ -50,8 +50,8 @@
 namespace tk {
 namespace {
 
-constexpr int BM = 256, BN = 256, BK = 64;     // a pair's tile
-constexpr int HM = BM / 2, HN = BN / 2;          // one CTA's operand rows
+constexpr int BM = 256, BN = 256, BK = 64;  // a pair's tile
+constexpr int HM = BM / 2, HN = BN / 2;     // one CTA's operand rows
 constexpr int A_BYTES = HM * BK * 2, B_BYTES = HN * BK * 2;
 constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
 // An epilogue warp turns 32 rows x 16 columns through its own 2.5 KB, so that
@@ -59,6 +59,7 @@ constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
 // 16-byte accesses).
 constexpr int TURN = 16;
 constexpr int PITCH = TURN + 4;
+
 // kPlain: eight epilogue warps, six stages.  kWide: sixteen warps for dz where
 // the K loop is short (the logits of 2384 rows by 30011 words at 768 columns,
 // 12 K blocks: 177 -> 166 us; at 64 K blocks five stages cost 3 %).  kChunked:
@@ -104,12 +105,12 @@ struct GemmParams {
     int planes;    // 1 (fp16 operands) or 2 (fp32)
     int chunk;     // K blocks per accumulator chunk
     int max_units; // tiles x K splits the workspace of a split reduction holds
-    int64_t vocab0, vocab;  // the piece's first column, all columns
     int group;     // M tiles that neighbouring CTAs share
     unsigned* err;
     // kStats / kDlogits
+    int64_t vocab0, vocab;  // the piece's first column, all columns
     const float* bias2;  // bias * log2(e), or NULL
-    float2* part;           // [rows][n_tiles][kParts] maximum and sum
+    float2* part;        // [rows][n_tiles][kParts] maximum and sum
     const float* lse2;
     const float* grow;   // g_i / max |g|
     const int* target;
@@ -1142,7 +1143,7 @@ ce_dbias_kernel(const float* partial, int chunks, int64_t dz_ld, int64_t cols, c
 // ---- host --------------------------------------------------------------------------
 
 constexpr int64_t kDzBytes = 512ll << 20;   // one piece's dz
-constexpr int64_t kMaxSize = 0x7FFFFF00;
+constexpr int64_t kMaxSize = 0x7FFFFF00, kMaxTiles = 1 << 30;
 
 size_t align(size_t v) { return round_up(v, 1024); }
 
@@ -1169,6 +1170,8 @@ int check(const char* who, const tk_linear_ce_desc_t& d) {
     TK_CHECK_ARG(d.reduction == TK_REDUCE_NONE || d.reduction == TK_REDUCE_MEAN || d.reduction == TK_REDUCE_SUM, "%s: bad reduction %d", who, d.reduction);
     TK_CHECK_ARG(d.rows >= 0 && d.cols >= 1 && d.vocab >= 1, "%s: rows must not be negative, cols and vocab must be positive", who);
     if (d.rows > kMaxSize || d.cols > kMaxSize || d.vocab > kMaxSize) TK_FAIL(TK_ERR_UNSUPPORTED, "%s: sizes must be below 2^31 - 256", who);
+    const int64_t m = ceil_div(d.rows, BM), n = ceil_div(d.vocab, BN), k = ceil_div(d.cols, BN);
+    if (m * n > kMaxTiles || m * k > kMaxTiles || n * k > kMaxTiles) TK_FAIL(TK_ERR_UNSUPPORTED, "%s: a product has more than 2^30 tiles of 256 x 256", who);
     return TK_OK;
 }
 

@@ -1306,6 +1306,8 @@ int tk_residual_norm_backward(const tk_residual_norm_grad_desc_t* desc, void* wo
         if (desc->dgate != nullptr && d.gate != nullptr) TK_CUDA_TRY(cudaMemsetAsync(desc->dgate, 0, row * d.gate_rows, s));
         return TK_OK;
     }
+    TK_CHECK_ARG(d.post_norm || (!desc->dpost_weight && !desc->dpost_bias), "tk_residual_norm_backward: dpost_weight and dpost_bias need post_norm");
+    TK_CHECK_ARG(d.gate || !desc->dgate, "tk_residual_norm_backward: dgate without a gate");
     TK_CHECK_ARG(d.x && d.f && d.stats && aligned16(d.stats), "tk_residual_norm_backward: x, f and 16-byte aligned stats are needed");
     TK_CHECK_ARG(desc->grad_x_new || desc->grad_h, "tk_residual_norm_backward: no incoming gradient");
     RnParams p = params(d);
