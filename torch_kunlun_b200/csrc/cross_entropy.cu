@@ -897,64 +897,130 @@ struct PackJob {
     bool vec;          // 16-byte aligned rows, cols a multiple of 8
 };
 
+// Packs row r of the planes from a row of src (NULL: zeros).
 template <typename T, int PLANES>
-__device__ __forceinline__ void pack_rows(const PackJob<T>& j, int64_t live, int64_t rows, float s, int64_t block, int64_t blocks) {
+__device__ __forceinline__ void pack_row(const PackJob<T>& j, const T* from, int64_t r, float s) {
     const void* end = j.src + j.rows * j.cols;
-    for (int64_t r = block; r < rows; r += blocks) {
-        const T* from = r < live ? j.src + (j.index != nullptr ? static_cast<int64_t>(j.index[r]) : r) * j.cols : nullptr;
-        __half* to = j.dst + r * j.ld;
-        for (int64_t c = static_cast<int64_t>(threadIdx.x) * 8; c < j.ld; c += blockDim.x * 8) {
-            float v[8];
-            if (from == nullptr) {
+    __half* to = j.dst + r * j.ld;
+    for (int64_t c = static_cast<int64_t>(threadIdx.x) * 8; c < j.ld; c += blockDim.x * 8) {
+        float v[8];
+        if (from == nullptr) {
 #pragma unroll
-                for (int i = 0; i < 8; ++i) v[i] = 0.0f;
-            } else if (j.vec) {
-                if constexpr (sizeof(T) == 2) {
-                    *reinterpret_cast<uint4*>(to + c) = *reinterpret_cast<const uint4*>(from + c);
-                    continue;
-                } else {
-                    const float4 a = *reinterpret_cast<const float4*>(from + c), b = *reinterpret_cast<const float4*>(from + c + 4);
-                    v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w;
-                    v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
-                }
+            for (int i = 0; i < 8; ++i) v[i] = 0.0f;
+        } else if (j.vec) {
+            if constexpr (sizeof(T) == 2) {
+                *reinterpret_cast<uint4*>(to + c) = *reinterpret_cast<const uint4*>(from + c);
+                continue;
             } else {
-                load8_any(from + c, j.cols - c, j.src, end, v);
+                const float4 a = *reinterpret_cast<const float4*>(from + c), b = *reinterpret_cast<const float4*>(from + c + 4);
+                v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w;
+                v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
             }
-            uint32_t hi[4], lo[4];
-#pragma unroll
-            for (int t = 0; t < 4; ++t) {
-                const float a = v[2 * t] * s, b = v[2 * t + 1] * s;
-                hi[t] = half2_bits(a, b);
-                const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&hi[t]));
-                // a non-finite value is all in its high plane
-                lo[t] = half2_bits(isfinite(f.x) ? a - f.x : 0.0f, isfinite(f.y) ? b - f.y : 0.0f);
-            }
-            *reinterpret_cast<uint4*>(to + c) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-            if constexpr (PLANES == 2) *reinterpret_cast<uint4*>(to + j.plane + c) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+        } else {
+            load8_any(from + c, j.cols - c, j.src, end, v);
         }
+        uint32_t hi[4], lo[4];
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+            const float a = v[2 * t] * s, b = v[2 * t + 1] * s;
+            hi[t] = half2_bits(a, b);
+            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&hi[t]));
+            // a non-finite value is all in its high plane
+            lo[t] = half2_bits(isfinite(f.x) ? a - f.x : 0.0f, isfinite(f.y) ? b - f.y : 0.0f);
+        }
+        *reinterpret_cast<uint4*>(to + c) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+        if constexpr (PLANES == 2) *reinterpret_cast<uint4*>(to + j.plane + c) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+    }
+}
+
+// W's rows and the bias in base 2: blocks [0, w_blocks), the rest.
+template <typename T, int PLANES>
+__device__ __forceinline__ void pack_weight_and_bias(const PackJob<T>& w, float s, int block, int w_blocks, const T* bias, float* bias2) {
+    if (block < w_blocks) {
+        for (int64_t r = block; r < w.rows; r += w_blocks) pack_row<T, PLANES>(w, w.src + r * w.cols, r, s);
+    } else {
+        const int64_t i = static_cast<int64_t>(block - w_blocks) * blockDim.x + threadIdx.x;
+        if (i < w.rows) bias2[i] = load_f(bias, i) * kLog2e;
     }
 }
 
 constexpr int kPackThreads = 128;
 
-// Packs x's listed rows (zero rows after them up to a multiple of BK), W
-// where it is not read in place, and the bias in base 2: blocks [0, x_blocks),
-// the next w_blocks, the rest.
+// Packs x's listed rows (zero rows after them up to a multiple of BK; blocks
+// [0, x_blocks)), W where it is not read in place, and the bias in base 2.
 template <typename T, int PLANES>
 __global__ void __launch_bounds__(kPackThreads)
 ce_pack_kernel(const PackJob<T> x, const PackJob<T> w, const Scalars* sc, int x_blocks, int w_blocks, const T* bias, float* bias2) {
     pdl_wait();
     const int b = static_cast<int>(blockIdx.x);
-    if (b < x_blocks) {
-        const int64_t live = sc->count;
-        pack_rows<T, PLANES>(x, live, (live + BK - 1) / BK * BK, PLANES == 2 ? plane_scale(sc->amax_x) : 1.0f, b, x_blocks);
-    } else if (b < x_blocks + w_blocks) {
-        pack_rows<T, PLANES>(w, w.rows, w.rows, PLANES == 2 ? plane_scale(sc->amax_w) : 1.0f, b - x_blocks, w_blocks);
-    } else {
-        const int64_t i = static_cast<int64_t>(b - x_blocks - w_blocks) * kPackThreads + threadIdx.x;
-        if (i < w.rows) bias2[i] = load_f(bias, i) * kLog2e;
+    if (b >= x_blocks) {
+        pack_weight_and_bias<T, PLANES>(w, PLANES == 2 ? plane_scale(sc->amax_w) : 1.0f, b - x_blocks, w_blocks, bias, bias2);
+        return;
     }
+    const int64_t live = sc->count;
+    const float s = PLANES == 2 ? plane_scale(sc->amax_x) : 1.0f;
+    for (int64_t r = b; r < (live + BK - 1) / BK * BK; r += x_blocks)
+        pack_row<T, PLANES>(x, r < live ? x.src + static_cast<int64_t>(x.index[r]) * x.cols : nullptr, r, s);
 }
+
+// ce_index_kernel and ce_pack_kernel in one launch, for up to 1024 rows of
+// fp16: every block that packs a row lists the rows itself, block 0 writes the
+// list down (8 rows by 30011 words: the forward pass 24 -> 22 us).
+constexpr int kListRows = 1024;
+
+__global__ void __launch_bounds__(kPackThreads)
+ce_list_pack_kernel(const int64_t* target, int rows, int64_t vocab, int64_t ignore, int* index, int* packed_target, Scalars* sc, float* row_loss_out,
+                    const PackJob<__half> x, const PackJob<__half> w, int x_blocks, int w_blocks, const __half* bias, float* bias2) {
+    pdl_wait();
+    const int b = static_cast<int>(blockIdx.x);
+    if (b >= x_blocks) {
+        pack_weight_and_bias<__half, 1>(w, 1.0f, b - x_blocks, w_blocks, bias, bias2);
+        return;
+    }
+    constexpr int WARPS = kPackThreads / 32, SPANS = kListRows / 32;
+    __shared__ unsigned used[SPANS];
+    __shared__ int before[SPANS], total, mine;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    for (int s = warp; s < SPANS; s += WARPS) {
+        const int r = s * 32 + lane;
+        const unsigned u = __ballot_sync(0xFFFFFFFFu, r < rows && target[r] != ignore);
+        if (lane == 0) used[s] = u;
+    }
+    __syncthreads();
+    if (warp == 0) {
+        const int v = __popc(used[lane]);
+        int s = v;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const int o = __shfl_up_sync(0xFFFFFFFFu, s, d);
+            if (lane >= d) s += o;
+        }
+        before[lane] = s - v;
+        if (lane == 31) total = s;
+    }
+    __syncthreads();
+    for (int s = warp; s < SPANS; s += WARPS) {
+        const int r = s * 32 + lane;
+        if ((used[s] >> lane) & 1u) {
+            const int at = before[s] + __popc(used[s] & ((1u << lane) - 1u));
+            if (at == b) mine = r;
+            if (b == 0) {
+                const int64_t t = target[r];
+                index[at] = r;
+                packed_target[at] = t >= 0 && t < vocab ? static_cast<int>(t) : -1;  // -1: the loss is NaN
+            }
+        } else if (b == 0 && r < rows && row_loss_out != nullptr) {
+            row_loss_out[r] = 0.0f;
+        }
+    }
+    __syncthreads();
+    if (b == 0 && threadIdx.x == 0) {
+        sc->count = total;
+        sc->rows_done = 0;
+    }
+    if (b < (total + BK - 1) / BK * BK) pack_row<__half, 1>(x, b < total ? x.src + static_cast<int64_t>(mine) * x.cols : nullptr, b, 1.0f);
+}
+static_assert(kListRows == 32 * 32, "one warp sums the spans");
 
 // This lane's part of the dot product of two rows, in one order however the
 // rows are aligned.
@@ -1306,25 +1372,42 @@ int gemm(const CUtensorMap& a, const CUtensorMap& b, const GemmParams& p, int64_
 
 int blocks_for(int64_t rows) { return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(rows, 148 * 16))); }
 
-// The kept operands (x's listed rows; W unless it is read in place; the bias).
+// The list of rows and the kept operands (x's listed rows; W unless it is read
+// in place; the bias).
 template <typename T, int PLANES>
-int pack(const tk_linear_ce_desc_t& d, const Plan& p, uint8_t* st, cudaStream_t s) {
+int list_and_pack(const tk_linear_ce_desc_t& d, const Plan& p, uint8_t* st, cudaStream_t s) {
     const T* x = static_cast<const T*>(d.x);
     const T* w = static_cast<const T*>(d.weight);
+    const T* bias = static_cast<const T*>(d.bias);
     Scalars* sc = reinterpret_cast<Scalars*>(st + p.s_scalars);
-    const int* index = reinterpret_cast<const int*>(st + p.s_index);
+    int* index = reinterpret_cast<int*>(st + p.s_index);
+    int* target = reinterpret_cast<int*>(st + p.s_target);
+    float* bias2 = reinterpret_cast<float*>(st + p.s_bias);
+    float* row_loss = d.reduction == TK_REDUCE_NONE ? d.loss : nullptr;
     const bool eight = d.cols % 8 == 0;
-    if constexpr (PLANES == 2)
-        CE_TRY(launch_chain("cross entropy amax", ce_amax_kernel, dim3(148 * 4, 2), dim3(256), 0, s, x, w, index, sc, d.cols, d.vocab));
     const PackJob<T> jx = {x, index, reinterpret_cast<__half*>(st + p.s_x), d.rows, d.cols, p.ld, p.rows_pad * p.ld,
                            eight && (reinterpret_cast<uintptr_t>(x) & 15) == 0};
     const PackJob<T> jw = {w, nullptr, reinterpret_cast<__half*>(st + p.s_w), d.vocab, d.cols, p.ld, d.vocab * p.ld,
                            eight && (reinterpret_cast<uintptr_t>(w) & 15) == 0};
-    const int x_blocks = blocks_for(p.rows_pad), w_blocks = p.w_direct ? 0 : blocks_for(d.vocab);
+    const int w_blocks = p.w_direct ? 0 : blocks_for(d.vocab);
     const int64_t b_blocks = d.bias != nullptr ? ceil_div(d.vocab, kPackThreads) : 0;
+    if constexpr (PLANES == 1) {
+        if (d.rows > 0 && d.rows <= kListRows) {
+            const int x_blocks = static_cast<int>(p.rows_read);
+            return launch_chain("cross entropy pack", ce_list_pack_kernel, dim3(static_cast<unsigned>(x_blocks + w_blocks + b_blocks)), dim3(kPackThreads),
+                                0, s, d.target, static_cast<int>(d.rows), d.vocab, d.ignore_index, index, target, sc, row_loss, jx, jw, x_blocks,
+                                w_blocks, bias, bias2);
+        }
+    }
+    auto* list = d.rows <= kIndexThreads ? ce_index_kernel<1> : ce_index_kernel<8>;
+    list<<<1, kIndexThreads, 0, s>>>(d.target, d.rows, d.vocab, d.ignore_index, index, target, sc, row_loss);
+    CE_TRY(launch_status("cross entropy index"));
+    if (d.rows == 0) return TK_OK;
+    if constexpr (PLANES == 2)
+        CE_TRY(launch_chain("cross entropy amax", ce_amax_kernel, dim3(148 * 4, 2), dim3(256), 0, s, x, w, static_cast<const int*>(index), sc, d.cols, d.vocab));
+    const int x_blocks = blocks_for(p.rows_read);
     return launch_chain("cross entropy pack", ce_pack_kernel<T, PLANES>, dim3(static_cast<unsigned>(x_blocks + w_blocks + b_blocks)), dim3(kPackThreads), 0,
-                        s, jx, jw, static_cast<const Scalars*>(sc), x_blocks, w_blocks, static_cast<const T*>(d.bias),
-                        reinterpret_cast<float*>(st + p.s_bias));
+                        s, jx, jw, static_cast<const Scalars*>(sc), x_blocks, w_blocks, bias, bias2);
 }
 
 template <typename T>
@@ -1392,17 +1475,12 @@ int tk_linear_ce(const tk_linear_ce_desc_t* desc, void* workspace, size_t worksp
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     uint8_t* ws = static_cast<uint8_t*>(workspace);
     uint8_t* st = d.state != nullptr ? static_cast<uint8_t*>(d.state) : ws + (p.fwd_bytes - p.state_bytes);
-    auto* index = d.rows <= kIndexThreads ? ce_index_kernel<1> : ce_index_kernel<8>;
-    index<<<1, kIndexThreads, 0, s>>>(d.target, d.rows, d.vocab, d.ignore_index, reinterpret_cast<int*>(st + p.s_index),
-                                                reinterpret_cast<int*>(st + p.s_target), reinterpret_cast<Scalars*>(st + p.s_scalars),
-                                                d.reduction == TK_REDUCE_NONE ? d.loss : nullptr);
-    CE_TRY(launch_status("cross entropy index"));
+    if (p.f16) {
+        CE_TRY((list_and_pack<__half, 1>(d, p, st, s)));
+    } else {
+        CE_TRY((list_and_pack<float, 2>(d, p, st, s)));
+    }
     if (d.rows > 0) {
-        if (p.f16) {
-            CE_TRY((pack<__half, 1>(d, p, st, s)));
-        } else {
-            CE_TRY((pack<float, 2>(d, p, st, s)));
-        }
         const Operand w = weight_operand(d, p, st);
         CUtensorMap tx, tw;
         CE_TRY(make_map(&tx, st + p.s_x, d.cols, p.rows_read, p.planes, p.ld, p.rows_pad * p.ld, HM));
