@@ -60,25 +60,36 @@ constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
 constexpr int TURN = 16;
 constexpr int PITCH = TURN + 4;
 
-// kPlain: eight epilogue warps, six stages.  kWide: sixteen warps for dz where
-// the K loop is short (the logits of 2384 rows by 30011 words at 768 columns,
-// 12 K blocks: 177 -> 166 us; at 64 K blocks five stages cost 3 %).  kChunked:
-// sums in registers, 128 columns per thread.  kPlanes: the same for fp32
-// operands.
-enum Mode { kPlain, kWide, kChunked, kPlanes };
+// kPlain: eight epilogue warps, six stages.  kWide: sixteen warps for dz and dW
+// where the K loop is short (dz of 2384 rows by 30011 words at 768 columns, 12
+// K blocks: 177 -> 166 us; at 64 K blocks five stages cost 3 %; dW of 9 rows,
+// 110320 x 325: 101 -> 90 us; dx of 122 rows, 1199 x 235: 12.0 -> 12.5, and the
+// statistics of 9 x 325 by 110320: 31.0 -> 32.7, so they stay plain).
+// kChunked: sums in registers, 128 columns per thread.  kPlanes: the same for
+// fp32 operands.  kPlanesWide: sixteen warps where fp32's K loop is one chunk (13 x 64 by 82545
+// words: logits 25 -> 19, dz 52 -> 29, dW 35 -> 22 us).
+enum Mode { kPlain, kWide, kChunked, kPlanes, kPlanesWide };
 constexpr int kWideBlocks = 24;  // K blocks up to which kWide is taken
 
 template <int MODE>
 struct Config {
-    static constexpr int STAGES = MODE == kWide ? 5 : 6;
-    static constexpr int EPI_WARPS = MODE == kWide ? 16 : 8;
+    static constexpr int PLANES = MODE == kPlanes || MODE == kPlanesWide ? 2 : 1;
+    static constexpr bool CHUNKED = MODE == kChunked || MODE == kPlanes;
+    static constexpr bool WIDE = MODE == kWide || MODE == kPlanesWide;
+    static constexpr int STAGES = MODE == kWide ? 5 : MODE == kPlanesWide ? 4 : 6;  // a multiple of PLANES
+    static constexpr int EPI_WARPS = WIDE ? 16 : 8;
     static constexpr int COLS = BN / (EPI_WARPS / 4);  // of a tile row, per warp
     static constexpr int THREADS = 64 + 32 * EPI_WARPS;
     static constexpr int TURN_BYTES = EPI_WARPS * 32 * PITCH * 4;
     static constexpr int SMEM = STAGES * STAGE_BYTES + TURN_BYTES + 1024 + 256;
     static_assert(SMEM <= 232448, "shared memory budget");
 };
-constexpr int kParts = BN / Config<kPlain>::COLS;  // statistics per row of a tile
+
+// K blocks per accumulator chunk: 24 steps of 16 (two blocks, three products)
+// where every output is binary32, 64 for the loss of fp16 operands (measured at
+// 4096 columns: the loss 1e-6 off without chunks, and the same time).
+constexpr int kChunkF32 = 2, kChunkStats = 16;
+
 constexpr int TMEM_COLS = 512;
 
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
@@ -110,7 +121,7 @@ struct GemmParams {
     // kStats / kDlogits
     int64_t vocab0, vocab;  // the piece's first column, all columns
     const float* bias2;  // bias * log2(e), or NULL
-    float2* part;        // [rows][n_tiles][kParts] maximum and sum
+    float2* part;        // [rows][n_tiles][BN / COLS] maximum and sum
     const float* lse2;
     const float* grow;   // g_i / max |g|
     const int* target;
@@ -363,9 +374,8 @@ ce_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
     constexpr bool A_MN = EPI == kGradW, B_MN = EPI == kGradX || EPI == kGradW;
     constexpr uint32_t IDESC = idesc_f16(BM, BN, A_MN, B_MN);
     using C = Config<MODE>;
-    constexpr bool CHUNKED = MODE == kChunked || MODE == kPlanes;
-    constexpr int PLANES = MODE == kPlanes ? 2 : 1;
-    static_assert(MODE != kWide || EPI == kDlogits, "wide epilogues are for dz");
+    constexpr bool CHUNKED = C::CHUNKED;
+    constexpr int PLANES = C::PLANES;
     constexpr int STAGES = C::STAGES, EPI_WARPS = C::EPI_WARPS, COLS = C::COLS;
     static_assert(STAGES % PLANES == 0, "both planes' stages are neighbours");
     extern __shared__ __align__(1024) uint8_t smem_raw[];
@@ -603,6 +613,7 @@ ce_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
                         });
                     }
                 } else {
+                    if (col >= p.out_cols && sh.splits == 1) return;
 #pragma unroll
                     for (int h = 0; h < 32; h += TURN) {
                         turn_in(buf_turn, lane, acc + h);
@@ -665,7 +676,7 @@ ce_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
 #pragma unroll
                 for (int c = 0; c < COLS; c += 32) take(c, v + c);
             }
-            if constexpr (EPI == kStats) p.part[(m * p.n_tiles + nt) * kParts + share] = make_float2(top, sum);
+            if constexpr (EPI == kStats) p.part[(m * p.n_tiles + nt) * (BN / COLS) + share] = make_float2(top, sum);
         }
     }
     tc_fence_before();
@@ -897,47 +908,65 @@ struct PackJob {
     bool vec;          // 16-byte aligned rows, cols a multiple of 8
 };
 
-// Packs row r of the planes from a row of src (NULL: zeros).
+// Packs the octet at column c of the planes' row r from a row of src (NULL:
+// zeros).
 template <typename T, int PLANES>
-__device__ __forceinline__ void pack_row(const PackJob<T>& j, const T* from, int64_t r, float s) {
-    const void* end = j.src + j.rows * j.cols;
-    __half* to = j.dst + r * j.ld;
-    for (int64_t c = static_cast<int64_t>(threadIdx.x) * 8; c < j.ld; c += blockDim.x * 8) {
-        float v[8];
-        if (from == nullptr) {
+__device__ __forceinline__ void pack_octet(const PackJob<T>& j, const T* from, int64_t r, int64_t c, float s) {
+    __half* to = j.dst + r * j.ld + c;
+    float v[8];
+    if (from == nullptr) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = 0.0f;
-        } else if (j.vec) {
-            if constexpr (sizeof(T) == 2) {
-                *reinterpret_cast<uint4*>(to + c) = *reinterpret_cast<const uint4*>(from + c);
-                continue;
-            } else {
-                const float4 a = *reinterpret_cast<const float4*>(from + c), b = *reinterpret_cast<const float4*>(from + c + 4);
-                v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w;
-                v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
-            }
+        for (int i = 0; i < 8; ++i) v[i] = 0.0f;
+    } else if (j.vec) {
+        if constexpr (sizeof(T) == 2) {
+            *reinterpret_cast<uint4*>(to) = *reinterpret_cast<const uint4*>(from + c);
+            return;
         } else {
-            load8_any(from + c, j.cols - c, j.src, end, v);
+            const float4 a = *reinterpret_cast<const float4*>(from + c), b = *reinterpret_cast<const float4*>(from + c + 4);
+            v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w;
+            v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
         }
-        uint32_t hi[4], lo[4];
-#pragma unroll
-        for (int t = 0; t < 4; ++t) {
-            const float a = v[2 * t] * s, b = v[2 * t + 1] * s;
-            hi[t] = half2_bits(a, b);
-            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&hi[t]));
-            // a non-finite value is all in its high plane
-            lo[t] = half2_bits(isfinite(f.x) ? a - f.x : 0.0f, isfinite(f.y) ? b - f.y : 0.0f);
-        }
-        *reinterpret_cast<uint4*>(to + c) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-        if constexpr (PLANES == 2) *reinterpret_cast<uint4*>(to + j.plane + c) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+    } else {
+        load8_any(from + c, j.cols - c, j.src, j.src + j.rows * j.cols, v);
     }
+    uint32_t hi[4], lo[4];
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+        const float a = v[2 * t] * s, b = v[2 * t + 1] * s;
+        hi[t] = half2_bits(a, b);
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&hi[t]));
+        // a non-finite value is all in its high plane
+        lo[t] = half2_bits(isfinite(f.x) ? a - f.x : 0.0f, isfinite(f.y) ? b - f.y : 0.0f);
+    }
+    *reinterpret_cast<uint4*>(to) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+    if constexpr (PLANES == 2) *reinterpret_cast<uint4*>(to + j.plane) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
 }
 
-// W's rows and the bias in base 2: blocks [0, w_blocks), the rest.
+template <typename T, int PLANES>
+__device__ __forceinline__ void pack_row(const PackJob<T>& j, const T* from, int64_t r, float s) {
+    for (int64_t c = static_cast<int64_t>(threadIdx.x) * 8; c < j.ld; c += blockDim.x * 8) pack_octet<T, PLANES>(j, from, r, c, s);
+}
+
+// W's octets and the bias in base 2: blocks [0, w_blocks), the rest.  Octets are
+// dealt out over rows, since a row may have few (110320 x 325 in fp16: 64 -> 32
+// us against a row per block; 82545 x 64 in fp32: 22 -> 7).
 template <typename T, int PLANES>
 __device__ __forceinline__ void pack_weight_and_bias(const PackJob<T>& w, float s, int block, int w_blocks, const T* bias, float* bias2) {
     if (block < w_blocks) {
-        for (int64_t r = block; r < w.rows; r += w_blocks) pack_row<T, PLANES>(w, w.src + r * w.cols, r, s);
+        const int64_t row = w.ld / 8, octets = w.rows * row, step = static_cast<int64_t>(w_blocks) * blockDim.x;
+        int64_t i = static_cast<int64_t>(block) * blockDim.x + threadIdx.x;
+        int64_t r = i / row, o = i - r * row;
+        const int64_t dr = step / row, dn = step - dr * row;
+#pragma unroll 2
+        for (; i < octets; i += step) {
+            pack_octet<T, PLANES>(w, w.src + r * w.cols, r, 8 * o, s);
+            r += dr;
+            o += dn;
+            if (o >= row) {
+                o -= row;
+                ++r;
+            }
+        }
     } else {
         const int64_t i = static_cast<int64_t>(block - w_blocks) * blockDim.x + threadIdx.x;
         if (i < w.rows) bias2[i] = load_f(bias, i) * kLog2e;
@@ -965,7 +994,7 @@ ce_pack_kernel(const PackJob<T> x, const PackJob<T> w, const Scalars* sc, int x_
 
 // ce_index_kernel and ce_pack_kernel in one launch, for up to 1024 rows of
 // fp16: every block that packs a row lists the rows itself, block 0 writes the
-// list down (8 rows by 30011 words: the forward pass 24 -> 22 us).
+// list down (8 rows by 30011 words, both directions: 23.7 -> 22.9 us).
 constexpr int kListRows = 1024;
 
 __global__ void __launch_bounds__(kPackThreads)
@@ -1222,6 +1251,7 @@ struct Plan {
     int64_t piece;           // vocabulary columns per piece (a multiple of BN)
     int64_t pieces;
     int64_t acc_ld;
+    int64_t parts;           // statistics per row
     int split_units;
     int db_chunks;
     // state: kept from the forward to the backward pass
@@ -1241,11 +1271,18 @@ int check(const char* who, const tk_linear_ce_desc_t& d) {
     return TK_OK;
 }
 
-// K blocks per accumulator chunk: 24 steps of 16 (two blocks, three products)
-// where every output is binary32, 64 for the loss of fp16 operands (measured at
-// 4096 columns: the loss 1e-6 off without chunks, and the same time).  A K loop
-// of fp16 no longer than a chunk needs no sum in registers.
-constexpr int kChunkF32 = 2, kChunkStats = 16;
+template <int EPI>
+Mode mode_of(int planes, int64_t k_blocks) {
+    if (planes == 2) return k_blocks <= kChunkF32 ? kPlanesWide : kPlanes;
+    if (EPI == kStats) return k_blocks <= kChunkStats ? kPlain : kChunked;
+    return (EPI == kDlogits || EPI == kGradW) && k_blocks <= kWideBlocks ? kWide : kPlain;
+}
+
+// Statistics per row and tile.
+int stats_parts(int planes, int64_t cols) {
+    const Mode m = mode_of<kStats>(planes, ceil_div(cols, BK));
+    return BN / (m == kPlanesWide ? Config<kPlanesWide>::COLS : Config<kChunked>::COLS);
+}
 
 Plan make_plan(const tk_linear_ce_desc_t& d) {
     Plan p = {};
@@ -1279,7 +1316,8 @@ Plan make_plan(const tk_linear_ce_desc_t& d) {
     p.s_bias = take(d.bias != nullptr ? static_cast<size_t>(d.vocab) * sizeof(float) : 0);
     p.state_bytes = at;
     at = 0;
-    p.w_part = take(static_cast<size_t>(kParts * p.n_tiles) * p.rows_pad * sizeof(float2));
+    p.parts = stats_parts(p.planes, d.cols) * p.n_tiles;
+    p.w_part = take(static_cast<size_t>(p.parts) * p.rows_pad * sizeof(float2));
     p.w_loss = take(p.rows_pad * sizeof(float));
     p.fwd_bytes = at + p.state_bytes;  // a call without a state keeps its own
     at = 0;
@@ -1357,17 +1395,16 @@ int gemm_launch(const CUtensorMap& a, const CUtensorMap& b, const GemmParams& p,
     return TK_OK;
 }
 
+// k_most: the most K blocks there can be, where the device's list decides.
 template <int EPI>
-int gemm(const CUtensorMap& a, const CUtensorMap& b, const GemmParams& p, int64_t most_units, cudaStream_t s) {
-    if (p.planes == 2) return gemm_launch<EPI, kPlanes>(a, b, p, most_units, s);
-    const int64_t blocks = p.k_blocks < 0 ? INT64_MAX : p.k_blocks;
-    if constexpr (EPI == kStats) {
-        if (blocks > p.chunk) return gemm_launch<EPI, kChunked>(a, b, p, most_units, s);
+int gemm(const CUtensorMap& a, const CUtensorMap& b, const GemmParams& p, int64_t most_units, cudaStream_t s, int64_t k_most = 0) {
+    switch (mode_of<EPI>(p.planes, p.k_blocks >= 0 ? p.k_blocks : k_most)) {
+        case kPlanes: return gemm_launch<EPI, kPlanes>(a, b, p, most_units, s);
+        case kPlanesWide: return gemm_launch<EPI, kPlanesWide>(a, b, p, most_units, s);
+        case kWide: return gemm_launch<EPI, EPI == kDlogits || EPI == kGradW ? kWide : kPlain>(a, b, p, most_units, s);
+        case kChunked: return gemm_launch<EPI, EPI == kStats ? kChunked : kPlain>(a, b, p, most_units, s);
+        default: return gemm_launch<EPI, kPlain>(a, b, p, most_units, s);
     }
-    if constexpr (EPI == kDlogits) {
-        if (blocks <= kWideBlocks) return gemm_launch<EPI, kWide>(a, b, p, most_units, s);
-    }
-    return gemm_launch<EPI, kPlain>(a, b, p, most_units, s);
 }
 
 int blocks_for(int64_t rows) { return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(rows, 148 * 16))); }
@@ -1389,7 +1426,7 @@ int list_and_pack(const tk_linear_ce_desc_t& d, const Plan& p, uint8_t* st, cuda
                            eight && (reinterpret_cast<uintptr_t>(x) & 15) == 0};
     const PackJob<T> jw = {w, nullptr, reinterpret_cast<__half*>(st + p.s_w), d.vocab, d.cols, p.ld, d.vocab * p.ld,
                            eight && (reinterpret_cast<uintptr_t>(w) & 15) == 0};
-    const int w_blocks = p.w_direct ? 0 : blocks_for(d.vocab);
+    const int w_blocks = p.w_direct ? 0 : blocks_for(ceil_div(d.vocab * (p.ld / 8), kPackThreads));
     const int64_t b_blocks = d.bias != nullptr ? ceil_div(d.vocab, kPackThreads) : 0;
     if constexpr (PLANES == 1) {
         if (d.rows > 0 && d.rows <= kListRows) {
@@ -1417,7 +1454,7 @@ int rows_loss(const tk_linear_ce_desc_t& d, const Plan& p, uint8_t* st, uint8_t*
     return launch_chain("cross entropy rows", ce_rows_kernel<T>, dim3(grid), dim3(32 * kRowWarps), 0, s, static_cast<const T*>(d.x),
                         static_cast<const T*>(d.weight), static_cast<const T*>(d.bias), reinterpret_cast<const int*>(st + p.s_index),
                         reinterpret_cast<const int*>(st + p.s_target), reinterpret_cast<Scalars*>(st + p.s_scalars),
-                        reinterpret_cast<const float2*>(ws + p.w_part), static_cast<int>(kParts * p.n_tiles), d.cols, vec,
+                        reinterpret_cast<const float2*>(ws + p.w_part), static_cast<int>(p.parts), d.cols, vec,
                         reinterpret_cast<float*>(st + p.s_lse), reinterpret_cast<float*>(ws + p.w_loss), static_cast<int>(d.reduction), d.loss);
 }
 
@@ -1584,7 +1621,7 @@ int tk_linear_ce_backward(const tk_linear_ce_grad_desc_t* desc, void* workspace,
             r.out = static_cast<uint8_t*>(desc->dweight) + v0 * d.cols * esz;
             r.out_vec = cols16 && (reinterpret_cast<uintptr_t>(r.out) & 15) == 0;
             r.out_rows = width;
-            CE_TRY(gemm<kGradW>(tdz_mn, tx_mn, r, std::max<int64_t>(r.m_tiles * col_tiles, p.split_units), s));
+            CE_TRY(gemm<kGradW>(tdz_mn, tx_mn, r, std::max<int64_t>(r.m_tiles * col_tiles, p.split_units), s, ceil_div(d.rows, BK)));
             if (2 * r.m_tiles * col_tiles <= p.split_units)  // else no tile is split
                 CE_TRY(launch_chain("cross entropy split", ce_split_kernel<kGradW>, dim3(static_cast<unsigned>(p.split_units) * 8), dim3(256), 0, s, r));
         }
