@@ -174,6 +174,15 @@ def test_residual_norm_many_rows_and_gate_segments():
     check_norm((2, 1500, 4096), F16, "rms", True, "sample", seed=3)
 
 
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("cols", [1, 2, 3, 7, 8, 9, 16, 17, 24, 31, 40, 63, 64, 65, 100, 104, 120, 127, 128, 129])
+@pytest.mark.parametrize("kind,post,gate,p", [("layer", False, "none", 0.1), ("rms", True, "sample", 0.2), ("layer", True, "token", 0.0)])
+def test_residual_norm_narrow_rows(cols, dtype, kind, post, gate, p):
+    # several rows to a warp; row counts that leave lanes of the last warp without one
+    check_norm((3, 67, cols), dtype, kind, post, gate, p=p, seed=cols)
+    check_norm((1, 1, cols), dtype, kind, post, gate, p=p, seed=cols + 1)
+
+
 def test_residual_norm_gate_over_two_leading_dimensions():
     t = norm_inputs((3, 4, 5, 40), F32, "layer", True, "none", 2)
     t["gate"] = rnd((3, 4, 1, 40), 8, F32)

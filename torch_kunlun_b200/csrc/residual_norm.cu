@@ -22,7 +22,8 @@
 // the forward pass had it before it was rounded: from the rounded x_new the
 // binary16 gradient of weight came out up to 1.5 times as far off.
 //
-// HBM bounds both directions: 4 tensors forward, 6 backward.  A group of W warps holds a row in
+// HBM bounds both directions: 4 tensors forward, 6 backward.  A group of W
+// warps (or some lanes of a warp, where rows are narrow) holds a row in
 // registers, 8 * NV columns per thread, as pairs for the two-wide binary32
 // instructions (one per element made the kernels issue-bound: 8192 x 4096 with
 // both norms took 93 us forward, 2.4 TB/s, at 63 % issue); a CTA runs several
@@ -33,9 +34,9 @@
 // barrier, otherwise the group the 16-byte vectors that cover the row.  CTAs
 // own contiguous rows; column sums stay in registers until a CTA's rows end,
 // and a second kernel adds the CTAs' partial sums in a fixed order, so no
-// gradient depends on timing.  Where a CTA cannot hold a row's columns and their
-// sums, a pass of its own adds the columns, from the row statistics and the two
-// row means that the first pass leaves.
+// gradient depends on timing.  Where a CTA cannot hold a row's columns and
+// their sums, a pass of its own adds the columns, from the row statistics and
+// the two row means that the first pass leaves.
 #include <cuda_fp16.h>
 
 #include <algorithm>
@@ -61,7 +62,7 @@ struct RnParams {
     float* partial;  // backward: [4][units][cols], then the gate's [2 * units][cols]
     int64_t rows, cols, gate_period;  // row r uses gate row r / gate_period
     int units;                        // row ranges: clusters of `cluster` CTAs
-    int cluster, warps, groups, stages;
+    int cluster, warps, lanes, groups, stages;  // a row has warps * lanes threads of a CTA
     float a, eps, inv_cols;
     bool layer, drop;
     DropoutParams dropout;
@@ -171,11 +172,17 @@ constexpr int kTailPad = 32;  // bytes of a row's copy beyond the row: both 16-b
 // offset, an octet is shifted out of the vectors that cover it, and a lane
 // stores the whole vector that its octet and its neighbour's fill (the warp's
 // outer lanes and the row's end store element by element).
-template <typename T, int NV, bool VEC>
+//
+// NARROW (NV 1): a row has p.lanes threads, a power of two below 32, and a warp
+// several rows, whose lanes name only one another in shuffles and barriers: the
+// rows of a warp need not end together.
+template <typename T, int NV, bool VEC, bool NARROW = false>
 struct Lane {
+    static_assert(!NARROW || NV == 1, "a narrow row is one octet to a lane");
     static constexpr int E = 8 * NV, P = E / 2;
     [[maybe_unused]] static constexpr int PARTS = sizeof(T) / 2;  // 16-byte vectors of an octet
-    int t, lane, warp, group, gthreads, rank, tensors;
+    int t, lane, lanes, warp, group, gthreads, rank, tensors;  // lane, lanes: of the warp, or of the narrow row
+    unsigned mask;   // those lanes
     int col0, cols;  // first column of the CTA's slice, columns of a row
     uint32_t ring;   // this thread's (VEC) or this group's copies
     uint32_t image;  // bytes of one row's copy (not VEC)
@@ -185,10 +192,12 @@ struct Lane {
     const RnParams& p;
 
     __device__ Lane(const RnParams& pr, uint8_t* smem, int tensors_) : tensors(tensors_), p(pr) {
-        gthreads = p.warps * 32;
+        gthreads = NARROW ? p.lanes : p.warps * 32;
         group = threadIdx.x / gthreads;
         t = threadIdx.x - group * gthreads;
-        lane = threadIdx.x & 31;
+        lanes = NARROW ? p.lanes : 32;
+        lane = threadIdx.x & (lanes - 1);
+        mask = NARROW ? ((1u << lanes) - 1u) << ((threadIdx.x & 31) - lane) : 0xFFFFFFFFu;
         warp = t >> 5;
         rank = p.cluster > 1 ? static_cast<int>(cluster_ctarank()) : 0;
         col0 = rank * gthreads * E;
@@ -246,8 +255,8 @@ struct Lane {
     }
     // Threads of the group wait for one another.
     __device__ __forceinline__ void group_sync() const {
-        if (p.warps == 1) {
-            __syncwarp();
+        if (NARROW || p.warps == 1) {
+            __syncwarp(mask);
         } else {
             named_barrier_sync(1 + group, gthreads);
         }
@@ -341,7 +350,7 @@ struct Lane {
                 const uint32_t off = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(to)) & 15u;
                 uint32_t u[W + 5];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) u[i] = __shfl_up_sync(0xFFFFFFFFu, o[W - 4 + i], 1);
+                for (int i = 0; i < 4; ++i) u[i] = __shfl_up_sync(mask, o[W - 4 + i], 1, lanes);
 #pragma unroll
                 for (int i = 0; i < W; ++i) u[4 + i] = o[i];
                 if (off == 0) {
@@ -358,7 +367,7 @@ struct Lane {
                 }
                 // what no whole store covers: the head of a first or partial
                 // octet, the tail where the next lane stores no whole vector
-                const bool next = lane < 31 && (full || col(8 * k) + 15 < cols);
+                const bool next = lane < lanes - 1 && (full || col(8 * k) + 15 < cols);
                 const int count = full ? 8 : min(8, max(0, cols - col(8 * k)));        // elements of the octet in the row
                 const int split = static_cast<int>((16u * PARTS - off) / sizeof(T));  // elements in its own vectors
                 const uint32_t head = (1u << min(split, 8)) - 1u;
@@ -401,6 +410,12 @@ struct Lane {
     // barrier per sum is enough.
     template <int N>
     __device__ __forceinline__ float2 row_sum(float2 s) {
+        if constexpr (NARROW) {
+#pragma unroll
+            for (int m = 8; m > 0; m >>= 1)
+                if (m < lanes) s = lanes_add<N>(s, m, mask);
+            return s;
+        }
 #pragma unroll
         for (int m = 16; m > 0; m >>= 1) s = lanes_add<N>(s, m);
         if (red_n == 1) return s;
@@ -426,10 +441,10 @@ struct Lane {
         return s;
     }
     template <int N>
-    static __device__ __forceinline__ float2 lanes_add(float2 s, int m) {
-        const float x = __shfl_xor_sync(0xFFFFFFFFu, s.x, m);
+    static __device__ __forceinline__ float2 lanes_add(float2 s, int m, unsigned mask = 0xFFFFFFFFu) {
+        const float x = __shfl_xor_sync(mask, s.x, m);
         if (N == 1) return make_float2(s.x + x, 0.0f);
-        return add2(s, make_float2(x, __shfl_xor_sync(0xFFFFFFFFu, s.y, m)));
+        return add2(s, make_float2(x, __shfl_xor_sync(mask, s.y, m)));
     }
     // mean and rstd of v over the row (mean 0 for an rms norm); the mean
     // square is taken about the mean, of values held in registers.
@@ -530,10 +545,10 @@ struct Lane {
 
 // Parameter vectors stay in registers for up to 24 columns per thread; wider
 // shares read them again for each row (from L1).
-template <typename T, int NV, bool VEC, bool POST>
+template <typename T, int NV, bool VEC, bool POST, bool NARROW = false>
 __global__ void __launch_bounds__(kMaxThreads, 1) residual_norm_kernel(const RnParams p) {
     extern __shared__ __align__(16) uint8_t smem[];
-    using L = Lane<T, NV, VEC>;
+    using L = Lane<T, NV, VEC, NARROW>;
     constexpr int P = L::P;
     constexpr bool KEPT = NV <= 3;
     L ln(p, smem, 2);
@@ -605,8 +620,8 @@ __global__ void __launch_bounds__(kMaxThreads, 1) residual_norm_kernel(const RnP
 // Adds `acc` over the CTA's groups and writes the CTA's columns, as fp32
 // partial sums or (to_final) as the finished gradient.  Every thread of the
 // CTA takes part; `buf` is the ring's memory, idle at this point.
-template <typename T, int NV, bool VEC>
-__device__ __forceinline__ void flush_columns(const Lane<T, NV, VEC>& ln, float* buf, const float2 (&acc)[4 * NV],
+template <typename T, int NV, bool VEC, bool NARROW>
+__device__ __forceinline__ void flush_columns(const Lane<T, NV, VEC, NARROW>& ln, float* buf, const float2 (&acc)[4 * NV],
                                               float* partial, T* final_row) {
     const RnParams& p = ln.p;
     const int width = ln.gthreads * 8 * NV;
@@ -617,6 +632,7 @@ __device__ __forceinline__ void flush_columns(const Lane<T, NV, VEC>& ln, float*
         __syncthreads();
         for (int c = threadIdx.x; c < width && ln.col0 + c < p.cols; c += blockDim.x) {
             float s = 0.0f;
+#pragma unroll 8
             for (int g = 0; g < p.groups; ++g) s += buf[g * width + c];
             if (final_row != nullptr) {
                 final_row[ln.col0 + c] = from_f<T>(s);
@@ -640,10 +656,10 @@ __device__ __forceinline__ void flush_columns(const Lane<T, NV, VEC>& ln, float*
 }
 
 // SUMS: keeps the column sums; otherwise leaves p.means for the column pass.
-template <typename T, int NV, bool VEC, bool POST, bool GATE, bool SUMS>
+template <typename T, int NV, bool VEC, bool POST, bool GATE, bool SUMS, bool NARROW = false>
 __global__ void __launch_bounds__(kMaxThreads, 1) residual_norm_backward_kernel(const RnParams p) {
     extern __shared__ __align__(16) uint8_t smem[];
-    using L = Lane<T, NV, VEC>;
+    using L = Lane<T, NV, VEC, NARROW>;
     constexpr int P = L::P;
     L ln(p, smem, 4);
     float* const buf = reinterpret_cast<float*>(smem + 2 * sizeof(float2) * ((ln.red_stride + 1) & ~1));
@@ -800,7 +816,7 @@ __global__ void __launch_bounds__(kMaxThreads, 1) residual_norm_backward_kernel(
                 // goes to the unit's first or last slot
                 const bool whole = seg_lo == seg_gate * p.gate_period && seg_hi == (seg_gate + 1) * p.gate_period;
                 float* slot = p.partial + (4 * static_cast<int64_t>(p.units) + 2 * unit + (seg_lo == unit_lo ? 0 : 1)) * p.cols;
-                flush_columns<T, NV, VEC>(ln, buf, dgt, slot, whole ? static_cast<T*>(p.dgate) + seg_gate * p.cols : nullptr);
+                flush_columns<T, NV, VEC, NARROW>(ln, buf, dgt, slot, whole ? static_cast<T*>(p.dgate) + seg_gate * p.cols : nullptr);
             }
         }
         seg_lo = seg_hi;
@@ -810,11 +826,11 @@ __global__ void __launch_bounds__(kMaxThreads, 1) residual_norm_backward_kernel(
     }
     if constexpr (SUMS) {
     const int64_t plane = static_cast<int64_t>(p.units) * p.cols;
-    flush_columns<T, NV, VEC>(ln, buf, dw, p.partial + unit * p.cols, nullptr);
-    flush_columns<T, NV, VEC>(ln, buf, db, p.partial + plane + unit * p.cols, nullptr);
+    flush_columns<T, NV, VEC, NARROW>(ln, buf, dw, p.partial + unit * p.cols, nullptr);
+    flush_columns<T, NV, VEC, NARROW>(ln, buf, db, p.partial + plane + unit * p.cols, nullptr);
     if constexpr (POST) {
-        flush_columns<T, NV, VEC>(ln, buf, dpw, p.partial + 2 * plane + unit * p.cols, nullptr);
-        flush_columns<T, NV, VEC>(ln, buf, dpb, p.partial + 3 * plane + unit * p.cols, nullptr);
+        flush_columns<T, NV, VEC, NARROW>(ln, buf, dpw, p.partial + 2 * plane + unit * p.cols, nullptr);
+        flush_columns<T, NV, VEC, NARROW>(ln, buf, dpb, p.partial + 3 * plane + unit * p.cols, nullptr);
     }
     }
 }
@@ -1052,11 +1068,24 @@ __global__ void __launch_bounds__(1024) residual_norm_columns_kernel(const RnPar
 enum Pass { kForward, kSums2, kSums5, kNoSums };
 
 struct Geometry {
-    int nv, warps, cluster, groups;
+    int nv, warps, cluster, lanes, groups;
+    bool narrow() const { return lanes < 32; }
 };
 
+// Half a warp's columns: up to here the lanes of one warp take several rows
+// (100000 x 64 in fp16: forward 57 -> 18 us, backward 75 -> 22; 400000 x 8: 214
+// -> 9 and 284 -> 16; 100000 x 63 with a post norm: 139 -> 47 and 177 -> 58.
+// Calls with too few rows to fill the GPU gain nothing: 75 x 64 the same, 75 x
+// 63 5.0 -> 5.5 and 7.5 -> 8.1).
+constexpr int kNarrowCols = 128;
+
 Geometry geometry(int64_t cols, bool f16, Pass pass, bool post) {
-    Geometry best = {1, 1, 1, 1};
+    if (cols <= kNarrowCols) {
+        int lanes = 1;
+        while (lanes * 8 < cols) lanes *= 2;
+        return {1, 1, 1, lanes, 256 / lanes};
+    }
+    Geometry best = {1, 1, 1, 32, 1};
     int64_t best_cost = INT64_MAX;
     const int nv_max = pass == kForward ? (f16 ? 4 : cols > 4096 ? 2 : 1) : pass == kSums5 || !f16 ? 1 : 2;
     for (int nv = nv_max; nv >= 1; --nv) {
@@ -1071,7 +1100,7 @@ Geometry geometry(int64_t cols, bool f16, Pass pass, bool post) {
         const int64_t cost = warps * cluster * (2 + nv) * (cluster > 1 ? 2 : 1);
         if (cost < best_cost) {
             best_cost = cost;
-            best = {nv, static_cast<int>(warps), cluster, 1};
+            best = {nv, static_cast<int>(warps), cluster, 32, 1};
         }
     }
     best.groups = best.cluster > 1 ? 1 : std::max(1, 8 / best.warps);
@@ -1081,7 +1110,9 @@ Geometry geometry(int64_t cols, bool f16, Pass pass, bool post) {
 using Kernel = void (*)(RnParams);
 
 template <typename T, bool VEC>
-Kernel forward_kernel(int nv, bool post) {
+Kernel forward_kernel(const Geometry& g, bool post) {
+    if (g.narrow()) return post ? residual_norm_kernel<T, 1, VEC, true, true> : residual_norm_kernel<T, 1, VEC, false, true>;
+    const int nv = g.nv;
     if constexpr (sizeof(T) == 2) {
         if (nv == 4) return post ? residual_norm_kernel<T, 4, VEC, true> : residual_norm_kernel<T, 4, VEC, false>;
         if (nv == 3) return residual_norm_kernel<T, 3, VEC, false>;
@@ -1090,16 +1121,18 @@ Kernel forward_kernel(int nv, bool post) {
     return post ? residual_norm_kernel<T, 1, VEC, true> : residual_norm_kernel<T, 1, VEC, false>;
 }
 
-template <typename T, int NV, bool VEC, bool SUMS>
+template <typename T, int NV, bool VEC, bool SUMS, bool NARROW = false>
 Kernel backward_kernel_of(bool post, bool gate) {
-    if (post) return gate ? residual_norm_backward_kernel<T, NV, VEC, true, true, SUMS> : residual_norm_backward_kernel<T, NV, VEC, true, false, SUMS>;
-    return gate ? residual_norm_backward_kernel<T, NV, VEC, false, true, SUMS> : residual_norm_backward_kernel<T, NV, VEC, false, false, SUMS>;
+    if (post)
+        return gate ? residual_norm_backward_kernel<T, NV, VEC, true, true, SUMS, NARROW> : residual_norm_backward_kernel<T, NV, VEC, true, false, SUMS, NARROW>;
+    return gate ? residual_norm_backward_kernel<T, NV, VEC, false, true, SUMS, NARROW> : residual_norm_backward_kernel<T, NV, VEC, false, false, SUMS, NARROW>;
 }
 
 template <typename T, bool VEC>
-Kernel backward_kernel(int nv, bool post, bool gate, bool sums) {
+Kernel backward_kernel(const Geometry& g, bool post, bool gate, bool sums) {
+    if (g.narrow()) return backward_kernel_of<T, 1, VEC, true, true>(post, gate);  // never without sums
     if constexpr (sizeof(T) == 2) {
-        if (nv == 2) return sums ? residual_norm_backward_kernel<T, 2, VEC, false, false, true> : backward_kernel_of<T, 2, VEC, false>(post, gate);
+        if (g.nv == 2) return sums ? residual_norm_backward_kernel<T, 2, VEC, false, false, true> : backward_kernel_of<T, 2, VEC, false>(post, gate);
     }
     return sums ? backward_kernel_of<T, 1, VEC, true>(post, gate) : backward_kernel_of<T, 1, VEC, false>(post, gate);
 }
@@ -1172,7 +1205,7 @@ constexpr size_t kSmemPerSm = 220 * 1024;
 constexpr int kSmemMost = 227 * 1024;
 
 size_t stage_bytes(const Geometry& g, bool f16, bool vec, int tensors) {
-    const size_t row = static_cast<size_t>(g.warps) * 32 * g.nv * (f16 ? 16 : 32);
+    const size_t row = static_cast<size_t>(g.warps) * g.lanes * g.nv * (f16 ? 16 : 32);
     return (row + (vec ? 0 : kTailPad)) * g.groups * tensors;
 }
 
@@ -1182,10 +1215,11 @@ size_t stage_bytes(const Geometry& g, bool f16, bool vec, int tensors) {
 size_t configure(RnParams& p, const Geometry& g, bool f16, bool vec, int tensors, bool backward) {
     p.cluster = g.cluster;
     p.warps = g.warps;
+    p.lanes = g.lanes;
     p.groups = g.groups;
     const size_t one = stage_bytes(g, f16, vec, tensors);
-    const size_t fold = backward && g.groups > 1 ? static_cast<size_t>(g.warps) * 32 * g.groups * 8 * g.nv * sizeof(float) : 0;
-    const int resident = std::max(1, 512 / (g.warps * 32 * g.groups));  // CTAs that registers admit
+    const size_t fold = backward && g.groups > 1 ? static_cast<size_t>(g.warps) * g.lanes * g.groups * 8 * g.nv * sizeof(float) : 0;
+    const int resident = std::max(1, 512 / (g.warps * g.lanes * g.groups));  // CTAs that registers admit
     p.stages = 3;
     while (p.stages > (vec ? 1 : 2) && (red_bytes(g) + p.stages * one + 1024) * resident > kSmemPerSm) --p.stages;
     return red_bytes(g) + std::max(p.stages * one, fold);
@@ -1198,7 +1232,7 @@ int launch(Kernel k, const RnParams& p, size_t smem, cudaStream_t s, const char*
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(static_cast<unsigned>(p.units) * p.cluster);
-    cfg.blockDim = dim3(p.warps * 32 * p.groups);
+    cfg.blockDim = dim3(p.warps * p.lanes * p.groups);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = s;
     cfg.attrs = attr;
@@ -1213,7 +1247,7 @@ int launch(Kernel k, const RnParams& p, size_t smem, cudaStream_t s, const char*
 
 int resident_ctas(Kernel k, const RnParams& p, size_t smem, int& per_sm) {
     TK_CUDA_TRY(cudaFuncSetAttribute(reinterpret_cast<const void*>(k), cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemMost));
-    TK_CUDA_TRY(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, reinterpret_cast<const void*>(k), p.warps * 32 * p.groups, smem));
+    TK_CUDA_TRY(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, reinterpret_cast<const void*>(k), p.warps * p.lanes * p.groups, smem));
     if (per_sm < 1) TK_FAIL(TK_ERR_CUDA, "residual norm: the kernel does not fit an SM");
     return TK_OK;
 }
@@ -1272,8 +1306,8 @@ int tk_residual_norm(const tk_residual_norm_desc_t* desc, void* stream) {
     const bool f16 = d.dtype == TK_DTYPE_F16, vec = vectorised(p);
     const Geometry g = geometry(p.cols, f16, kForward, d.post_norm != 0);
     const size_t smem = configure(p, g, f16, vec, 2, false);
-    const Kernel k = f16 ? (vec ? forward_kernel<__half, true>(g.nv, d.post_norm) : forward_kernel<__half, false>(g.nv, d.post_norm))
-                         : (vec ? forward_kernel<float, true>(g.nv, d.post_norm) : forward_kernel<float, false>(g.nv, d.post_norm));
+    const Kernel k = f16 ? (vec ? forward_kernel<__half, true>(g, d.post_norm) : forward_kernel<__half, false>(g, d.post_norm))
+                         : (vec ? forward_kernel<float, true>(g, d.post_norm) : forward_kernel<float, false>(g, d.post_norm));
     int per_sm = 0;
     if (int rc = resident_ctas(k, p, smem, per_sm)) return rc;
     p.units = max_units(current_device(), p.rows, g, per_sm);
@@ -1324,8 +1358,8 @@ int tk_residual_norm_backward(const tk_residual_norm_grad_desc_t* desc, void* wo
     const bool wide = is_wide(d);
     const Geometry g = geometry(p.cols, f16, wide ? kNoSums : gate || post ? kSums5 : kSums2, post);
     const size_t smem = configure(p, g, f16, vec, 4, !wide);
-    const Kernel k = f16 ? (vec ? backward_kernel<__half, true>(g.nv, post, gate, !wide) : backward_kernel<__half, false>(g.nv, post, gate, !wide))
-                         : (vec ? backward_kernel<float, true>(g.nv, post, gate, !wide) : backward_kernel<float, false>(g.nv, post, gate, !wide));
+    const Kernel k = f16 ? (vec ? backward_kernel<__half, true>(g, post, gate, !wide) : backward_kernel<__half, false>(g, post, gate, !wide))
+                         : (vec ? backward_kernel<float, true>(g, post, gate, !wide) : backward_kernel<float, false>(g, post, gate, !wide));
     int per_sm = 0;
     if (int rc = resident_ctas(k, p, smem, per_sm)) return rc;
     p.units = max_units(current_device(), p.rows, g, std::min(per_sm, kBackwardPerSm));
