@@ -183,6 +183,14 @@ def test_residual_norm_narrow_rows(cols, dtype, kind, post, gate, p):
     check_norm((1, 1, cols), dtype, kind, post, gate, p=p, seed=cols + 1)
 
 
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("shape", [(50, 3, 64), (301, 2, 8), (3001, 2, 5), (40, 5, 63), (33, 7, 256), (700, 4, 200), (2, 2, 1000), (9, 20, 129), (5000, 6, 16)])
+@pytest.mark.parametrize("post,p", [(False, 0.0), (True, 0.1)])
+def test_residual_norm_short_gate_rows(shape, dtype, post, p):
+    # groups of a block that take whole gate rows, the last block's with fewer than the others
+    check_norm(shape, dtype, "layer", post, "sample", p=p, seed=shape[0])
+
+
 def test_residual_norm_gate_over_two_leading_dimensions():
     t = norm_inputs((3, 4, 5, 40), F32, "layer", True, "none", 2)
     t["gate"] = rnd((3, 4, 1, 40), 8, F32)

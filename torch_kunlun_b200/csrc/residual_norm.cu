@@ -509,23 +509,41 @@ struct Lane {
             drop(keep(row), v);
         }
     }
-    // Runs f(row, stage) over the group's rows [begin, end), a step of `groups`
-    // apart, with the copies of the rows ahead under way.
-    template <typename Fetch, typename F>
+    // The group's walk over rows: a step of `groups` apart, or (OWN) whole gate
+    // rows of gate_period rows, a step of `groups` gate rows apart.
+    template <bool OWN>
+    struct Walk {
+        int64_t row;
+        int left;  // OWN: rows of this gate row from here on
+        __device__ __forceinline__ void next(const RnParams& p) {
+            if constexpr (OWN) {
+                ++row;
+                if (--left == 0) {
+                    left = static_cast<int>(p.gate_period);
+                    row += static_cast<int64_t>(p.groups - 1) * p.gate_period;
+                }
+            } else {
+                row += p.groups;
+            }
+        }
+    };
+    // Runs f(walk, stage) over the group's rows from `begin` to below `end`, with
+    // the copies of the rows ahead under way.
+    template <bool OWN, typename Fetch, typename F>
     __device__ __forceinline__ void rows(int64_t begin, int64_t end, Fetch fetch_row, F f) const {
         const int ahead = p.stages - 1;
+        Walk<OWN> at = {begin, OWN ? static_cast<int>(p.gate_period) : 0}, next = at;
         for (int i = 0; i < ahead; ++i) {
-            const int64_t r = begin + static_cast<int64_t>(i) * p.groups;
-            if (r < end) fetch_row(r, i);
+            if (next.row < end) fetch_row(next.row, i);
             cp_async_commit();
+            next.next(p);
         }
         int stage = 0;
-        for (int64_t r = begin; r < end; r += p.groups) {
-            const int64_t next = r + static_cast<int64_t>(ahead) * p.groups;
+        for (; at.row < end; at.next(p)) {
             int ns = stage + ahead;
             if (ns >= p.stages) ns -= p.stages;
             if constexpr (VEC) {
-                if (next < end) fetch_row(next, ns);
+                if (next.row < end) fetch_row(next.row, ns);
                 cp_async_commit();
                 cp_async_wait(ahead);
             } else {
@@ -533,10 +551,11 @@ struct Lane {
                 // are read, before that stage is filled again (stages >= 2)
                 cp_async_wait(ahead - 1);
                 group_sync();
-                if (next < end) fetch_row(next, ns);
+                if (next.row < end) fetch_row(next.row, ns);
                 cp_async_commit();
             }
-            f(r, stage);
+            next.next(p);
+            f(at, stage);
             if (++stage == p.stages) stage = 0;
         }
         cp_async_wait(0);
@@ -565,15 +584,15 @@ __global__ void __launch_bounds__(kMaxThreads, 1) residual_norm_kernel(const RnP
             if (p.post_bias != nullptr) ln.vector(p.post_bias, 0.0f, pb);
         }
     }
-    ln.rows(
+    ln.template rows<false>(
         begin, end,
         [&](int64_t r, int stage) {
             const int64_t at = r * p.cols;
             ln.fetch(p.x, at, stage, 0);
             ln.fetch(p.f, at, stage, 1);
         },
-        [&](int64_t r, int stage) {
-            const int64_t at = r * p.cols;
+        [&](const auto& walk, int stage) {
+            const int64_t r = walk.row, at = r * p.cols;
             float2 u[P], x[P];
             ln.row_values(p.f, at, stage, 1, u);
             float4 st = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -656,15 +675,21 @@ __device__ __forceinline__ void flush_columns(const Lane<T, NV, VEC, NARROW>& ln
 }
 
 // SUMS: keeps the column sums; otherwise leaves p.means for the column pass.
-template <typename T, int NV, bool VEC, bool POST, bool GATE, bool SUMS, bool NARROW = false>
+// kGateOwn: groups take whole gate rows and finish their gradients alone.
+enum Gate { kNoGate, kGate, kGateOwn };
+
+template <typename T, int NV, bool VEC, bool POST, Gate GATED, bool SUMS, bool NARROW = false>
 __global__ void __launch_bounds__(kMaxThreads, 1) residual_norm_backward_kernel(const RnParams p) {
     extern __shared__ __align__(16) uint8_t smem[];
     using L = Lane<T, NV, VEC, NARROW>;
     constexpr int P = L::P;
+    constexpr bool GATE = GATED != kNoGate, OWN = GATED == kGateOwn;
     L ln(p, smem, 4);
     float* const buf = reinterpret_cast<float*>(smem + 2 * sizeof(float2) * ((ln.red_stride + 1) & ~1));
     const int64_t unit = blockIdx.x / p.cluster;
-    const int64_t unit_lo = unit_begin(unit, p.rows, p.units), unit_hi = unit_begin(unit + 1, p.rows, p.units);
+    // a unit is a range of rows, or of gate rows
+    const int64_t each = OWN ? p.gate_period : 1;
+    const int64_t unit_lo = unit_begin(unit, p.rows / each, p.units) * each, unit_hi = unit_begin(unit + 1, p.rows / each, p.units) * each;
     const bool gate_sums = GATE && SUMS && p.gate_period > 1;  // else each row writes its own gradient
     Raw<T, L::E> w, pw, gate;
     ln.vector(p.weight, 1.0f, w);
@@ -679,19 +704,20 @@ __global__ void __launch_bounds__(kMaxThreads, 1) residual_norm_backward_kernel(
     }
     int64_t gate_row = -1;
     // a segment: the rows of this unit that share a gate row (all of them
-    // where no sum of the gate's gradient is kept)
+    // where the CTA's groups do not add up a gate's gradient together)
     int64_t seg_lo = unit_lo;
     while (seg_lo < unit_hi) {
-        const int64_t seg_gate = gate_sums ? seg_lo / p.gate_period : 0;
-        const int64_t seg_hi = gate_sums ? min(unit_hi, (seg_gate + 1) * p.gate_period) : unit_hi;
+        const int64_t seg_gate = gate_sums && !OWN ? seg_lo / p.gate_period : 0;
+        const int64_t seg_hi = gate_sums && !OWN ? min(unit_hi, (seg_gate + 1) * p.gate_period) : unit_hi;
         if constexpr (GATE && SUMS) {
 #pragma unroll
             for (int i = 0; i < P; ++i) dgt[i] = make_float2(0.0f, 0.0f);
         }
         float4 next_st = make_float4(0.0f, 0.0f, 0.0f, 0.0f);  // read a row ahead
-        if (seg_lo + ln.group < seg_hi) next_st = p.stats[seg_lo + ln.group];
-        ln.rows(
-            seg_lo + ln.group, seg_hi,
+        const int64_t first = seg_lo + ln.group * each;
+        if (first < seg_hi) next_st = p.stats[first];
+        ln.template rows<OWN>(
+            first, seg_hi,
             [&](int64_t r, int stage) {
                 const int64_t at = r * p.cols;
                 if (p.gx != nullptr) ln.fetch(p.gx, at, stage, 0);
@@ -701,10 +727,12 @@ __global__ void __launch_bounds__(kMaxThreads, 1) residual_norm_backward_kernel(
                 }
                 ln.fetch(p.f, at, stage, 3);
             },
-            [&](int64_t r, int stage) {
-                const int64_t at = r * p.cols;
+            [&](const auto& walk, int stage) {
+                const int64_t r = walk.row, at = r * p.cols;
                 const float4 st = next_st;
-                if (r + p.groups < seg_hi) next_st = p.stats[r + p.groups];
+                auto after = walk;
+                after.next(p);
+                if (after.row < seg_hi) next_st = p.stats[after.row];
                 const uint32_t keep = p.drop ? ln.keep(at) : 0u;
                 if constexpr (GATE) {
                     const int64_t k = p.gate_period == p.rows ? 0 : r / p.gate_period;
@@ -774,6 +802,13 @@ __global__ void __launch_bounds__(kMaxThreads, 1) residual_norm_backward_kernel(
                         if constexpr (SUMS) {
 #pragma unroll
                             for (int i = 0; i < P; ++i) dgt[i] = fma2(u[i], g[i], dgt[i]);
+                            if constexpr (OWN) {
+                                if (walk.left == 1) {
+                                    ln.store(p.dgate, gate_row * p.cols, dgt);
+#pragma unroll
+                                    for (int i = 0; i < P; ++i) dgt[i] = make_float2(0.0f, 0.0f);
+                                }
+                            }
                         }
                     } else if (p.gate_period == 1 && p.dgate != nullptr) {
 #pragma unroll
@@ -810,7 +845,7 @@ __global__ void __launch_bounds__(kMaxThreads, 1) residual_norm_backward_kernel(
                 }
                 if (p.df != nullptr) ln.store(p.df, at, g);
             });
-        if constexpr (GATE && SUMS) {
+        if constexpr (GATE && SUMS && !OWN) {
             if (gate_sums && p.dgate != nullptr) {
                 // whole segments are finished here; one that other units share
                 // goes to the unit's first or last slot
@@ -1121,20 +1156,31 @@ Kernel forward_kernel(const Geometry& g, bool post) {
     return post ? residual_norm_kernel<T, 1, VEC, true> : residual_norm_kernel<T, 1, VEC, false>;
 }
 
+template <typename T, int NV, bool VEC, bool SUMS, bool NARROW, Gate GATED>
+Kernel backward_kernel_of(bool post) {
+    return post ? residual_norm_backward_kernel<T, NV, VEC, true, GATED, SUMS, NARROW> : residual_norm_backward_kernel<T, NV, VEC, false, GATED, SUMS, NARROW>;
+}
+
 template <typename T, int NV, bool VEC, bool SUMS, bool NARROW = false>
-Kernel backward_kernel_of(bool post, bool gate) {
-    if (post)
-        return gate ? residual_norm_backward_kernel<T, NV, VEC, true, true, SUMS, NARROW> : residual_norm_backward_kernel<T, NV, VEC, true, false, SUMS, NARROW>;
-    return gate ? residual_norm_backward_kernel<T, NV, VEC, false, true, SUMS, NARROW> : residual_norm_backward_kernel<T, NV, VEC, false, false, SUMS, NARROW>;
+Kernel backward_kernel_of(bool post, Gate gate) {
+    if constexpr (SUMS) {
+        if (gate == kGateOwn) return backward_kernel_of<T, NV, VEC, SUMS, NARROW, kGateOwn>(post);
+    }
+    return gate != kNoGate ? backward_kernel_of<T, NV, VEC, SUMS, NARROW, kGate>(post) : backward_kernel_of<T, NV, VEC, SUMS, NARROW, kNoGate>(post);
 }
 
 template <typename T, bool VEC>
-Kernel backward_kernel(const Geometry& g, bool post, bool gate, bool sums) {
+Kernel backward_kernel(const Geometry& g, bool post, Gate gate, bool sums) {
     if (g.narrow()) return backward_kernel_of<T, 1, VEC, true, true>(post, gate);  // never without sums
     if constexpr (sizeof(T) == 2) {
-        if (g.nv == 2) return sums ? residual_norm_backward_kernel<T, 2, VEC, false, false, true> : backward_kernel_of<T, 2, VEC, false>(post, gate);
+        if (g.nv == 2) return sums ? residual_norm_backward_kernel<T, 2, VEC, false, kNoGate, true> : backward_kernel_of<T, 2, VEC, false>(post, gate);
     }
     return sums ? backward_kernel_of<T, 1, VEC, true>(post, gate) : backward_kernel_of<T, 1, VEC, false>(post, gate);
+}
+
+template <typename T>
+Kernel backward_kernel(const Geometry& g, bool vec, bool post, Gate gate, bool sums) {
+    return vec ? backward_kernel<T, true>(g, post, gate, sums) : backward_kernel<T, false>(g, post, gate, sums);
 }
 
 template <typename T, bool VEC>
@@ -1252,6 +1298,20 @@ int resident_ctas(Kernel k, const RnParams& p, size_t smem, int& per_sm) {
     return TK_OK;
 }
 
+// Whether groups take whole gate rows: by the rows that one group works off in
+// turn, where the groups of a CTA that share a gate row add up its gradient in
+// about the time of two rows (samples x tokens x columns, backward and column
+// sums: 20000 x 3 x 64 in fp16 155 -> 18 us, 50000 x 2 x 8 537 -> 13, 4000 x 25 x
+// 64 52 -> 37, 2000 x 8 x 200 59 -> 18; 3000 x 40 x 128 in fp32 127 -> 131).
+bool whole_gate_rows(const RnParams& p, const Geometry& g, int64_t resident) {
+    if (g.groups == 1 || p.gate_period > INT32_MAX) return false;
+    const int64_t gates = p.rows / p.gate_period;
+    const int64_t own = ceil_div(gates, std::min(resident, ceil_div(gates, g.groups)) * g.groups) * p.gate_period;
+    const int64_t units = std::min(resident, ceil_div(p.rows, g.groups));
+    const int64_t shared = ceil_div(gates, units) * (ceil_div(std::min(p.gate_period, ceil_div(p.rows, units)), g.groups) + 2);
+    return own <= shared;
+}
+
 // CTAs per SM the backward pass may use: its partial sums are sized by it.
 constexpr int kBackwardPerSm = 4;
 
@@ -1358,11 +1418,19 @@ int tk_residual_norm_backward(const tk_residual_norm_grad_desc_t* desc, void* wo
     const bool wide = is_wide(d);
     const Geometry g = geometry(p.cols, f16, wide ? kNoSums : gate || post ? kSums5 : kSums2, post);
     const size_t smem = configure(p, g, f16, vec, 4, !wide);
-    const Kernel k = f16 ? (vec ? backward_kernel<__half, true>(g, post, gate, !wide) : backward_kernel<__half, false>(g, post, gate, !wide))
-                         : (vec ? backward_kernel<float, true>(g, post, gate, !wide) : backward_kernel<float, false>(g, post, gate, !wide));
+    Gate gated = gate ? kGate : kNoGate;
+    const auto pick = [&] { return f16 ? backward_kernel<__half>(g, vec, post, gated, !wide) : backward_kernel<float>(g, vec, post, gated, !wide); };
+    Kernel k = pick();
     int per_sm = 0;
     if (int rc = resident_ctas(k, p, smem, per_sm)) return rc;
     p.units = max_units(current_device(), p.rows, g, std::min(per_sm, kBackwardPerSm));
+    if (!wide && p.dgate != nullptr && p.gate_period > 1 &&
+        whole_gate_rows(p, g, static_cast<int64_t>(sm_count(current_device())) * std::min(per_sm, kBackwardPerSm) / g.cluster)) {
+        gated = kGateOwn;
+        k = pick();
+        if (int rc = resident_ctas(k, p, smem, per_sm)) return rc;
+        p.units = max_units(current_device(), p.rows / p.gate_period, g, std::min(per_sm, kBackwardPerSm));
+    }
     const int pass_units = column_units(current_device(), p.rows, p.cols, vec);
     const size_t means = wide ? round_up(static_cast<size_t>(p.rows) * sizeof(float2), 16) : 0;
     const size_t need = means + static_cast<size_t>(6) * (wide ? pass_units : p.units) * p.cols * sizeof(float);
@@ -1382,7 +1450,7 @@ int tk_residual_norm_backward(const tk_residual_norm_grad_desc_t* desc, void* wo
             TK_FAIL(TK_ERR_CUDA, "residual norm column pass launch failed: %s", cudaGetErrorString(e));
         }
     }
-    const bool gate_items = p.dgate != nullptr && p.gate_period > 1;
+    const bool gate_items = p.dgate != nullptr && p.gate_period > 1 && gated != kGateOwn;
     return f16 ? columns<__half>(p, *desc, gate_items, s) : columns<float>(p, *desc, gate_items, s);
 }
 
