@@ -1030,16 +1030,17 @@ __global__ void __launch_bounds__(kPassThreads, 4) residual_norm_column_pass_ker
 
 constexpr int kColLanes = 32;
 
-// The units' partial sums added in a fixed order, rounded once: blockDim.y
-// units at a time.  The first `vectors` items are the parameter vectors asked
-// for (plane[i] of the partial sums to out[i]); the others finish gate rows
-// that several units share: item vectors + g gate row g, or (by_unit, fewer
-// units than gate rows) item vectors + c the gate row that unit c ends and unit
-// c + 1 continues.
+// The units' partial sums added in a fixed order, rounded once.  The first
+// `vectors` items are the parameter vectors asked for (plane[i] of the partial
+// sums to out[i]), blockDim.y units at a time.  The others finish gate rows that
+// several units share, `share` units at a time and blockDim.y / share gate rows
+// per item: gate row g, or (by_unit, fewer units than gate rows) the gate row
+// that unit g ends and unit g + 1 continues, for g below `gates`.
 struct ColumnJobs {
     void* out[4];
     int plane[4];
-    int vectors, col_blocks;
+    int vectors, col_blocks, share;
+    int64_t gates;
     bool by_unit;
 };
 
@@ -1049,33 +1050,39 @@ __global__ void __launch_bounds__(1024) residual_norm_columns_kernel(const RnPar
     __shared__ float part[32][kColLanes + 1];
     const int item = static_cast<int>(blockIdx.x) / j.col_blocks;
     const int64_t c = static_cast<int64_t>(blockIdx.x - item * j.col_blocks) * kColLanes + threadIdx.x;
-    const int step = static_cast<int>(blockDim.y);
+    const bool vector = item < j.vectors;
+    const int share = vector ? static_cast<int>(blockDim.y) : j.share;
+    const int sub = vector ? 0 : static_cast<int>(threadIdx.y) / share, y = static_cast<int>(threadIdx.y) - sub * share;
     float s = 0.0f;
-    T* out;
-    if (item < j.vectors) {
+    T* out = nullptr;  // none: nothing to finish
+    if (vector) {
         out = static_cast<T*>(j.out[item]);
         if (c < p.cols) {
             const float* src = p.partial + static_cast<int64_t>(j.plane[item]) * p.units * p.cols + c;
 #pragma unroll 4
-            for (int u = threadIdx.y; u < p.units; u += step) s += src[static_cast<int64_t>(u) * p.cols];
+            for (int u = y; u < p.units; u += share) s += src[static_cast<int64_t>(u) * p.cols];
         }
     } else {
-        int64_t row = item - j.vectors, first;
-        if (j.by_unit) {
-            const int64_t start = unit_begin(row + 1, p.rows, p.units);
-            first = unit_of(start / p.gate_period * p.gate_period, p.rows, p.units);
-            if (start % p.gate_period == 0 || first != row) return;
-            row = start / p.gate_period;
-        } else {
-            first = unit_of(row * p.gate_period, p.rows, p.units);
+        const int per = static_cast<int>(blockDim.y) / share;
+        int64_t row = static_cast<int64_t>(item - j.vectors) * per + sub, first = 0, last = 0;
+        if (sub < per && row < j.gates) {
+            bool mine = true;
+            if (j.by_unit) {
+                const int64_t start = unit_begin(row + 1, p.rows, p.units);
+                first = unit_of(start / p.gate_period * p.gate_period, p.rows, p.units);
+                mine = start % p.gate_period != 0 && first == row;
+                row = start / p.gate_period;
+            } else {
+                first = unit_of(row * p.gate_period, p.rows, p.units);
+            }
+            last = unit_of((row + 1) * p.gate_period - 1, p.rows, p.units);
+            // else one unit held the row and finished it, or another item does
+            if (mine && first != last) out = static_cast<T*>(p.dgate) + row * p.cols;
         }
-        const int64_t last = unit_of((row + 1) * p.gate_period - 1, p.rows, p.units);
-        if (first == last) return;  // one unit held the row and finished it
-        out = static_cast<T*>(p.dgate) + row * p.cols;
-        if (c < p.cols) {
+        if (out != nullptr && c < p.cols) {
             const float* src = p.partial + 4 * static_cast<int64_t>(p.units) * p.cols + c;
 #pragma unroll 4
-            for (int64_t u = first + threadIdx.y; u <= last; u += step) {
+            for (int64_t u = first + y; u <= last; u += share) {
                 const int64_t slot = 2 * u + (unit_begin(u, p.rows, p.units) / p.gate_period == row ? 0 : 1);
                 s += src[slot * p.cols];
             }
@@ -1083,9 +1090,9 @@ __global__ void __launch_bounds__(1024) residual_norm_columns_kernel(const RnPar
     }
     part[threadIdx.y][threadIdx.x] = s;
     __syncthreads();
-    if (threadIdx.y == 0 && c < p.cols) {
+    if (y == 0 && out != nullptr && c < p.cols) {
         s = 0.0f;
-        for (int i = 0; i < step; ++i) s += part[i][threadIdx.x];
+        for (int i = 0; i < share; ++i) s += part[threadIdx.y + i][threadIdx.x];
         out[c] = from_f<T>(s);
     }
 }
@@ -1337,10 +1344,15 @@ int columns(const RnParams& p, const tk_residual_norm_grad_desc_t& g, bool gate_
         j.plane[j.vectors++] = i;
     }
     j.col_blocks = static_cast<int>(ceil_div(p.cols, kColLanes));
-    j.by_unit = gate_items && p.rows / p.gate_period > p.units;
-    const int items = j.vectors + (!gate_items ? 0 : j.by_unit ? p.units - 1 : static_cast<int>(p.rows / p.gate_period));
-    if (items == 0) return TK_OK;
+    const int64_t gates = p.rows / p.gate_period;
+    j.by_unit = gate_items && gates > p.units;
+    j.gates = !gate_items ? 0 : j.by_unit ? p.units - 1 : gates;
     const int rows = std::max(1, std::min(32, (p.units + 3) / 4));  // about four partial sums per thread
+    // and two of a gate row (a block for each gate row: 300 of 30 x 256 took 42
+    // us, now 5, 4000 of 100 x 64 13, now 5; 7 of 333 x 1151 8.4, now 9.2)
+    j.share = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(rows, (p.units / gates + 2 + 1) / 2)));
+    const int items = j.vectors + static_cast<int>(ceil_div(j.gates, rows / j.share));
+    if (items == 0) return TK_OK;
     cudaError_t e = launch_pdl(residual_norm_columns_kernel<T>, dim3(static_cast<unsigned>(items) * j.col_blocks), dim3(kColLanes, rows), 0, s, p, j);
     if (e != cudaSuccess) {
         cudaGetLastError();
