@@ -504,6 +504,10 @@ typedef struct {
                   * backward pass needs; NULL where there is none */
 } tk_linear_ce_desc_t;
 
+/* The state's size and layout follow from dtype, rows, cols and vocab alone, so
+ * the backward pass may be given the weight at another address.  The workspace
+ * sizes also go by weight's address: an fp16 weight of cols % 8 == 0 off a
+ * 16-byte boundary is packed into the workspace of each pass. */
 TK_API size_t tk_linear_ce_state_size(const tk_linear_ce_desc_t* desc);
 TK_API size_t tk_linear_ce_workspace_size(const tk_linear_ce_desc_t* desc);
 TK_API int tk_linear_ce(const tk_linear_ce_desc_t* desc, void* workspace, size_t workspace_bytes,

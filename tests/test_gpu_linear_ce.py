@@ -377,3 +377,45 @@ def test_training_operators_in_one_step():
         for k, name in (("g", "weight"), ("b", "bias"), ("pg", "post_weight"), ("pb", "post_bias"), ("gate", "gate")):
             R.assert_within(cpu(dev[i][k].grad), *got[name], f"{name} {i}")
         assert torch.isfinite(cpu(dev[i]["w1"].grad)).all() and cpu(dev[i]["w1"].grad).any()
+
+
+def off_boundary(t):
+    """A copy whose data start 2 (fp16) or 4 (fp32) bytes off a 16-byte boundary."""
+    b = torch.empty(t.numel() + 1, dtype=t.dtype, device=t.device)
+    v = b[1:].view(t.shape)
+    v.copy_(t)
+    assert v.data_ptr() % 16 == t.element_size()
+    return v
+
+
+@pytest.mark.parametrize("bias", [True, False])
+@pytest.mark.parametrize("before", ["on", "off"])
+@pytest.mark.parametrize("after", ["on", "off"])
+def test_linear_ce_saved_tensors_come_back_at_another_address(before, after, bias):
+    """Saved-tensor hooks (offloading, packing) hand the weight back in other
+    memory: on a 16-byte boundary or off it, whatever it was in the forward pass."""
+    t, target = ce_inputs(300, 96, 1000, F16, bias, 30, seed=21)
+    want = run_ce(t, target, "mean", torch.tensor(512.0))
+    dev = {k: v.to(DEV) for k, v in t.items()}
+    if before == "off":
+        dev["weight"] = off_boundary(dev["weight"])
+    dev = {k: v.requires_grad_() for k, v in dev.items()}
+    move = off_boundary if after == "off" else torch.clone
+    with torch.autograd.graph.saved_tensors_hooks(lambda v: v.detach(), lambda v: move(v) if v.dtype == F16 else v):
+        loss = ops.linear_cross_entropy(dev["x"], dev["weight"], target.to(DEV), dev.get("bias"))
+    grads = torch.autograd.grad(loss, list(dev.values()), torch.tensor(512.0).to(DEV))
+    assert torch.equal(loss.detach().cpu(), want["loss"])
+    for k, g in zip(dev, grads):
+        assert torch.equal(g.cpu(), want[k]), k
+
+
+@pytest.mark.parametrize("dtype,d", [(F16, 64), (F16, 65), (F32, 64)])
+def test_linear_ce_saved_on_the_host(dtype, d):
+    t, target = ce_inputs(40, d, 300, dtype, True, 5, seed=22)
+    want = run_ce(t, target, "sum", torch.tensor(1.0))
+    dev = {k: v.to(DEV).requires_grad_() for k, v in t.items()}
+    with torch.autograd.graph.saved_tensors_hooks(lambda v: v.cpu(), lambda v: v.to(DEV)):
+        loss = ops.linear_cross_entropy(dev["x"], dev["weight"], target.to(DEV), dev["bias"], reduction="sum")
+    grads = torch.autograd.grad(loss, list(dev.values()))
+    for k, g in zip(dev, grads):
+        assert torch.equal(g.cpu(), want[k]), k

@@ -225,3 +225,24 @@ def test_linear_ce_workspace_is_bounded_by_its_pieces(dtype, rows, vocab):
     acc = pad * 64 * 4
     split = 2 * 148 * 128 * 256 * 4
     assert L.tk_linear_ce_backward_workspace_size(ctypes.byref(g)) <= packed + dz + acc + split + 4 * pad + 8192
+
+
+@pytest.mark.parametrize("dtype", [0, 1])
+@pytest.mark.parametrize("cols", [96, 97])
+def test_linear_ce_state_size_does_not_depend_on_addresses(dtype, cols):
+    # the backward pass may see the weight at another address, and a caller may ask before it has one
+    L = C.lib()
+    size = lambda **kw: L.tk_linear_ce_state_size(ctypes.byref(_ce_desc(dtype=dtype, rows=300, cols=cols, vocab=1000, **kw)))  # noqa: E731
+    sizes = {size(weight=w, bias=b) for w in (None, 1024, 1026, 1032) for b in (None, 1024)}
+    assert len(sizes) == 1 and sizes.pop() > 0
+
+
+def test_linear_ce_workspaces_have_room_for_a_weight_off_the_boundary():
+    L = C.lib()
+    g = C.LinearCeGradDesc()
+    sizes = []
+    for weight in (1024, 1026):
+        g.fwd = _ce_desc(rows=300, cols=96, vocab=1000, weight=weight)
+        sizes.append((L.tk_linear_ce_workspace_size(ctypes.byref(g.fwd)), L.tk_linear_ce_backward_workspace_size(ctypes.byref(g))))
+    packed = 1000 * 96 * 2
+    assert all(off >= on + packed for on, off in zip(*sizes))

@@ -1243,7 +1243,9 @@ constexpr int64_t kMaxSize = 0x7FFFFF00, kMaxTiles = 1 << 30;
 size_t align(size_t v) { return round_up(v, 1024); }
 
 struct Plan {
-    bool f16, w_direct;
+    bool f16;
+    bool w_kept;             // W is packed into the state: by type and width, never by address
+    bool w_direct;           // W is read in place; neither: packed into the workspace of each pass
     int planes;
     int64_t rows_pad, ld;    // packed rows and their length
     int64_t rows_read;       // rows that the products read; tiles end in zeros of their own
@@ -1255,10 +1257,10 @@ struct Plan {
     int split_units;
     int db_chunks;
     // state: kept from the forward to the backward pass
-    size_t s_scalars, s_index, s_target, s_lse, s_x, s_w, s_bias, state_bytes;
+    size_t s_scalars, s_index, s_target, s_lse, s_x, s_bias, s_w, state_bytes;
     // workspaces
-    size_t w_part, w_loss, fwd_bytes;
-    size_t b_grow, b_dz, b_acc, b_split, b_db, bwd_bytes;
+    size_t w_part, w_loss, w_w, fwd_bytes;
+    size_t b_grow, b_dz, b_acc, b_split, b_db, b_w, bwd_bytes;
 };
 
 int check(const char* who, const tk_linear_ce_desc_t& d) {
@@ -1291,7 +1293,11 @@ Plan make_plan(const tk_linear_ce_desc_t& d) {
     p.rows_pad = static_cast<int64_t>(round_up(static_cast<size_t>(std::max<int64_t>(d.rows, 1)), kRowPad));
     p.rows_read = static_cast<int64_t>(round_up(static_cast<size_t>(std::max<int64_t>(d.rows, 1)), BK));
     p.ld = static_cast<int64_t>(round_up(static_cast<size_t>(d.cols), 8));
-    p.w_direct = p.f16 && d.cols % 8 == 0 && (reinterpret_cast<uintptr_t>(d.weight) & 15) == 0;
+    // The state's layout follows from sizes and types alone: the backward pass
+    // may see the weight at another address than the forward pass did.
+    p.w_kept = !p.f16 || d.cols % 8 != 0;
+    p.w_direct = !p.w_kept && (reinterpret_cast<uintptr_t>(d.weight) & 15) == 0;
+    const size_t w_bytes = static_cast<size_t>(p.planes) * d.vocab * p.ld * 2;
     p.n_tiles = ceil_div(d.vocab, BN);
     // pieces of equal size whose dz planes fit kDzBytes (one tile at least)
     const int64_t most = std::max<int64_t>(1, kDzBytes / (p.rows_pad * 2 * p.planes * BN));
@@ -1312,13 +1318,14 @@ Plan make_plan(const tk_linear_ce_desc_t& d) {
     p.s_target = take(p.rows_pad * sizeof(int));
     p.s_lse = take(p.rows_pad * sizeof(float));
     p.s_x = take(static_cast<size_t>(p.planes) * p.rows_pad * p.ld * 2);
-    p.s_w = take(p.w_direct ? 0 : static_cast<size_t>(p.planes) * d.vocab * p.ld * 2);
-    p.s_bias = take(d.bias != nullptr ? static_cast<size_t>(d.vocab) * sizeof(float) : 0);
+    p.s_bias = take(static_cast<size_t>(d.vocab) * sizeof(float));  // with a bias or without
+    p.s_w = take(p.w_kept ? w_bytes : 0);
     p.state_bytes = at;
     at = 0;
     p.parts = stats_parts(p.planes, d.cols) * p.n_tiles;
     p.w_part = take(static_cast<size_t>(p.parts) * p.rows_pad * sizeof(float2));
     p.w_loss = take(p.rows_pad * sizeof(float));
+    p.w_w = take(p.w_kept || p.w_direct ? 0 : w_bytes);
     p.fwd_bytes = at + p.state_bytes;  // a call without a state keeps its own
     at = 0;
     p.b_grow = take(p.rows_pad * sizeof(float));
@@ -1326,6 +1333,7 @@ Plan make_plan(const tk_linear_ce_desc_t& d) {
     p.b_acc = take(p.pieces > 1 ? static_cast<size_t>(p.rows_pad) * p.acc_ld * sizeof(float) : 0);
     p.b_split = take(static_cast<size_t>(p.split_units) * BM * BN * sizeof(float));
     p.b_db = take(d.bias != nullptr ? static_cast<size_t>(p.db_chunks) * p.piece * sizeof(float) : 0);
+    p.b_w = take(p.w_kept || p.w_direct ? 0 : w_bytes);
     p.bwd_bytes = at;
     return p;
 }
@@ -1409,24 +1417,32 @@ int gemm(const CUtensorMap& a, const CUtensorMap& b, const GemmParams& p, int64_
 
 int blocks_for(int64_t rows) { return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(rows, 148 * 16))); }
 
-// The list of rows and the kept operands (x's listed rows; W unless it is read
-// in place; the bias).
+// W as planes at `to`.
+template <typename T>
+PackJob<T> weight_job(const tk_linear_ce_desc_t& d, const Plan& p, __half* to) {
+    return {static_cast<const T*>(d.weight), nullptr, to, d.vocab, d.cols, p.ld, d.vocab * p.ld,
+            d.cols % 8 == 0 && (reinterpret_cast<uintptr_t>(d.weight) & 15) == 0};
+}
+
+int weight_blocks(const tk_linear_ce_desc_t& d, const Plan& p) {
+    return p.w_direct ? 0 : blocks_for(ceil_div(d.vocab * (p.ld / 8), kPackThreads));
+}
+
+// The list of rows, x's listed rows, W unless it is read in place (to `w_at`),
+// and the bias.
 template <typename T, int PLANES>
-int list_and_pack(const tk_linear_ce_desc_t& d, const Plan& p, uint8_t* st, cudaStream_t s) {
+int list_and_pack(const tk_linear_ce_desc_t& d, const Plan& p, uint8_t* st, uint8_t* w_at, cudaStream_t s) {
     const T* x = static_cast<const T*>(d.x);
-    const T* w = static_cast<const T*>(d.weight);
     const T* bias = static_cast<const T*>(d.bias);
     Scalars* sc = reinterpret_cast<Scalars*>(st + p.s_scalars);
     int* index = reinterpret_cast<int*>(st + p.s_index);
     int* target = reinterpret_cast<int*>(st + p.s_target);
     float* bias2 = reinterpret_cast<float*>(st + p.s_bias);
     float* row_loss = d.reduction == TK_REDUCE_NONE ? d.loss : nullptr;
-    const bool eight = d.cols % 8 == 0;
     const PackJob<T> jx = {x, index, reinterpret_cast<__half*>(st + p.s_x), d.rows, d.cols, p.ld, p.rows_pad * p.ld,
-                           eight && (reinterpret_cast<uintptr_t>(x) & 15) == 0};
-    const PackJob<T> jw = {w, nullptr, reinterpret_cast<__half*>(st + p.s_w), d.vocab, d.cols, p.ld, d.vocab * p.ld,
-                           eight && (reinterpret_cast<uintptr_t>(w) & 15) == 0};
-    const int w_blocks = p.w_direct ? 0 : blocks_for(ceil_div(d.vocab * (p.ld / 8), kPackThreads));
+                           d.cols % 8 == 0 && (reinterpret_cast<uintptr_t>(x) & 15) == 0};
+    const PackJob<T> jw = weight_job<T>(d, p, reinterpret_cast<__half*>(w_at));
+    const int w_blocks = weight_blocks(d, p);
     const int64_t b_blocks = d.bias != nullptr ? ceil_div(d.vocab, kPackThreads) : 0;
     if constexpr (PLANES == 1) {
         if (d.rows > 0 && d.rows <= kListRows) {
@@ -1441,7 +1457,7 @@ int list_and_pack(const tk_linear_ce_desc_t& d, const Plan& p, uint8_t* st, cuda
     CE_TRY(launch_status("cross entropy index"));
     if (d.rows == 0) return TK_OK;
     if constexpr (PLANES == 2)
-        CE_TRY(launch_chain("cross entropy amax", ce_amax_kernel, dim3(148 * 4, 2), dim3(256), 0, s, x, w, static_cast<const int*>(index), sc, d.cols, d.vocab));
+        CE_TRY(launch_chain("cross entropy amax", ce_amax_kernel, dim3(148 * 4, 2), dim3(256), 0, s, x, jw.src, static_cast<const int*>(index), sc, d.cols, d.vocab));
     const int x_blocks = blocks_for(p.rows_read);
     return launch_chain("cross entropy pack", ce_pack_kernel<T, PLANES>, dim3(static_cast<unsigned>(x_blocks + w_blocks + b_blocks)), dim3(kPackThreads), 0,
                         s, jx, jw, static_cast<const Scalars*>(sc), x_blocks, w_blocks, bias, bias2);
@@ -1463,9 +1479,9 @@ struct Operand {
     int64_t ld, plane;
 };
 
-Operand weight_operand(const tk_linear_ce_desc_t& d, const Plan& p, const uint8_t* st) {
+Operand weight_operand(const tk_linear_ce_desc_t& d, const Plan& p, const uint8_t* w_at) {
     if (p.w_direct) return {static_cast<const uint8_t*>(d.weight), d.cols, d.vocab * d.cols};
-    return {st + p.s_w, p.ld, d.vocab * p.ld};
+    return {w_at, p.ld, d.vocab * p.ld};
 }
 
 GemmParams base_params(const tk_linear_ce_desc_t& d, const Plan& p, const uint8_t* st) {
@@ -1512,13 +1528,14 @@ int tk_linear_ce(const tk_linear_ce_desc_t* desc, void* workspace, size_t worksp
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     uint8_t* ws = static_cast<uint8_t*>(workspace);
     uint8_t* st = d.state != nullptr ? static_cast<uint8_t*>(d.state) : ws + (p.fwd_bytes - p.state_bytes);
+    uint8_t* w_at = p.w_kept ? st + p.s_w : ws + p.w_w;
     if (p.f16) {
-        CE_TRY((list_and_pack<__half, 1>(d, p, st, s)));
+        CE_TRY((list_and_pack<__half, 1>(d, p, st, w_at, s)));
     } else {
-        CE_TRY((list_and_pack<float, 2>(d, p, st, s)));
+        CE_TRY((list_and_pack<float, 2>(d, p, st, w_at, s)));
     }
     if (d.rows > 0) {
-        const Operand w = weight_operand(d, p, st);
+        const Operand w = weight_operand(d, p, w_at);
         CUtensorMap tx, tw;
         CE_TRY(make_map(&tx, st + p.s_x, d.cols, p.rows_read, p.planes, p.ld, p.rows_pad * p.ld, HM));
         CE_TRY(make_map(&tw, w.base, d.cols, d.vocab, p.planes, w.ld, w.plane, HN));
@@ -1565,7 +1582,13 @@ int tk_linear_ce_backward(const tk_linear_ce_grad_desc_t* desc, void* workspace,
     CE_TRY(launch_chain("cross entropy gradient rows", ce_grad_rows_kernel, dim3(static_cast<unsigned>(1 + zero_blocks)), dim3(1024), 0, s,
                         desc->grad_loss, static_cast<int>(d.reduction), index, sc, grow, p.planes, d.target, d.ignore_index, d.rows,
                         static_cast<int64_t>(d.cols * esz), static_cast<uint8_t*>(desc->dx)));
-    const Operand w = weight_operand(d, p, st);
+    uint8_t* w_at = p.w_kept ? st + p.s_w : ws + p.b_w;
+    if (!p.w_kept && !p.w_direct) {
+        CE_TRY(launch_chain("cross entropy pack", ce_pack_kernel<__half, 1>, dim3(static_cast<unsigned>(weight_blocks(d, p))), dim3(kPackThreads), 0, s,
+                            PackJob<__half>{}, weight_job<__half>(d, p, reinterpret_cast<__half*>(w_at)), static_cast<const Scalars*>(sc), 0,
+                            weight_blocks(d, p), static_cast<const __half*>(nullptr), static_cast<float*>(nullptr)));
+    }
+    const Operand w = weight_operand(d, p, w_at);
     const int64_t x_plane = p.rows_pad * p.ld, dz_plane = p.rows_pad * p.piece;
     CUtensorMap tx, tx_mn;
     CE_TRY(make_map(&tx, st + p.s_x, d.cols, p.rows_read, p.planes, p.ld, x_plane, HM));
