@@ -517,9 +517,11 @@ TK_API int tk_linear_ce(const tk_linear_ce_desc_t* desc, void* workspace, size_t
  * not read), grad_loss the gradient of the loss ([rows] or one value).  dx
  * [rows, cols], dweight [vocab, cols] and dbias [vocab] may be NULL.  The
  * logits are computed again in pieces of the vocabulary; softmax - onehot is
- * held as binary16 (two planes for fp32) scaled by the largest |grad_loss|.
- * Deterministic.  The state's scalars are written, so two backward passes of
- * one state must not run at the same time. */
+ * held as binary16 (two planes for fp32), so each of its entries is known to
+ * 2^-39 at least, and no closer: below 2^-28 in fp16 and 2^-17 in fp32 an entry
+ * has fewer than 11 and 22 bits.  A row's dx depends on that row's grad_loss
+ * alone; a non-finite grad_loss makes its row of dx and all of dweight and dbias
+ * non-finite.  Deterministic; the state is only read. */
 typedef struct {
     tk_linear_ce_desc_t fwd;
     const float* grad_loss;

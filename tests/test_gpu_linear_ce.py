@@ -419,3 +419,68 @@ def test_linear_ce_saved_on_the_host(dtype, d):
     grads = torch.autograd.grad(loss, list(dev.values()))
     for k, g in zip(dev, grads):
         assert torch.equal(g.cpu(), want[k]), k
+
+
+@pytest.mark.parametrize("dtype,low,high", [(F16, -4, 4), (F32, -12, 3)])
+def test_linear_ce_each_row_has_its_own_gradient(dtype, low, high):
+    """Gradients of the rows over many decades: every row of dx is as exact,
+    relative to its own gradient, as with all gradients 1, and is the same
+    whatever the other rows' gradients are."""
+    n, d, v = 64, 72, 5000
+    t, target = ce_inputs(n, d, v, dtype, True, 6, seed=41)
+    g = (10.0 ** torch.linspace(low, high, n, dtype=torch.float64)).float()
+    g[1::2] *= -1
+    g[7] = 0
+    got = check_ce(t, target, "none", g)
+    value, bound = R.linear_ce64(t["x"], t["weight"], target, t["bias"], reduction="none", grad=torch.ones(n))["x"]
+    own = g.double()[:, None]
+    # linear in g_i: the error of a gradient of 1, times |g_i|, and the result's own rounding
+    R.assert_within(got["x"], own * value, own.abs() * bound + R.ulp(own * value, dtype), "x")
+    other = g.clone()
+    other[::3] = 1.0
+    again = run_ce(t, target, "none", other)
+    same = torch.ones(n, dtype=torch.bool)
+    same[::3] = False
+    assert torch.equal(got["x"][same], again["x"][same])
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+def test_linear_ce_subnormal_and_far_row_gradients(dtype):
+    # a row far below the others adds nothing to dW that its rounding shows; alone it is all of it
+    n, d, v = 40, 64, 300
+    t, target = ce_inputs(n, d, v, dtype, True, seed=42)
+    g = torch.full((n,), 2.0 ** -140)
+    got = run_ce(t, target, "none", g)
+    assert all(torch.isfinite(got[k]).all() for k in got)
+    t["x"][3] *= 2.0 ** -9
+    for big in (1.0, 2.0 ** -20):
+        g = torch.full((n,), 2.0 ** -24 * big)
+        g[3] = 512 * big
+        check_ce(t, target, "none", g)
+        g[3] = 0
+        g[4] = -big
+        check_ce(t, target, "none", g)
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+def test_linear_ce_non_finite_row_gradients_stay_in_their_rows(dtype):
+    n = 70
+    t, target = ce_inputs(n, 96, 400, dtype, True, 8, seed=43)
+    live = (target != -100).nonzero()[:, 0]
+    g = loss_grad(n, "none")
+    bad = torch.zeros(n, dtype=torch.bool)
+    bad[live[[5, 9]]] = True
+    g[bad] = 0.0
+    clean = run_ce(t, target, "none", g)
+    for values in ([float("nan"), 1.0], [float("inf"), 1.0], [float("nan"), float("-inf")]):
+        g[bad] = torch.tensor(values)
+        got = run_ce(t, target, "none", g)
+        assert torch.equal(got["loss"], clean["loss"])
+        assert torch.equal(got["x"][~bad], clean["x"][~bad])
+        assert not torch.isfinite(got["x"][live[5]]).any()
+        assert not torch.isfinite(got["weight"]).any() and not torch.isfinite(got["bias"]).any()
+
+
+def test_linear_ce_row_gradients_over_several_pieces():
+    t, target = ce_inputs(14000, 72, 20003, F16, True, 14000 // 3, seed=44)
+    check_ce(t, target, "none", loss_grad(14000, "none") * 64)

@@ -16,10 +16,15 @@
 // GEMMs read it in place (dz and x^T / W^T in MN-major shared-memory tiles, so
 // nothing is transposed).
 //
-// binary16 dz: softmax - onehot lies in [-1, 1]; rows are scaled by g_i / max
-// |g| and 2^14, so values down to 2^-28 of the largest gradient keep all 11
-// bits and the rest lose at most 2^-39 of it.  The scale is taken out again
-// in binary32 when dx and dW are rounded.
+// binary16 dz: softmax - onehot lies in [-1, 1] and is held at 2^14 times its
+// value, so entries down to 2^-28 keep all 11 bits (22 with fp32's two planes,
+// down to 2^-17) and no entry loses more than 2^-39.  One g for all rows is
+// applied in binary32 when dx, dW and db are rounded.  Where rows have gradients
+// of their own, g_i = m_i 2^k_i with m_i in [1, 2): dz takes m_i, dx's row takes
+// 2^k_i in its epilogue, so rows do not touch one another whatever their
+// gradients (one NaN, or six decades between them, would otherwise spoil the
+// others' dx), and dW reads x's rows times 2^k_i, their largest |x g| in [2^14,
+// 2^15): again 2^-39 of the largest is all that a term can lose.
 //
 // fp32 operands are split into two binary16 planes of a power-of-two multiple
 // (hi = rn(v s), lo = rn(v s - hi), the tensor's largest value in [2^14,
@@ -43,6 +48,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <climits>
 
 #include "tk_internal.h"
 #include "tk_ptx.cuh"
@@ -102,14 +108,19 @@ struct Scalars {
     unsigned amax_x;     // binary32 bits of the largest finite |x|, |W| (fp32 operands)
     unsigned amax_w;
     unsigned rows_done;  // blocks of ce_rows_kernel that finished
-    float gmax;          // max |g_i|
-    float dx_scale, dw_scale, db_scale;  // accumulators -> gradients
+};
+
+// Device scalars of one backward pass: accumulators -> gradients.
+struct GradScalars {
+    float dx_scale, dw_scale, db_scale;
+    int top;  // largest exponent of x_i g_i, where rows have gradients of their own
 };
 
 enum Epilogue { kStats, kDlogits, kGradX, kGradW };
 
 struct GemmParams {
     const Scalars* sc;
+    const GradScalars* gs;
     int n_tiles;
     int m_tiles;   // < 0: from sc->count
     int k_blocks;  // < 0: from sc->count
@@ -123,7 +134,7 @@ struct GemmParams {
     const float* bias2;  // bias * log2(e), or NULL
     float2* part;        // [rows][n_tiles][BN / COLS] maximum and sum
     const float* lse2;
-    const float* grow;   // g_i / max |g|
+    const float* grow;   // kDlogits, kGradX: g_i; NULL: one for all rows
     const int* target;
     __half* dz;          // [planes][rows_pad][dz_ld]
     int64_t dz_ld, dz_plane;
@@ -261,6 +272,20 @@ __device__ __forceinline__ float plane_scale(unsigned amax_bits) {
     return exp2f(static_cast<float>(max(-126, min(126, 14 - e))));
 }
 
+// g = mantissa * 2^exponent, the mantissa in [1, 2) (below 1 for subnormal and
+// zero g; a NaN or infinity is its own mantissa).
+__device__ __forceinline__ int exponent_of(float g) {
+    const int e = static_cast<int>(__float_as_uint(g) >> 23 & 0xFFu);
+    return e == 255 ? 0 : max(e, 1) - 127;
+}
+__device__ __forceinline__ float pow2(int e) {  // 2^e, 0 below the subnormal numbers, at most 2^127
+    return __uint_as_float(e >= -126 ? static_cast<uint32_t>(min(127, e) + 127) << 23 : e >= -149 ? 1u << (e + 149) : 0u);
+}
+__device__ __forceinline__ float mantissa_of(float g) {
+    const uint32_t b = __float_as_uint(g), e = b >> 23 & 0xFFu;
+    return e == 255 ? g : e == 0 ? g * pow2(126) : __uint_as_float((b & 0x807FFFFFu) | 0x3F800000u);
+}
+
 // 32 consecutive columns of one row: base-2 logits from the accumulators.
 __device__ __forceinline__ void logits2(const float* acc, float k, const float* bias2, int64_t col, int64_t vocab, float (&y)[32]) {
     if (bias2 != nullptr) {
@@ -346,6 +371,7 @@ __device__ __forceinline__ void finish(const GemmParams& p, int64_t m, int64_t r
         }
     }
     const int64_t at = (EPI == kGradX ? p.index[m] : m) * p.out_cols + col;
+    if (EPI == kGradX && p.grow != nullptr) scale *= pow2(exponent_of(p.grow[m]));
 #pragma unroll
     for (int i = 0; i < N; ++i) v[i] *= scale;
     if constexpr (N == 4) {  // out_cols a multiple of 16 bytes, out 16-byte aligned
@@ -555,8 +581,8 @@ ce_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
         const int rows = p.sc->count;
         float scale = 1.0f;
         if constexpr (EPI == kStats || EPI == kDlogits) scale = z_scale(p);
-        if constexpr (EPI == kGradX) scale = p.sc->dx_scale;
-        if constexpr (EPI == kGradW) scale = p.sc->dw_scale;
+        if constexpr (EPI == kGradX) scale = p.gs->dx_scale;
+        if constexpr (EPI == kGradW) scale = p.gs->dw_scale;
         int local = 0;
         bool ok = true;
         for (int u = first_unit; u < sh.units && ok; u += unit_step) {
@@ -569,7 +595,7 @@ ce_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
             float top = -INFINITY, sum = 0.0f;  // kStats
             const bool live = m < rows;         // kDlogits
             const float lse = EPI == kDlogits && live ? p.lse2[m] : 0.0f;
-            const float g = EPI == kDlogits && live ? p.grow[m] * kDzScale : 0.0f;
+            const float g = EPI == kDlogits && live ? (p.grow != nullptr ? mantissa_of(p.grow[m]) * kDzScale : kDzScale) : 0.0f;
             const int64_t hit = EPI == kDlogits && live ? p.target[m] - p.vocab0 : -1;
             // rows that the warp works for: dz is read (as K) up to a multiple of BK
             const int64_t limit = EPI == kGradW ? p.out_rows : EPI == kDlogits ? (rows + BK - 1) / BK * BK : rows;
@@ -697,7 +723,7 @@ __global__ void __launch_bounds__(256) ce_split_kernel(const GemmParams p) {
     if (sh.splits <= 1) return;
     const int tiles = sh.m_tiles * p.n_tiles;
     const int64_t limit = EPI == kGradX ? p.sc->count : p.out_rows;
-    const float scale = EPI == kGradX ? p.sc->dx_scale : p.sc->dw_scale;
+    const float scale = EPI == kGradX ? p.gs->dx_scale : p.gs->dw_scale;
     const int quad = threadIdx.x % 64, group = threadIdx.x / 64;
     const int shares = sh.splits >= 16 ? 4 : 1, rows = 4 / shares;
     const int share = shares == 4 ? group : 0;
@@ -1134,10 +1160,12 @@ ce_rows_kernel(const T* x, const T* w, const T* bias, const int* index, const in
     }
 }
 
-// Block 0: g_i / max |g| per packed row, the maximum, and the gradients'
-// scales.  The others: zero gradients for the ignored rows.
+static_assert(kDzScale == 16384.0f, "2^14, in the exponents below");
+
+// Block 0: the gradients' scales, and g_i per packed row where each has its
+// own.  The others: zero gradients for the ignored rows.
 __global__ void __launch_bounds__(1024)
-ce_grad_rows_kernel(const float* grad, int reduction, const int* index, Scalars* sc, float* grow, int planes, const int64_t* target,
+ce_grad_rows_kernel(const float* grad, int reduction, const int* index, const Scalars* sc, GradScalars* gs, float* grow, int planes, const int64_t* target,
                     int64_t ignore, int64_t all_rows, int64_t row_bytes, uint8_t* dx) {
     pdl_wait();
     if (blockIdx.x > 0) {
@@ -1153,36 +1181,89 @@ ce_grad_rows_kernel(const float* grad, int reduction, const int* index, Scalars*
         }
         return;
     }
-    __shared__ unsigned warp_top[32];
     const int rows = sc->count;
-    const float g1 = reduction == TK_REDUCE_NONE ? 0.0f : reduction == TK_REDUCE_MEAN ? grad[0] / static_cast<float>(rows) : grad[0];
-    unsigned top = reduction == TK_REDUCE_NONE ? 0u : __float_as_uint(g1) & 0x7FFFFFFFu;
-    if (reduction == TK_REDUCE_NONE)
-        for (int i = threadIdx.x; i < rows; i += 1024) top = max(top, __float_as_uint(grad[index[i]]) & 0x7FFFFFFFu);
-    top = __reduce_max_sync(0xFFFFFFFFu, top);
-    if ((threadIdx.x & 31) == 0) warp_top[threadIdx.x >> 5] = top;
-    __syncthreads();
-    top = __reduce_max_sync(0xFFFFFFFFu, warp_top[threadIdx.x & 31]);
-    const float gmax = rows > 0 ? __uint_as_float(top) : 0.0f;
-    for (int i = threadIdx.x; i < rows; i += 1024) {
-        const float g = reduction == TK_REDUCE_NONE ? grad[index[i]] : g1;
-        grow[i] = gmax == 0.0f ? 0.0f : __fdiv_rn(g, gmax);
-    }
+    const bool own = reduction == TK_REDUCE_NONE;
+    if (own)
+        for (int i = threadIdx.x; i < rows; i += 1024) grow[i] = grad[index[i]];
     if (threadIdx.x == 0) {
-        const float unit = gmax / kDzScale;
-        sc->gmax = gmax;
-        sc->db_scale = unit;
-        sc->dx_scale = planes == 2 ? unit / plane_scale(sc->amax_w) : unit;
-        sc->dw_scale = planes == 2 ? unit / plane_scale(sc->amax_x) : unit;
+        // no rows: every sum is zero
+        const float g = own ? 1.0f : rows == 0 ? 0.0f : reduction == TK_REDUCE_MEAN ? grad[0] / static_cast<float>(rows) : grad[0];
+        const float unit = g / kDzScale;
+        gs->db_scale = own ? 1.0f : unit;  // the sums take 2^(k_i - 14) row by row
+        gs->dx_scale = planes == 2 ? unit / plane_scale(sc->amax_w) : unit;
+        gs->dw_scale = planes == 2 ? unit / plane_scale(sc->amax_x) : unit;  // ce_scale_rows_kernel adds x's exponent
+        gs->top = INT_MIN;
+    }
+}
+
+constexpr int kNoTop = -100000;  // below every exponent of a finite x_i g_i
+
+// The largest exponent of x_i g_i over the packed rows, a warp to a row.
+__global__ void __launch_bounds__(256)
+ce_top_kernel(const __half* x, int64_t ld, const Scalars* sc, GradScalars* gs, const float* grow) {
+    pdl_wait();
+    const int lane = threadIdx.x & 31, rows = sc->count;
+    int top = kNoTop;
+    for (int r = blockIdx.x * 8 + static_cast<int>(threadIdx.x >> 5); r < rows; r += gridDim.x * 8) {
+        const float g = grow[r];
+        if (g == 0.0f || !isfinite(g)) continue;
+        uint32_t most = 0;  // binary16 bits of the row's largest finite |x|
+        for (int64_t c = lane * 8; c < ld; c += 32 * 8) {
+            const uint4 u = *reinterpret_cast<const uint4*>(x + r * ld + c);
+            for (uint32_t w : {u.x, u.y, u.z, u.w})
+                for (uint32_t h : {w & 0x7FFFu, w >> 16 & 0x7FFFu})
+                    if (h < 0x7C00u) most = max(most, h);
+        }
+        most = __reduce_max_sync(0xFFFFFFFFu, most);
+        if (most != 0) top = max(top, exponent_of(__half2float(__ushort_as_half(static_cast<unsigned short>(most)))) + exponent_of(g));
+    }
+    if (lane == 0) atomicMax(&gs->top, top);
+}
+
+// x's packed rows (zero rows up to a multiple of BK included) times 2^k_i and
+// the power of two that takes the largest into [2^14, 2^15), for dW.
+template <int PLANES>
+__global__ void __launch_bounds__(kPackThreads)
+ce_scale_rows_kernel(const __half* x, __half* to, int64_t ld, int64_t plane, const Scalars* sc, GradScalars* gs, const float* grow) {
+    pdl_wait();
+    const int64_t live = sc->count;
+    const int shift = gs->top > kNoTop ? 14 - gs->top : 0;
+    if (blockIdx.x == 0 && threadIdx.x == 0) {  // in two steps: the exponent can be past a power of two's
+        const int half = shift / 2;
+        gs->dw_scale = gs->dw_scale * pow2(-half) * pow2(half - shift);
+    }
+    for (int64_t r = blockIdx.x; r < (live + BK - 1) / BK * BK; r += gridDim.x) {
+        const float g = r < live ? grow[r] : 0.0f;
+        const int e = isfinite(g) ? exponent_of(g) + shift : 0;
+        const float a = g == 0.0f ? 0.0f : pow2(e / 2), b = pow2(e - e / 2);  // a row that `top` does not bound takes no part
+        for (int64_t c = static_cast<int64_t>(threadIdx.x) * 8; c < ld; c += kPackThreads * 8) {
+            const int64_t at = r * ld + c;
+            const uint4 h = *reinterpret_cast<const uint4*>(x + at);
+            uint4 l = make_uint4(0, 0, 0, 0);
+            if constexpr (PLANES == 2) l = *reinterpret_cast<const uint4*>(x + plane + at);
+            const uint32_t hs[4] = {h.x, h.y, h.z, h.w}, ls[4] = {l.x, l.y, l.z, l.w};
+            uint32_t hi[4], lo[4];
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+                const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&hs[t])), d = __half22float2(*reinterpret_cast<const __half2*>(&ls[t]));
+                const float v0 = (f.x + d.x) * a * b, v1 = (f.y + d.y) * a * b;  // exact: hi + lo has 22 bits
+                hi[t] = half2_bits(v0, v1);
+                const float2 q = __half22float2(*reinterpret_cast<const __half2*>(&hi[t]));
+                lo[t] = half2_bits(isfinite(q.x) ? v0 - q.x : 0.0f, isfinite(q.y) ? v1 - q.y : 0.0f);
+            }
+            *reinterpret_cast<uint4*>(to + at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+            if constexpr (PLANES == 2) *reinterpret_cast<uint4*>(to + plane + at) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+        }
     }
 }
 
 constexpr int kDbThreads = 256;
 
-// Column sums of a piece's dz: chunk blockIdx.y of the rows, 8 columns per
-// lane, 8 rows at a time, into partial[chunk][dz_ld].
+// Column sums of a piece's dz, rows times 2^(k_i - 14) where each has its own
+// gradient: chunk blockIdx.y of the rows, 8 columns per lane, 8 rows at a time,
+// into partial[chunk][dz_ld].
 __global__ void __launch_bounds__(kDbThreads)
-ce_dbias_part_kernel(const __half* dz, int64_t dz_ld, int64_t dz_plane, const Scalars* sc, float* partial) {
+ce_dbias_part_kernel(const __half* dz, int64_t dz_ld, int64_t dz_plane, const Scalars* sc, const float* grow, float* partial) {
     pdl_wait();
     __shared__ float sums[8][32][9];
     const int rows = sc->count;
@@ -1200,11 +1281,12 @@ ce_dbias_part_kernel(const __half* dz, int64_t dz_ld, int64_t dz_plane, const Sc
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
                 const __half2* h = reinterpret_cast<const __half2*>(&u[k]);
+                const float a = grow != nullptr && r + 8 * k < hi ? pow2(exponent_of(grow[r + 8 * k]) - 14) : 1.0f;
 #pragma unroll
                 for (int t = 0; t < 4; ++t) {
                     const float2 f = __half22float2(h[t]);
-                    s[2 * t] += f.x;
-                    s[2 * t + 1] += f.y;
+                    s[2 * t] = fmaf(f.x, a, s[2 * t]);
+                    s[2 * t + 1] = fmaf(f.y, a, s[2 * t + 1]);
                 }
             }
         }
@@ -1221,13 +1303,13 @@ ce_dbias_part_kernel(const __half* dz, int64_t dz_ld, int64_t dz_plane, const Sc
 }
 
 __global__ void __launch_bounds__(256)
-ce_dbias_kernel(const float* partial, int chunks, int64_t dz_ld, int64_t cols, const Scalars* sc, void* out, int out_f32) {
+ce_dbias_kernel(const float* partial, int chunks, int64_t dz_ld, int64_t cols, const GradScalars* gs, void* out, int out_f32) {
     pdl_wait();
     const int64_t c = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
     if (c >= cols) return;
     float s = 0.0f;
     for (int i = 0; i < chunks; ++i) s += partial[i * dz_ld + c];
-    s *= sc->db_scale;
+    s *= gs->db_scale;
     if (out_f32) {
         static_cast<float*>(out)[c] = s;
     } else {
@@ -1260,7 +1342,7 @@ struct Plan {
     size_t s_scalars, s_index, s_target, s_lse, s_x, s_bias, s_w, state_bytes;
     // workspaces
     size_t w_part, w_loss, w_w, fwd_bytes;
-    size_t b_grow, b_dz, b_acc, b_split, b_db, b_w, bwd_bytes;
+    size_t b_scalars, b_grow, b_dz, b_acc, b_split, b_db, b_w, b_x, bwd_bytes;
 };
 
 int check(const char* who, const tk_linear_ce_desc_t& d) {
@@ -1328,7 +1410,10 @@ Plan make_plan(const tk_linear_ce_desc_t& d) {
     p.w_w = take(p.w_kept || p.w_direct ? 0 : w_bytes);
     p.fwd_bytes = at + p.state_bytes;  // a call without a state keeps its own
     at = 0;
-    p.b_grow = take(p.rows_pad * sizeof(float));
+    const bool own = d.reduction == TK_REDUCE_NONE;  // each row has its own gradient
+    p.b_scalars = take(sizeof(GradScalars));
+    p.b_grow = take(own ? p.rows_pad * sizeof(float) : 0);
+    p.b_x = take(own ? static_cast<size_t>(p.planes) * p.rows_pad * p.ld * 2 : 0);
     p.b_dz = take(static_cast<size_t>(p.planes) * p.rows_pad * p.piece * 2);
     p.b_acc = take(p.pieces > 1 ? static_cast<size_t>(p.rows_pad) * p.acc_ld * sizeof(float) : 0);
     p.b_split = take(static_cast<size_t>(p.split_units) * BM * BN * sizeof(float));
@@ -1573,26 +1658,38 @@ int tk_linear_ce_backward(const tk_linear_ce_grad_desc_t* desc, void* workspace,
     if (!desc->dx && !desc->dweight && !desc->dbias) return TK_OK;
     uint8_t* ws = static_cast<uint8_t*>(workspace);
     uint8_t* st = static_cast<uint8_t*>(d.state);
-    Scalars* sc = reinterpret_cast<Scalars*>(st + p.s_scalars);
+    const Scalars* sc = reinterpret_cast<const Scalars*>(st + p.s_scalars);
     const int* index = reinterpret_cast<const int*>(st + p.s_index);
-    float* grow = reinterpret_cast<float*>(ws + p.b_grow);
+    GradScalars* gs = reinterpret_cast<GradScalars*>(ws + p.b_scalars);
+    const bool own = d.reduction == TK_REDUCE_NONE;
+    float* grow = own ? reinterpret_cast<float*>(ws + p.b_grow) : nullptr;
     __half* dz = reinterpret_cast<__half*>(ws + p.b_dz);
     const size_t esz = dtype_size(d.dtype);
     const int zero_blocks = desc->dx != nullptr ? static_cast<int>(std::min<int64_t>(ceil_div(d.rows, 32), 148 * 2)) : 0;
     CE_TRY(launch_chain("cross entropy gradient rows", ce_grad_rows_kernel, dim3(static_cast<unsigned>(1 + zero_blocks)), dim3(1024), 0, s,
-                        desc->grad_loss, static_cast<int>(d.reduction), index, sc, grow, p.planes, d.target, d.ignore_index, d.rows,
+                        desc->grad_loss, static_cast<int>(d.reduction), index, sc, gs, grow, p.planes, d.target, d.ignore_index, d.rows,
                         static_cast<int64_t>(d.cols * esz), static_cast<uint8_t*>(desc->dx)));
     uint8_t* w_at = p.w_kept ? st + p.s_w : ws + p.b_w;
     if (!p.w_kept && !p.w_direct) {
         CE_TRY(launch_chain("cross entropy pack", ce_pack_kernel<__half, 1>, dim3(static_cast<unsigned>(weight_blocks(d, p))), dim3(kPackThreads), 0, s,
-                            PackJob<__half>{}, weight_job<__half>(d, p, reinterpret_cast<__half*>(w_at)), static_cast<const Scalars*>(sc), 0,
+                            PackJob<__half>{}, weight_job<__half>(d, p, reinterpret_cast<__half*>(w_at)), sc, 0,
                             weight_blocks(d, p), static_cast<const __half*>(nullptr), static_cast<float*>(nullptr)));
     }
     const Operand w = weight_operand(d, p, w_at);
     const int64_t x_plane = p.rows_pad * p.ld, dz_plane = p.rows_pad * p.piece;
+    const __half* x_dw = reinterpret_cast<const __half*>(st + p.s_x);
+    if (own && desc->dweight) {
+        __half* to = reinterpret_cast<__half*>(ws + p.b_x);
+        CE_TRY(launch_chain("cross entropy row exponents", ce_top_kernel, dim3(static_cast<unsigned>(std::min<int64_t>(ceil_div(d.rows, 8), 148 * 8))), dim3(256),
+                            0, s, x_dw, p.ld, sc, gs, static_cast<const float*>(grow)));
+        CE_TRY(launch_chain("cross entropy row scales", p.planes == 2 ? ce_scale_rows_kernel<2> : ce_scale_rows_kernel<1>,
+                            dim3(static_cast<unsigned>(blocks_for(p.rows_read))), dim3(kPackThreads), 0, s, x_dw, to, p.ld, x_plane, sc, gs,
+                            static_cast<const float*>(grow)));
+        x_dw = to;
+    }
     CUtensorMap tx, tx_mn;
     CE_TRY(make_map(&tx, st + p.s_x, d.cols, p.rows_read, p.planes, p.ld, x_plane, HM));
-    CE_TRY(make_map(&tx_mn, st + p.s_x, d.cols, p.rows_read, p.planes, p.ld, x_plane, BK));
+    CE_TRY(make_map(&tx_mn, x_dw, d.cols, p.rows_read, p.planes, p.ld, x_plane, BK));
     const int64_t row_tiles = ceil_div(d.rows, BM), col_tiles = ceil_div(d.cols, BN);
     const bool cols16 = d.cols * esz % 16 == 0;
     for (int64_t i = 0; i < p.pieces; ++i) {
@@ -1616,12 +1713,14 @@ int tk_linear_ce_backward(const tk_linear_ce_grad_desc_t* desc, void* workspace,
         if (desc->dbias) {
             float* part = reinterpret_cast<float*>(ws + p.b_db);
             CE_TRY(launch_chain("cross entropy bias sums", ce_dbias_part_kernel, dim3(static_cast<unsigned>(p.piece / 256), p.db_chunks), dim3(kDbThreads), 0, s,
-                                static_cast<const __half*>(dz), p.piece, g.dz_plane, static_cast<const Scalars*>(sc), part));
+                                static_cast<const __half*>(dz), p.piece, g.dz_plane, sc, static_cast<const float*>(grow), part));
             CE_TRY(launch_chain("cross entropy bias sums", ce_dbias_kernel, dim3(static_cast<unsigned>(ceil_div(width, 256))), dim3(256), 0, s,
-                                static_cast<const float*>(part), p.db_chunks, p.piece, width, static_cast<const Scalars*>(sc),
+                                static_cast<const float*>(part), p.db_chunks, p.piece, width, static_cast<const GradScalars*>(gs),
                                 static_cast<void*>(static_cast<uint8_t*>(desc->dbias) + v0 * esz), p.f16 ? 0 : 1));
         }
         GemmParams r = base_params(d, p, st);
+        r.gs = gs;
+        r.grow = grow;
         r.out_cols = d.cols;
         r.out_f32 = p.f16 ? 0 : 1;
         r.n_tiles = static_cast<int>(col_tiles);
