@@ -423,7 +423,7 @@ TK_API int tk_dropout(tk_dtype_t dtype, const void* x, void* y, int64_t n, doubl
  * sqrt(mean square + eps).  NULL weights stand for 1, NULL biases for 0, a
  * NULL gate for 1.  gate is [gate_rows, cols]: row r uses gate row
  * r / (rows / gate_rows) (1: one for each channel; the batch size: one for
- * each sample; rows: one for each token).  Sums and statistics are fp32; each
+ * each sample; rows: one for each token; 0 where rows is 0).  Sums and statistics are fp32; each
  * output is rounded once.  stats (NULL or 16-byte aligned, [rows][4]) receives
  * mean and rstd of f (post norm only) and of x_new for the backward pass.
  * cols <= 32768; with dropout rows * cols < 2^34.  Outputs must not overlap inputs.  Extends layer_norm

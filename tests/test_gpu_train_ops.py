@@ -373,3 +373,13 @@ def test_train_op_refusals():
     y, _ = ops.residual_norm(leaf, x)
     with pytest.raises(RuntimeError, match="create_graph"):
         torch.autograd.grad(y, leaf, torch.ones(4, 16, dtype=F16).to(DEV), create_graph=True)
+
+
+@pytest.mark.parametrize("shape", [(0, 4, 16), (3, 0, 16), (0, 16), (0, 0, 8)])
+@pytest.mark.parametrize("gate", ["sample", "token"])
+def test_residual_norm_empty_batch_with_a_gate_for_each_sample(shape, gate):
+    t = norm_inputs(shape, F16, "layer", True, gate, 1)
+    none = torch.zeros(shape, dtype=F16)
+    got = run_norm(t, "layer", True, 1.0, 0.1, none, none)
+    assert got["h"].shape == got["x"].shape == shape and got["gate"].shape == t["gate"].shape
+    assert not got["weight"].any() and not got["gate"].any()

@@ -246,3 +246,15 @@ def test_linear_ce_workspaces_have_room_for_a_weight_off_the_boundary():
         sizes.append((L.tk_linear_ce_workspace_size(ctypes.byref(g.fwd)), L.tk_linear_ce_backward_workspace_size(ctypes.byref(g))))
     packed = 1000 * 96 * 2
     assert all(off >= on + packed for on, off in zip(*sizes))
+
+
+@pytest.mark.parametrize("gate_rows", [0, 1, 5])
+def test_residual_norm_without_rows_takes_any_gate(gate_rows):
+    L = C.lib()
+    d = _norm_desc(rows=0, gate=1024, gate_rows=gate_rows)
+    assert L.tk_residual_norm(ctypes.byref(d), None) == 0
+    g = C.ResidualNormGradDesc()
+    g.fwd = d
+    assert L.tk_residual_norm_backward_workspace_size(ctypes.byref(g)) > 0
+    assert L.tk_residual_norm_backward(ctypes.byref(g), None, 0, None) == 0
+    assert L.tk_residual_norm(ctypes.byref(_norm_desc(rows=0, gate=1024, gate_rows=-1)), None) == 1

@@ -1207,7 +1207,8 @@ int check(const char* who, const tk_residual_norm_desc_t& d) {
     TK_CHECK_ARG(d.p >= 0.0 && d.p <= 1.0, "%s: p must be in [0, 1], got %g", who, d.p);
     if (d.p > 0.0 && d.rows * d.cols >= (1ll << 34)) TK_FAIL(TK_ERR_UNSUPPORTED, "%s: dropout of 2^34 elements or more", who);
     TK_CHECK_ARG(d.post_norm || (d.post_weight == nullptr && d.post_bias == nullptr), "%s: post_weight and post_bias need post_norm", who);
-    TK_CHECK_ARG(d.gate == nullptr || (d.gate_rows >= 1 && d.rows % d.gate_rows == 0), "%s: gate_rows must divide rows", who);
+    // no rows: a gate for each sample of an empty batch has none either
+    TK_CHECK_ARG(d.gate == nullptr || (d.gate_rows >= 1 && d.rows % d.gate_rows == 0) || (d.gate_rows == 0 && d.rows == 0), "%s: gate_rows must divide rows", who);
     return TK_OK;
 }
 
