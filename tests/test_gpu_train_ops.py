@@ -383,3 +383,22 @@ def test_residual_norm_empty_batch_with_a_gate_for_each_sample(shape, gate):
     got = run_norm(t, "layer", True, 1.0, 0.1, none, none)
     assert got["h"].shape == got["x"].shape == shape and got["gate"].shape == t["gate"].shape
     assert not got["weight"].any() and not got["gate"].any()
+
+
+@pytest.mark.parametrize("grad", [False, True])
+@pytest.mark.parametrize("call", [lambda x, y: ops.dropout(x, 0.1, 1), lambda x, y: ops.residual_norm(x, y)[1], lambda x, y: ops.residual_norm(y, x)[1],
+                                  lambda x, y: ops.residual_norm(y, y, x[0])[1], lambda x, y: ops.residual_norm(y, y, gate=x)[1],
+                                  lambda x, y: ops.linear_cross_entropy(x, y, TARGET.to(DEV)), lambda x, y: ops.linear_cross_entropy(y, x, TARGET.to(DEV)),
+                                  lambda x, y: ops.linear_cross_entropy(y, y, TARGET.to(DEV), x[0, :6])])
+def test_train_ops_refuse_forward_mode(call, grad):
+    """A dual tensor is refused, whether it also requires a gradient or not: its
+    tangent would be lost."""
+    x, y = rnd((6, 16), 1).to(DEV).requires_grad_(grad), rnd((6, 16), 2).to(DEV)
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(x, torch.ones_like(x))
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            call(dual, y)
+    call(x, y)
+
+
+TARGET = torch.arange(6)

@@ -54,6 +54,12 @@ bool needs_grad(std::initializer_list<at::Tensor> ts) {
     return false;
 }
 
+// A dual tensor would come back without its tangent where no gradient is wanted.
+void check_no_tangent(const char* op, std::initializer_list<at::Tensor> ts) {
+    for (const at::Tensor& t : ts)
+        TORCH_CHECK(!t.defined() || !t._fw_grad(0).defined(), "kunlun ", op, ": forward-mode derivatives are not implemented");
+}
+
 void check_single_backward(const char* op) {
     TORCH_CHECK(!at::GradMode::is_enabled(), "kunlun ", op, ": gradients of its backward pass (create_graph=True) are not implemented");
 }
@@ -317,6 +323,7 @@ at::Tensor linear_cross_entropy(const at::Tensor& x_in, const at::Tensor& weight
     const at::Tensor weight = param(weight_in, x_in, op, "weight"), bias = param(bias_in, x_in, op, "bias");
     TORCH_CHECK(!bias.defined() || (bias.dim() == 1 && bias.size(0) == weight.size(0)),
                 "kunlun linear_cross_entropy: bias must be [", weight.size(0), "], got ", bias.sizes());
+    check_no_tangent(op, {x_in, weight, bias});
     const int64_t cols = x_in.size(-1), rows = x_in.numel() / cols;
     const at::Tensor x = x_in.contiguous().view({rows, cols}), target = target_in.contiguous().view({rows});
     at::Tensor loss;
@@ -332,6 +339,7 @@ at::Tensor linear_cross_entropy(const at::Tensor& x_in, const at::Tensor& weight
 at::Tensor dropout(const at::Tensor& x, double p, uint64_t seed, uint64_t offset) {
     check_input(x, "dropout");
     TORCH_CHECK(p >= 0.0 && p <= 1.0, "kunlun dropout: p must be in [0, 1], got ", p);
+    check_no_tangent("dropout", {x});
     if (needs_grad({x})) return Dropout::apply(x, p, static_cast<int64_t>(seed), static_cast<int64_t>(offset));
     at::AutoDispatchBelowADInplaceOrView guard;
     return dropout_run(x, p, seed, offset);
@@ -368,6 +376,7 @@ std::tuple<at::Tensor, at::Tensor> residual_norm(
         TORCH_CHECK(ok, "kunlun residual_norm: gate must be [", cols, "] or x's shape ", x.sizes(),
                     " with 1 in place of some last dimensions before the columns, got ", gate.sizes());
     }
+    check_no_tangent(op, {x, f, weight, bias, post_weight, post_bias, gate});
     const NormOptions o = {rms, post_norm, residual_scale, eps, p, static_cast<int64_t>(seed), static_cast<int64_t>(offset)};
     if (needs_grad({x, f, weight, bias, post_weight, post_bias, gate})) {
         const variable_list r = ResidualNorm::apply(x, f, optional(weight), optional(bias), optional(post_weight),
