@@ -402,3 +402,40 @@ def test_train_ops_refuse_forward_mode(call, grad):
 
 
 TARGET = torch.arange(6)
+
+
+@pytest.mark.parametrize("spoil,match", [(lambda v: v.cpu(), "expected"), (lambda v: v.to(F32) if v.dtype == F16 else v.to(F16), "expected"),
+                                         (lambda v: v[:1], "expected")])
+@pytest.mark.parametrize("call", ["norm", "loss"])
+def test_train_ops_refuse_other_saved_tensors(call, spoil, match):
+    """What saved-tensor hooks hand back is looked at before its pointer is used."""
+    x = rnd((2, 3, 16), 1).to(DEV).requires_grad_()
+    with torch.autograd.graph.saved_tensors_hooks(lambda v: v, lambda v: spoil(v.detach())):
+        if call == "norm":
+            y = ops.residual_norm(x, x.detach(), rnd((16,), 2).to(DEV), post_norm=True, gate=rnd((2, 1, 16), 3).to(DEV))[1].float().sum()
+        else:
+            y = ops.linear_cross_entropy(x, rnd((9, 16), 4).to(DEV), torch.zeros(2, 3, dtype=torch.int64).to(DEV), rnd((9,), 5).to(DEV))
+    with pytest.raises(RuntimeError, match=match):
+        y.backward()
+
+
+@pytest.mark.parametrize("kind,post,gate", [("layer", True, "sample"), ("rms", False, "none")])
+def test_residual_norm_saved_tensors_come_back_strided_or_from_the_host(kind, post, gate):
+    shape = (4, 19, 96)
+    t = norm_inputs(shape, F16, kind, post, gate, 3)
+    gx, gh = rnd(shape, 8), rnd(shape, 9)
+    want = run_norm(t, kind, post, 1.0, 0.2, gx, gh)
+
+    def strided(v):
+        return v.transpose(0, 1).contiguous().transpose(0, 1) if v.dim() > 1 else v.clone()
+
+    def off(v):
+        b = torch.empty(v.numel() + 8, dtype=v.dtype, device=DEV)
+        b[1:1 + v.numel()].copy_(v.reshape(-1))
+        return b[1:1 + v.numel()].view(v.shape) if v.dtype == F16 else v
+
+    for pack, unpack in ((lambda v: v.cpu(), lambda v: v.to(DEV)), (lambda v: v, strided), (lambda v: v, off)):
+        with torch.autograd.graph.saved_tensors_hooks(pack, unpack):
+            got = run_norm(t, kind, post, 1.0, 0.2, gx, gh)
+        for k in want:
+            assert torch.equal(got[k], want[k]), k

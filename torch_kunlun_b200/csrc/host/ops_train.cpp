@@ -64,6 +64,15 @@ void check_single_backward(const char* op) {
     TORCH_CHECK(!at::GradMode::is_enabled(), "kunlun ", op, ": gradients of its backward pass (create_graph=True) are not implemented");
 }
 
+// A saved tensor as the kernels take it.  Saved-tensor hooks may hand back other
+// tensors than were saved, so what the pointers rest on is looked at again.
+at::Tensor restored(const at::Tensor& t, at::Device device, at::ScalarType type, at::IntArrayRef sizes, const char* op, const char* name) {
+    TORCH_CHECK(t.defined() && t.device() == device && t.scalar_type() == type && t.sizes().equals(sizes), "kunlun ", op, ": the saved ", name,
+                " came back as ", t.defined() ? t.toString() : "nothing", " ", t.defined() ? t.sizes() : at::IntArrayRef(), " on ",
+                t.defined() ? t.device() : at::Device(at::kCPU), ", expected ", type, " ", sizes, " on ", device);
+    return t.contiguous();
+}
+
 // A contiguous tensor on the current device, allocated without a trip through
 // the dispatcher: these ops allocate up to nine tensors a call.
 at::Tensor fresh(at::IntArrayRef shape, at::ScalarType type) {
@@ -165,17 +174,19 @@ struct ResidualNorm : torch::autograd::Function<ResidualNorm> {
         }
         auto [x_new, h] = norm_run(x, f, weight, bias, post_weight, post_bias, gate, o, stats);
         ctx->save_for_backward({x, f, weight, post_weight, post_bias, gate, stats});
-        ctx->saved_data["flags"] = std::vector<bool>{o.rms,
-                                                     o.post,
-                                                     x.requires_grad(),
-                                                     f.requires_grad(),
-                                                     weight.defined() && weight.requires_grad(),
-                                                     bias.defined() && bias.requires_grad(),
-                                                     post_weight.defined() && post_weight.requires_grad(),
-                                                     post_bias.defined() && post_bias.requires_grad(),
-                                                     gate.defined() && gate.requires_grad()};
+        // a bit for each tensor given, and for each that wants a gradient
+        int64_t given = 0, wanted = 0;
+        const at::Tensor* const inputs[7] = {&x, &f, &weight, &bias, &post_weight, &post_bias, &gate};
+        for (int i = 0; i < 7; ++i) {
+            if (!inputs[i]->defined()) continue;
+            given |= 1 << i;
+            if (inputs[i]->requires_grad()) wanted |= 1 << i;
+        }
+        std::vector<int64_t> ints = {o.rms, o.post, o.seed, o.offset, given, wanted, static_cast<int64_t>(x.scalar_type()), x.device().index(), x.dim()};
+        ints.insert(ints.end(), x.sizes().begin(), x.sizes().end());
+        if (gate.defined()) ints.insert(ints.end(), gate.sizes().begin(), gate.sizes().end());
+        ctx->saved_data["ints"] = std::move(ints);
         ctx->saved_data["reals"] = std::vector<double>{o.scale, o.eps, o.p};
-        ctx->saved_data["random"] = std::vector<int64_t>{o.seed, o.offset};
         ctx->set_materialize_grads(false);
         return {x_new, h};
     }
@@ -186,25 +197,33 @@ struct ResidualNorm : torch::autograd::Function<ResidualNorm> {
         at::Tensor gx = grads[0], gh = grads[1];
         if (!gx.defined() && !gh.defined()) return out;
         const variable_list saved = ctx->get_saved_variables();
-        const at::Tensor &x = saved[0], &f = saved[1], &weight = saved[2], &post_weight = saved[3],
-                         &post_bias = saved[4], &gate = saved[5], &stats = saved[6];
-        const auto flag = ctx->saved_data["flags"].toBoolList();
+        const auto ints = ctx->saved_data["ints"].toIntVector();
         const auto real = ctx->saved_data["reals"].toDoubleVector();
-        const auto random = ctx->saved_data["random"].toIntVector();
-        const NormOptions o = {flag[0], flag[1], real[0], real[1], real[2], random[0], random[1]};
+        const NormOptions o = {ints[0] != 0, ints[1] != 0, real[0], real[1], real[2], ints[2], ints[3]};
+        const auto given = [&](int i) { return (ints[4] >> i & 1) != 0; };
+        const auto wanted = [&](int i) { return (ints[5] >> i & 1) != 0; };
+        const at::ScalarType type = static_cast<at::ScalarType>(ints[6]);
+        const at::Device device(c10::DeviceType::PrivateUse1, static_cast<at::DeviceIndex>(ints[7]));
+        const at::IntArrayRef shapes = at::IntArrayRef(ints).slice(9), sizes = shapes.slice(0, ints[8]), gate_sizes = shapes.slice(ints[8]);
+        const int64_t cols = sizes.back(), rows = c10::multiply_integers(sizes) / cols;
+        const auto again = [&](int i, const char* name, at::IntArrayRef shape) { return restored(saved[i], device, type, shape, "residual_norm", name); };
+        const at::Tensor x = again(0, "x", sizes), f = again(1, "f", sizes),
+                         weight = given(2) ? again(2, "weight", cols) : at::Tensor(),
+                         post_weight = given(4) ? again(3, "post_weight", cols) : at::Tensor(),
+                         post_bias = given(5) ? again(4, "post_bias", cols) : at::Tensor(),
+                         gate = given(6) ? again(5, "gate", gate_sizes) : at::Tensor(),
+                         stats = restored(saved[6], device, at::kFloat, {rows, 4}, "residual_norm", "statistics");
         if (gx.defined()) gx = gx.contiguous();
         if (gh.defined()) gh = gh.contiguous();
-        const int dev = x.device().index();
+        const int dev = device.index();
         DeviceScope g(dev);
-        const at::ScalarType type = x.scalar_type();
-        const int64_t cols = x.size(-1);
-        if (flag[2]) out[0] = fresh(x.sizes(), type);
-        if (flag[3]) out[1] = fresh(x.sizes(), type);
-        if (flag[4]) out[2] = fresh({cols}, type);
-        if (flag[5]) out[3] = fresh({cols}, type);
-        if (flag[6]) out[4] = fresh({cols}, type);
-        if (flag[7]) out[5] = fresh({cols}, type);
-        if (flag[8]) out[6] = fresh(gate.sizes(), type);
+        if (wanted(0)) out[0] = fresh(x.sizes(), type);
+        if (wanted(1)) out[1] = fresh(x.sizes(), type);
+        if (wanted(2)) out[2] = fresh({cols}, type);
+        if (wanted(3)) out[3] = fresh({cols}, type);
+        if (wanted(4)) out[4] = fresh({cols}, type);
+        if (wanted(5)) out[5] = fresh({cols}, type);
+        if (wanted(6)) out[6] = fresh(gate.sizes(), type);
         tk_residual_norm_grad_desc_t d = {};
         d.fwd = norm_desc(x, o, weight, post_weight, post_bias, gate);
         d.fwd.x = ptr(x);
@@ -271,7 +290,8 @@ struct LinearCrossEntropy : torch::autograd::Function<LinearCrossEntropy> {
         at::Tensor loss = ce_run(ce_desc(x, weight, target, bias, ignore_index, reduction), x, &state);
         ctx->save_for_backward({x, weight, target, bias, state});
         ctx->saved_data["ints"] = std::vector<int64_t>{ignore_index, reduction, x.requires_grad(), weight.requires_grad(),
-                                                       bias.defined() && bias.requires_grad()};
+                                                       bias.defined() && bias.requires_grad(), bias.defined(), x.size(0), x.size(1), weight.size(0),
+                                                       state.numel(), static_cast<int64_t>(x.scalar_type()), x.device().index()};
         ctx->set_materialize_grads(false);
         return loss;
     }
@@ -281,9 +301,17 @@ struct LinearCrossEntropy : torch::autograd::Function<LinearCrossEntropy> {
         variable_list out(6);
         if (!grads[0].defined()) return out;
         const variable_list saved = ctx->get_saved_variables();
-        const at::Tensor &x = saved[0], &weight = saved[1], &target = saved[2], &bias = saved[3], &state = saved[4];
         const auto ints = ctx->saved_data["ints"].toIntVector();
-        const int dev = x.device().index();
+        const at::Device device(c10::DeviceType::PrivateUse1, static_cast<at::DeviceIndex>(ints[11]));
+        const int64_t rows = ints[6], cols = ints[7], vocab = ints[8];
+        const at::ScalarType type = static_cast<at::ScalarType>(ints[10]);
+        const auto again = [&](int i, const char* name, at::ScalarType t, at::IntArrayRef shape) {
+            return restored(saved[i], device, t, shape, "linear_cross_entropy", name);
+        };
+        const at::Tensor x = again(0, "x", type, {rows, cols}), weight = again(1, "weight", type, {vocab, cols}),
+                         target = again(2, "target", at::kLong, rows), bias = ints[5] ? again(3, "bias", type, vocab) : at::Tensor(),
+                         state = again(4, "state", at::kByte, ints[9]);
+        const int dev = device.index();
         DeviceScope g(dev);
         const at::Tensor grad = grads[0].contiguous();
         if (ints[2]) out[0] = fresh(x.sizes(), x.scalar_type());
