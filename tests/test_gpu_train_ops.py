@@ -439,3 +439,37 @@ def test_residual_norm_saved_tensors_come_back_strided_or_from_the_host(kind, po
             got = run_norm(t, kind, post, 1.0, 0.2, gx, gh)
         for k in want:
             assert torch.equal(got[k], want[k]), k
+
+
+@pytest.mark.parametrize("call", ["norm with a channel gate", "norm with a sample gate", "norm with a token gate", "loss"])
+def test_train_ops_form_the_gradients_that_are_asked_for(call):
+    """autograd.grad for some of the inputs that require gradients: the others'
+    are not even allocated, and those asked for are the same."""
+    if call != "loss":
+        t = norm_inputs((2, 512, 4096), F16, "layer", True, call.split()[3], 1)
+        g = rnd((2, 512, 4096), 9).to(DEV)
+        large = "f"
+    else:
+        t = {"x": rnd((8, 256), 1), "weight": rnd((60000, 256), 2, F16, 0.1), "bias": rnd((60000,), 3)}
+        target, g = torch.arange(8).to(DEV), torch.tensor(64.0).to(DEV)
+        large = "weight"
+
+    def peak(names):
+        dev = {k: v.to(DEV).requires_grad_() for k, v in t.items()}
+        if call != "loss":
+            y = ops.residual_norm(dev["x"], dev["f"], post_norm=True, p=0.1, seed=5, **{k: dev[k] for k in t if k not in ("x", "f")})[1]
+        else:
+            y = ops.linear_cross_entropy(dev["x"], dev["weight"], target, dev["bias"])
+        kunlun.synchronize()
+        kunlun.reset_peak_memory_stats()
+        before = kunlun.memory_allocated()
+        grads = torch.autograd.grad(y, [dev[k] for k in names], g)
+        kunlun.synchronize()
+        return kunlun.max_memory_allocated() - before, dict(zip(names, (v.cpu() for v in grads)))
+
+    whole, every = peak(list(t))
+    for names in [[k] for k in t if k != large] + [[k for k in t if k != large]]:
+        part, some = peak(names)
+        assert whole - part >= t[large].numel() * 2, names
+        for k in names:
+            assert torch.equal(some[k], every[k]), k

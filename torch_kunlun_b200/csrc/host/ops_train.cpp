@@ -73,6 +73,16 @@ at::Tensor restored(const at::Tensor& t, at::Device device, at::ScalarType type,
     return t.contiguous();
 }
 
+// The tensor inputs, of those in `given`, whose gradients this backward pass has
+// been asked for (an input that requires none, or that autograd.grad leaves out,
+// is not).
+unsigned wanted_gradients(AutogradContext* ctx, unsigned given) {
+    unsigned wanted = 0;
+    for (size_t i = 0, edge = 0; given >> i != 0; ++i)
+        if (given >> i & 1u) wanted |= (ctx->needs_input_grad(edge++) ? 1u : 0u) << i;
+    return wanted;
+}
+
 // A contiguous tensor on the current device, allocated without a trip through
 // the dispatcher: these ops allocate up to nine tensors a call.
 at::Tensor fresh(at::IntArrayRef shape, at::ScalarType type) {
@@ -174,15 +184,11 @@ struct ResidualNorm : torch::autograd::Function<ResidualNorm> {
         }
         auto [x_new, h] = norm_run(x, f, weight, bias, post_weight, post_bias, gate, o, stats);
         ctx->save_for_backward({x, f, weight, post_weight, post_bias, gate, stats});
-        // a bit for each tensor given, and for each that wants a gradient
-        int64_t given = 0, wanted = 0;
+        int64_t given = 0;  // a bit for each tensor
         const at::Tensor* const inputs[7] = {&x, &f, &weight, &bias, &post_weight, &post_bias, &gate};
-        for (int i = 0; i < 7; ++i) {
-            if (!inputs[i]->defined()) continue;
-            given |= 1 << i;
-            if (inputs[i]->requires_grad()) wanted |= 1 << i;
-        }
-        std::vector<int64_t> ints = {o.rms, o.post, o.seed, o.offset, given, wanted, static_cast<int64_t>(x.scalar_type()), x.device().index(), x.dim()};
+        for (int i = 0; i < 7; ++i)
+            if (inputs[i]->defined()) given |= 1 << i;
+        std::vector<int64_t> ints = {o.rms, o.post, o.seed, o.offset, given, static_cast<int64_t>(x.scalar_type()), x.device().index(), x.dim()};
         ints.insert(ints.end(), x.sizes().begin(), x.sizes().end());
         if (gate.defined()) ints.insert(ints.end(), gate.sizes().begin(), gate.sizes().end());
         ctx->saved_data["ints"] = std::move(ints);
@@ -201,10 +207,11 @@ struct ResidualNorm : torch::autograd::Function<ResidualNorm> {
         const auto real = ctx->saved_data["reals"].toDoubleVector();
         const NormOptions o = {ints[0] != 0, ints[1] != 0, real[0], real[1], real[2], ints[2], ints[3]};
         const auto given = [&](int i) { return (ints[4] >> i & 1) != 0; };
-        const auto wanted = [&](int i) { return (ints[5] >> i & 1) != 0; };
-        const at::ScalarType type = static_cast<at::ScalarType>(ints[6]);
-        const at::Device device(c10::DeviceType::PrivateUse1, static_cast<at::DeviceIndex>(ints[7]));
-        const at::IntArrayRef shapes = at::IntArrayRef(ints).slice(9), sizes = shapes.slice(0, ints[8]), gate_sizes = shapes.slice(ints[8]);
+        const unsigned wanted = wanted_gradients(ctx, static_cast<unsigned>(ints[4]));
+        if (wanted == 0) return out;
+        const at::ScalarType type = static_cast<at::ScalarType>(ints[5]);
+        const at::Device device(c10::DeviceType::PrivateUse1, static_cast<at::DeviceIndex>(ints[6]));
+        const at::IntArrayRef shapes = at::IntArrayRef(ints).slice(8), sizes = shapes.slice(0, ints[7]), gate_sizes = shapes.slice(ints[7]);
         const int64_t cols = sizes.back(), rows = c10::multiply_integers(sizes) / cols;
         const auto again = [&](int i, const char* name, at::IntArrayRef shape) { return restored(saved[i], device, type, shape, "residual_norm", name); };
         const at::Tensor x = again(0, "x", sizes), f = again(1, "f", sizes),
@@ -217,13 +224,13 @@ struct ResidualNorm : torch::autograd::Function<ResidualNorm> {
         if (gh.defined()) gh = gh.contiguous();
         const int dev = device.index();
         DeviceScope g(dev);
-        if (wanted(0)) out[0] = fresh(x.sizes(), type);
-        if (wanted(1)) out[1] = fresh(x.sizes(), type);
-        if (wanted(2)) out[2] = fresh({cols}, type);
-        if (wanted(3)) out[3] = fresh({cols}, type);
-        if (wanted(4)) out[4] = fresh({cols}, type);
-        if (wanted(5)) out[5] = fresh({cols}, type);
-        if (wanted(6)) out[6] = fresh(gate.sizes(), type);
+        if (wanted >> 0 & 1) out[0] = fresh(x.sizes(), type);
+        if (wanted >> 1 & 1) out[1] = fresh(x.sizes(), type);
+        if (wanted >> 2 & 1) out[2] = fresh({cols}, type);
+        if (wanted >> 3 & 1) out[3] = fresh({cols}, type);
+        if (wanted >> 4 & 1) out[4] = fresh({cols}, type);
+        if (wanted >> 5 & 1) out[5] = fresh({cols}, type);
+        if (wanted >> 6 & 1) out[6] = fresh(gate.sizes(), type);
         tk_residual_norm_grad_desc_t d = {};
         d.fwd = norm_desc(x, o, weight, post_weight, post_bias, gate);
         d.fwd.x = ptr(x);
@@ -289,9 +296,8 @@ struct LinearCrossEntropy : torch::autograd::Function<LinearCrossEntropy> {
         at::Tensor state;
         at::Tensor loss = ce_run(ce_desc(x, weight, target, bias, ignore_index, reduction), x, &state);
         ctx->save_for_backward({x, weight, target, bias, state});
-        ctx->saved_data["ints"] = std::vector<int64_t>{ignore_index, reduction, x.requires_grad(), weight.requires_grad(),
-                                                       bias.defined() && bias.requires_grad(), bias.defined(), x.size(0), x.size(1), weight.size(0),
-                                                       state.numel(), static_cast<int64_t>(x.scalar_type()), x.device().index()};
+        ctx->saved_data["ints"] = std::vector<int64_t>{ignore_index, reduction, bias.defined(), x.size(0), x.size(1), weight.size(0), state.numel(),
+                                                       static_cast<int64_t>(x.scalar_type()), x.device().index()};
         ctx->set_materialize_grads(false);
         return loss;
     }
@@ -302,21 +308,23 @@ struct LinearCrossEntropy : torch::autograd::Function<LinearCrossEntropy> {
         if (!grads[0].defined()) return out;
         const variable_list saved = ctx->get_saved_variables();
         const auto ints = ctx->saved_data["ints"].toIntVector();
-        const at::Device device(c10::DeviceType::PrivateUse1, static_cast<at::DeviceIndex>(ints[11]));
-        const int64_t rows = ints[6], cols = ints[7], vocab = ints[8];
-        const at::ScalarType type = static_cast<at::ScalarType>(ints[10]);
+        const unsigned wanted = wanted_gradients(ctx, ints[2] ? 0b1111u : 0b111u);  // x, weight, target, bias
+        if (wanted == 0) return out;
+        const int64_t rows = ints[3], cols = ints[4], vocab = ints[5];
+        const at::ScalarType type = static_cast<at::ScalarType>(ints[7]);
+        const at::Device device(c10::DeviceType::PrivateUse1, static_cast<at::DeviceIndex>(ints[8]));
         const auto again = [&](int i, const char* name, at::ScalarType t, at::IntArrayRef shape) {
             return restored(saved[i], device, t, shape, "linear_cross_entropy", name);
         };
         const at::Tensor x = again(0, "x", type, {rows, cols}), weight = again(1, "weight", type, {vocab, cols}),
-                         target = again(2, "target", at::kLong, rows), bias = ints[5] ? again(3, "bias", type, vocab) : at::Tensor(),
-                         state = again(4, "state", at::kByte, ints[9]);
+                         target = again(2, "target", at::kLong, rows), bias = ints[2] ? again(3, "bias", type, vocab) : at::Tensor(),
+                         state = again(4, "state", at::kByte, ints[6]);
         const int dev = device.index();
         DeviceScope g(dev);
         const at::Tensor grad = grads[0].contiguous();
-        if (ints[2]) out[0] = fresh(x.sizes(), x.scalar_type());
-        if (ints[3]) out[1] = fresh(weight.sizes(), x.scalar_type());
-        if (ints[4]) out[3] = fresh(bias.sizes(), x.scalar_type());
+        if (wanted & 1u) out[0] = fresh(x.sizes(), type);
+        if (wanted & 2u) out[1] = fresh(weight.sizes(), type);
+        if (wanted & 8u) out[3] = fresh(bias.sizes(), type);
         tk_linear_ce_grad_desc_t d = {};
         d.fwd = ce_desc(x, weight, target, bias, ints[0], ints[1]);
         d.fwd.state = state.data_ptr();
