@@ -504,8 +504,10 @@ typedef struct {
                   * backward pass needs; NULL where there is none */
 } tk_linear_ce_desc_t;
 
-/* The state's size and layout follow from dtype, rows, cols and vocab alone, so
- * the backward pass may be given the weight at another address.  The workspace
+/* The state holds x's listed rows as binary16 planes (room for all rows) and
+ * three words per row, the bias, and where dtype is fp32 or cols % 8 != 0 the weight as
+ * planes too.  Its size and layout follow from dtype, rows, cols and vocab alone,
+ * so the backward pass may be given the weight at another address.  The workspace
  * sizes also go by weight's address: an fp16 weight of cols % 8 == 0 off a
  * 16-byte boundary is packed into the workspace of each pass. */
 TK_API size_t tk_linear_ce_state_size(const tk_linear_ce_desc_t* desc);
@@ -513,8 +515,8 @@ TK_API size_t tk_linear_ce_workspace_size(const tk_linear_ce_desc_t* desc);
 TK_API int tk_linear_ce(const tk_linear_ce_desc_t* desc, void* workspace, size_t workspace_bytes,
                         void* stream);
 
-/* Its gradients: fwd is the forward call's descriptor with its state (loss is
- * not read), grad_loss the gradient of the loss ([rows] or one value).  dx
+/* Its gradients: fwd is the forward call's descriptor with its state (x and loss
+ * are not read: the state holds x's rows), grad_loss the gradient of the loss ([rows] or one value).  dx
  * [rows, cols], dweight [vocab, cols] and dbias [vocab] may be NULL.  The
  * logits are computed again in pieces of the vocabulary; softmax - onehot is
  * held as binary16 (two planes for fp32), so each of its entries is known to

@@ -484,3 +484,29 @@ def test_linear_ce_non_finite_row_gradients_stay_in_their_rows(dtype):
 def test_linear_ce_row_gradients_over_several_pieces():
     t, target = ce_inputs(14000, 72, 20003, F16, True, 14000 // 3, seed=44)
     check_ce(t, target, "none", loss_grad(14000, "none") * 64)
+
+
+@pytest.mark.parametrize("d", [1024, 1000, 1001])
+def test_linear_ce_holds_its_input_once(d):
+    # from forward to backward: the state, which has x's rows, and not x besides
+    t, target = ce_inputs(4096, d, 300, F16, False, 500, seed=51)
+    w, tg = t["weight"].to(DEV).requires_grad_(), target.to(DEV)
+    kunlun.synchronize()
+    before = kunlun.memory_allocated()
+    loss = ops.linear_cross_entropy(t["x"].to(DEV), w, tg)
+    kunlun.synchronize()
+    f = _capi.LinearCeDesc()
+    f.dtype, f.rows, f.cols, f.vocab, f.reduction = 0, 4096, d, 300, 1
+    assert kunlun.memory_allocated() - before <= _capi.lib().tk_linear_ce_state_size(ctypes.byref(f)) + (1 << 20)
+    got, = torch.autograd.grad(loss, w, torch.tensor(64.0).to(DEV))
+    assert torch.equal(got.cpu(), run_ce(t, target, "mean", torch.tensor(64.0))["weight"])
+
+
+def test_linear_ce_input_changed_after_the_forward_pass():
+    t, target = ce_inputs(50, 64, 200, F16, True, 5, seed=52)
+    want = run_ce(t, target, "mean", torch.tensor(64.0))
+    dev = {k: v.to(DEV).requires_grad_(k != "x") for k, v in t.items()}
+    loss = ops.linear_cross_entropy(dev["x"], dev["weight"], target.to(DEV), dev["bias"])
+    dev["x"].zero_()
+    got = torch.autograd.grad(loss, [dev["weight"], dev["bias"]], torch.tensor(64.0).to(DEV))
+    assert torch.equal(got[0].cpu(), want["weight"]) and torch.equal(got[1].cpu(), want["bias"])

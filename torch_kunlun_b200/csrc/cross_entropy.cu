@@ -1650,7 +1650,7 @@ int tk_linear_ce_backward(const tk_linear_ce_grad_desc_t* desc, void* workspace,
         if (desc->dbias) TK_CUDA_TRY(cudaMemsetAsync(desc->dbias, 0, static_cast<size_t>(d.vocab) * dtype_size(d.dtype), s));
         return TK_OK;
     }
-    TK_CHECK_ARG(d.x && d.weight && d.target && d.state && desc->grad_loss, "tk_linear_ce_backward: NULL pointer");
+    TK_CHECK_ARG(d.weight && d.target && d.state && desc->grad_loss, "tk_linear_ce_backward: NULL pointer");
     TK_CHECK_ARG((reinterpret_cast<uintptr_t>(d.state) & 15) == 0, "tk_linear_ce_backward: state must be 16-byte aligned");
     const Plan p = make_plan(d);
     if (workspace == nullptr || workspace_bytes < p.bwd_bytes || (reinterpret_cast<uintptr_t>(workspace) & 1023) != 0)

@@ -258,9 +258,9 @@ struct ResidualNorm : torch::autograd::Function<ResidualNorm> {
 tk_linear_ce_desc_t ce_desc(const at::Tensor& x, const at::Tensor& weight, const at::Tensor& target, const at::Tensor& bias,
                             int64_t ignore_index, int64_t reduction) {
     tk_linear_ce_desc_t d = {};
-    d.dtype = tk_dtype(x.scalar_type());
-    d.rows = x.size(0);
-    d.cols = x.size(1);
+    d.dtype = tk_dtype(weight.scalar_type());
+    d.rows = target.size(0);
+    d.cols = weight.size(1);
     d.vocab = weight.size(0);
     d.x = ptr(x);
     d.weight = ptr(weight);
@@ -295,7 +295,7 @@ struct LinearCrossEntropy : torch::autograd::Function<LinearCrossEntropy> {
         const at::Tensor bias = or_undefined(bias_in);
         at::Tensor state;
         at::Tensor loss = ce_run(ce_desc(x, weight, target, bias, ignore_index, reduction), x, &state);
-        ctx->save_for_backward({x, weight, target, bias, state});
+        ctx->save_for_backward({weight, target, bias, state});  // the state holds x's rows
         ctx->saved_data["ints"] = std::vector<int64_t>{ignore_index, reduction, bias.defined(), x.size(0), x.size(1), weight.size(0), state.numel(),
                                                        static_cast<int64_t>(x.scalar_type()), x.device().index()};
         ctx->set_materialize_grads(false);
@@ -316,17 +316,16 @@ struct LinearCrossEntropy : torch::autograd::Function<LinearCrossEntropy> {
         const auto again = [&](int i, const char* name, at::ScalarType t, at::IntArrayRef shape) {
             return restored(saved[i], device, t, shape, "linear_cross_entropy", name);
         };
-        const at::Tensor x = again(0, "x", type, {rows, cols}), weight = again(1, "weight", type, {vocab, cols}),
-                         target = again(2, "target", at::kLong, rows), bias = ints[2] ? again(3, "bias", type, vocab) : at::Tensor(),
-                         state = again(4, "state", at::kByte, ints[6]);
+        const at::Tensor weight = again(0, "weight", type, {vocab, cols}), target = again(1, "target", at::kLong, rows),
+                         bias = ints[2] ? again(2, "bias", type, vocab) : at::Tensor(), state = again(3, "state", at::kByte, ints[6]);
         const int dev = device.index();
         DeviceScope g(dev);
         const at::Tensor grad = grads[0].contiguous();
-        if (wanted & 1u) out[0] = fresh(x.sizes(), type);
+        if (wanted & 1u) out[0] = fresh({rows, cols}, type);
         if (wanted & 2u) out[1] = fresh(weight.sizes(), type);
         if (wanted & 8u) out[3] = fresh(bias.sizes(), type);
         tk_linear_ce_grad_desc_t d = {};
-        d.fwd = ce_desc(x, weight, target, bias, ints[0], ints[1]);
+        d.fwd = ce_desc(at::Tensor(), weight, target, bias, ints[0], ints[1]);
         d.fwd.state = state.data_ptr();
         d.grad_loss = grad.numel() > 0 ? grad.data_ptr<float>() : nullptr;
         d.dx = ptr(out[0]);
