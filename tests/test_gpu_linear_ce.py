@@ -510,3 +510,42 @@ def test_linear_ce_input_changed_after_the_forward_pass():
     dev["x"].zero_()
     got = torch.autograd.grad(loss, [dev["weight"], dev["bias"]], torch.tensor(64.0).to(DEV))
     assert torch.equal(got[0].cpu(), want["weight"]) and torch.equal(got[1].cpu(), want["bias"])
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("d,v", [(64, 300), (512, 1000), (768, 5003), (2048, 700)])
+def test_linear_ce_of_rows_whose_target_dominates(dtype, d, v):
+    """Target logits of 5 to 500 far above the others: no loss is negative, and a
+    small one is as exact as its logits' differences, whatever their size."""
+    n = 200
+    t, target = ce_inputs(n, d, v, dtype, True, seed=d + v)
+    w = t["weight"].double()[target]
+    size = 10.0 ** torch.linspace(0.7, 2.7, n, dtype=torch.float64)
+    t["x"] = (size[:, None] * w / w.square().sum(1, keepdim=True)).to(dtype)
+    X, W = t["x"].double(), t["weight"].double()
+    z = X @ W.T + t["bias"].double()
+    hit = z.gather(1, target[:, None])
+    want = torch.log1p((z - hit).exp().scatter(1, target[:, None], 0.0).sum(1))
+    assert (want < 1e-6).sum() > 20 and (want > 1e-3).any()
+    # a logit's error: each step of 16 (three products for fp32) cut to binary32, the planes' 2^-20, the bias
+    mag = X.abs() @ W.abs().T + t["bias"].double().abs()
+    e = ((d * (1 if dtype == F16 else 3) / 16 + 16) * 2.0 ** -23 + (0 if dtype == F16 else 2.0 ** -20)) * mag
+    e = e.amax(1) + e.gather(1, target[:, None])[:, 0]
+    # the others' exponentials move by the differences' errors, and 2^-18 for exponentials and logarithm; the sum, the
+    # target's 1 among its terms, is rounded at each of 32 additions in a row and then 32 + v / 2048 joins: a half
+    # step, 2^-24, each, whatever the loss
+    for reduction in ("none", "sum"):
+        got = run_ce(t, target, reduction)["loss"]
+        assert (got >= 0).all()
+        value, bound = (want, want * (torch.expm1(e) + 2.0 ** -18) + (64 + v / 2048) * 2.0 ** -24)
+        if reduction == "sum":
+            value, bound = value.sum(), bound.sum()
+        R.assert_within(got, value, bound, f"loss {reduction}")
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+def test_linear_ce_of_one_word_is_zero(dtype):
+    t, target = ce_inputs(300, 72, 1, dtype, True, seed=3)
+    t["x"] *= 50
+    got = run_ce(t, target, "none", torch.ones(300))
+    assert not got["loss"].any()

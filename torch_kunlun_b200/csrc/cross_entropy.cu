@@ -9,8 +9,11 @@
 // its row count from that list on the device.
 //
 // Forward: one tcgen05 GEMM whose epilogue keeps, per row and 128 columns,
-// the maximum and the sum of exponentials (base 2); a small kernel joins them
-// and computes the target's logit as a dot product of its own.  Backward: the
+// the maximum and the sum of exponentials (base 2), and the target's logit; a
+// small kernel joins them.  logsumexp and the target's logit carry the same
+// rounding, so no loss is negative and that of a row whose target dominates is
+// not lost in it (with a dot product of its own for the target, 512 columns and
+// logits of 500 gave losses of -2.7e-3).  Backward: the
 // vocabulary is taken in pieces whose dz fits a workspace; per piece the
 // logits are computed again, the epilogue stores dz as binary16, and two
 // GEMMs read it in place (dz and x^T / W^T in MN-major shared-memory tiles, so
@@ -133,6 +136,7 @@ struct GemmParams {
     int64_t vocab0, vocab;  // the piece's first column, all columns
     const float* bias2;  // bias * log2(e), or NULL
     float2* part;        // [rows][n_tiles][BN / COLS] maximum and sum
+    float* hit2;         // kStats: the target's logit, base 2
     const float* lse2;
     const float* grow;   // kDlogits, kGradX: g_i; NULL: one for all rows
     const int* target;
@@ -593,10 +597,10 @@ ce_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
             const int64_t m = m0 + lane;
             const int64_t col0 = static_cast<int64_t>(nt) * BN + share * COLS;
             float top = -INFINITY, sum = 0.0f;  // kStats
-            const bool live = m < rows;         // kDlogits
+            const bool live = m < rows;         // kStats, kDlogits
             const float lse = EPI == kDlogits && live ? p.lse2[m] : 0.0f;
             const float g = EPI == kDlogits && live ? (p.grow != nullptr ? mantissa_of(p.grow[m]) * kDzScale : kDzScale) : 0.0f;
-            const int64_t hit = EPI == kDlogits && live ? p.target[m] - p.vocab0 : -1;
+            const int64_t hit = (EPI == kStats || EPI == kDlogits) && live ? p.target[m] - p.vocab0 : -1;
             // rows that the warp works for: dz is read (as K) up to a multiple of BK
             const int64_t limit = EPI == kGradW ? p.out_rows : EPI == kDlogits ? (rows + BK - 1) / BK * BK : rows;
             const bool idle = m0 >= limit;
@@ -606,6 +610,13 @@ ce_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
                 if constexpr (EPI == kStats) {
                     float y[32];
                     logits2(acc, scale, p.bias2, col, p.vocab, y);
+                    if (hit >= col && hit < col + 32) {
+                        const int j = static_cast<int>(hit - col);
+                        float h = y[0];
+#pragma unroll
+                        for (int i = 1; i < 32; ++i) h = i == j ? y[i] : h;
+                        p.hit2[m] = h;
+                    }
                     float cm = y[0];
 #pragma unroll
                     for (int i = 1; i < 32; ++i) cm = fmaxf(cm, y[i]);
@@ -1077,64 +1088,31 @@ ce_list_pack_kernel(const int64_t* target, int rows, int64_t vocab, int64_t igno
 }
 static_assert(kListRows == 32 * 32, "one warp sums the spans");
 
-// This lane's part of the dot product of two rows, in one order however the
-// rows are aligned.
-template <typename T>
-__device__ __forceinline__ float dot_lane(const T* a, const T* b, int64_t n, int lane, bool vec) {
-    constexpr int V = 16 / sizeof(T);
-    float s[4] = {};
-#pragma unroll 4
-    for (int64_t c = lane * V; c < n; c += 32 * V) {
-        alignas(16) T x[V];
-        alignas(16) T y[V];
-        if (vec) {  // both rows 16-byte aligned, n a multiple of V
-            *reinterpret_cast<uint4*>(x) = *reinterpret_cast<const uint4*>(a + c);
-            *reinterpret_cast<uint4*>(y) = *reinterpret_cast<const uint4*>(b + c);
-        } else {
-#pragma unroll
-            for (int i = 0; i < V; ++i) {
-                x[i] = c + i < n ? a[c + i] : T(0.0f);
-                y[i] = c + i < n ? b[c + i] : T(0.0f);
-            }
-        }
-#pragma unroll
-        for (int i = 0; i < V; ++i) s[i % 4] = fmaf(load_f(x, i), load_f(y, i), s[i % 4]);
-    }
-    return (s[0] + s[1]) + (s[2] + s[3]);
-}
-
 constexpr int kRowWarps = 8;
 
-// A warp joins the statistics of a row, computes its target's logit and forms
-// its loss: lse2 (base 2) for the backward pass, the loss per packed row, and
-// per row where asked for.  The block that finishes last adds the losses of
+// A warp joins the statistics of a row and forms its loss: lse2 (base 2) for the
+// backward pass, the loss per packed row, and per row where asked for.  The block that finishes last adds the losses of
 // all rows, in a fixed order.
-template <typename T>
 __global__ void __launch_bounds__(32 * kRowWarps)
-ce_rows_kernel(const T* x, const T* w, const T* bias, const int* index, const int* target, Scalars* sc, const float2* part,
-               int parts, int64_t cols, bool vec, float* lse2, float* loss, int reduction, float* out) {
+ce_rows_kernel(const int* index, const int* target, Scalars* sc, const float2* part, int parts, const float* hit2, float* lse2, float* loss, int reduction,
+               float* out) {
     pdl_wait();
     const int rows = sc->count;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     for (int m = blockIdx.x * kRowWarps + warp; m < rows; m += gridDim.x * kRowWarps) {
-        const int t = target[m], r = index[m];
         float top = -INFINITY, sum = 0.0f;
         const float2* row = part + static_cast<int64_t>(m) * parts;
 #pragma unroll 4
         for (int i = lane; i < parts; i += 32) join(top, sum, row[i].x, row[i].y);
-        float hit = t >= 0 ? dot_lane(x + r * cols, w + t * cols, cols, lane, vec) : 0.0f;
 #pragma unroll
-        for (int k = 16; k > 0; k >>= 1) {
-            join(top, sum, __shfl_xor_sync(0xFFFFFFFFu, top, k), __shfl_xor_sync(0xFFFFFFFFu, sum, k));
-            hit += __shfl_xor_sync(0xFFFFFFFFu, hit, k);
-        }
+        for (int k = 16; k > 0; k >>= 1) join(top, sum, __shfl_xor_sync(0xFFFFFFFFu, top, k), __shfl_xor_sync(0xFFFFFFFFu, sum, k));
         if (lane == 0) {
-            if (bias != nullptr && t >= 0) hit += load_f(bias, t);
-            const float l2 = top + log2f(sum);
-            const float v = t >= 0 ? l2 * kLn2 - hit : NAN;
-            lse2[m] = t >= 0 ? l2 : NAN;
+            // top >= hit2 and sum >= 1: the loss is never negative
+            const bool inside = target[m] >= 0;
+            const float l2 = log2f(sum), v = inside ? (top - hit2[m] + l2) * kLn2 : NAN;
+            lse2[m] = inside ? top + l2 : NAN;
             loss[m] = v;
-            if (reduction == TK_REDUCE_NONE) out[r] = v;
+            if (reduction == TK_REDUCE_NONE) out[index[m]] = v;
         }
     }
     if (reduction == TK_REDUCE_NONE) return;
@@ -1341,7 +1319,7 @@ struct Plan {
     // state: kept from the forward to the backward pass
     size_t s_scalars, s_index, s_target, s_lse, s_x, s_bias, s_w, state_bytes;
     // workspaces
-    size_t w_part, w_loss, w_w, fwd_bytes;
+    size_t w_part, w_hit, w_loss, w_w, fwd_bytes;
     size_t b_scalars, b_grow, b_dz, b_acc, b_split, b_db, b_w, b_x, bwd_bytes;
 };
 
@@ -1406,6 +1384,7 @@ Plan make_plan(const tk_linear_ce_desc_t& d) {
     at = 0;
     p.parts = stats_parts(p.planes, d.cols) * p.n_tiles;
     p.w_part = take(static_cast<size_t>(p.parts) * p.rows_pad * sizeof(float2));
+    p.w_hit = take(p.rows_pad * sizeof(float));
     p.w_loss = take(p.rows_pad * sizeof(float));
     p.w_w = take(p.w_kept || p.w_direct ? 0 : w_bytes);
     p.fwd_bytes = at + p.state_bytes;  // a call without a state keeps its own
@@ -1548,14 +1527,11 @@ int list_and_pack(const tk_linear_ce_desc_t& d, const Plan& p, uint8_t* st, uint
                         s, jx, jw, static_cast<const Scalars*>(sc), x_blocks, w_blocks, bias, bias2);
 }
 
-template <typename T>
 int rows_loss(const tk_linear_ce_desc_t& d, const Plan& p, uint8_t* st, uint8_t* ws, cudaStream_t s) {
     const int grid = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(ceil_div(d.rows, kRowWarps), 148 * 8)));
-    const bool vec = d.cols * sizeof(T) % 16 == 0 && ((reinterpret_cast<uintptr_t>(d.x) | reinterpret_cast<uintptr_t>(d.weight)) & 15) == 0;
-    return launch_chain("cross entropy rows", ce_rows_kernel<T>, dim3(grid), dim3(32 * kRowWarps), 0, s, static_cast<const T*>(d.x),
-                        static_cast<const T*>(d.weight), static_cast<const T*>(d.bias), reinterpret_cast<const int*>(st + p.s_index),
+    return launch_chain("cross entropy rows", ce_rows_kernel, dim3(grid), dim3(32 * kRowWarps), 0, s, reinterpret_cast<const int*>(st + p.s_index),
                         reinterpret_cast<const int*>(st + p.s_target), reinterpret_cast<Scalars*>(st + p.s_scalars),
-                        reinterpret_cast<const float2*>(ws + p.w_part), static_cast<int>(p.parts), d.cols, vec,
+                        reinterpret_cast<const float2*>(ws + p.w_part), static_cast<int>(p.parts), reinterpret_cast<const float*>(ws + p.w_hit),
                         reinterpret_cast<float*>(st + p.s_lse), reinterpret_cast<float*>(ws + p.w_loss), static_cast<int>(d.reduction), d.loss);
 }
 
@@ -1627,9 +1603,11 @@ int tk_linear_ce(const tk_linear_ce_desc_t* desc, void* workspace, size_t worksp
         GemmParams g = base_params(d, p, st);
         g.n_tiles = static_cast<int>(p.n_tiles);
         g.part = reinterpret_cast<float2*>(ws + p.w_part);
+        g.hit2 = reinterpret_cast<float*>(ws + p.w_hit);
+        g.target = reinterpret_cast<const int*>(st + p.s_target);
         CE_TRY(gemm<kStats>(tx, tw, g, p.n_tiles * ceil_div(d.rows, BM), s));
     }
-    if (d.rows > 0 || d.reduction != TK_REDUCE_NONE) CE_TRY(p.f16 ? rows_loss<__half>(d, p, st, ws, s) : rows_loss<float>(d, p, st, ws, s));
+    if (d.rows > 0 || d.reduction != TK_REDUCE_NONE) CE_TRY(rows_loss(d, p, st, ws, s));
     return TK_OK;
 }
 
