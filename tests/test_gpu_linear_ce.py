@@ -549,3 +549,33 @@ def test_linear_ce_of_one_word_is_zero(dtype):
     t["x"] *= 50
     got = run_ce(t, target, "none", torch.ones(300))
     assert not got["loss"].any()
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("d,v", [(64, 300), (768, 5003), (1032, 300), (1500, 777), (4096, 700)])
+def test_linear_ce_gradient_of_rows_whose_target_dominates(dtype, d, v):
+    """The softmax of the backward pass is that of the forward pass's logits: where
+    the target has all of it, its entry of dz is zero up to logsumexp's rounding,
+    however large the logits."""
+    n = 100
+    t, target = ce_inputs(n, d, v, dtype, False, seed=d + v)
+    w = t["weight"].double()[target]
+    size = 10.0 ** torch.linspace(1.7, 2.7, n, dtype=torch.float64)
+    t["x"] = (size[:, None] * w / w.square().sum(1, keepdim=True)).to(dtype)
+    X, W = t["x"].double(), t["weight"].double()
+    z = X @ W.T
+    lse = torch.logsumexp(z, 1)
+    dz = (z - lse[:, None]).exp()
+    hit = z.gather(1, target[:, None])
+    rest = (z - hit).exp().scatter(1, target[:, None], 0.0).sum(1, keepdim=True)
+    dz.scatter_(1, target[:, None], -rest / (1 + rest))
+    others = dz.scatter(1, target[:, None], 0.0).abs()
+    assert (others < 1e-6).all()
+    # the target's entry: logsumexp / ln 2 and its difference from the logit are rounded (a half step, 2^-24, each) and
+    # held to the sum's 64 + v / 2048 half steps, the exponential to 2^-22; the others' are below 1e-6 and 1 % exact
+    e_hit = 2.0 ** -23 * (lse.abs() / 0.6931 + 64 + v / 2048) + 2.0 ** -22
+    e_dz = (0.01 * others + 2.0 ** -39).scatter(1, target[:, None], e_hit[:, None])
+    value = dz @ W
+    bound = e_dz @ W.abs() + (d + v) * 2.0 ** -23 * (dz.abs() @ W.abs()) + R.ulp(value, dtype)
+    got = run_ce(t, target, "sum", torch.tensor(1.0), wanted=("x",))["x"]
+    R.assert_within(got, value, bound, "x")
