@@ -485,7 +485,8 @@ TK_API int tk_residual_norm_backward(const tk_residual_norm_grad_desc_t* desc, v
  * and the gradients NaN.  reduction: one loss per row, or their mean over the
  * rows with a target (NaN without any) or sum.  Losses are fp32.  fp16
  * products are exact and summed in fp32; fp32 operands enter as two binary16
- * planes each (22 bits, or 2^-40 of the tensor's largest value).  Sizes below
+ * planes each (22 bits, or 2^-40 of the largest value of weight, or of the row
+ * of x: rows do not touch one another's losses).  Sizes below
  * 2^31 - 256, and no product of more than 2^30 tiles of 256 x 256.  A loss
  * beside mse_loss; the reference has none of this kind. */
 typedef enum { TK_REDUCE_NONE = 0, TK_REDUCE_MEAN = 1, TK_REDUCE_SUM = 2 } tk_reduction_t;
@@ -505,8 +506,8 @@ typedef struct {
 } tk_linear_ce_desc_t;
 
 /* The state holds x's listed rows as binary16 planes (room for all rows) and
- * three words per row, the bias, and where dtype is fp32 or cols % 8 != 0 the weight as
- * planes too.  Its size and layout follow from dtype, rows, cols and vocab alone,
+ * four words per row, the bias, and where dtype is fp32 or cols % 8 != 0 the
+ * weight as planes too.  Its size and layout follow from dtype, rows, cols and vocab alone,
  * so the backward pass may be given the weight at another address.  The workspace
  * sizes also go by weight's address: an fp16 weight of cols % 8 == 0 off a
  * 16-byte boundary is packed into the workspace of each pass. */

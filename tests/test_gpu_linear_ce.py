@@ -579,3 +579,33 @@ def test_linear_ce_gradient_of_rows_whose_target_dominates(dtype, d, v):
     bound = e_dz @ W.abs() + (d + v) * 2.0 ** -23 * (dz.abs() @ W.abs()) + R.ulp(value, dtype)
     got = run_ce(t, target, "sum", torch.tensor(1.0), wanted=("x",))["x"]
     R.assert_within(got, value, bound, "x")
+
+
+@pytest.mark.parametrize("dtype,size", [(F16, 2.0 ** 13), (F32, 2.0 ** 40), (F32, 2.0 ** 100)])
+def test_linear_ce_a_far_larger_row_leaves_the_others_alone(dtype, size):
+    """The losses and gradients of rows do not depend on another row's size, as
+    padding that the caller weighs with zero may have any."""
+    n = 60
+    t, target = ce_inputs(n, 72, 500, dtype, True, 5, seed=61)
+    at = int((target != -100).nonzero()[3])
+    rest = torch.arange(n) != at
+    g = loss_grad(n, "none")
+    g[at] = 0
+    t["x"][at] = t["x"][at].clamp(-1, 1)
+    want = run_ce(t, target, "none", g)
+    t["x"][at] *= size
+    got = run_ce(t, target, "none", g)
+    assert torch.equal(got["loss"][rest], want["loss"][rest]) and torch.equal(got["x"][rest], want["x"][rest])
+    assert torch.equal(got["weight"], want["weight"]) and torch.equal(got["bias"], want["bias"])
+    t["x"][at] = torch.finfo(dtype).min
+    got = run_ce(t, target, "none", g)
+    assert torch.equal(got["loss"][rest], want["loss"][rest]) and torch.equal(got["x"][rest], want["x"][rest])
+
+
+@pytest.mark.parametrize("reduction", ["none", "sum"])
+def test_linear_ce_fp32_rows_of_many_sizes(reduction):
+    n = 90
+    t, target = ce_inputs(n, 100, 400, F32, True, 7, seed=62)
+    t["x"] *= (2.0 ** torch.linspace(-100, 4, n))[:, None]
+    t["x"][5] = 0
+    check_ce(t, target, reduction, loss_grad(n, reduction))

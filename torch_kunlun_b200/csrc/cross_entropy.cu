@@ -30,9 +30,9 @@
 // 2^15): again 2^-39 of the largest is all that a term can lose.
 //
 // fp32 operands are split into two binary16 planes of a power-of-two multiple
-// (hi = rn(v s), lo = rn(v s - hi), the tensor's largest value in [2^14,
-// 2^15)), 22 bits or 2^-40 of the largest value, and a product is the sum
-// hi*hi + hi*lo + lo*hi: a K block takes two stages, one for each plane of both
+// (hi = rn(v s), lo = rn(v s - hi), the largest value of W and of each row of x
+// in [2^14, 2^15)), 22 bits or 2^-40 of that largest value, and a product is the
+// sum hi*hi + hi*lo + lo*hi: a K block takes two stages, one for each plane of both
 // operands, and three products.
 //
 // GEMM kernel (persistent pairs of CTAs, one CTA per SM):
@@ -53,7 +53,6 @@
 
 #include <algorithm>
 #include <atomic>
-#include <climits>
 
 #include "tk_internal.h"
 #include "tk_ptx.cuh"
@@ -111,15 +110,14 @@ constexpr int kRowPad = 256;  // rows of a tile: packed rows have room up to a m
 // Device scalars of one call.
 struct Scalars {
     int count;           // rows with a target
-    unsigned amax_x;     // binary32 bits of the largest finite |x|, |W| (fp32 operands)
-    unsigned amax_w;
+    unsigned amax_w;     // binary32 bits of the largest finite |W| (fp32 operands)
     unsigned rows_done;  // blocks of ce_rows_kernel that finished
 };
 
 // Device scalars of one backward pass: accumulators -> gradients.
 struct GradScalars {
     float dx_scale, dw_scale, db_scale;
-    int top;  // largest exponent of x_i g_i, where rows have gradients of their own
+    int top;  // largest exponent of x_i g_i, where x's rows are scaled for dW
 };
 
 enum Epilogue { kStats, kDlogits, kGradX, kGradW };
@@ -141,6 +139,7 @@ struct GemmParams {
     float2* part;        // [rows][n_tiles][BN / COLS] maximum and sum
     float* hit2;         // kStats: the target's logit, base 2
     const float* lse2;
+    const float* xs;     // kStats, kDlogits: what the rows' planes were multiplied by; NULL: 1 (fp16 operands)
     const float* grow;   // kDlogits, kGradX: g_i; NULL: one for all rows
     const int* target;
     __half* dz;          // [planes][rows_pad][dz_ld]
@@ -396,9 +395,9 @@ __device__ __forceinline__ void finish(const GemmParams& p, int64_t m, int64_t r
     }
 }
 
-// The scale that takes an accumulator to a base-2 logit.
-__device__ __forceinline__ float z_scale(const GemmParams& p) {
-    return p.planes == 1 ? kLog2e : kLog2e / plane_scale(p.sc->amax_x) / plane_scale(p.sc->amax_w);
+// The scale that takes an accumulator of row m to a base-2 logit.
+__device__ __forceinline__ float z_scale(const GemmParams& p, int64_t m) {
+    return p.xs == nullptr ? kLog2e : kLog2e / p.xs[m] / plane_scale(p.sc->amax_w);
 }
 
 template <int EPI, int MODE>
@@ -587,7 +586,6 @@ ce_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
         float* const buf_turn = turn_buf + (warp - 2) * 32 * PITCH;
         const int rows = p.sc->count;
         float scale = 1.0f;
-        if constexpr (EPI == kStats || EPI == kDlogits) scale = z_scale(p);
         if constexpr (EPI == kGradX) scale = p.gs->dx_scale;
         if constexpr (EPI == kGradW) scale = p.gs->dw_scale;
         int local = 0;
@@ -601,6 +599,7 @@ ce_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
             const int64_t col0 = static_cast<int64_t>(nt) * BN + share * COLS;
             float top = -INFINITY, sum = 0.0f;  // kStats
             const bool live = m < rows;         // kStats, kDlogits
+            if constexpr (EPI == kStats || EPI == kDlogits) scale = live ? z_scale(p, m) : 0.0f;
             const float lse = EPI == kDlogits && live ? p.lse2[m] : 0.0f;
             const float g = EPI == kDlogits && live ? (p.grow != nullptr ? mantissa_of(p.grow[m]) * kDzScale : kDzScale) : 0.0f;
             const int64_t hit = (EPI == kStats || EPI == kDlogits) && live ? p.target[m] - p.vocab0 : -1;
@@ -841,7 +840,6 @@ ce_index_kernel(const int64_t* target, int64_t rows, int64_t vocab, int64_t igno
     }
     if (threadIdx.x == 0) {
         sc->count = base;
-        sc->amax_x = 0;
         sc->amax_w = 0;
         sc->rows_done = 0;
     }
@@ -879,18 +877,12 @@ __device__ __forceinline__ unsigned amax_span(const float* p, int64_t n, int64_t
     return top;
 }
 
-// Largest finite |v| of x's listed rows (blockIdx.y 0) and of W (1).
-__global__ void __launch_bounds__(256) ce_amax_kernel(const float* x, const float* w, const int* index, Scalars* sc, int64_t cols, int64_t vocab) {
+// Largest finite |W|.
+__global__ void __launch_bounds__(256) ce_amax_kernel(const float* w, int64_t n, Scalars* sc) {
     pdl_wait();
-    const bool is_w = blockIdx.y == 1;
-    unsigned top = 0;
-    if (is_w) {
-        top = amax_span(w, vocab * cols, blockIdx.x, gridDim.x);
-    } else {
-        for (int64_t r = blockIdx.x; r < sc->count; r += gridDim.x) top = max(top, amax_span(x + static_cast<int64_t>(index[r]) * cols, cols, 0, 1));
-    }
+    unsigned top = amax_span(w, n, blockIdx.x, gridDim.x);
     top = __reduce_max_sync(0xFFFFFFFFu, top);
-    if ((threadIdx.x & 31) == 0 && top != 0) atomicMax(is_w ? &sc->amax_w : &sc->amax_x, top);
+    if ((threadIdx.x & 31) == 0 && top != 0) atomicMax(&sc->amax_w, top);
 }
 
 // Eight consecutive elements of a row whose address is off a 16-byte boundary:
@@ -1015,11 +1007,24 @@ __device__ __forceinline__ void pack_weight_and_bias(const PackJob<T>& w, float 
 
 constexpr int kPackThreads = 128;
 
+// What a row's planes are multiplied by: its largest value goes to [2^14, 2^15).
+// A row of zeros takes the largest scale, so that it bounds no other row's.
+__device__ __forceinline__ float row_scale(const float* row, int64_t cols) {
+    __shared__ unsigned tops[kPackThreads / 32];
+    const unsigned top = __reduce_max_sync(0xFFFFFFFFu, amax_span(row, cols, 0, 1));
+    __syncthreads();  // the last row's maxima are read
+    if ((threadIdx.x & 31) == 0) tops[threadIdx.x >> 5] = top;
+    __syncthreads();
+    unsigned all = 0;
+    for (int i = 0; i < kPackThreads / 32; ++i) all = max(all, tops[i]);
+    return all == 0 ? pow2(126) : plane_scale(all);
+}
+
 // Packs x's listed rows (zero rows after them up to a multiple of BK; blocks
 // [0, x_blocks)), W where it is not read in place, and the bias in base 2.
 template <typename T, int PLANES>
 __global__ void __launch_bounds__(kPackThreads)
-ce_pack_kernel(const PackJob<T> x, const PackJob<T> w, const Scalars* sc, int x_blocks, int w_blocks, const T* bias, float* bias2) {
+ce_pack_kernel(const PackJob<T> x, const PackJob<T> w, const Scalars* sc, int x_blocks, int w_blocks, const T* bias, float* bias2, float* xs) {
     pdl_wait();
     const int b = static_cast<int>(blockIdx.x);
     if (b >= x_blocks) {
@@ -1027,9 +1032,15 @@ ce_pack_kernel(const PackJob<T> x, const PackJob<T> w, const Scalars* sc, int x_
         return;
     }
     const int64_t live = sc->count;
-    const float s = PLANES == 2 ? plane_scale(sc->amax_x) : 1.0f;
-    for (int64_t r = b; r < (live + BK - 1) / BK * BK; r += x_blocks)
-        pack_row<T, PLANES>(x, r < live ? x.src + static_cast<int64_t>(x.index[r]) * x.cols : nullptr, r, s);
+    for (int64_t r = b; r < (live + BK - 1) / BK * BK; r += x_blocks) {
+        const T* row = r < live ? x.src + static_cast<int64_t>(x.index[r]) * x.cols : nullptr;
+        float s = 1.0f;
+        if constexpr (PLANES == 2) {
+            if (row != nullptr) s = row_scale(row, x.cols);
+            if (threadIdx.x == 0) xs[r] = s;
+        }
+        pack_row<T, PLANES>(x, row, r, s);
+    }
 }
 
 // ce_index_kernel and ce_pack_kernel in one launch, for up to 1024 rows of
@@ -1143,11 +1154,14 @@ ce_rows_kernel(const int* index, const int* target, Scalars* sc, const float2* p
 
 static_assert(kDzScale == 16384.0f, "2^14, in the exponents below");
 
-// Block 0: the gradients' scales, and g_i per packed row where each has its
-// own.  The others: zero gradients for the ignored rows.
+constexpr int kNoTop = -100000;  // below every exponent of a finite x_i g_i
+
+// Block 0: the gradients' scales, g_i per packed row where each has its own, and
+// (fp32 operands) the largest exponent of x_i g_i.  The others: zero gradients
+// for the ignored rows.
 __global__ void __launch_bounds__(1024)
-ce_grad_rows_kernel(const float* grad, int reduction, const int* index, const Scalars* sc, GradScalars* gs, float* grow, int planes, const int64_t* target,
-                    int64_t ignore, int64_t all_rows, int64_t row_bytes, uint8_t* dx) {
+ce_grad_rows_kernel(const float* grad, int reduction, const int* index, const Scalars* sc, GradScalars* gs, float* grow, const float* xs,
+                    const int64_t* target, int64_t ignore, int64_t all_rows, int64_t row_bytes, uint8_t* dx) {
     pdl_wait();
     if (blockIdx.x > 0) {
         const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -1164,22 +1178,30 @@ ce_grad_rows_kernel(const float* grad, int reduction, const int* index, const Sc
     }
     const int rows = sc->count;
     const bool own = reduction == TK_REDUCE_NONE;
-    if (own)
-        for (int i = threadIdx.x; i < rows; i += 1024) grow[i] = grad[index[i]];
+    int top = kNoTop;
+    for (int i = threadIdx.x; i < rows && (own || xs != nullptr); i += 1024) {
+        float g = 1.0f;
+        if (own) grow[i] = g = grad[index[i]];
+        if (xs != nullptr && g != 0.0f && isfinite(g)) top = max(top, 14 - exponent_of(xs[i]) + exponent_of(g));
+    }
+    __shared__ int tops[32];
+    top = __reduce_max_sync(0xFFFFFFFFu, top);
+    if ((threadIdx.x & 31) == 0) tops[threadIdx.x >> 5] = top;
+    __syncthreads();
+    if (threadIdx.x < 32) top = __reduce_max_sync(0xFFFFFFFFu, tops[threadIdx.x]);
     if (threadIdx.x == 0) {
         // no rows: every sum is zero
         const float g = own ? 1.0f : rows == 0 ? 0.0f : reduction == TK_REDUCE_MEAN ? grad[0] / static_cast<float>(rows) : grad[0];
         const float unit = g / kDzScale;
         gs->db_scale = own ? 1.0f : unit;  // the sums take 2^(k_i - 14) row by row
-        gs->dx_scale = planes == 2 ? unit / plane_scale(sc->amax_w) : unit;
-        gs->dw_scale = planes == 2 ? unit / plane_scale(sc->amax_x) : unit;  // ce_scale_rows_kernel adds x's exponent
-        gs->top = INT_MIN;
+        gs->dx_scale = xs != nullptr ? unit / plane_scale(sc->amax_w) : unit;
+        gs->dw_scale = unit;  // ce_scale_rows_kernel adds the exponent of x's rows
+        gs->top = top;
     }
 }
 
-constexpr int kNoTop = -100000;  // below every exponent of a finite x_i g_i
-
-// The largest exponent of x_i g_i over the packed rows, a warp to a row.
+// The largest exponent of x_i g_i over the packed rows of fp16 operands, a warp
+// to a row.
 __global__ void __launch_bounds__(256)
 ce_top_kernel(const __half* x, int64_t ld, const Scalars* sc, GradScalars* gs, const float* grow) {
     pdl_wait();
@@ -1201,11 +1223,12 @@ ce_top_kernel(const __half* x, int64_t ld, const Scalars* sc, GradScalars* gs, c
     if (lane == 0) atomicMax(&gs->top, top);
 }
 
-// x's packed rows (zero rows up to a multiple of BK included) times 2^k_i and
-// the power of two that takes the largest into [2^14, 2^15), for dW.
+// x's packed rows (zero rows up to a multiple of BK included) times 2^k_i, with
+// one scale for all rows, the power of two that takes the largest into [2^14,
+// 2^15), for dW.
 template <int PLANES>
 __global__ void __launch_bounds__(kPackThreads)
-ce_scale_rows_kernel(const __half* x, __half* to, int64_t ld, int64_t plane, const Scalars* sc, GradScalars* gs, const float* grow) {
+ce_scale_rows_kernel(const __half* x, __half* to, int64_t ld, int64_t plane, const Scalars* sc, GradScalars* gs, const float* grow, const float* xs) {
     pdl_wait();
     const int64_t live = sc->count;
     const int shift = gs->top > kNoTop ? 14 - gs->top : 0;
@@ -1214,8 +1237,8 @@ ce_scale_rows_kernel(const __half* x, __half* to, int64_t ld, int64_t plane, con
         gs->dw_scale = gs->dw_scale * pow2(-half) * pow2(half - shift);
     }
     for (int64_t r = blockIdx.x; r < (live + BK - 1) / BK * BK; r += gridDim.x) {
-        const float g = r < live ? grow[r] : 0.0f;
-        const int e = isfinite(g) ? exponent_of(g) + shift : 0;
+        const float g = r >= live ? 0.0f : grow != nullptr ? grow[r] : 1.0f;
+        const int e = exponent_of(g) + shift - (PLANES == 2 && r < live ? exponent_of(xs[r]) : 0);
         const float a = g == 0.0f ? 0.0f : pow2(e / 2), b = pow2(e - e / 2);  // a row that `top` does not bound takes no part
         for (int64_t c = static_cast<int64_t>(threadIdx.x) * 8; c < ld; c += kPackThreads * 8) {
             const int64_t at = r * ld + c;
@@ -1320,7 +1343,7 @@ struct Plan {
     int split_units;
     int db_chunks;
     // state: kept from the forward to the backward pass
-    size_t s_scalars, s_index, s_target, s_lse, s_x, s_bias, s_w, state_bytes;
+    size_t s_scalars, s_index, s_target, s_lse, s_xs, s_x, s_bias, s_w, state_bytes;
     // workspaces
     size_t w_part, w_hit, w_loss, w_w, fwd_bytes;
     size_t b_scalars, b_grow, b_dz, b_acc, b_split, b_db, b_w, b_x, bwd_bytes;
@@ -1381,6 +1404,7 @@ Plan make_plan(const tk_linear_ce_desc_t& d) {
     p.s_index = take(p.rows_pad * sizeof(int));
     p.s_target = take(p.rows_pad * sizeof(int));
     p.s_lse = take(p.rows_pad * sizeof(float));
+    p.s_xs = take(p.planes == 2 ? p.rows_pad * sizeof(float) : 0);
     p.s_x = take(static_cast<size_t>(p.planes) * p.rows_pad * p.ld * 2);
     p.s_bias = take(static_cast<size_t>(d.vocab) * sizeof(float));  // with a bias or without
     p.s_w = take(p.w_kept ? w_bytes : 0);
@@ -1396,7 +1420,7 @@ Plan make_plan(const tk_linear_ce_desc_t& d) {
     const bool own = d.reduction == TK_REDUCE_NONE;  // each row has its own gradient
     p.b_scalars = take(sizeof(GradScalars));
     p.b_grow = take(own ? p.rows_pad * sizeof(float) : 0);
-    p.b_x = take(own ? static_cast<size_t>(p.planes) * p.rows_pad * p.ld * 2 : 0);
+    p.b_x = take(own || p.planes == 2 ? static_cast<size_t>(p.planes) * p.rows_pad * p.ld * 2 : 0);
     p.b_dz = take(static_cast<size_t>(p.planes) * p.rows_pad * p.piece * 2);
     p.b_acc = take(p.pieces > 1 ? static_cast<size_t>(p.rows_pad) * p.acc_ld * sizeof(float) : 0);
     p.b_split = take(static_cast<size_t>(p.split_units) * BM * BN * sizeof(float));
@@ -1525,10 +1549,10 @@ int list_and_pack(const tk_linear_ce_desc_t& d, const Plan& p, uint8_t* st, uint
     CE_TRY(launch_status("cross entropy index"));
     if (d.rows == 0) return TK_OK;
     if constexpr (PLANES == 2)
-        CE_TRY(launch_chain("cross entropy amax", ce_amax_kernel, dim3(148 * 4, 2), dim3(256), 0, s, x, jw.src, static_cast<const int*>(index), sc, d.cols, d.vocab));
+        CE_TRY(launch_chain("cross entropy amax", ce_amax_kernel, dim3(148 * 4), dim3(256), 0, s, jw.src, d.vocab * d.cols, sc));
     const int x_blocks = blocks_for(p.rows_read);
     return launch_chain("cross entropy pack", ce_pack_kernel<T, PLANES>, dim3(static_cast<unsigned>(x_blocks + w_blocks + b_blocks)), dim3(kPackThreads), 0,
-                        s, jx, jw, static_cast<const Scalars*>(sc), x_blocks, w_blocks, bias, bias2);
+                        s, jx, jw, static_cast<const Scalars*>(sc), x_blocks, w_blocks, bias, bias2, reinterpret_cast<float*>(st + p.s_xs));
 }
 
 int rows_loss(const tk_linear_ce_desc_t& d, const Plan& p, uint8_t* st, uint8_t* ws, cudaStream_t s) {
@@ -1559,6 +1583,7 @@ GemmParams base_params(const tk_linear_ce_desc_t& d, const Plan& p, const uint8_
     g.group = 8;
     g.max_units = p.split_units;
     g.err = device_error_word(current_device());
+    g.xs = p.planes == 2 ? reinterpret_cast<const float*>(st + p.s_xs) : nullptr;
     g.bias2 = d.bias != nullptr ? reinterpret_cast<const float*>(st + p.s_bias) : nullptr;
     g.vocab = d.vocab;
     return g;
@@ -1644,29 +1669,31 @@ int tk_linear_ce_backward(const tk_linear_ce_grad_desc_t* desc, void* workspace,
     const int* index = reinterpret_cast<const int*>(st + p.s_index);
     GradScalars* gs = reinterpret_cast<GradScalars*>(ws + p.b_scalars);
     const bool own = d.reduction == TK_REDUCE_NONE;
+    const float* xs = p.planes == 2 ? reinterpret_cast<const float*>(st + p.s_xs) : nullptr;
     float* grow = own ? reinterpret_cast<float*>(ws + p.b_grow) : nullptr;
     __half* dz = reinterpret_cast<__half*>(ws + p.b_dz);
     const size_t esz = dtype_size(d.dtype);
     const int zero_blocks = desc->dx != nullptr ? static_cast<int>(std::min<int64_t>(ceil_div(d.rows, 32), 148 * 2)) : 0;
     CE_TRY(launch_chain("cross entropy gradient rows", ce_grad_rows_kernel, dim3(static_cast<unsigned>(1 + zero_blocks)), dim3(1024), 0, s,
-                        desc->grad_loss, static_cast<int>(d.reduction), index, sc, gs, grow, p.planes, d.target, d.ignore_index, d.rows,
+                        desc->grad_loss, static_cast<int>(d.reduction), index, sc, gs, grow, xs, d.target, d.ignore_index, d.rows,
                         static_cast<int64_t>(d.cols * esz), static_cast<uint8_t*>(desc->dx)));
     uint8_t* w_at = p.w_kept ? st + p.s_w : ws + p.b_w;
     if (!p.w_kept && !p.w_direct) {
         CE_TRY(launch_chain("cross entropy pack", ce_pack_kernel<__half, 1>, dim3(static_cast<unsigned>(weight_blocks(d, p))), dim3(kPackThreads), 0, s,
                             PackJob<__half>{}, weight_job<__half>(d, p, reinterpret_cast<__half*>(w_at)), sc, 0,
-                            weight_blocks(d, p), static_cast<const __half*>(nullptr), static_cast<float*>(nullptr)));
+                            weight_blocks(d, p), static_cast<const __half*>(nullptr), static_cast<float*>(nullptr), static_cast<float*>(nullptr)));
     }
     const Operand w = weight_operand(d, p, w_at);
     const int64_t x_plane = p.rows_pad * p.ld, dz_plane = p.rows_pad * p.piece;
     const __half* x_dw = reinterpret_cast<const __half*>(st + p.s_x);
-    if (own && desc->dweight) {
+    if ((own || p.planes == 2) && desc->dweight) {
         __half* to = reinterpret_cast<__half*>(ws + p.b_x);
-        CE_TRY(launch_chain("cross entropy row exponents", ce_top_kernel, dim3(static_cast<unsigned>(std::min<int64_t>(ceil_div(d.rows, 8), 148 * 8))), dim3(256),
-                            0, s, x_dw, p.ld, sc, gs, static_cast<const float*>(grow)));
+        if (p.planes == 1)
+            CE_TRY(launch_chain("cross entropy row exponents", ce_top_kernel, dim3(static_cast<unsigned>(std::min<int64_t>(ceil_div(d.rows, 8), 148 * 8))), dim3(256),
+                                0, s, x_dw, p.ld, sc, gs, static_cast<const float*>(grow)));
         CE_TRY(launch_chain("cross entropy row scales", p.planes == 2 ? ce_scale_rows_kernel<2> : ce_scale_rows_kernel<1>,
                             dim3(static_cast<unsigned>(blocks_for(p.rows_read))), dim3(kPackThreads), 0, s, x_dw, to, p.ld, x_plane, sc, gs,
-                            static_cast<const float*>(grow)));
+                            static_cast<const float*>(grow), xs));
         x_dw = to;
     }
     CUtensorMap tx, tx_mn;

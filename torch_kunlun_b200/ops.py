@@ -143,9 +143,12 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Te
     target [...] is int64.  Rows whose target is ignore_index take no part (loss
     and gradient 0, whatever x holds there) and cost nothing; any other target
     outside [0, V) makes its loss NaN.  reduction is "mean" (over the rows with a
-    target), "sum" or "none" (target's shape).  Products are those of the tensors' own
-    values summed in fp32, not the int16-quantised ones of ``linear``.
-    Differentiable in x, weight and bias."""
+    target), "sum" or "none" (target's shape); a row's loss and its row of x's
+    gradient depend on that row alone.  Products are those of the tensors' own
+    values (float32 to 22 bits) summed in fp32, not the int16-quantised ones of
+    ``linear``.  In the backward pass softmax - onehot is held to 11 bits for
+    float16 and 22 for float32, and to 2**-39 at most.  Differentiable in x, weight
+    and bias."""
     if reduction not in REDUCTION:
         raise ValueError(f"reduction must be one of {sorted(REDUCTION)}, got {reduction!r}")
     return _C.linear_cross_entropy(x, weight, target, bias, int(ignore_index), REDUCTION[reduction])
