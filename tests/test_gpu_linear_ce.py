@@ -609,3 +609,46 @@ def test_linear_ce_fp32_rows_of_many_sizes(reduction):
     t["x"] *= (2.0 ** torch.linspace(-100, 4, n))[:, None]
     t["x"][5] = 0
     check_ce(t, target, reduction, loss_grad(n, reduction))
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("n,d,v,reduction", [(50, 64, 200, "none"), (300, 96, 1000, "mean"), (70, 100, 333, "sum"), (16384, 64, 20003, "mean")])
+def test_linear_ce_gradients_of_misaligned_tensors(n, d, v, reduction, dtype):
+    """Every tensor, results among them, off a 16-byte boundary and at offsets of
+    its own, over one and several pieces of the vocabulary: the aligned call's bits."""
+    t, target = ce_inputs(n, d, v, dtype, True, n // 9, seed=n + d)
+    g = loss_grad(n, reduction).reshape(-1)
+    want = run_ce(t, target, reduction, g if reduction == "none" else g[0])
+    L, desc, hold = _capi.lib(), _capi.LinearCeGradDesc(), []
+
+    def off(v, k):
+        b = torch.full((v.numel() + 8,), 7.0 if v.is_floating_point() else 7, dtype=v.dtype, device="cuda")
+        b[k:k + v.numel()] = v.reshape(-1).cuda()
+        hold.append(b)
+        return b[k:k + v.numel()].view(v.shape)
+
+    def room(size):
+        b = torch.full((size + 1024,), 255, dtype=torch.uint8, device="cuda")
+        hold.append(b)
+        return (b.data_ptr() + 1023) // 1024 * 1024
+
+    f = desc.fwd
+    f.dtype, f.rows, f.cols, f.vocab, f.ignore_index, f.reduction = int(dtype == F32), n, d, v, -100, ["none", "mean", "sum"].index(reduction)
+    ins = {"x": off(t["x"], 1), "weight": off(t["weight"], 3), "bias": off(t["bias"], 1)}
+    loss, gl, tg = off(torch.zeros(n if reduction == "none" else 1), 1), off(g, 1), off(target, 1)
+    outs = {k: off(torch.zeros_like(t[k]), i + 1) for i, k in enumerate(t)}
+    f.x, f.weight, f.bias, f.target, f.loss = (u.data_ptr() for u in (ins["x"], ins["weight"], ins["bias"], tg, loss))
+    assert all(u.data_ptr() % 16 for u in (*ins.values(), *outs.values(), loss, gl, tg))
+    desc.grad_loss, desc.dx, desc.dweight, desc.dbias = gl.data_ptr(), outs["x"].data_ptr(), outs["weight"].data_ptr(), outs["bias"].data_ptr()
+    f.state = room(L.tk_linear_ce_state_size(ctypes.byref(f)))
+    sizes = L.tk_linear_ce_workspace_size(ctypes.byref(f)), L.tk_linear_ce_backward_workspace_size(ctypes.byref(desc))
+    torch.cuda.synchronize()
+    _capi.check(L.tk_linear_ce(ctypes.byref(f), room(sizes[0]), sizes[0], None), "tk_linear_ce")
+    _capi.check(L.tk_linear_ce_backward(ctypes.byref(desc), room(sizes[1]), sizes[1], None), "tk_linear_ce_backward")
+    torch.cuda.synchronize()
+    assert torch.equal(loss.cpu(), want["loss"].reshape(-1))
+    for i, k in enumerate(t):
+        assert torch.equal(outs[k].cpu(), want[k]), k
+        rim = outs[k].numel() + i + 1
+        whole = torch.as_strided(outs[k], (outs[k].numel() + 8,), (1,), 0).cpu()
+        assert (whole[:i + 1] == 7).all() and (whole[rim:] == 7).all(), k  # nothing beside the result is written

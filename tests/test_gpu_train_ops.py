@@ -473,3 +473,62 @@ def test_train_ops_form_the_gradients_that_are_asked_for(call):
         assert whole - part >= t[large].numel() * 2, names
         for k in names:
             assert torch.equal(some[k], every[k]), k
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("shape", [(3, 7, 24), (2, 9, 96), (5, 31, 256), (3, 40, 1000), (2, 5, 4096), (2, 3, 9000), (1, 2, 20000)])
+@pytest.mark.parametrize("kind,post,gate,p", [("layer", True, "sample", 0.1), ("rms", False, "none", 0.0), ("rms", True, "channel", 0.3), ("layer", False, "token", 0.0)])
+def test_residual_norm_gradients_of_misaligned_tensors(shape, dtype, kind, post, gate, p):
+    """Every tensor off a 16-byte boundary, each by an offset of its own, at widths
+    that vectors would fit, against the 64-bit values; nothing beside a result is
+    written."""
+    t = norm_inputs(shape, dtype, kind, post, gate, sum(shape))
+    gx, gh = rnd(shape, 8, dtype), rnd(shape, 9, dtype)
+    hold = []
+
+    def off(v, k):
+        b = torch.full((v.numel() + 8,), 7.0, dtype=v.dtype, device="cuda")
+        b[k:k + v.numel()] = v.reshape(-1).cuda()
+        hold.append((b, k, v.numel()))
+        return hold[-1][0][k:k + v.numel()].data_ptr()
+
+    d = shape[-1]
+    rows = t["x"].numel() // d
+    step = 8 if dtype == F16 else 4  # elements of 16 bytes
+    g = C.ResidualNormGradDesc()
+    f = g.fwd
+    f.dtype, f.norm, f.rows, f.cols, f.post_norm = int(dtype == F32), int(kind == "rms"), rows, d, int(post)
+    f.residual_scale, f.eps, f.p, f.seed, f.offset = 0.75, 1e-5, p, 77, 5
+    for i, k in enumerate(t):
+        setattr(f, k, off(t[k], 1 + i % (step - 1)))
+    f.gate_rows = t["gate"].numel() // d if "gate" in t else 0
+    inputs = len(hold)
+    names = ["x_new", "h"] + list(t)
+    where = {}
+    for i, k in enumerate(names):
+        like = t[k] if k in t else t["x"]
+        where[k] = (len(hold), like.shape)
+        at = off(torch.zeros_like(like), 1 + (2 * i + 1) % (step - 1))
+        if k in ("x_new", "h"):
+            setattr(f, k, at)
+        else:
+            setattr(g, "d" + k, at)
+    g.grad_x_new, g.grad_h = off(gx, 3), off(gh, 2)
+    stats = torch.zeros(rows, 4, device="cuda")
+    f.stats = stats.data_ptr()
+    L = C.lib()
+    size = L.tk_residual_norm_backward_workspace_size(C.ctypes.byref(g))
+    ws = torch.full((size,), 255, dtype=torch.uint8, device="cuda")
+    torch.cuda.synchronize()
+    C.check(L.tk_residual_norm(C.ctypes.byref(f), None), "tk_residual_norm")
+    C.check(L.tk_residual_norm_backward(C.ctypes.byref(g), ws.data_ptr(), size, None), "tk_residual_norm_backward")
+    torch.cuda.synchronize()
+    want = R.residual_norm64(t["x"], t["f"], t.get("weight"), t.get("bias"), post, t.get("post_weight"), t.get("post_bias"), t.get("gate"),
+                             kind == "rms", 0.75, 1e-5, R.keep_mask(shape, p, 77, 5) if p > 0 else None, p, gx, gh)
+    for k, (i, s) in where.items():
+        b, at, n = hold[i]
+        value, bound = want[k]
+        got = b.cpu()
+        R.assert_within(got[at:at + n].view(s), value.reshape(s), bound.expand_as(value).reshape(s), k)
+        assert (got[:at] == 7).all() and (got[at + n:] == 7).all(), k
+    assert inputs == len(t)
