@@ -56,9 +56,14 @@ def _norm64(v, rms, eps):
 
 
 def residual_norm64(x, f, weight=None, bias=None, post=False, post_weight=None, post_bias=None, gate=None,
-                    rms=False, scale=1.0, eps=1e-5, keep=None, p=0.0, gx=None, gh=None):
+                    rms=False, scale=1.0, eps=1e-5, keep=None, p=0.0, gx=None, gh=None, chain=None):
     """{name: (value, bound)} in float64 on the rounded inputs; gradients when
-    gx / gh are given (the missing one counts as zero)."""
+    gx / gh are given (the missing one counts as zero).
+
+    `chain` None: bounds that also admit a backward pass from the rounded x_new
+    and column sums of all rows one after the other.  A number: bounds for the
+    unrounded x_new, with results rounded to nearest and at most `chain` additions
+    on a term's way through a column sum."""
     dtype = x.dtype
     d = {n: t.double() for n, t in dict(x=x, f=f, w=weight, b=bias, pw=post_weight, pb=post_bias, gate=gate,
                                         gx=gx, gh=gh).items() if t is not None}
@@ -83,7 +88,7 @@ def residual_norm64(x, f, weight=None, bias=None, post=False, post_weight=None, 
         return out
     zero = torch.zeros_like(x_new)
     vx, vh = d.get("gx", zero), d.get("gh", zero)
-    c_b = c_n + HALF_STEP[dtype] * an                 # n from the rounded x_new
+    c_b = c_n + (HALF_STEP[dtype] * an if chain is None else 0.0)  # n from the rounded x_new
     t = vh * w
     mean = (lambda v: torch.zeros_like(v[..., :1])) if rms else (lambda v: v.mean(-1, keepdim=True))
     both = lambda v: v.mean(-1, keepdim=True)  # noqa: E731
@@ -95,7 +100,7 @@ def residual_norm64(x, f, weight=None, bias=None, post=False, post_weight=None, 
 
     def total(name, v, err, mag, over=dims, shape=None):
         s = v.sum(over, keepdim=shape is not None)
-        e = (err + (rows + 64) * U32 * mag).sum(over, keepdim=shape is not None)
+        e = (err + (rows + 64 if chain is None else chain) * U32 * mag).sum(over, keepdim=shape is not None)
         out[name] = (s, ulp(s, dtype) + e)
 
     out["x"] = (scale * g, ulp(scale * g, dtype) + abs(scale) * e_g)
@@ -122,6 +127,25 @@ def residual_norm64(x, f, weight=None, bias=None, post=False, post_weight=None, 
         e_gu = rq * (spread(e_t) + 2 * (c_q + K * U32) * spread(m_t))
     out["f"] = (gu, ulp(gu, dtype) + e_gu)
     return out
+
+
+def column_chain(rows, gate_rows=None):
+    """Additions on a term's way through a column sum of `rows` rows of more than
+    128 columns that one CTA holds: the rows of one of 148 or more row ranges, or of
+    a gate row that a group takes whole, then the range's groups (up to 8), four to
+    19 ranges per thread and 32 threads, and a product's rounding."""
+    return max(-(-rows // 148), rows // gate_rows if gate_rows else 0) + 64
+
+
+# Norm of the error over norm of the value.  Rounding a result is off by half a
+# step at most, 2^-11 of the norm in binary16; binary32 errors of the terms, up to
+# K half steps each with signs of their own, add sqrt(K) twice over (the
+# statistics' and the sums'), 14 to 28 half steps: 32 in all.
+NORM_ERROR = {torch.float16: 2.0 ** -11 + 32 * U32, torch.float32: 32 * U32}
+
+
+def norm_error(got, want):
+    return float((got.double() - want).norm() / want.norm().clamp_min(1e-300))
 
 
 def linear_ce64(x, w, target, bias=None, ignore=-100, reduction="mean", grad=None):

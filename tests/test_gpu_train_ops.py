@@ -532,3 +532,22 @@ def test_residual_norm_gradients_of_misaligned_tensors(shape, dtype, kind, post,
         R.assert_within(got[at:at + n].view(s), value.reshape(s), bound.expand_as(value).reshape(s), k)
         assert (got[:at] == 7).all() and (got[at + n:] == 7).all(), k
     assert inputs == len(t)
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("shape", [(3, 37, 768), (1, 3000, 256), (4, 500, 1000), (7, 33, 1151), (2, 1500, 4096), (16, 301, 136), (600, 5, 200)])
+@pytest.mark.parametrize("kind,post,gate,p", [("layer", False, "none", 0.0), ("layer", True, "channel", 0.1), ("rms", True, "sample", 0.0), ("rms", False, "token", 0.1)])
+def test_residual_norm_gradients_within_tight_bounds(shape, dtype, kind, post, gate, p):
+    """Bounds that an x_new rounded to binary16, or a missing or wrong term, does
+    not meet (test_train_ops_cpu.py): element by element and in norm."""
+    t = norm_inputs(shape, dtype, kind, post, gate, sum(shape))
+    gx, gh = rnd(shape, 8, dtype), rnd(shape, 9, dtype)
+    got = run_norm(t, kind, post, 1.25, p, gx, gh)
+    rows = t["x"].numel() // shape[-1]
+    want = R.residual_norm64(t["x"], t["f"], t.get("weight"), t.get("bias"), post, t.get("post_weight"), t.get("post_bias"), t.get("gate"),
+                             kind == "rms", 1.25, 1e-5, R.keep_mask(shape, p, 77, 5) if p > 0 else None, p, gx, gh,
+                             chain=R.column_chain(rows, shape[0] if gate == "sample" else None))
+    for k, v in got.items():
+        value, bound = want[k]
+        R.assert_within(v, value.reshape(v.shape), bound.expand_as(value).reshape(v.shape), f"{k} {shape} {dtype} {kind}")
+        assert R.norm_error(v, value.reshape(v.shape)) <= R.NORM_ERROR[dtype], k

@@ -258,3 +258,89 @@ def test_residual_norm_without_rows_takes_any_gate(gate_rows):
     assert L.tk_residual_norm_backward_workspace_size(ctypes.byref(g)) > 0
     assert L.tk_residual_norm_backward(ctypes.byref(g), None, 0, None) == 0
     assert L.tk_residual_norm(ctypes.byref(_norm_desc(rows=0, gate=1024, gate_rows=-1)), None) == 1
+
+
+def _norm_gradients(t, gx, gh, keep, p, rms, mistake=None):
+    """The residual norm's results from its formulas in binary64, rounded once;
+    `mistake` leaves one thing out or takes it wrong."""
+    d = {k: v.double() for k, v in t.items()}
+    gx, gh = gx.double(), gh.double()
+    mean = (lambda v: 0.0) if rms else (lambda v: v.mean(-1, keepdim=True))
+
+    def norm(v):
+        r = ((v - mean(v)).square().mean(-1, keepdim=True) + 1e-5).rsqrt()
+        return (v - mean(v)) * r, r
+
+    def back(n, r, g):
+        a = 0.0 if mistake == "mean" else mean(g)
+        return r * (g - a - (0.0 if mistake == "product mean" else n * (g * n).mean(-1, keepdim=True)))
+
+    drop = keep.double() / (1 - p)
+    q, rq = norm(d["f"])
+    u = drop * (q * d["post_weight"] + d["post_bias"])
+    x_new = d["x"] + d["gate"] * u
+    if mistake == "rounded":
+        x_new = x_new.to(t["x"].dtype).double()
+    n, r = norm(x_new)
+    g = gx + back(n, r, gh * (1.0 if mistake == "weight" else d["weight"]))
+    gu = g * (1.0 if mistake == "gate" else d["gate"]) * (1.0 if mistake == "mask" else drop)
+    rows = (0, 1)
+    out = {"x": g, "weight": (gh * n).sum(rows), "bias": gh.sum(rows), "gate": (g * u).sum(rows),
+           "post_weight": (gu * (q if mistake != "row" else q * (torch.arange(q.shape[1]) > 0)[:, None])).sum(rows), "post_bias": gu.sum(rows),
+           "f": back(q, rq, gu * (1.0 if mistake == "post weight" else d["post_weight"]))}
+    return {k: v.to(t["x"].dtype) for k, v in out.items()}
+
+
+@pytest.mark.parametrize("shape", [(3, 37, 768), (1, 3000, 256)])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+@pytest.mark.parametrize("rms", [False, True])
+def test_residual_norm_bounds_tell_mistakes(shape, dtype, rms):
+    """The bounds for the unrounded x_new admit the formulas' rounded values and
+    none of these mistakes."""
+    g = torch.Generator().manual_seed(12)
+    n = lambda s, scale=1.0, mean=0.0: (torch.randn(s, generator=g) * scale + mean).to(dtype)  # noqa: E731
+    d = shape[-1]
+    t = {"x": n(shape, 1.0, 0.5), "f": n(shape, 0.7), "weight": n(d, 0.1, 1.0), "bias": n(d, 0.1), "post_weight": n(d, 0.1, 1.0),
+         "post_bias": n(d, 0.1), "gate": n(d, 0.3, 0.5)}
+    gx, gh, keep = n(shape), n(shape), torch.rand(shape, generator=g) > 0.1
+    rows = shape[0] * shape[1]
+    want = R.residual_norm64(t["x"], t["f"], t["weight"], t["bias"], True, t["post_weight"], t["post_bias"], t["gate"], rms, 1.0, 1e-5,
+                             keep, 0.1, gx, gh, chain=R.column_chain(rows))
+
+    def beyond(mistake):
+        got = _norm_gradients(t, gx, gh, keep, 0.1, rms, mistake)
+        off = set()
+        for k, v in got.items():
+            value, bound = want[k]
+            if ((v.double() - value).abs() > bound.expand_as(value)).any() or R.norm_error(v, value) > R.NORM_ERROR[dtype]:
+                off.add(k)
+        return off
+
+    assert not beyond(None)
+    expected = {"product mean": {"x", "f", "gate"}, "weight": {"x", "f"}, "gate": {"f", "post_weight", "post_bias"},
+                "mask": {"f", "post_weight", "post_bias"}, "post weight": {"f"}, "row": {"post_weight"}}
+    if not rms:
+        expected["mean"] = {"x", "f"}
+    for mistake, outputs in expected.items():
+        assert outputs <= beyond(mistake), mistake
+
+
+def test_residual_norm_bounds_tell_a_rounded_x_new():
+    """Gradients from x_new rounded to binary16, without a norm behind the block:
+    admitted by the wide bounds, beyond the tight ones."""
+    g = torch.Generator().manual_seed(12)
+    shape = (3, 37, 768)
+    n = lambda s, scale=1.0, mean=0.0: (torch.randn(s, generator=g) * scale + mean).half()  # noqa: E731
+    x, f, w, gx, gh = n(shape, 1.0, 0.5), n(shape, 0.7), n(768, 0.1, 1.0), n(shape), n(shape)
+    tight = R.residual_norm64(x, f, w, gx=gx, gh=gh, chain=R.column_chain(111))["weight"]
+    wide = R.residual_norm64(x, f, w, gx=gx, gh=gh)["weight"]
+
+    def weight_gradient(x_new):
+        c = x_new - x_new.mean(-1, keepdim=True)
+        return (gh.double() * c * (c.square().mean(-1, keepdim=True) + 1e-5).rsqrt()).sum((0, 1)).half()
+
+    x_new = x.double() + f.double()
+    off = lambda got, want: int(((got.double() - want[0]).abs() > want[1]).sum())  # noqa: E731
+    assert off(weight_gradient(x_new), tight) == 0
+    rounded = weight_gradient(x_new.half().double())
+    assert off(rounded, wide) == 0 and off(rounded, tight) > 4
