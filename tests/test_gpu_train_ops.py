@@ -551,3 +551,45 @@ def test_residual_norm_gradients_within_tight_bounds(shape, dtype, kind, post, g
         value, bound = want[k]
         R.assert_within(v, value.reshape(v.shape), bound.expand_as(value).reshape(v.shape), f"{k} {shape} {dtype} {kind}")
         assert R.norm_error(v, value.reshape(v.shape)) <= R.NORM_ERROR[dtype], k
+
+
+def test_train_ops_captured_with_their_backward_passes():
+    """Two steps captured through the public calls, forward and backward, replayed
+    in turn on new values in the same inputs, against ordinary calls."""
+    def values(seed):
+        return [rnd((4, 16, 64), seed), rnd((4, 16, 64), seed + 1), rnd((64,), seed + 2, F16, 0.1, 1.0), rnd((1000, 64), seed + 3, F16, 0.3)]
+
+    def step(x, f, w, head, target, offset):
+        y, h = ops.residual_norm(x, f, w, post_norm=True, p=0.1, seed=3, offset=offset)
+        loss = ops.linear_cross_entropy(ops.dropout(h, 0.1, 5, offset), head, target)
+        return [y.detach(), loss.detach()] + list(torch.autograd.grad([y, loss], [x, f, w, head], [torch.ones_like(y), one]))
+
+    one = torch.tensor(64.0).to(DEV)
+    target = torch.randint(-1, 1000, (4, 16), generator=torch.Generator().manual_seed(2))
+    target = torch.where(target < 0, -100, target).to(DEV)
+    s = kunlun.Stream()
+    graphs = []
+    for k in range(2):
+        leaves = [v.to(DEV).requires_grad_() for v in values(10 * k)]
+        kunlun.synchronize()
+        with kunlun.stream(s):
+            step(*leaves, target, k)
+            s.synchronize()
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=torch.cuda.ExternalStream(s.stream_id)):
+                out = step(*leaves, target, k)
+        graphs.append((graph, leaves, out))
+    torch.cuda.synchronize()
+    for seed in (100, 200):
+        for k, (graph, leaves, out) in enumerate(graphs):
+            with torch.no_grad():
+                for leaf, v in zip(leaves, values(seed + 50 * k)):
+                    leaf.copy_(v.to(DEV))
+        kunlun.synchronize()
+        for graph, _, _ in graphs:
+            graph.replay()
+        torch.cuda.synchronize()
+        for k, (_, leaves, out) in enumerate(graphs):
+            want = step(*[v.to(DEV).requires_grad_() for v in values(seed + 50 * k)], target, k)
+            for a, b in zip(out, want):
+                assert torch.equal(a.cpu(), b.cpu())
