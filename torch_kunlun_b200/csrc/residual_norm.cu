@@ -1102,8 +1102,10 @@ __global__ void __launch_bounds__(1024) residual_norm_columns_kernel(const RnPar
 // NV octets per thread, W warps per row and CTA, CTAs per row.  A warp's work
 // for a row is about two octets' worth of sums and addresses and NV octets, so
 // the least W * (2 + NV) is taken (8192 x 4096 with both norms, forward: NV 1
-// 91 us, 2 58 us, 4 60 us).  Registers rule some out: NV 3 with a post norm
-// spills; the backward pass keeps two sums per column up to NV 2 (NV 3: 154
+// 91 us, 2 58 us, 4 60 us).  Registers rule some out, at 128 for up to 512
+// threads: NV 3 with a post norm spills 212 to 284 bytes (43690 x 768: 55.5 us,
+// with NV 4 53.7; without one it spills 48 to 88 and stays, as fp32 NV 2 with one
+// does at 64 to 256); the backward pass keeps two sums per column up to NV 2 (NV 3: 154
 // against 93 us), five at NV 1 (NV 2: 198 against 153 us).  fp32 doubles the
 // bytes of a row's copy: NV 1 (2331 x 1151 forward: 32 us, with NV 2 40 us),
 // and forward 2 where that spares a cluster.
