@@ -507,22 +507,22 @@ typedef struct {
 
 /* The state holds x's listed rows as binary16 planes (room for all rows) and
  * four words per row, the bias, and where dtype is fp32 or cols % 8 != 0 the
- * weight as planes too.  Its size and layout follow from dtype, rows, cols and vocab alone,
- * so the backward pass may be given the weight at another address.  The workspace
- * sizes also go by weight's address: an fp16 weight of cols % 8 == 0 off a
- * 16-byte boundary is packed into the workspace of each pass. */
+ * weight as planes too.  Its size and layout follow from dtype, rows, cols and
+ * vocab alone, so the backward pass may be given the weight at another address.
+ * The workspace sizes also go by weight's address: an fp16 weight of cols % 8 == 0
+ * off a 16-byte boundary is packed into the workspace of each pass. */
 TK_API size_t tk_linear_ce_state_size(const tk_linear_ce_desc_t* desc);
 TK_API size_t tk_linear_ce_workspace_size(const tk_linear_ce_desc_t* desc);
 TK_API int tk_linear_ce(const tk_linear_ce_desc_t* desc, void* workspace, size_t workspace_bytes,
                         void* stream);
 
 /* Its gradients: fwd is the forward call's descriptor with its state (x and loss
- * are not read: the state holds x's rows), grad_loss the gradient of the loss ([rows] or one value).  dx
- * [rows, cols], dweight [vocab, cols] and dbias [vocab] may be NULL.  The
- * logits are computed again in pieces of the vocabulary; softmax - onehot is
- * held as binary16 (two planes for fp32), so each of its entries is known to
- * 2^-39 at least, and no closer: below 2^-28 in fp16 and 2^-17 in fp32 an entry
- * has fewer than 11 and 22 bits.  A row's dx depends on that row's grad_loss
+ * are not read: the state holds x's rows), grad_loss the gradient of the loss
+ * ([rows] or one value).  dx [rows, cols], dweight [vocab, cols] and dbias [vocab]
+ * may be NULL.  The logits are computed again in pieces of the vocabulary;
+ * softmax - onehot is held as binary16 (two planes for fp32): 11 (22) bits, and
+ * an entry of any size may be 2^-39 off, so one below 2^-28 (2^-17) has fewer.
+ * A row's dx depends on that row's grad_loss
  * alone; a non-finite grad_loss makes its row of dx and all of dweight and dbias
  * non-finite.  Deterministic; the state is only read. */
 typedef struct {

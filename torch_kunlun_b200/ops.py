@@ -147,8 +147,8 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Te
     gradient depend on that row alone.  Products are those of the tensors' own
     values (float32 to 22 bits) summed in fp32, not the int16-quantised ones of
     ``linear``.  In the backward pass softmax - onehot is held to 11 bits for
-    float16 and 22 for float32, and no closer than 2**-39.  Differentiable in x, weight
-    and bias."""
+    float16 and 22 for float32, and an entry of any size may be 2**-39 off.
+    Differentiable in x, weight and bias."""
     if reduction not in REDUCTION:
         raise ValueError(f"reduction must be one of {sorted(REDUCTION)}, got {reduction!r}")
     return _C.linear_cross_entropy(x, weight, target, bias, int(ignore_index), REDUCTION[reduction])
